@@ -83,6 +83,25 @@ class GemmArgs(C.Structure):
                 ("ws_bytes", C.c_size_t), ("norm_ls", C.c_float)]
 
 
+class RopeScaling(C.Structure):
+    """e2cuda_rope_scaling: how rotary frequencies reach past the trained length (0: the kind's default)."""
+
+    _fields_ = [("kind", C.c_int), ("original", C.c_int), ("factor", C.c_float), ("fast", C.c_float), ("slow", C.c_float),
+                ("gain", C.c_float)]
+
+
+class Pages(C.Structure):
+    """e2cuda_pages: the description of a paged key/value cache."""
+
+    _fields_ = [("k", vp), ("v", vp), ("table", vp), ("len", vp), ("refs", vp), ("ws", vp), ("type", C.c_int),
+                ("layers", C.c_int), ("n_pages", C.c_int), ("page", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("max_seqs", C.c_int), ("max_blocks", C.c_int)]
+
+
+F32, BF16, F16 = 0, 1, 2
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_BY_ROTATIONS, ROPE_BY_PAIRS = 0, 1, 2, 3, 4
+ROPE_INTERLEAVED, ROPE_TRANSPOSE = 1, 2
+
 EPI_F32, EPI_RESID, EPI_I32, EPI_GELU, EPI_QKV, EPI_NORMADD, EPI_GELUQ, EPI_QKVPB = 0, 1, 2, 3, 4, 5, 6, 7
 
 
@@ -118,6 +137,20 @@ API = [
                                        C.c_float, vp]),
     ("e2cuda_attention_window", C.c_int, [vp, vp, vp, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                           C.c_float, C.c_int, vp]),
+    ("e2cuda_rope_table", C.c_int, [vp, vp, C.c_int, C.c_int, C.c_float, C.POINTER(RopeScaling), vp]),
+    ("e2cuda_rope", C.c_int, [vp, C.c_int, C.c_int, vp, C.c_int, C.c_int, vp, vp, C.c_int, C.c_int, vp, C.c_int, C.c_int,
+                              C.c_int, C.c_int, vp]),
+    ("e2cuda_pages_ws_bytes", C.c_size_t, [C.c_int, C.c_int]),
+    ("e2cuda_pages_fork", C.c_int, [vp, vp, vp, C.c_int, vp]),
+    ("e2cuda_pages_append", C.c_int, [vp, vp, vp, C.c_int, vp]),
+    ("e2cuda_pages_free", C.c_int, [vp, vp, C.c_int, vp]),
+    ("e2cuda_pages_compact", C.c_int, [vp, vp, vp]),
+    ("e2cuda_pages_copy", C.c_int, [vp, vp, vp, C.c_int, vp]),
+    ("e2cuda_pages_store", C.c_int, [vp, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, vp, C.c_int,
+                                     C.c_int, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp]),
+    ("e2cuda_pages_attention_ws_bytes", C.c_size_t, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    ("e2cuda_pages_attention", C.c_int, [vp, C.c_int, vp, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                         C.c_int, C.c_float, vp, C.c_int, vp, vp, C.c_size_t, vp]),
     ("e2cuda_ffn_create", vp, [C.POINTER(Q8W), C.POINTER(Q8W), C.POINTER(Q8W), f32p, C.c_float, C.c_int]),
     ("e2cuda_ffn_destroy", None, [vp]),
     ("e2cuda_ffn_forward", C.c_int, [vp, vp, C.c_int, vp, vp]),
@@ -315,6 +348,178 @@ def attention_window(q, k, vt, valid, B: int, S: int, H: int, KV: int, D: int, s
     _ok(lib().e2cuda_attention_window(_ptr(q), _ptr(k), _ptr(vt), vt.shape[-1], _ptr(valid), _ptr(ctx), B, S, H, KV, D,
                                       scale, window, _stream(stream)), "attention_window")
     return ctx
+
+
+# ------------------------------------------------------------------------------------ prompt cache
+_types: dict = {}
+
+
+def _type(t) -> int:
+    """The E2CUDA_* element type of a tensor."""
+    if not _types:
+        torch = _torch()
+        _types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    try:
+        return _types[t.dtype]
+    except KeyError:
+        raise E2CudaError(f"element type {t.dtype}: fp32, bf16 or fp16") from None
+
+
+def _rows(t, what: str) -> int:
+    """Elements between the rows of a [rows][heads][head_dim] tensor whose heads lie side by side."""
+    s = t.stride()
+    if len(s) != 3 or (s[2] != 1 and t.shape[2] > 1) or (s[1] != t.shape[2] and t.shape[1] > 1):
+        raise E2CudaError(f"{what}: [rows][heads][head_dim] with the heads of a row side by side, got strides {tuple(s)}")
+    return s[0] if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _ints(t, count: int, what: str) -> int:
+    """The address of a device int32 list of `count` entries."""
+    if t.dtype != _torch().int32 or t.dim() != 1 or t.shape[0] != count or not t.is_cuda or (count > 1 and t.stride(0) != 1):
+        raise E2CudaError(f"{what}: a contiguous device int32 list of {count}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _table(cos, sin) -> tuple[int, int]:
+    """(positions, rot) of a rotary table."""
+    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()) or _type(cos) or _type(sin) \
+            or not (cos.is_cuda and sin.is_cuda):
+        raise E2CudaError("rotary table: contiguous device fp32 cos and sin of the same [positions][rot / 2]")
+    return cos.shape[0], 2 * cos.shape[1]
+
+
+def rope_table(positions: int, rot: int, theta: float = 1e4, scaling: RopeScaling | None = None, stream=None):
+    """cos, sin [positions][rot / 2] fp32 of the angles position * theta^(-2 i / rot), scaled for long
+    contexts as `scaling` says."""
+    torch = _torch()
+    cos = torch.empty((positions, rot // 2), dtype=torch.float32, device="cuda")
+    sin = torch.empty_like(cos)
+    _ok(lib().e2cuda_rope_table(cos.data_ptr(), sin.data_ptr(), positions, rot, theta,
+                                None if scaling is None else C.byref(scaling), _stream(stream)), "rope_table")
+    return cos, sin
+
+
+def rope(x, cos, sin, pos=None, interleaved: bool = False, backward: bool = False, out=None, dtype=None, stream=None):
+    """x [T][heads][head_dim] with the pairs of each head's first 2 * cos.shape[1] dimensions rotated at
+    positions pos [T] int32 (None: 0..T-1). backward: the transposed rotation, which takes a gradient
+    with respect to the result to one with respect to x. out may be x; dtype: the result's type
+    (x's own, or 16 bits for an fp32 x)."""
+    torch = _torch()
+    T, H, D = x.shape
+    positions, rot = _table(cos, sin)
+    if out is None:
+        out = torch.empty((T, H, D), dtype=dtype or x.dtype, device=x.device)
+    elif out.shape != x.shape:
+        raise E2CudaError(f"rope: out {tuple(out.shape)} for x {tuple(x.shape)}")
+    _ok(lib().e2cuda_rope(x.data_ptr(), _rows(x, "rope"), _type(x), out.data_ptr(), _rows(out, "rope out"), _type(out),
+                          cos.data_ptr(), sin.data_ptr(), positions, rot, None if pos is None else _ints(pos, T, "rope pos"), T, H,
+                          D, (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_TRANSPOSE if backward else 0), _stream(stream)),
+        "rope")
+    return out
+
+
+class PageCache:
+    """A paged key/value cache (e2cuda_pages) over the caller's tensors: k, v
+    [layers][n_pages][page][kv_heads][head_dim] bf16 or fp16, table [max_seqs][max_blocks], length
+    [max_seqs] and refs [n_pages] int32 (length and refs zero when new). PageCache.new makes them.
+    Sequence and count lists are device int32 tensors; every method only queues work."""
+
+    def __init__(self, k, v, table, length, refs):
+        torch = _torch()
+        if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype or not (k.is_contiguous() and v.is_contiguous()):
+            raise E2CudaError("PageCache: contiguous k and v of the same [layers][n_pages][page][kv_heads][head_dim] and type")
+        for t, shape in ((table, (length.shape[0], table.shape[-1])), (length, (length.shape[0],)), (refs, (k.shape[1],))):
+            if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+                raise E2CudaError(f"PageCache: a contiguous int32 tensor of {shape}, got {t.dtype} {tuple(t.shape)}")
+        if not all(t.is_cuda and t.device == k.device for t in (k, v, table, length, refs)):
+            raise E2CudaError("PageCache: all tensors on one CUDA device")
+        self.k, self.v, self.table, self.length, self.refs = k, v, table, length, refs
+        layers, n_pages, page, kv, dim = k.shape
+        self.ws = torch.empty(lib().e2cuda_pages_ws_bytes(n_pages, length.shape[0]) // 4, dtype=torch.int32, device=k.device)
+        self._scratch: dict = {}  # the attention's, by stream
+        self.pages = Pages(k.data_ptr(), v.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.ws.data_ptr(),
+                           _type(k), layers, n_pages, page, kv, dim, table.shape[0], table.shape[1])
+        self._p = C.addressof(self.pages)
+
+    @classmethod
+    def new(cls, layers: int, n_pages: int, page: int, kv_heads: int, head_dim: int, max_seqs: int, max_blocks: int, dtype):
+        torch = _torch()
+        shape = (layers, n_pages, page, kv_heads, head_dim)
+        ints = dict(dtype=torch.int32, device="cuda")
+        return cls(torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"),
+                   torch.zeros((max_seqs, max_blocks), **ints), torch.zeros(max_seqs, **ints), torch.zeros(n_pages, **ints))
+
+    def fork(self, parents, children, stream=None) -> None:
+        """Each child, a free sequence, maps its parent's pages."""
+        n = children.shape[0]
+        _ok(lib().e2cuda_pages_fork(self._p, _ints(parents, n, "fork"), _ints(children, n, "fork"), n, _stream(stream)), "fork")
+
+    def append(self, seqs, counts, stream=None) -> None:
+        """Sequence seqs[i] grows by counts[i] tokens; a partly filled page that others map is copied first."""
+        n = seqs.shape[0]
+        _ok(lib().e2cuda_pages_append(self._p, _ints(seqs, n, "append"), _ints(counts, n, "append"), n, _stream(stream)),
+            "append")
+
+    def free(self, seqs, stream=None) -> None:
+        n = seqs.shape[0]
+        _ok(lib().e2cuda_pages_free(self._p, _ints(seqs, n, "free"), n, _stream(stream)), "free")
+
+    def compact(self, used=None, stream=None) -> None:
+        """The pages in use move to the pool's low end; used (device int32 [1]) gets their count."""
+        _ok(lib().e2cuda_pages_compact(self._p, None if used is None else _ints(used, 1, "compact"), _stream(stream)), "compact")
+
+    def copy(self, src, dst, stream=None) -> None:
+        """Page src[i]'s keys and values, in every layer, to page dst[i]."""
+        n = src.shape[0]
+        _ok(lib().e2cuda_pages_copy(self._p, _ints(src, n, "copy"), _ints(dst, n, "copy"), n, _stream(stream)), "copy")
+
+    def store(self, layer: int, q, k, v, cos, sin, seqs, q_start, interleaved: bool = False, out=None, stream=None):
+        """The batch's q [T][heads][head_dim] and k, v [T][kv_heads][head_dim] (fp32 or the cache's type) of
+        `layer`: q and k rotated at their tokens' positions, k and v written to the cache; returns the
+        rotated q in the cache's type. Entry i's rows q_start[i]..q_start[i+1]-1 are the last tokens of
+        sequence seqs[i], which append has grown."""
+        T, H, D = q.shape
+        p, n = self.pages, seqs.shape[0]
+        if k.shape != (T, p.kv_heads, p.head_dim) or v.shape != k.shape or D != p.head_dim or not q.dtype == k.dtype == v.dtype:
+            raise E2CudaError(f"store: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} of one type for a cache of "
+                              f"{p.kv_heads} heads of {p.head_dim}")
+        positions, rot = _table(cos, sin)
+        if out is None:
+            out = q.new_empty((T, H, D), dtype=self.k.dtype)
+        elif out.shape != q.shape or out.dtype != self.k.dtype:
+            raise E2CudaError(f"store: out {tuple(out.shape)} {out.dtype}")
+        _ok(lib().e2cuda_pages_store(self._p, layer, _type(q), q.data_ptr(), _rows(q, "store q"), k.data_ptr(), _rows(k, "store k"),
+                                     v.data_ptr(), _rows(v, "store v"), out.data_ptr(), _rows(out, "store out"), cos.data_ptr(),
+                                     sin.data_ptr(), positions, rot, ROPE_INTERLEAVED if interleaved else 0,
+                                     _ints(seqs, n, "store seqs"), _ints(q_start, n + 1, "store q_start"), n, T, H,
+                                     _stream(stream)), "store")
+        return out
+
+    def attention(self, layer: int, q, seqs, q_start, max_q: int, shared: int = 0, causal: bool = True, window: int = -1,
+                  scale: float | None = None, lse: bool = False, out=None, stream=None):
+        """Attention of q [T][heads][head_dim] over the batch's cached tokens (the batch as in store; max_q:
+        an upper bound of an entry's rows). The first `shared` tokens of every sequence lie in the same
+        pages and are read once for the batch. Returns out, or (out, lse [T][heads])."""
+        T, H, D = q.shape
+        p, n = self.pages, seqs.shape[0]
+        if D != p.head_dim or q.dtype != self.k.dtype:
+            raise E2CudaError(f"attention: q {tuple(q.shape)} {q.dtype} for a cache of heads of {p.head_dim} {self.k.dtype}")
+        if out is None:
+            out = q.new_empty((T, H, D))
+        elif out.shape != q.shape or out.dtype != q.dtype:
+            raise E2CudaError(f"attention: out {tuple(out.shape)} {out.dtype}")
+        sums = q.new_empty((T, H), dtype=_torch().float32) if lse else None
+        st = _stream(stream)
+        need = lib().e2cuda_pages_attention_ws_bytes(self._p, n, T, max_q, H, shared)
+        ws = self._scratch.get(st)
+        if ws is None or ws.numel() < need:
+            with _torch().cuda.stream(stream):  # its memory is reused in that stream's order
+                ws = self._scratch[st] = q.new_empty(max(need, 16), dtype=_torch().uint8)
+        _ok(lib().e2cuda_pages_attention(self._p, layer, q.data_ptr(), _rows(q, "attention q"), _ints(seqs, n, "attention seqs"),
+                                         _ints(q_start, n + 1, "attention q_start"), n, T, max_q, H, shared, causal, window,
+                                         1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(),
+                                         _rows(out, "attention out"), _ptr(sums), ws.data_ptr(), ws.numel(), st), "attention")
+        return (out, sums) if lse else out
 
 
 class FFN:

@@ -66,6 +66,9 @@ static const char *status_name(int s) {
     case 0x105: return "drain of in-flight copies timed out";
     case 0x106: return "token id outside the embedding table";
     case 0x107: return "dynamic shared memory not 1024-byte aligned (kernel skipped)";
+    case 0x108: return "position outside the rotary table";
+    case 0x109: return "not enough free pages (the append did nothing)";
+    case 0x10a: return "sequence, count or page outside the cache (that entry was left out)";
     default: return "unknown device failure";
     }
 }

@@ -205,6 +205,40 @@ int e2c_attention_win(const void *q, const void *k, const void *vt, int ldvt, co
 int e2c_attention_wide(const void *q, const void *k, const void *vt, int ldvt, const uint8_t *valid, float *ctx,
                        int B, int S, int H, int KV, float scale, int window, int *status, void *stream);
 
+/* ---- rotary positions (rope.cu) */
+enum { E2C_F32 = 0, E2C_BF16 = 1, E2C_F16 = 2 }; /* element types, E2CUDA_F32.. */
+/* cs/sn [positions][half] = gain * cos/sin(position * freq[i]); freq: host, half <= 256 */
+int e2c_rope_table(float *cs, float *sn, int positions, int half, const double *freq, double gain, void *stream);
+/* x [T] rows of H heads of D (row stride ldx elements) -> y; pos NULL: row t is position t. Types
+ * equal, or fp32 -> 16 bits. A position outside the table records 0x108 and uses position 0. */
+int e2c_rope(const void *x, int64_t ldx, int x_type, void *y, int64_t ldy, int y_type, const float *cs, const float *sn,
+             int positions, int half, const int32_t *pos, int T, int H, int D, int inter, int transpose, int *status,
+             void *stream);
+
+/* ---- a paged key/value cache (pages.cu, rope.cu, attention_pages.cu). k, v point at one layer for
+ * the store and the attention, at layer 0 for the page operations; a layer is
+ * [n_pages][page][KV][D] of `type` (16 bits). */
+typedef struct {
+    void *k, *v;
+    int32_t *table;      /* [max_seqs][max_blocks] */
+    int32_t *len, *refs; /* [max_seqs], [n_pages] */
+    int32_t *ws;         /* e2c_pages_ws_ints() */
+    int type, layers, n_pages, page, KV, D, max_seqs, max_blocks;
+} e2c_pages;
+size_t e2c_pages_ws_ints(int n_pages, int max_seqs);
+int e2c_pages_store(const e2c_pages *pc, int x_type, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
+                    int64_t ldv, void *q_out, int64_t ldo, const float *cs, const float *sn, int positions, int half, int inter,
+                    const int32_t *seqs, const int32_t *q_start, int n, int T, int H, int *status, void *stream);
+int e2c_pages_copy(const e2c_pages *pc, const int32_t *src, const int32_t *dst, int n, int *status, void *stream);
+int e2c_pages_fork(const e2c_pages *pc, const int32_t *parents, const int32_t *children, int n, int *status, void *stream);
+int e2c_pages_append(const e2c_pages *pc, const int32_t *seqs, const int32_t *counts, int n, int *status, void *stream);
+int e2c_pages_free(const e2c_pages *pc, const int32_t *seqs, int n, int *status, void *stream);
+int e2c_pages_compact(const e2c_pages *pc, int32_t *used, int *status, void *stream);
+size_t e2c_pages_attention_ws_bytes(int n, int T, int max_q, int H, int KV, int D, int shared);
+int e2c_pages_attention(const e2c_pages *pc, const void *q, int64_t ldq, const int32_t *seqs, const int32_t *q_start, int n, int T,
+                        int max_q, int H, int shared, int causal, int window, float scale, void *out, int64_t ldo, float *lse,
+                        void *ws, size_t ws_bytes, int *status, void *stream);
+
 /* ---- self-test of the bounded wait (selftest.cu): one warp waits on an mbarrier that receives
  * its arrival first (arrive != 0) or never (arrive == 0). *completed is 1 if the wait completed, 0
  * if it gave up after its bound (~2 s) and recorded `code` (0x101..0x105) in *status. */

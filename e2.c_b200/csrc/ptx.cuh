@@ -22,7 +22,10 @@ enum {
     E2C_ERR_WAIT_ATTN = 0x104,      // attention softmax / correction gave up
     E2C_ERR_WAIT_DRAIN = 0x105,     // teardown gave up draining in-flight copies
     E2C_ERR_BAD_TOKEN = 0x106,      // a token id outside the table (row 0 used instead)
-    E2C_ERR_SMEM_ALIGN = 0x107      // dynamic shared memory not 1024-byte aligned: the kernel did nothing
+    E2C_ERR_SMEM_ALIGN = 0x107,     // dynamic shared memory not 1024-byte aligned: the kernel did nothing
+    E2C_ERR_BAD_POSITION = 0x108,   // a position outside the rotary table
+    E2C_ERR_NO_PAGES = 0x109,       // fewer free pages than an append needs: it did nothing
+    E2C_ERR_BAD_SEQ = 0x10a         // a sequence, count or page outside the cache (that entry is left out)
 };
 
 E2C_DEV uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }

@@ -1,0 +1,384 @@
+// rope.cu — rotary positions on the heads of token rows, and the same fused with the write of a
+// token's key and value into its page of the cache.
+//
+// A pair (a, b) of a head at position p with the angle's cos c and sin s becomes
+//   a' = a c - b s,  b' = b c + a s          (its transpose, the gradient: s -> -s)
+// for the rot / 2 pairs (i, i + rot/2), or (2i, 2i+1) interleaved; dimensions past rot pass through.
+//
+// Bound: memory. One thread owns V pairs (V elements = 16 bytes of the output type) of up to four
+// heads of one token, so a pair's cos and sin are read once for four heads and every thread has up to
+// eight 16-byte loads in flight; all arithmetic is in 32 bits with one rounding at the store. Rows
+// that 16-byte accesses do not fit (an odd stride, a rot whose halves are not multiples of V, an
+// unaligned base) take V = 1.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "launch.h"
+#include "pages.cuh"
+#include "pdl.h"
+#include "ptx.cuh"
+
+namespace {
+
+constexpr int HPT = 4;      // heads per thread
+constexpr int BLOCK = 128;  // threads per block: decode-sized calls spread over more SMs than with 256
+
+template <typename T>
+E2C_DEV float to_f(T x);
+template <>
+E2C_DEV float to_f(float x) {
+    return x;
+}
+template <>
+E2C_DEV float to_f(__nv_bfloat16 x) {
+    return __bfloat162float(x);
+}
+template <>
+E2C_DEV float to_f(__half x) {
+    return __half2float(x);
+}
+template <typename T>
+E2C_DEV T from_f(float x);
+template <>
+E2C_DEV float from_f(float x) {
+    return x;
+}
+template <>
+E2C_DEV __nv_bfloat16 from_f(float x) {
+    return __float2bfloat16_rn(x);
+}
+template <>
+E2C_DEV __half from_f(float x) {
+    return __float2half_rn(x);
+}
+
+// N consecutive values as floats; N * sizeof(T) is a multiple of 16 with 16-byte alignment, or N = 1
+template <typename T, int N>
+E2C_DEV void load(const T *p, float (&r)[N]) {
+    if constexpr (N == 1) {
+        r[0] = to_f<T>(*p);
+    } else {
+        constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i += PER) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(p + i);
+            const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+            for (int j = 0; j < PER; j++) r[i + j] = to_f<T>(e[j]);
+        }
+    }
+}
+template <typename T, int N>
+E2C_DEV void store(T *p, const float (&r)[N]) {
+    if constexpr (N == 1) {
+        *p = from_f<T>(r[0]);
+    } else {
+        constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N; i += PER) {
+            uint4 w;
+            T *e = reinterpret_cast<T *>(&w);
+#pragma unroll
+            for (int j = 0; j < PER; j++) e[j] = from_f<T>(r[i + j]);
+            *reinterpret_cast<uint4 *>(p + i) = w;
+        }
+    }
+}
+
+// V pairs of one head: the raw values at the two places, and the rotation
+template <typename TI, typename TO, int V>
+struct Pairs {
+    float a[V], b[V];
+    // pairs j V .. j V + V - 1 of the head at x
+    E2C_DEV void get(const TI *x, int j, int half, bool inter) {
+        if (!inter) {
+            load<TI, V>(x + j * V, a);
+            load<TI, V>(x + half + j * V, b);
+        } else if constexpr (V == 1) {
+            a[0] = to_f<TI>(x[2 * j]);
+            b[0] = to_f<TI>(x[2 * j + 1]);
+        } else {
+            load<TI, V>(x + 2 * j * V, a);
+            load<TI, V>(x + 2 * j * V + V, b);
+        }
+    }
+    E2C_DEV void put(TO *y, int j, int half, bool inter, const float (&c)[V], const float (&s)[V]) {
+        if (!inter || V == 1) {
+            float u[V], w[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                u[i] = a[i] * c[i] - b[i] * s[i];
+                w[i] = b[i] * c[i] + a[i] * s[i];
+            }
+            if (inter) {
+                y[2 * j] = from_f<TO>(u[0]);
+                y[2 * j + 1] = from_f<TO>(w[0]);
+            } else {
+                store<TO, V>(y + j * V, u);
+                store<TO, V>(y + half + j * V, w);
+            }
+        } else {
+            // a holds elements 0 .. V-1 of the 2 V interleaved ones, b the others
+            float u[V], w[V];
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                u[i] = a[i] * c[i / 2] - a[i + 1] * s[i / 2];
+                u[i + 1] = a[i + 1] * c[i / 2] + a[i] * s[i / 2];
+                w[i] = b[i] * c[(V + i) / 2] - b[i + 1] * s[(V + i) / 2];
+                w[i + 1] = b[i + 1] * c[(V + i) / 2] + b[i] * s[(V + i) / 2];
+            }
+            store<TO, V>(y + 2 * j * V, u);
+            store<TO, V>(y + 2 * j * V + V, w);
+        }
+    }
+};
+
+struct RopeArgs {
+    const void *x;
+    void *y;
+    int64_t ldx, ldy;
+    const float *cs, *sn;
+    const int32_t *pos;
+    int positions, half, T, H, D, inter, copy_rest;
+    float sign;
+    int *status;
+};
+
+// one thread: rotation unit j (V pairs, or V pass-through elements past them) of heads 4 hg .. 4 hg + 3
+template <typename TI, typename TO, int V>
+__global__ void __launch_bounds__(BLOCK) k_rope(const RopeArgs p, int units, int hgroups) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int64_t u = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
+    const int t = (int)(u / (units * hgroups));
+    if (t >= p.T) return;
+    const int rem = (int)(u - (int64_t)t * (units * hgroups));
+    const int hg = rem / units, j = rem - hg * units;
+    const int h0 = hg * HPT, nh = min(HPT, p.H - h0);
+    const TI *x = static_cast<const TI *>(p.x) + t * p.ldx + (int64_t)h0 * p.D;
+    TO *y = static_cast<TO *>(p.y) + t * p.ldy + (int64_t)h0 * p.D;
+    const int nrot = p.half / V;
+    if (j < nrot) {
+        Pairs<TI, TO, V> r[HPT];
+#pragma unroll
+        for (int h = 0; h < HPT; h++)
+            if (h < nh) r[h].get(x + h * p.D, j, p.half, p.inter);
+        int at = p.pos ? p.pos[t] : t;
+        if ((unsigned)at >= (unsigned)p.positions) {
+            record_status(p.status, E2C_ERR_BAD_POSITION);
+            at = 0;
+        }
+        float c[V], s[V];
+        load<float, V>(p.cs + (int64_t)at * p.half + j * V, c);
+        load<float, V>(p.sn + (int64_t)at * p.half + j * V, s);
+#pragma unroll
+        for (int i = 0; i < V; i++) s[i] *= p.sign;
+#pragma unroll
+        for (int h = 0; h < HPT; h++)
+            if (h < nh) r[h].put(y + h * p.D, j, p.half, p.inter, c, s);
+    } else {
+        const int e = 2 * p.half + (j - nrot) * V;
+        float a[HPT][V];
+#pragma unroll
+        for (int h = 0; h < HPT; h++)
+            if (h < nh) load<TI, V>(x + h * p.D + e, a[h]);
+#pragma unroll
+        for (int h = 0; h < HPT; h++)
+            if (h < nh) store<TO, V>(y + h * p.D + e, a[h]);
+    }
+}
+
+struct StoreArgs {
+    const void *q, *k, *v;
+    int64_t ldq, ldk, ldv;
+    void *q_out;
+    int64_t ldo;
+    const float *cs, *sn;
+    int positions, half, inter;
+    const int32_t *seqs, *q_start;
+    int n, T, H;
+    e2c_pages pc;  // k and v at the layer
+    int *status;
+};
+
+// One thread: unit j of up to four heads of one token, as k_rope; the heads are H query heads and KV
+// key heads (rotated) and KV value heads (passed through). The input loads are issued before the
+// chain of lookups (token -> sequence -> length -> page) that the stores wait for.
+template <typename TI, typename TO, int V>
+__global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, int units, int qgroups, int kgroups, int vunits) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int rot_units = units * (qgroups + kgroups), per_token = rot_units + vunits * kgroups;
+    const int64_t u = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
+    const int t = (int)(u / per_token);
+    if (t >= p.T) return;
+    const int rem = (int)(u - (int64_t)t * per_token);
+    const int D = p.pc.D, KV = p.pc.KV;
+    const bool is_v = rem >= rot_units;
+    const int r2 = is_v ? rem - rot_units : rem, per = is_v ? vunits : units;
+    int hg = r2 / per;
+    const int j = r2 - hg * per;
+    const bool is_q = !is_v && hg < qgroups;
+    if (!is_v && !is_q) hg -= qgroups;
+    const int h0 = hg * HPT, nh = min(HPT, (is_q ? p.H : KV) - h0);
+    const TI *x = is_q ? static_cast<const TI *>(p.q) + t * p.ldq
+                       : is_v ? static_cast<const TI *>(p.v) + t * p.ldv : static_cast<const TI *>(p.k) + t * p.ldk;
+    x += (int64_t)h0 * D;
+    const int nrot = p.half / V;
+    const bool turn = !is_v && j < nrot;
+    const int e = is_v ? j * V : 2 * p.half + (j - nrot) * V;  // the first element passed through
+    Pairs<TI, TO, V> r[HPT];
+#pragma unroll
+    for (int h = 0; h < HPT; h++)
+        if (h < nh) {
+            if (turn)
+                r[h].get(x + h * D, j, p.half, p.inter);
+            else
+                load<TI, V>(x + h * D + e, r[h].a);
+        }
+    int last;
+    const int i = e2c_token_seq(p.q_start, p.n, p.T, t, last);
+    const int seq = i < 0 ? -1 : p.seqs[i];
+    const bool ok = (unsigned)seq < (unsigned)p.pc.max_seqs;
+    const int at = ok ? p.pc.len[seq] - (last - t) : -1;
+    // a token without a place (its sequence is not in the cache, or is shorter than its queries, or
+    // longer than the table or the rotary table) is not written
+    if (at < 0 || at >= p.positions) {
+        record_status(p.status, at >= p.positions ? E2C_ERR_BAD_POSITION : E2C_ERR_BAD_SEQ);
+        return;
+    }
+    TO *y;
+    if (is_q) {
+        y = static_cast<TO *>(p.q_out) + t * p.ldo;
+    } else {
+        const int blk = at / p.pc.page, page = blk < p.pc.max_blocks ? p.pc.table[(int64_t)seq * p.pc.max_blocks + blk] : -1;
+        if ((unsigned)page >= (unsigned)p.pc.n_pages) {
+            record_status(p.status, E2C_ERR_BAD_SEQ);
+            return;
+        }
+        const int64_t row = (int64_t)page * p.pc.page + (at - blk * p.pc.page);
+        y = static_cast<TO *>(is_v ? p.pc.v : p.pc.k) + row * (KV * D);
+    }
+    y += (int64_t)h0 * D;
+    if (turn) {
+        float c[V], s[V];
+        load<float, V>(p.cs + (int64_t)at * p.half + j * V, c);
+        load<float, V>(p.sn + (int64_t)at * p.half + j * V, s);
+#pragma unroll
+        for (int h = 0; h < HPT; h++)
+            if (h < nh) r[h].put(y + h * D, j, p.half, p.inter, c, s);
+    } else {
+#pragma unroll
+        for (int h = 0; h < HPT; h++)
+            if (h < nh) store<TO, V>(y + h * D + e, r[h].a);
+    }
+}
+
+struct Freqs {
+    double f[256];
+};
+
+// cos and sin of position * frequency, in 64 bits: at position 10^6 a 32-bit product would be off by
+// 0.06 radians
+__global__ void __launch_bounds__(256) k_rope_table(float *cs, float *sn, int64_t total, int half, const __grid_constant__ Freqs fr,
+                                                    double gain) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (u >= total) return;
+    const int64_t p = u / half;
+    double s, c;
+    sincos((double)p * fr.f[u - p * half], &s, &c);
+    cs[u] = (float)(c * gain);
+    sn[u] = (float)(s * gain);
+}
+
+int launched(const char *what) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return 0;
+    e2c_set_msg("%s launch: %s", what, cudaGetErrorString(e));
+    return -2;
+}
+
+bool fits16(const void *p, int64_t ld, int bytes) { return ((uintptr_t)p & 15) == 0 && (ld * bytes) % 16 == 0; }
+
+template <typename TI, typename TO>
+int rope_as(const RopeArgs &a, bool vec, cudaStream_t st) {
+    constexpr int VV = 16 / sizeof(TO);
+    const int V = vec ? VV : 1;
+    const int units = a.half / V + (a.copy_rest ? (a.D - 2 * a.half) / V : 0), hgroups = (a.H + HPT - 1) / HPT;
+    const int64_t total = (int64_t)a.T * units * hgroups;
+    if (total == 0) return 0;
+    const int64_t blocks = (total + BLOCK - 1) / BLOCK;
+    if (blocks > 0x7fffffff) {
+        e2c_set_msg("rope: too many tokens for one call");
+        return -1;
+    }
+    if (vec)
+        e2c_launch(k_rope<TI, TO, VV>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, hgroups);
+    else
+        e2c_launch(k_rope<TI, TO, 1>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, hgroups);
+    return launched("rope");
+}
+
+template <typename TI, typename TO>
+int store_as(const StoreArgs &a, bool vec, cudaStream_t st) {
+    constexpr int VV = 16 / sizeof(TO);
+    const int V = vec ? VV : 1, D = a.pc.D;
+    const int units = a.half / V + (D - 2 * a.half) / V, vunits = D / V;
+    const int qg = (a.H + HPT - 1) / HPT, kg = (a.pc.KV + HPT - 1) / HPT;
+    const int64_t blocks = ((int64_t)a.T * (units * (qg + kg) + vunits * kg) + BLOCK - 1) / BLOCK;
+    if (blocks > 0x7fffffff) {
+        e2c_set_msg("pages_store: too many tokens for one call");
+        return -1;
+    }
+    if (vec)
+        e2c_launch(k_pages_store<TI, TO, VV>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, qg, kg, vunits);
+    else
+        e2c_launch(k_pages_store<TI, TO, 1>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, qg, kg, vunits);
+    return launched("pages_store");
+}
+
+}  // namespace
+
+extern "C" int e2c_rope_table(float *cs, float *sn, int positions, int half, const double *freq, double gain, void *stream) {
+    Freqs fr;
+    for (int i = 0; i < half; i++) fr.f[i] = freq[i];
+    const int64_t total = (int64_t)positions * half;
+    e2c_launch(k_rope_table, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, cs, sn, total, half, fr,
+               gain);
+    return launched("rope_table");
+}
+
+extern "C" int e2c_rope(const void *x, int64_t ldx, int x_type, void *y, int64_t ldy, int y_type, const float *cs, const float *sn,
+                        int positions, int half, const int32_t *pos, int T, int H, int D, int inter, int transpose, int *status,
+                        void *stream) {
+    RopeArgs a = {x, y, ldx, ldy, cs, sn, pos, positions, half, T, H, D, inter, x != y, transpose ? -1.f : 1.f, status};
+    const int xb = x_type == E2C_F32 ? 4 : 2, yb = y_type == E2C_F32 ? 4 : 2, V = 16 / yb;
+    const bool vec = half % V == 0 && D % V == 0 && fits16(x, ldx, xb) && fits16(y, ldy, yb) && fits16(cs, 0, 4) && fits16(sn, 0, 4);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (x_type == E2C_F32 && y_type == E2C_F32) return rope_as<float, float>(a, vec, st);
+    if (x_type == E2C_F32 && y_type == E2C_BF16) return rope_as<float, __nv_bfloat16>(a, vec, st);
+    if (x_type == E2C_F32 && y_type == E2C_F16) return rope_as<float, __half>(a, vec, st);
+    if (x_type == E2C_BF16 && y_type == E2C_BF16) return rope_as<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
+    if (x_type == E2C_F16 && y_type == E2C_F16) return rope_as<__half, __half>(a, vec, st);
+    e2c_set_msg("rope: types %d -> %d", x_type, y_type);
+    return -1;
+}
+
+extern "C" int e2c_pages_store(const e2c_pages *pc, int x_type, const void *q, int64_t ldq, const void *k, int64_t ldk,
+                               const void *v, int64_t ldv, void *q_out, int64_t ldo, const float *cs, const float *sn,
+                               int positions, int half, int inter, const int32_t *seqs, const int32_t *q_start, int n, int T, int H,
+                               int *status, void *stream) {
+    StoreArgs a = {q, k, v, ldq, ldk, ldv, q_out, ldo, cs, sn, positions, half, inter, seqs, q_start, n, T, H, *pc, status};
+    const int xb = x_type == E2C_F32 ? 4 : 2;
+    const bool vec = half % 8 == 0 && fits16(q, ldq, xb) && fits16(k, ldk, xb) && fits16(v, ldv, xb) && fits16(q_out, ldo, 2) &&
+                     fits16(cs, 0, 4) && fits16(sn, 0, 4);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (pc->type == E2C_BF16)
+        return x_type == E2C_F32 ? store_as<float, __nv_bfloat16>(a, vec, st) : store_as<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
+    return x_type == E2C_F32 ? store_as<float, __half>(a, vec, st) : store_as<__half, __half>(a, vec, st);
+}

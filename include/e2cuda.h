@@ -7,6 +7,8 @@
  *   - activation quantiser          replaces e2_i8_quantize      (e2.c src/kernels.h:72)
  *   - W8A8 GEMM + fused epilogues   replaces e2_i8_gemm          (e2.c src/int8.h:96-97)
  *   - bf16 flash attention          replaces attention_blocked   (e2.c src/text.c:780-815)
+ *   - the prompt cache              rotary positions, a paged key/value cache and attention over it for
+ *                                   causal or prefix towers (no counterpart in e2.c)
  *   - the synthetic encoder         the text tower's layer recipe (e2.c src/text.c:924-984) over
  *                                   the kernels above, batch API shaped like e2_hip_text_embed_batch
  *                                   (e2.c include/e2hip.h:44-50)
@@ -191,6 +193,118 @@ int e2cuda_attention_gqa(const void *q, const void *k, const void *vt, int ldvt,
  * the value dimensions). */
 int e2cuda_attention_window(const void *q, const void *k, const void *vt, int ldvt, const uint8_t *valid,
                             float *ctx, int B, int S, int H, int KV, int D, float scale, int window, void *stream);
+
+/* ------------------------------------------------------------------ rotary positions */
+/* Element types of the calls below. */
+enum { E2CUDA_F32 = 0, E2CUDA_BF16 = 1, E2CUDA_F16 = 2 };
+
+/* How the frequencies theta^(-2 i / rot) of the rot / 2 pairs are scaled to reach past the length a
+ * model was trained on, by `factor` >= 1:
+ *   PLAIN         not at all
+ *   LINEAR        every frequency divided by factor
+ *   NTK           theta multiplied by factor^(rot / (rot - 2))
+ *   BY_ROTATIONS  a pair that makes at least `fast` (default 4) rotations over `original` positions
+ *                 keeps its frequency, one that makes at most `slow` (default 1) has it divided by
+ *                 factor; between them the share kept is linear in the rotations
+ *   BY_PAIRS      the same with the share linear in the pair index, between the pairs that make `fast`
+ *                 (default 32) and `slow` (default 1) rotations, rounded outward; cos and sin are
+ *                 multiplied by 0.1 ln(factor) + 1 unless `gain` says otherwise
+ * gain != 0 multiplies cos and sin. */
+enum {
+    E2CUDA_ROPE_PLAIN = 0,
+    E2CUDA_ROPE_LINEAR = 1,
+    E2CUDA_ROPE_NTK = 2,
+    E2CUDA_ROPE_BY_ROTATIONS = 3,
+    E2CUDA_ROPE_BY_PAIRS = 4
+};
+typedef struct e2cuda_rope_scaling {
+    int kind, original;
+    float factor, fast, slow, gain; /* fast, slow, gain: 0 for the kind's default */
+} e2cuda_rope_scaling;
+/* cos, sin (device fp32 [positions][rot / 2]) of every position's angles, computed in 64 bits. rot even,
+ * 2..512; s NULL: PLAIN. */
+int e2cuda_rope_table(float *cos_t, float *sin_t, int positions, int rot, float theta, const e2cuda_rope_scaling *s,
+                      void *stream);
+
+/* x: T rows of `heads` heads of head_dim (head h at h * head_dim; rows ldx elements apart) -> y, rows ldy
+ * apart. Pairs (i, i + rot/2) of a head's first rot dimensions, or (2i, 2i + 1) with INTERLEAVED, are
+ * rotated by the angles of row t's position pos[t] (device; NULL: t); the rest is copied. TRANSPOSE
+ * applies the transposed matrix: the gradient with respect to x from the one with respect to y.
+ * Types: equal, or fp32 -> 16 bits. y may be x (equal types and rows). A position outside the table
+ * is taken as position 0 and reported by e2cuda_check. */
+enum { E2CUDA_ROPE_INTERLEAVED = 1, E2CUDA_ROPE_TRANSPOSE = 2 };
+int e2cuda_rope(const void *x, int ldx, int x_type, void *y, int ldy, int y_type, const float *cos_t, const float *sin_t,
+                int positions, int rot, const int32_t *pos, int T, int heads, int head_dim, int flags, void *stream);
+
+/* ------------------------------------------------------------------ prompt cache */
+/* A paged key/value cache: device memory that the caller owns, described here. Its whole state is on
+ * the device, so every call below only queues work (and can be captured in a graph). A sequence's tokens
+ * [b * page, (b + 1) * page) lie in page table[seq][b]; several sequences may map one page, and refs counts
+ * them. A new cache has len and refs zero; the other arrays need no initial value.
+ *
+ * Calls on one cache must be ordered (one stream, or events). The calls take device lists of sequences;
+ * no sequence may be named twice in one call (except as a parent). An entry that is outside the cache is
+ * left out and reported by e2cuda_check. */
+typedef struct e2cuda_pages {
+    void *k, *v;    /* [layers][n_pages][page][kv_heads][head_dim], 16-byte aligned                */
+    int32_t *table; /* [max_seqs][max_blocks]                                                      */
+    int32_t *len;   /* [max_seqs] tokens held; 0: the sequence is free                             */
+    int32_t *refs;  /* [n_pages] sequences that map the page; 0: free. 16-byte aligned             */
+    int32_t *ws;    /* e2cuda_pages_ws_bytes() of scratch                                          */
+    int type;       /* E2CUDA_BF16 or E2CUDA_F16                                                   */
+    int layers, n_pages;
+    int page;       /* tokens of a page: a power of two, 8..1024                                   */
+    int kv_heads, head_dim; /* head_dim 64, 128 or 256                                             */
+    int max_seqs, max_blocks;
+} e2cuda_pages;
+size_t e2cuda_pages_ws_bytes(int n_pages, int max_seqs);
+
+/* Each child (a free sequence) maps its parent's pages: no data moves. */
+int e2cuda_pages_fork(const e2cuda_pages *pc, const int32_t *parents, const int32_t *children, int n, void *stream);
+/* Sequence seqs[i] grows by counts[i] tokens, whose keys and values are then stored. Blocks past the
+ * old ones get the lowest free pages, in the list's order. A partly filled last page that other
+ * sequences map too is first copied (every layer) to a page of the sequence's own; which pages are
+ * shared is judged before the call changes anything. With too few free pages the whole call does
+ * nothing and is reported by e2cuda_check. */
+int e2cuda_pages_append(const e2cuda_pages *pc, const int32_t *seqs, const int32_t *counts, int n, void *stream);
+/* The sequences' pages lose one mapping each; the sequences become free. */
+int e2cuda_pages_free(const e2cuda_pages *pc, const int32_t *seqs, int n, void *stream);
+/* The pages in use move to the pool's low end: the k-th one past the used count to the k-th hole
+ * below it. used (device, or NULL) gets the count: pages [0, used) are then in use, the rest is free. */
+int e2cuda_pages_compact(const e2cuda_pages *pc, int32_t *used, void *stream);
+/* Page src[i]'s keys and values, in every layer, copied to page dst[i] (src[i] < 0: none). No dst may
+ * be another entry's src or dst. Tables and counts are the caller's to change. */
+int e2cuda_pages_copy(const e2cuda_pages *pc, const int32_t *src, const int32_t *dst, int n, void *stream);
+
+/* The batch of a store or attention call: entry i is sequence seqs[i], whose last q_start[i + 1] -
+ * q_start[i] tokens are rows q_start[i].. of the call's T rows (device lists; q_start has n + 1 entries, from 0
+ * to T). Row t's position follows from its sequence's length. */
+
+/* q and k rotated at their tokens' positions (as e2cuda_rope; flags: INTERLEAVED), k and v written to the
+ * tokens' places in the cache, q to q_out (rows ldo apart, the cache's type). q, k, v: rows of heads of head_dim,
+ * fp32 or the cache's type; q_out may be q. Rows without a place are left out and reported. */
+int e2cuda_pages_store(const e2cuda_pages *pc, int layer, int x_type, const void *q, int ldq, const void *k, int ldk,
+                       const void *v, int ldv, void *q_out, int ldo, const float *cos_t, const float *sin_t, int positions,
+                       int rot, int flags, const int32_t *seqs, const int32_t *q_start, int n, int T, int heads,
+                       void *stream);
+
+/* Attention of the batch's rows over their sequences' cached tokens:
+ *   out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j,   lse[t][h] = log sum_j exp(scale * q[t][h] . k_j)
+ * over the tokens j in sight of t's position p: j < len, with `causal` j <= p, with window >= 0
+ * |p - j| <= window. Query head h reads key head h / (heads / kv_heads); at most 128 query heads for one key
+ * head. q, out: rows of heads of head_dim in the cache's type, 16-byte aligned, ld a multiple of 8. lse: fp32
+ * [T][heads] or NULL. A row that sees nothing gets zeros and -infinity. What the cache holds past a sequence's
+ * length is never used, whatever its value.
+ *
+ * shared (a multiple of page): the first `shared` tokens of every sequence of the batch lie in the same
+ * pages, as after a fork; their keys are then read once for the batch instead of once for each
+ * sequence. 0 asks for nothing of the tables. max_q: an upper bound of an entry's rows.
+ *
+ * ws: e2cuda_pages_attention_ws_bytes() of 16-byte aligned scratch that no other call uses meanwhile. */
+size_t e2cuda_pages_attention_ws_bytes(const e2cuda_pages *pc, int n, int T, int max_q, int heads, int shared);
+int e2cuda_pages_attention(const e2cuda_pages *pc, int layer, const void *q, int ldq, const int32_t *seqs,
+                           const int32_t *q_start, int n, int T, int max_q, int heads, int shared, int causal, int window,
+                           float scale, void *out, int ldo, float *lse, void *ws, size_t ws_bytes, void *stream);
 
 /* ------------------------------------------------------------------ fused FFN block (config 1) */
 typedef struct e2cuda_ffn e2cuda_ffn;
