@@ -127,6 +127,13 @@ E2C_DEV void tma_load_2d(uint32_t dst, const CUtensorMap *m, int x, int y, uint3
         "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
+E2C_DEV void tma_load_3d(uint32_t dst, const CUtensorMap *m, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
 // 2D tile store from this CTA's shared memory (bulk-group completion). Rows / columns outside the
 // tensor are not written.
 E2C_DEV void tma_store_2d(const CUtensorMap *m, uint32_t src, int x, int y) {
@@ -355,6 +362,12 @@ E2C_DEV uint64_t smem_desc_sw64(uint32_t addr) {
     d |= (uint64_t)1 << 46;             // descriptor version (sm_100)
     d |= (uint64_t)4 << 61;             // SWIZZLE_64B
     return d;
+}
+
+// A B operand stored with its N dimension contiguous (MN-major): panels of 64 N elements (rows of 128
+// bytes, one row per k, 128-byte swizzle), `panel` bytes apart; 8-row groups of k 1024 bytes apart.
+E2C_DEV uint64_t smem_desc_sw128_mn(uint32_t addr, uint32_t panel) {
+    return smem_desc_sw128(addr) | (uint64_t)((panel >> 4) & 0x3FFFu) << 16;  // leading byte offset
 }
 
 // Instruction descriptors (M = 128, K-major A and B, dense).

@@ -72,6 +72,35 @@ static int tmap_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int
     return 0;
 }
 
+int e2c_tmap_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner, uint64_t mid,
+                uint64_t outer, uint64_t mid_stride, uint64_t outer_stride, uint32_t box_inner, uint32_t box_mid,
+                uint32_t box_outer) {
+    encode_tiled_fn enc = get_encode();
+    if (!enc) {
+        e2c_set_msg("tensor map: cuTensorMapEncodeTiled unavailable");
+        return -1;
+    }
+    if (box_inner * (uint32_t)elem_bytes != 128 || ((uintptr_t)base & 15) || (mid_stride & 15) || (outer_stride & 15)) {
+        e2c_set_msg("tensor map: 128-byte boxes, 16-byte aligned base and strides required");
+        return -1;
+    }
+    const cuuint64_t dims[3] = { inner, mid, outer };
+    const cuuint64_t strides[2] = { mid_stride, outer_stride };
+    const cuuint32_t box[3] = { box_inner, box_mid, box_outer };
+    const cuuint32_t estr[3] = { 1, 1, 1 };
+    memset(m, 0, sizeof *m);
+    const CUresult r = enc(m, dt, 3, (void *)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        e2c_set_msg("tensor map: encode failed (%d) for %llu x %llu x %llu, box %u x %u x %u", (int)r,
+                    (unsigned long long)inner, (unsigned long long)mid, (unsigned long long)outer, box_inner, box_mid,
+                    box_outer);
+        return -1;
+    }
+    return 0;
+}
+
 int e2c_tmap_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
                 uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer) {
     return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 128);
