@@ -45,36 +45,59 @@ namespace {
 constexpr int TR = 128;  // rows of an item
 constexpr int TK = 128;  // keys of a tile
 constexpr int NTHREADS = 512;
+// Registers a thread: at launch, and after the split (warps 0..3, 4..11, 12..15)
+constexpr int LAUNCH_REGS = 128, LOAD_REGS = 112, SOFTMAX_REGS = 168, EPI_REGS = 64;
+static_assert(LOAD_REGS + 2 * SOFTMAX_REGS + EPI_REGS == 4 * LAUNCH_REGS, "the split is what the block was launched with");
 constexpr int NI = 8;  // item descriptors in flight
 constexpr float kRescaleLog2 = 8.0f;
+
+// A wait of a whole warp, bounded by its number of (sleeping) tries: up to 1.3 s. It is small on
+// purpose: with ptx.cuh's mbar_wait inlined at every wait the kernel was 234 KB of code, whose
+// instruction fetches took most of a tile's time (128-wide heads, 4096 tokens: 905 us a call).
+constexpr uint32_t kTryNs = 10000, kTries = 1u << 17;
+E2C_DEV bool wait_warp(uint32_t bar, uint32_t parity, int *status, int code) {
+    bool ok = false;
+#pragma unroll 1
+    for (uint32_t i = 0; i < kTries && !ok; i++) ok = mbar_try_wait_sleep(bar, parity, kTryNs);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) record_status(status, code);
+    return ok;
+}
+
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 
 template <int D>
 struct Cfg {
-    static constexpr int NQ = D == 256 ? 1 : 2;                 // Q buffers
-    static constexpr int NO = D == 256 ? 1 : 2;                 // O buffers in tensor memory
-    static constexpr int PANELS = D / 64;                       // 64 of the head's dimensions each
-    // a stage: one panel of a K tile (128 keys x 64), or VROWS keys of a V tile (VROWS x D)
-    static constexpr int STAGE = 16384;
-    static constexpr int NST = D == 64 ? 10 : 9;
-    static constexpr int VROWS = STAGE / (2 * D);
-    static constexpr bool CROSS = NQ == 2;  // an item's first QK is issued before the last PV of the one before
+    static constexpr int PANELS = D / 64;  // 64 of the head's dimensions each, 128 bytes a row
+    static constexpr int NQ = D == 256 ? 1 : 2;  // Q buffers
+    // K and V have a ring of NST stages each: of a tile, or for D = 256 of half a one (K: half of the
+    // head's dimensions, V: half of the keys)
+    static constexpr int KPARTS = D == 256 ? 2 : 1, VROWS = TK / KPARTS;
+    static constexpr int STAGE = TK * D * 2 / KPARTS;
+    static constexpr int NST = D == 64 ? 5 : 2;
+    // tensor memory: NS buffers of S (128 columns each), then NO of O (D columns each), 512 columns
+    static constexpr int NS = D == 256 ? 2 : 3;
+    static constexpr int NO = D == 64 ? 2 : 1;
+    static constexpr int O_COL = NS * 128;
+    // QK runs NS - 1 tiles ahead of PV; with two Q buffers across items too, with one an item's first
+    // QK follows the last PV of the item before
+    static constexpr bool CROSS = NQ == 2;
     static constexpr int Q_BYTES = TR * D * 2;
-    static constexpr int RING = NQ * Q_BYTES;
-    static constexpr int XM = RING + NST * STAGE;               // running maxima handed on [2][128]
+    static constexpr int K_OFF = NQ * Q_BYTES;
+    static constexpr int V_OFF = K_OFF + NST * STAGE;
+    static constexpr int XM = V_OFF + NST * STAGE;              // running maxima handed on [2][128]
     static constexpr int ML = XM + 2 * TR * 4;                  // item's (m, l) [2 items][2 groups][128] x 2
     static constexpr int ITEMS = ML + 2 * 2 * TR * 8;
     static constexpr int SCAN = ITEMS + NI * 64;
     static constexpr int BARS = SCAN + 256;
 };
-enum { SCAN_INTS = 64 };
 
 enum {
     B_QF,
     B_QE = B_QF + 2,
     B_SF = B_QE + 2,
-    B_PF = B_SF + 2,
-    B_PV = B_PF + 2,
+    B_PF = B_SF + 3,
+    B_PV = B_PF + 3,
     B_MX = B_PV + 2,  // [2][4 lane quadrants]
     B_OF = B_MX + 8,
     B_OE = B_OF + 2,
@@ -83,9 +106,11 @@ enum {
     B_ITF = B_MLE + 2,
     B_ITE = B_ITF + NI,
     B_DRAIN = B_ITE + NI,
-    B_STF,
-    B_STE = B_STF + 10,
-    B_NUM = B_STE + 10
+    B_KF,
+    B_KE = B_KF + 5,
+    B_VF = B_KE + 5,
+    B_VE = B_VF + 5,
+    B_NUM = B_VE + 5
 };
 template <int D>
 constexpr int smem_bytes() {
@@ -120,8 +145,8 @@ struct __align__(16) Item {
     int pos0;         // position of token t0
     int masked;       // prefix items: rows differ in what they see
     int prefix, dst;  // dst: TO_*
-    int slot;
-    int pad[3];
+    int slot, seq;    // seq: whose table maps the keys; -1: none (a page that is masked is read)
+    int pad[2];
 };
 static_assert(sizeof(Item) == 64, "descriptor");
 
@@ -177,13 +202,17 @@ E2C_DEV int span_of(const Args &p, int len, int nq, int r, int base, int &k0, in
     return (hi - k0 + TK - 1) / TK;
 }
 // tiles of all of an entry's row tiles, for one key head
-E2C_DEV int64_t tiles_of(const Args &p, const Entry &e, int base) {
-    if (e.nq <= 0) return 0;
-    const int nr = (e.nq + p.tpt - 1) / p.tpt;
+E2C_DEV int64_t tiles_of(const Args &p, int len, int nq, int base) {
+    if (nq <= 0) return 0;
+    const int nr = (nq + p.tpt - 1) / p.tpt;
+    const bool same = !p.causal && p.window < 0;  // every row tile sees every key
     int k0, klim;
-    if (!p.causal && p.window < 0) return (int64_t)nr * span_of(p, e.len, e.nq, 0, base, k0, klim);
     int64_t s = 0;
-    for (int r = 0; r < nr; r++) s += span_of(p, e.len, e.nq, r, base, k0, klim);
+#pragma unroll 1
+    for (int r = 0; r < nr; r++) {
+        s += span_of(p, len, nq, r, base, k0, klim);
+        if (same) return s * nr;
+    }
     return s;
 }
 
@@ -198,136 +227,151 @@ struct Plan {
     int64_t first_before;  // and the tiles before it
 };
 
-// every thread of the block; sums, mins and maxima over the entries
-E2C_DEV void make_plan(const Args &p, Plan &pl, int64_t *s64) {
+// Every thread of the block. Pass 0 sums over the entries and finds the longest; pass 1 finds the entry in
+// which this block's share begins (and leaves the joining kernel the tiles before each entry).
+struct PlanScratch {
+    int64_t sum[16], at;  // by warp; tiles before the block's first entry
+    int longest, least, masked, first, seq;
+};
+E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    int *s32 = reinterpret_cast<int *>(s64 + 18);
-    int64_t mine = 0, total = 0;
-    int best = -1, best_seq = 0, least = 0x7fffffff, flag = 0;
-    Entry e = {};
-    for (int base = 0; base < p.n; base += NTHREADS) {
-        const int i = base + tid;
-        if (i < p.n) {
-            e = entry_of(p, i, blockIdx.x == 0);
-            const int64_t t = tiles_of(p, e, p.shared) * p.pc.KV;
-            mine = base == 0 ? t : mine;
-            total += t;
-            if (e.nq > 0) {
-                if (e.len > best) {
-                    best = e.len;
-                    best_seq = e.seq;
-                }
-                least = min(least, e.len - e.nq);
-                flag |= e.len < p.shared || (p.causal && e.len - e.nq < p.shared - 1);
-            }
-        }
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        total += __shfl_xor_sync(0xffffffffu, total, d);
-        least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
-        flag |= __shfl_xor_sync(0xffffffffu, flag, d);
-        const int b = __shfl_xor_sync(0xffffffffu, best, d), bs = __shfl_xor_sync(0xffffffffu, best_seq, d);
-        if (b > best || (b == best && bs < best_seq)) {
-            best = b;
-            best_seq = bs;
-        }
-    }
-    // 16 warps: totals in s64[0..15]; the rest in 4 rows of s32
-    if (lane == 0) {
-        s64[w] = total;
-        s32[w] = best;
+    if (tid == 0) {
+        s.longest = -1;
+        s.least = 0x7fffffff;
+        s.masked = 0;
+        s.first = -1;
+        s.seq = 0x7fffffff;
     }
     __syncthreads();
-    int64_t Ws = 0;
-    for (int i = 0; i < 16; i++) {
-        Ws += s64[i];
-        best = max(best, s32[i]);
-    }
-    __syncthreads();
-    // the longest sequence's id, the least first position and the flag, one round each (the scratch is small)
-    if (lane == 0) {
-        s32[w] = least;
-    }
-    __syncthreads();
-    for (int i = 0; i < 16; i++) least = min(least, s32[i]);
-    __syncthreads();
-    if (lane == 0) s32[w] = flag;
-    __syncthreads();
-    for (int i = 0; i < 16; i++) flag |= s32[i];
-    pl.pmax = min(p.shared, max(best, 0));
-    pl.masked = flag || p.window >= 0;
     pl.npt = (p.T + p.tpt - 1) / p.tpt;
     pl.plo = 0;
-    pl.ptiles = 0;
-    pl.pseq = -1;
-    if (p.shared > 0 && best > 0) {
-        if (p.window >= 0) pl.plo = max(0, least - p.window) / TK * TK;
-        pl.ptiles = pl.plo < pl.pmax ? (pl.pmax - pl.plo + TK - 1) / TK : 0;
-    }
-    pl.Wp = (int64_t)pl.ptiles * pl.npt * p.pc.KV;
-    pl.W = pl.Wp + Ws;
-    // second pass: the longest sequence, the entry that this block's share begins in, and the tiles before
-    // each entry for the joining kernel
-    const int64_t blocks = min((int64_t)gridDim.x, pl.W);
-    const int64_t at = (int64_t)blockIdx.x < blocks ? max((int64_t)0, begin_of(blockIdx.x, pl.W, blocks) - pl.Wp) : -1;
-    int64_t run = 0;
-    __syncthreads();
-    if (tid == 0) {
-        s32[0] = -1;
-        s32[1] = 0x7fffffff;
-    }
-    for (int base = 0; base < p.n; base += NTHREADS) {
-        const int i = base + tid;
-        int64_t t = 0;
-        if (i < p.n) {
-            if (p.n > NTHREADS) {
-                e = entry_of(p, i, false);
-                mine = tiles_of(p, e, p.shared) * p.pc.KV;
+    Entry e = {};
+    int64_t mine = 0, at = -1;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+        int64_t run = 0;
+#pragma unroll 1
+        for (int base = 0; base < p.n; base += NTHREADS) {
+            const int i = base + tid;
+            if (pass == 0 || p.n > NTHREADS) {
+                e = {};
+                mine = 0;
+                if (i < p.n) {
+                    e = entry_of(p, i, pass == 0 && blockIdx.x == 0);
+                    mine = tiles_of(p, e.len, e.nq, p.shared) * p.pc.KV;
+                }
             }
-            t = mine;
-        }
-        int64_t x = t;
+            int64_t x = mine;
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
-            if (lane >= d) x += y;
-        }
-        __syncthreads();
-        if (lane == 31) s64[w] = x;
-        __syncthreads();
-        int64_t pre = run, all = 0;
-        for (int k = 0; k < 16; k++) {
-            if (k < w) pre += s64[k];
-            all += s64[k];
-        }
-        pre += x - t;
-        run += all;
-        if (i < p.n) {
-            if (t > 0 && at >= pre && at < pre + t) {
-                s32[0] = i;
-                s64[16] = pre;
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+                if (lane >= d) x += y;
             }
-            if (e.nq > 0 && e.len == best) atomicMin(&s32[1], e.seq);
-            if (blockIdx.x == 0 && p.shared > 0) p.before[i] = pre;
+            __syncthreads();  // the sums of the step before have been read
+            if (lane == 31) s.sum[w] = x;
+            if (pass == 0) {
+                if (p.shared > 0) {
+                    const int longest = __reduce_max_sync(0xffffffffu, e.nq > 0 ? e.len : -1);
+                    const int least = __reduce_min_sync(0xffffffffu, e.nq > 0 ? e.len - e.nq : 0x7fffffff);
+                    const bool masked = __any_sync(0xffffffffu, e.nq > 0 && (e.len < p.shared || (p.causal && e.len - e.nq < p.shared - 1)));
+                    if (lane == 0) {
+                        atomicMax(&s.longest, longest);
+                        atomicMin(&s.least, least);
+                        if (masked) s.masked = 1;
+                    }
+                }
+            } else if (e.nq > 0 && e.len == s.longest) {
+                atomicMin(&s.seq, e.seq);
+            }
+            __syncthreads();
+            int64_t before = run + x - mine;
+#pragma unroll 4
+            for (int k = 0; k < 16; k++) {
+                if (k < w) before += s.sum[k];
+                run += s.sum[k];
+            }
+            if (pass == 1 && i < p.n) {
+                if (at >= before && at < before + mine) {
+                    s.first = i;
+                    s.at = before;
+                }
+                if (blockIdx.x == 0 && p.shared > 0) p.before[i] = before;
+            }
+        }
+        if (pass == 0) {
+            const int longest = s.longest;
+            pl.pmax = min(p.shared, max(longest, 0));
+            pl.masked = s.masked || p.window >= 0;
+            if (p.window >= 0) pl.plo = max(0, s.least - p.window) / TK * TK;
+            pl.ptiles = pl.plo < pl.pmax ? (pl.pmax - pl.plo + TK - 1) / TK : 0;
+            pl.Wp = (int64_t)pl.ptiles * pl.npt * p.pc.KV;
+            pl.W = pl.Wp + run;
+            const int64_t blocks = min((int64_t)gridDim.x, pl.W);
+            if ((int64_t)blockIdx.x < blocks) at = max((int64_t)0, begin_of(blockIdx.x, pl.W, blocks) - pl.Wp);
         }
     }
     __syncthreads();
-    pl.first = s32[0];
-    pl.first_before = s64[16];
-    if (pl.ptiles) pl.pseq = s32[1];
+    pl.first = s.first;
+    pl.first_before = s.at;
+    pl.pseq = s.seq;
     if (blockIdx.x == 0 && tid == 0) {
         p.before[p.n] = pl.Wp;
         p.before[p.n + 1] = pl.W;
         p.before[p.n + 2] = pl.ptiles;
     }
-    __syncthreads();
 }
 
 E2C_DEV float ex2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+E2C_DEV float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// two fp32 operations in one instruction
+E2C_DEV float2 fma2(float2 a, float2 b, float2 c) {
+    float2 y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<uint64_t &>(y))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)), "l"(reinterpret_cast<uint64_t &>(c)));
+    return y;
+}
+E2C_DEV float2 add2(float2 a, float2 b) {
+    float2 y;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(y))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return y;
+}
+// f(0), f(1), .. with the index a constant expression
+template <int V>
+struct Const {
+    E2C_DEV constexpr operator int() const { return V; }
+};
+template <int N, int I = 0, typename F>
+E2C_DEV void static_for(F &&f) {
+    if constexpr (I < N) {
+        f(Const<I>());
+        static_for<N, I + 1>(f);
+    }
+}
+// 32 columns of tensor memory into r[B] .. r[B + 31]
+template <int B, int N>
+E2C_DEV void tmem_ld32_to(uint32_t taddr, uint32_t (&r)[N]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[B + 0]), "=r"(r[B + 1]), "=r"(r[B + 2]), "=r"(r[B + 3]), "=r"(r[B + 4]), "=r"(r[B + 5]), "=r"(r[B + 6]),
+          "=r"(r[B + 7]), "=r"(r[B + 8]), "=r"(r[B + 9]), "=r"(r[B + 10]), "=r"(r[B + 11]), "=r"(r[B + 12]), "=r"(r[B + 13]),
+          "=r"(r[B + 14]), "=r"(r[B + 15]), "=r"(r[B + 16]), "=r"(r[B + 17]), "=r"(r[B + 18]), "=r"(r[B + 19]), "=r"(r[B + 20]),
+          "=r"(r[B + 21]), "=r"(r[B + 22]), "=r"(r[B + 23]), "=r"(r[B + 24]), "=r"(r[B + 25]), "=r"(r[B + 26]), "=r"(r[B + 27]),
+          "=r"(r[B + 28]), "=r"(r[B + 29]), "=r"(r[B + 30]), "=r"(r[B + 31])
+        : "r"(taddr));
 }
 
 template <typename T>
@@ -347,19 +391,11 @@ __host__ __device__ constexpr uint32_t type_bits() {  // A and B formats of the 
     return sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? (1u << 7) | (1u << 10) : 0u;
 }
 
-// one producer step: a tile's place in its item and where its pages lie
-struct Tile {
-    int item;       // running item number; -1: no more tiles
-    int kvh, kk, nk, row;
-    int t0, prefix;
-    bool first;
-};
-
 template <typename T, int D>
 __global__ void __launch_bounds__(NTHREADS, 1)
     k_attention_pages(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQp,
-                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const Args p,
-                      const int q_box, const int qp_box) {
+                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const __grid_constant__ Args p, const int q_box, const int qp_box) {
     using C = Cfg<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     griddep_launch_dependents();
@@ -378,22 +414,26 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         for (int i = 0; i < 2; i++) {
             mbar_init(bar(B_QF + i), 1);
             mbar_init(bar(B_QE + i), 1);
-            mbar_init(bar(B_SF + i), 1);
-            mbar_init(bar(B_PF + i), 4);
             mbar_init(bar(B_PV + i), 1);
             mbar_init(bar(B_OF + i), 1);
             mbar_init(bar(B_OE + i), 4);
             mbar_init(bar(B_MLF + i), 8);
             mbar_init(bar(B_MLE + i), 4);
         }
+        for (int i = 0; i < 3; i++) {
+            mbar_init(bar(B_SF + i), 1);
+            mbar_init(bar(B_PF + i), 4);
+        }
         for (int i = 0; i < 8; i++) mbar_init(bar(B_MX + i), 1);
         for (int i = 0; i < NI; i++) {
             mbar_init(bar(B_ITF + i), 1);
-            mbar_init(bar(B_ITE + i), 13);  // MMA, 8 softmax and 4 epilogue warps
+            mbar_init(bar(B_ITE + i), 16);  // K, V, QK, PV, 8 softmax and 4 epilogue warps
         }
         for (int i = 0; i < C::NST; i++) {
-            mbar_init(bar(B_STF + i), 1);
-            mbar_init(bar(B_STE + i), 1);
+            mbar_init(bar(B_KF + i), 1);
+            mbar_init(bar(B_KE + i), 1);
+            mbar_init(bar(B_VF + i), 1);
+            mbar_init(bar(B_VE + i), 1);
         }
         mbar_init(bar(B_DRAIN), 1);
         fence_mbar_init();
@@ -409,100 +449,62 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     __syncthreads();
     tc_fence_after();
     griddep_wait();
-    const uint32_t tmem = *tmem_slot;  // S buffer i: columns 128 i .. +127; O buffer i: 256 + D i ..
+    const uint32_t tmem = *tmem_slot;
 
     Plan pl;
-    make_plan(p, pl, reinterpret_cast<int64_t *>(smem + C::SCAN));
-    const int64_t blocks = min((int64_t)gridDim.x, pl.W);
-    const int64_t L0 = (int64_t)blockIdx.x < blocks ? begin_of(blockIdx.x, pl.W, blocks) : 0;
-    const int64_t L1 = (int64_t)blockIdx.x < blocks ? begin_of(blockIdx.x + 1, pl.W, blocks) : 0;
+    make_plan(p, pl, *reinterpret_cast<PlanScratch *>(smem + C::SCAN));
 
-    // a consumer's copy of the next item; false after the last (or a failure). The slot is released at once.
-    auto take = [&](int &n, Item &it) -> bool {
+    // A consumer's copy of item n; false after the last one (or a failure). The slot is released at once.
+    auto take = [&](int n, Item &it) -> bool {
         const int s = n & (NI - 1);
-        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_ITF + s), (uint32_t)((n / NI) & 1), p.status, E2C_ERR_WAIT_ATTN))) return false;
+        if (!wait_warp(bar(B_ITF + s), (uint32_t)((n / NI) & 1), p.status, E2C_ERR_WAIT_ATTN)) return false;
         const int4 *d = reinterpret_cast<const int4 *>(items + s);
         int4 *o = reinterpret_cast<int4 *>(&it);
 #pragma unroll
         for (int k = 0; k < 4; k++) o[k] = d[k];
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_ITE + s));
-        n++;
         return it.ntok >= 0;
     };
 
-    if (warp == 0) {
-        // ---------------------------------------------------------------- items, Q, K and V loads
-        bool ok = true;
-        int ni = 0;                // items published
-        int64_t pos = L0;
-        // sequence entries, 32 at a time, one per lane
-        int ebase = -1;
-        Entry e = {};
-        int64_t etiles = 0;
-        int ei = pl.first, kvh = 0, r = 0;
-        bool placed = false;  // kvh, r and left are valid for entry ei
-        // the part being walked
-        Item it = {};
-        int seq = -1, j = 0;
-        it.nt = 0;
-        const int PB = min(p.pc.page, C::VROWS), NB = TK / PB;
-        const int row_blk = lane < NB ? lane : 0;
-
-        auto entry = [&](int i) {
-            if (ebase < 0 || i >= ebase + 32) {
-                ebase = i;
-                const int k = i + lane;
-                e = {};
-                etiles = 0;
-                if (k < p.n) {
-                    e = entry_of(p, k, false);
-                    etiles = tiles_of(p, e, p.shared);
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(LOAD_REGS));
+        if (warp == 0) {
+            // ------------------------------------------------------------ items and Q loads
+            const int64_t blocks = min((int64_t)gridDim.x, pl.W);
+            const bool at_work = (int64_t)blockIdx.x < blocks;
+            const int64_t L0 = at_work ? begin_of(blockIdx.x, pl.W, blocks) : 0;
+            const int64_t L1 = at_work ? begin_of(blockIdx.x + 1, pl.W, blocks) : 0;
+            // where a part of the item of tiles [s, end) goes: `whole` where it lies in this block
+            auto destination = [&](Item &it, int64_t s, int64_t end, int whole) {
+                it.dst = whole;
+                it.slot = 0;
+                if (s >= L0 && end <= L1) return;
+                it.dst = TO_SLOT;
+                it.slot = 2 * blockIdx.x + (s > L0 ? 1 : 0);
+                // an item's second block reports it to the joining kernel
+                if (p.shared == 0 && s < L0 && block_of(s, pl.W, blocks) == (int)blockIdx.x - 1 && lane == 0) {
+                    const int c0 = blockIdx.x - 1, c1 = block_of(end - 1, pl.W, blocks);
+                    p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, it.kvh, 2 * c0 + (s > begin_of(c0, pl.W, blocks) ? 1 : 0));
+                    p.split[2 * blockIdx.x + 1] = make_int4(c1, 0, 0, 0);
                 }
-            }
-        };
-        auto publish = [&]() -> bool {
-            const int s = ni & (NI - 1);
-            if (!__all_sync(0xffffffffu,
-                            mbar_wait(bar(B_ITE + s), (uint32_t)(((ni / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)))
-                return false;
-            if (lane == 0) {
-                const int4 *d = reinterpret_cast<const int4 *>(&it);
-                int4 *o = reinterpret_cast<int4 *>(items + s);
-#pragma unroll
-                for (int k = 0; k < 4; k++) o[k] = d[k];
-                mbar_arrive(bar(B_ITF + s));
-            }
+            };
+            if (p.shared == 0 && lane == 0 && at_work) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
             __syncwarp();
-            ni++;
-            return true;
-        };
-        // where a part goes: [s, s + nt) are the item's tiles, `undivided` where it goes whole
-        auto destination = [&](int64_t s, int64_t end, int undivided) {
-            if (s >= L0 && end <= L1) {
-                it.dst = undivided;
-                return;
-            }
-            it.dst = TO_SLOT;
-            it.slot = 2 * blockIdx.x + (s > L0 ? 1 : 0);
-            // an item's second block reports it to the joining kernel
-            if (p.shared == 0 && s < L0 && block_of(s, pl.W, blocks) == (int)blockIdx.x - 1 && lane == 0) {
-                const int c0 = blockIdx.x - 1, c1 = block_of(end - 1, pl.W, blocks);
-                p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, it.kvh, 2 * c0 + (s > begin_of(c0, pl.W, blocks) ? 1 : 0));
-                p.split[2 * blockIdx.x + 1] = make_int4(c1, 0, 0, 0);
-            }
-        };
-        if (p.shared == 0 && lane == 0 && pos < L1) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-        __syncwarp();
-
-        // the next tile, its pages asked for; publishes an item at its first tile
-        auto advance = [&](Tile &t) -> bool {
-            if (j == it.nt) {
-                if (pos >= L1) {
-                    t.item = -1;
-                    return true;
-                }
-                if (pos < pl.Wp) {
+            // sequence entries, 32 at a time, one per lane
+            int ebase = -1, ei = pl.first, kvh = 0, r = 0;
+            bool placed = false;  // kvh and r are valid for entry ei
+            Entry e = {};
+            int64_t etiles = 0, pos = L0;
+            Item it = {};
+            int n = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (bool more = true; more && ok; n++) {
+                more = pos < L1;
+                if (!more) {
+                    it.ntok = -1;
+                } else if (pos < pl.Wp) {
                     const int64_t q = pos / pl.ptiles;
                     const int j0 = (int)(pos - q * pl.ptiles);
                     it.prefix = 1;
@@ -513,49 +515,50 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     it.k0 = pl.plo + j0 * TK;
                     it.klim = pl.pmax;
                     it.masked = pl.masked;
-                    it.slot = 0;
-                    seq = pl.pseq;
-                    destination(q * pl.ptiles, (q + 1) * pl.ptiles, TO_DENSE);
+                    it.seq = pl.pseq;
+                    destination(it, q * pl.ptiles, (q + 1) * pl.ptiles, TO_DENSE);
                 } else {
-                    int nq, len, q0;
+                    int nq;
                     int64_t skip = 0;  // tiles of the item before this block's share
-                    if (!placed) {
-                        entry(ei);
-                        const int64_t c = __shfl_sync(0xffffffffu, etiles, ei - ebase);
-                        int64_t off = pos - pl.Wp - pl.first_before;
-                        kvh = (int)(off / c);
-                        skip = off - kvh * c;
-                        r = 0;
-                    } else if (r * p.tpt >= __shfl_sync(0xffffffffu, e.nq, ei - ebase)) {
-                        r = 0;
-                        if (++kvh == p.pc.KV) {
-                            kvh = 0;
-                            do {
-                                ei++;
-                                if (ei >= p.n) break;  // cannot happen: pos < L1 <= W
-                                entry(ei);
-                            } while (__shfl_sync(0xffffffffu, e.nq, ei - ebase) == 0);
-                            if (ei >= p.n) {
-                                t.item = -1;
-                                return true;
+                    for (;;) {  // to the next row tile: of this key head, of the next, of the next entry
+                        if (ebase < 0 || ei >= ebase + 32) {
+                            ebase = ei;
+                            e = {};
+                            etiles = 0;
+                            if (ei + lane < p.n) {
+                                e = entry_of(p, ei + lane, false);
+                                etiles = tiles_of(p, e.len, e.nq, p.shared);
                             }
                         }
+                        nq = __shfl_sync(0xffffffffu, e.nq, ei - ebase);
+                        if (!placed) {
+                            const int64_t c = __shfl_sync(0xffffffffu, etiles, ei - ebase), off = pos - pl.Wp - pl.first_before;
+                            kvh = (int)(off / c);
+                            skip = off - kvh * c;
+                            placed = true;
+                        }
+                        if (r * p.tpt < nq) break;
+                        r = 0;
+                        if (nq > 0 && ++kvh < p.pc.KV) break;
+                        kvh = 0;
+                        if (++ei >= p.n) break;  // cannot happen: pos < L1 <= W
+                    }
+                    if (ei >= p.n) {
+                        ok = false;
+                        break;
                     }
                     const int src = ei - ebase;
-                    seq = __shfl_sync(0xffffffffu, e.seq, src);
-                    len = __shfl_sync(0xffffffffu, e.len, src);
-                    q0 = __shfl_sync(0xffffffffu, e.q0, src);
-                    nq = __shfl_sync(0xffffffffu, e.nq, src);
-                    int k0, klim, nt = span_of(p, len, nq, r, p.shared, k0, klim);
-                    if (!placed) {
-                        while (skip >= nt) {
-                            skip -= nt;
-                            nt = span_of(p, len, nq, ++r, p.shared, k0, klim);
-                        }
-                        placed = true;
+                    const int len = __shfl_sync(0xffffffffu, e.len, src), q0 = __shfl_sync(0xffffffffu, e.q0, src);
+                    int k0, klim, nt;
+#pragma unroll 1
+                    for (;; r++) {
+                        nt = span_of(p, len, nq, r, p.shared, k0, klim);
+                        if (skip < nt) break;
+                        skip -= nt;
                     }
-                    if (len == 0) seq = -1;  // its table says nothing
                     const int64_t s = pos - skip;
+                    it.seq = __shfl_sync(0xffffffffu, e.seq, src);
+                    if (len == 0) it.seq = -1;  // its table says nothing
                     it.prefix = 0;
                     it.kvh = kvh;
                     it.t0 = q0 + r * p.tpt;
@@ -567,248 +570,257 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     it.len = len;
                     it.pos0 = len - nq + r * p.tpt;
                     it.masked = 1;
-                    it.slot = 0;
-                    destination(s, s + nt, p.shared > 0 ? TO_DENSE : TO_OUT);
+                    destination(it, s, s + nt, p.shared > 0 ? TO_DENSE : TO_OUT);
                     r++;
                 }
-                if (!publish()) return false;
-                pos += it.nt;
-                j = 0;
-            }
-            t.item = ni - 1;
-            t.kvh = it.kvh;
-            t.kk = it.k0 + j * TK;
-            t.nk = min(TK, it.klim - t.kk);
-            t.t0 = it.t0;
-            t.prefix = it.prefix;
-            t.first = j == 0;
-            const int key = t.kk + row_blk * PB;
-            int page = 0;
-            if (seq >= 0 && key < it.klim) page = p.pc.table[(int64_t)seq * p.pc.max_blocks + key / p.pc.page];
-            t.row = ((unsigned)page < (unsigned)p.pc.n_pages ? page : 0) * p.pc.page + (key & (p.pc.page - 1));
-            j++;
-            return true;
-        };
-        int st = 0;  // stages filled
-        auto stage = [&](uint32_t bytes, uint32_t &dst, uint32_t &b) -> bool {
-            const int s = st % C::NST;
-            if (!__all_sync(0xffffffffu,
-                            mbar_wait(bar(B_STE + s), (uint32_t)(((st / C::NST) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)))
-                return false;
-            dst = sbase + C::RING + s * C::STAGE;
-            b = bar(B_STF + s);
-            if (lane == 0) mbar_arrive_expect_tx(b, bytes);
-            __syncwarp();
-            st++;
-            return true;
-        };
-        int nq_loads = 0;
-        auto push_k = [&](const Tile &t) -> bool {
-            if (t.first) {
-                const int qb = t.item % C::NQ;
-                if (!__all_sync(0xffffffffu, mbar_wait(bar(B_QE + qb), (uint32_t)(((t.item / C::NQ) & 1) ^ 1), p.status,
-                                                       E2C_ERR_WAIT_PRODUCER)))
-                    return false;
+                const int sl = n & (NI - 1);
+                if (!(ok = wait_warp(bar(B_ITE + sl), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) break;
                 if (lane == 0) {
-                    const int box = t.prefix ? qp_box : q_box;
+                    const int4 *d = reinterpret_cast<const int4 *>(&it);
+                    int4 *o = reinterpret_cast<int4 *>(items + sl);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) o[k] = d[k];
+                    mbar_arrive(bar(B_ITF + sl));
+                }
+                __syncwarp();
+                if (!more) break;
+                pos += it.nt;
+                const int qb = n % C::NQ;
+                if (!(ok = wait_warp(bar(B_QE + qb), (uint32_t)(((n / C::NQ) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) break;
+                if (elect_one()) {
+                    const int box = it.prefix ? qp_box : q_box;
                     mbar_arrive_expect_tx(bar(B_QF + qb), (uint32_t)(C::PANELS * box * p.G * 128));
                     for (int i = 0; i < C::PANELS; i++)
-                        tma_load_3d(sbase + qb * C::Q_BYTES + i * (TR * 128), t.prefix ? &tmQp : &tmQ, 64 * i, t.kvh * p.G, t.t0,
+                        tma_load_3d(sbase + qb * C::Q_BYTES + i * (TR * 128), it.prefix ? &tmQp : &tmQ, 64 * i, it.kvh * p.G, it.t0,
                                     bar(B_QF + qb));
                 }
                 __syncwarp();
-                nq_loads = t.item + 1;
             }
-            const int nb = (t.nk + PB - 1) / PB;
-            for (int h = 0; h < C::PANELS; h++) {
-                uint32_t dst, b;
-                if (!stage((uint32_t)(nb * PB * 128), dst, b)) return false;
-                if (lane < nb) tma_load_2d(dst + lane * (PB * 128), &tmK, t.kvh * D + 64 * h, t.row, b);
-                __syncwarp();
-            }
-            return true;
-        };
-        auto push_v = [&](const Tile &t) -> bool {
-            const int nb = (t.nk + PB - 1) / PB;
-            constexpr int per = C::VROWS;
-            for (int h = 0; h * per < t.nk; h++) {
-                const int b0 = h * per / PB, bn = min(nb, (h + 1) * per / PB);
-                uint32_t dst, b;
-                if (!stage((uint32_t)((bn - b0) * PB * 128 * C::PANELS), dst, b)) return false;
-                if (lane >= b0 && lane < bn)
-                    for (int i = 0; i < C::PANELS; i++)
-                        tma_load_2d(dst + i * (per * 128) + (lane - b0) * (PB * 128), &tmV, t.kvh * D + 64 * i, t.row, b);
-                __syncwarp();
-            }
-            return true;
-        };
-
-        Tile cur, nxt, nn;
-        ok = advance(cur);
-        if (ok && cur.item >= 0) {
-            ok = advance(nxt) && push_k(cur);
-            while (ok) {
-                if (nxt.item >= 0)
-                    ok = advance(nn);
-                else
-                    nn.item = -1;
-                if (!ok) break;
-                if (nxt.item >= 0 && (C::CROSS || !nxt.first)) ok = push_k(nxt);
-                ok = ok && push_v(cur);
-                if (ok && nxt.item >= 0 && !(C::CROSS || !nxt.first)) ok = push_k(nxt);
-                if (nxt.item < 0) break;
-                cur = nxt;
-                nxt = nn;
-            }
-        }
-        if (ok) {
-            it.ntok = -1;
-            publish();
-        }
-        // every load that was issued has landed before the block may end
-        for (int i = nq_loads - C::NQ < 0 ? 0 : nq_loads - C::NQ; i < nq_loads; i++)
-            mbar_wait(bar(B_QF + i % C::NQ), (uint32_t)((i / C::NQ) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
-        for (int i = st - C::NST < 0 ? 0 : st - C::NST; i < st; i++)
-            mbar_wait(bar(B_STF + i % C::NST), (uint32_t)((i / C::NST) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
-    } else if (warp == 1) {
-        // ---------------------------------------------------------------- MMA issue
-        // QK of the next tile, then PV of this one (across items too, with two Q buffers)
-        const uint32_t idesc = (1u << 4) | type_bits<T>() | ((uint32_t)(128 >> 4) << 24);
-        bool ok = true;
-        int n = 0, st = 0;
-        Item it = {};
-        int left = 0, item = -1, kk = 0;  // of the tile that `step` gave last
-        struct Step {
-            int item, nk, g;
-            bool first, last;
-        };
-        int g = 0;
-        auto step = [&](Step &s) -> bool {
-            if (left == 0) {
-                if (!take(n, it)) {
-                    s.item = -1;
-                    return it.ntok < 0;
-                }
-                left = it.nt;
-                item++;
-                kk = it.k0;
-                s.first = true;
-            } else {
-                s.first = false;
-            }
-            s.item = item;
-            s.nk = min(TK, it.klim - kk);
-            s.g = g++;
-            kk += TK;
-            left--;
-            s.last = left == 0;
-            return true;
-        };
-        auto full = [&](int s) {
-            return __all_sync(0xffffffffu, mbar_wait(bar(B_STF + s % C::NST), (uint32_t)((s / C::NST) & 1), p.status, E2C_ERR_WAIT_MMA));
-        };
-        auto qk = [&](const Step &s) -> bool {
-            const int qb = s.item % C::NQ;
-            if (s.first && !__all_sync(0xffffffffu, mbar_wait(bar(B_QF + qb), (uint32_t)((s.item / C::NQ) & 1), p.status,
-                                                              E2C_ERR_WAIT_MMA)))
-                return false;
-            const uint32_t id = idesc | (p.neg << 13) | (uint32_t)(((s.nk + 15) >> 4) << 1) << 17;
-            const uint32_t d = tmem + (uint32_t)((s.g & 1) * 128);
-            for (int h = 0; h < C::PANELS; h++, st++) {
-                if (!full(st)) return false;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t kb = sbase + C::RING + (st % C::NST) * C::STAGE;
-                    const uint32_t qa = sbase + qb * C::Q_BYTES + h * (TR * 128);
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        mma_bf16(d, smem_desc_sw128(qa + k * 32), smem_desc_sw128(kb + k * 32), id, h != 0 || k != 0);
-                    mma_commit(bar(B_STE + st % C::NST));
-                }
-                __syncwarp();
-            }
-            if (lane == 0) {
-                mma_commit(bar(B_SF + (s.g & 1)));
-                if (s.last) mma_commit(bar(B_QE + qb));
-            }
-            __syncwarp();
-            return true;
-        };
-        auto pv = [&](const Step &s) -> bool {
-            const int ob = s.item % C::NO;
-            const uint32_t id = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // B: N contiguous
-            const uint32_t d = tmem + 256u + (uint32_t)(ob * D), a = tmem + (uint32_t)((s.g & 1) * 128);
-            const int nk16 = (s.nk + 15) & ~15;
-            bool waited = false;
-            for (int h = 0; h * C::VROWS < s.nk; h++, st++) {
-                if (!full(st)) return false;
-                const uint32_t vb = sbase + C::RING + (st % C::NST) * C::STAGE;
-                const int r0 = h * C::VROWS, here = min(C::VROWS, nk16 - r0);
-                if (s.nk < r0 + here) {
-                    // rows nk .. nk16 - 1 of every panel, 16 bytes a lane
-                    const int rows = r0 + here - s.nk;
-                    uint8_t *v = smem + C::RING + (st % C::NST) * C::STAGE + (s.nk - r0) * 128;
-                    for (int x = lane; x < C::PANELS * rows * 8; x += 32) {
-                        const int panel = x / (rows * 8), y = x - panel * (rows * 8);
-                        *reinterpret_cast<uint4 *>(v + panel * (C::VROWS * 128) + y * 16) = make_uint4(0, 0, 0, 0);
+            // every load that was issued has landed before the block may end
+            for (int i = n - C::NQ < 0 ? 0 : n - C::NQ; i < n; i++)
+                wait_warp(bar(B_QF + i % C::NQ), (uint32_t)((i / C::NQ) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
+        } else if (warp == 1) {
+            // ------------------------------------------------------------ MMA issue
+            // QK runs LOOK tiles ahead of PV; each has a cursor over the items
+            constexpr int LOOK = C::NS - 1;
+            const uint32_t idesc = (1u << 4) | type_bits<T>() | ((uint32_t)(128 >> 4) << 24);
+            Item iq = {}, iv = {};
+            int nq = 0, nv = 0, jq = 0, jv = 0;  // items taken; tile of the item
+            int ks = 0, vs = 0;                  // stages, and the parity of their round
+            uint32_t kp = 0, vp = 0;
+            int sq = 0, sv = 0;                  // S buffers
+            uint32_t pp = 0;                     // parity of P in S buffer sv
+            int gq = 0, gv = 0;
+            bool more = true, ok = true;         // more: QK has tiles left
+            auto qk = [&]() -> bool {
+                if (jq == iq.nt) {
+                    if (!take(nq, iq)) {
+                        more = false;
+                        return iq.ntok < 0;
                     }
-                    fence_proxy_async_smem();
+                    jq = 0;
+                    const int qb = nq % C::NQ;
+                    if (!wait_warp(bar(B_QF + qb), (uint32_t)((nq / C::NQ) & 1), p.status, E2C_ERR_WAIT_MMA)) return false;
+                    nq++;
+                }
+                const int qb = (nq - 1) % C::NQ, nk = min(TK, iq.klim - iq.k0 - jq * TK);
+                const uint32_t id = idesc | (p.neg << 13) | (uint32_t)(((nk + 15) >> 4) << 1) << 17;
+                const uint32_t d = tmem + (uint32_t)(sq * 128);
+                jq++;
+                uint64_t qd = smem_desc_sw128(sbase + qb * C::Q_BYTES);
+#pragma unroll
+                for (int h = 0; h < C::KPARTS; h++) {
+                    if (!wait_warp(bar(B_KF + ks), kp, p.status, E2C_ERR_WAIT_MMA)) return false;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        uint64_t kd = smem_desc_sw128(sbase + C::K_OFF + ks * C::STAGE);
+                        constexpr int PP = C::PANELS / C::KPARTS;
+#pragma unroll
+                        for (int k = 0; k < PP * 4; k++) {
+                            const int off = ((k >> 2) * (TR * 128) + (k & 3) * 32) >> 4;
+                            mma_bf16(d, qd + off, kd + off, id, h != 0 || k != 0);
+                        }
+                        mma_commit(bar(B_KE + ks));
+                        if (h == C::KPARTS - 1) {
+                            mma_commit(bar(B_SF + sq));
+                            if (jq == iq.nt) mma_commit(bar(B_QE + qb));
+                        }
+                    }
                     __syncwarp();
+                    qd += (C::PANELS / C::KPARTS * TR * 128) >> 4;
+                    if (++ks == C::NST) {
+                        ks = 0;
+                        kp ^= 1;
+                    }
                 }
-                if (!waited) {
-                    waited = true;
-                    if (!__all_sync(0xffffffffu, mbar_wait(bar(B_PF + (s.g & 1)), (uint32_t)((s.g >> 1) & 1), p.status,
-                                                           E2C_ERR_WAIT_MMA)))
-                        return false;
-                    if (s.first && !__all_sync(0xffffffffu, mbar_wait(bar(B_OE + ob), (uint32_t)(((s.item / C::NO) & 1) ^ 1),
-                                                                      p.status, E2C_ERR_WAIT_MMA)))
-                        return false;
+                if (++sq == C::NS) sq = 0;
+                gq++;
+                return true;
+            };
+            auto pv = [&]() -> bool {
+                if (jv == iv.nt) {
+                    if (!take(nv, iv)) return false;  // QK has taken it: it is there
+                    jv = 0;
+                    nv++;
                 }
-                tc_fence_after();
-                if (lane == 0) {
-                    for (int k = 0; k < here / 16; k++)
-                        mma_bf16_ts(d, a + (uint32_t)((r0 / 16 + k) * 8), smem_desc_sw128_mn(vb + k * 2048, C::VROWS * 128), id,
-                                    !s.first || h != 0 || k != 0);
-                    mma_commit(bar(B_STE + st % C::NST));
+                const int ob = (nv - 1) % C::NO, nk = min(TK, iv.klim - iv.k0 - jv * TK), nk16 = (nk + 15) & ~15;
+                const bool first = jv == 0;
+                const uint32_t id = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // B: N contiguous
+                const uint32_t d = tmem + (uint32_t)(C::O_COL + ob * D);
+                uint32_t a = tmem + (uint32_t)(sv * 128);
+                jv++;
+#pragma unroll 1
+                for (int r0 = 0; r0 < nk; r0 += C::VROWS) {
+                    if (!wait_warp(bar(B_VF + vs), vp, p.status, E2C_ERR_WAIT_MMA)) return false;
+                    const int here = min(C::VROWS, nk16 - r0), rows = r0 + here - nk;
+                    if (rows > 0) {  // rows nk .. nk16 - 1 of every panel are zeroed, 16 bytes a lane
+                        uint8_t *v = smem + C::V_OFF + vs * C::STAGE + (nk - r0) * 128;
+                        for (int x = lane; x < C::PANELS * rows * 8; x += 32) {
+                            const int panel = x / (rows * 8), y = x - panel * (rows * 8);
+                            *reinterpret_cast<uint4 *>(v + panel * (C::VROWS * 128) + y * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    if (r0 == 0) {
+                        if (!wait_warp(bar(B_PF + sv), pp, p.status, E2C_ERR_WAIT_MMA)) return false;
+                        if (first && !wait_warp(bar(B_OE + ob), (uint32_t)((((nv - 1) / C::NO) & 1) ^ 1), p.status, E2C_ERR_WAIT_MMA))
+                            return false;
+                    }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        uint64_t vd = smem_desc_sw128_mn(sbase + C::V_OFF + vs * C::STAGE, C::VROWS * 128);
+                        if (here == C::VROWS) {
+#pragma unroll
+                            for (int k = 0; k < C::VROWS / 16; k++)
+                                mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id, !first || r0 != 0 || k != 0);
+                        } else {
+#pragma unroll 1
+                            for (int k = 0; k < here / 16; k++) mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id, !first || r0 != 0 || k != 0);
+                        }
+                        mma_commit(bar(B_VE + vs));
+                        if (r0 + C::VROWS >= nk) {
+                            mma_commit(bar(B_PV + (gv & 1)));
+                            if (jv == iv.nt) mma_commit(bar(B_OF + ob));
+                        }
+                    }
+                    __syncwarp();
+                    a += C::VROWS / 2;
+                    if (++vs == C::NST) {
+                        vs = 0;
+                        vp ^= 1;
+                    }
                 }
-                __syncwarp();
+                if (++sv == C::NS) {
+                    sv = 0;
+                    pp ^= 1;
+                }
+                gv++;
+                return true;
+            };
+#pragma unroll 1
+            while (ok && (more || gv < gq)) {
+                const bool early = C::CROSS || jq != iq.nt;
+#pragma unroll 1
+                for (int half = 0; ok && half < 2; half++) {
+                    if ((half == 0) == early) {
+                        if (more) ok = qk();
+                    } else if (gv < gq && (gq - gv > LOOK || !more || !early)) {
+                        ok = pv();
+                    }
+                }
             }
-            if (lane == 0) {
-                mma_commit(bar(B_PV + (s.g & 1)));
-                if (s.last) mma_commit(bar(B_OF + ob));
-            }
+            // all products are done before the block frees tensor memory or ends
+            if (elect_one()) mma_commit(bar(B_DRAIN));
             __syncwarp();
-            return true;
-        };
-        Step cur, nxt;
-        ok = step(cur);
-        if (ok && cur.item >= 0) {
-            ok = qk(cur);
+            wait_warp(bar(B_DRAIN), 0, nullptr, E2C_ERR_WAIT_DRAIN);
+        } else {
+            // ------------------------------------------------------------ K loads (warp 2), V loads (warp 3)
+            const bool is_v = warp == 3;
+            const CUtensorMap *tm = is_v ? &tmV : &tmK;
+            const int F = is_v ? B_VF : B_KF, E = is_v ? B_VE : B_KE;
+            const uint32_t ring = sbase + (is_v ? C::V_OFF : C::K_OFF);
+            const int PB = min(p.pc.page, C::VROWS), shift = 31 - __clz(p.pc.page);
+            Item it = {};
+            int n = 0, j = 0, st = 0, total = 0;
+            uint32_t par = 1;
+            // the tile whose boxes are issued next, its rows asked for one tile before
+            int row = 0, kvh = 0, nk = 0;
+            bool ok = true, have = false, more = true;
+#pragma unroll 1
             while (ok) {
-                ok = step(nxt);
-                if (!ok) break;
-                if (nxt.item >= 0 && (C::CROSS || !nxt.first)) ok = qk(nxt);
-                ok = ok && pv(cur);
-                if (ok && nxt.item >= 0 && !(C::CROSS || !nxt.first)) ok = qk(nxt);
-                if (nxt.item < 0) break;
-                cur = nxt;
+                int row2 = 0, kvh2 = 0, nk2 = 0;
+                bool have2 = false;
+                if (more && j == it.nt) {
+                    more = take(n, it);
+                    ok = more || it.ntok < 0;
+                    n++;
+                    j = 0;
+                }
+                if (more) {
+                    const int kk = it.k0 + j * TK, key = kk + lane * PB;
+                    int page = 0;
+                    if (it.seq >= 0 && key < min(it.klim, kk + TK))
+                        page = p.pc.table[(int64_t)it.seq * p.pc.max_blocks + (key >> shift)];
+                    row2 = ((unsigned)page < (unsigned)p.pc.n_pages ? page << shift : 0) + (key & (p.pc.page - 1));
+                    nk2 = min(TK, it.klim - kk);
+                    kvh2 = it.kvh;
+                    have2 = true;
+                    j++;
+                }
+                if (have) {
+                    const int nb = (nk + PB - 1) / PB;
+                    // a K stage holds PANELS / KPARTS panels of every key, a V stage every panel of VROWS keys
+                    const int parts = is_v ? (nk + C::VROWS - 1) / C::VROWS : C::KPARTS;
+                    const int np = is_v ? C::PANELS : C::PANELS / C::KPARTS;
+                    const int pitch = (is_v ? C::VROWS : TK) * 128;
+#pragma unroll 1
+                    for (int h = 0; h < parts; h++) {
+                        const int b0 = is_v ? h * C::VROWS / PB : 0, b1 = is_v ? min(nb, (h + 1) * C::VROWS / PB) : nb;
+                        const int x = kvh * D + (is_v ? 0 : h * np * 64);
+                        if (!(ok = wait_warp(bar(E + st), par, p.status, E2C_ERR_WAIT_PRODUCER))) break;
+                        if (elect_one()) mbar_arrive_expect_tx(bar(F + st), (uint32_t)((b1 - b0) * PB * 128 * np));
+                        __syncwarp();
+                        uint32_t dst = ring + st * C::STAGE;
+#pragma unroll 1
+                        for (int b = b0; b < b1; b++, dst += PB * 128) {
+                            const int y = __shfl_sync(0xffffffffu, row, b);
+                            if (elect_one()) {
+#pragma unroll
+                                for (int i = 0; i < C::PANELS; i++)
+                                    if (i < np) tma_load_2d(dst + i * pitch, tm, x + 64 * i, y, bar(F + st));
+                            }
+                        }
+                        if (++st == C::NST) {
+                            st = 0;
+                            par ^= 1;
+                        }
+                        total++;
+                    }
+                } else if (!more) {
+                    break;
+                }
+                row = row2;
+                kvh = kvh2;
+                nk = nk2;
+                have = have2;
             }
+            for (int i = total - C::NST < 0 ? 0 : total - C::NST; i < total; i++)
+                wait_warp(bar(F + i % C::NST), (uint32_t)((i / C::NST) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
         }
-        // all products are done before the block frees tensor memory or ends
-        if (lane == 0) mma_commit(bar(B_DRAIN));
-        __syncwarp();
-        mbar_wait(bar(B_DRAIN), 0, nullptr, E2C_ERR_WAIT_DRAIN);
-    } else if (warp >= 4 && warp < 12) {
+    } else if (warp < 12) {
         // ---------------------------------------------------------------- softmax
+        // a row of 128 logits is held in registers, taken from the other warps' share
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFTMAX_REGS));
         const int quad = warp & 3, group = (warp - 4) >> 2, row = quad * 32 + lane;
         const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16);
         float *xm = reinterpret_cast<float *>(smem + C::XM);
         float2 *ml = reinterpret_cast<float2 *>(smem + C::ML);
         const int tok = row / p.G;
         bool ok = true;
-        int n = 0, g = 0;
+        int g = 0;
         Item it;
-        for (int item = 0; take(n, it); item++) {
+        for (int item = 0; take(item, it); item++) {
             const bool live = tok < it.ntok;
             const bool busy = quad * 32 < it.ntok * p.G;  // some row of this warp is live
             int lo = 0, hi = it.klim;
@@ -835,38 +847,43 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < it.nt; j++, g++) {
                 if ((g & 1) != group) continue;
-                const int b = g & 1, kk = it.k0 + j * TK, nk = min(TK, it.klim - kk);
-                if (!__all_sync(0xffffffffu, mbar_wait(bar(B_SF + b), (uint32_t)((g >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN))) {
+                const int b = g & 1, sb = g % C::NS, kk = it.k0 + j * TK, nk = min(TK, it.klim - kk);
+                if (!wait_warp(bar(B_SF + sb), (uint32_t)((g / C::NS) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t ts = ta + (uint32_t)(b * 128);
+                const uint32_t ts = ta + (uint32_t)(sb * 128);
                 const int chunks = (nk + 31) >> 5;
-                const int ra = lo - kk, rb = max(hi - kk, ra);  // columns [ra, rb) are seen
-                const bool mask = __any_sync(0xffffffffu, live && (ra > 0 || rb < TK));
+                uint32_t s[TK];
                 float mx = -INFINITY;
                 if (busy) {
-#pragma unroll 1
-                    for (int c = 0; c < chunks; c++) {
-                        uint32_t s[32];
-                        tmem_ld32(ts + 32 * c, s);
-                        tmem_wait_ld();
-                        if (mask) {
+                    static_for<4>([&](auto c) {
+                        if (c < chunks) {
+                            tmem_ld32_to<32 * c>(ts + 32 * c, s);
+                        } else {
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if ((unsigned)(32 * c + i - ra) >= (unsigned)(rb - ra)) s[i] = 0xff800000u;
+                            for (int i = 0; i < 32; i++) s[32 * c + i] = 0xff800000u;
                         }
+                    });
+                    tmem_wait_ld();
+                    const int ra = lo - kk, rb = max(hi - kk, ra);  // columns [ra, rb) are seen
+                    if (__any_sync(0xffffffffu, live && (ra > 0 || rb < TK))) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) mx = fmaxf(mx, __uint_as_float(s[i]));
+                        for (int i = 0; i < TK; i++)
+                            if ((unsigned)(i - ra) >= (unsigned)(rb - ra)) s[i] = 0xff800000u;
                     }
+                    float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int i = 0; i < TK; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) mm[k] = max3(mm[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+                    mx = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])) * p.c;
                 }
-                mx *= p.c;
                 // the running maximum, from the tile before
                 float before = -INFINITY;
                 if (g > 0) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(bar(B_MX + (b ^ 1) * 4 + quad), (uint32_t)(((g - 1) >> 1) & 1), p.status,
-                                                           E2C_ERR_WAIT_ATTN))) {
+                    if (!wait_warp(bar(B_MX + (b ^ 1) * 4 + quad), (uint32_t)(((g - 1) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                         ok = false;
                         break;
                     }
@@ -887,73 +904,69 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     }
                     if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                         // O holds the tiles before this one once their products are done
-                        if (!__all_sync(0xffffffffu, mbar_wait(bar(B_PV + (b ^ 1)), (uint32_t)(((g - 1) >> 1) & 1), p.status,
-                                                               E2C_ERR_WAIT_ATTN))) {
+                        if (!wait_warp(bar(B_PV + (b ^ 1)), (uint32_t)(((g - 1) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
-                        const uint32_t to = ta + 256u + (uint32_t)((item % C::NO) * D);
+                        const uint32_t to = ta + (uint32_t)(C::O_COL + item % C::NO * D);
 #pragma unroll 1
-                        for (int c = 0; c < D / 32; c++) {
-                            uint32_t o[32];
-                            tmem_ld32(to + 32 * c, o);
+                        for (int c = 0; c < D / 16; c++) {
+                            uint32_t o[16];
+                            tmem_ld16(to + 16 * c, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st32(to + 32 * c, o);
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st16(to + 16 * c, o);
                         }
                         tmem_wait_st();
                     }
-                    const float cc = p.c, mneg = -m;
-                    const bool any = m != -INFINITY;
-                    float sum = 0.f;
-#pragma unroll 1
-                    for (int c = 0; c < chunks; c++) {
-                        uint32_t s[32], pk[16];
-                        tmem_ld32(ts + 32 * c, s);
-                        tmem_wait_ld();
-                        if (mask) {
+                    // a row that has seen nothing yet has only -inf: any finite maximum gives it zeros
+                    const float2 cc = make_float2(p.c, p.c);
+                    const float mneg = m == -INFINITY ? 0.f : -m;
+                    const float2 mm = make_float2(mneg, mneg);
+                    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+                    static_for<4>([&](auto c) {
+                        if (c < chunks) {
+                            uint32_t pk[16];
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if ((unsigned)(32 * c + i - ra) >= (unsigned)(rb - ra)) s[i] = 0xff800000u;
+                            for (int i = 0; i < 16; i++) {
+                                float2 x = fma2(make_float2(__uint_as_float(s[32 * c + 2 * i]), __uint_as_float(s[32 * c + 2 * i + 1])), cc, mm);
+                                x.x = ex2_approx(x.x);
+                                x.y = ex2_approx(x.y);
+                                sum[i & 1] = add2(sum[i & 1], x);
+                                pk[i] = pack2<T>(x.x, x.y);
+                            }
+                            tmem_st16(ts + 16 * c, pk);
                         }
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float e0 = any ? ex2_approx(__fmaf_rn(__uint_as_float(s[2 * i]), cc, mneg)) : 0.f;
-                            const float e1 = any ? ex2_approx(__fmaf_rn(__uint_as_float(s[2 * i + 1]), cc, mneg)) : 0.f;
-                            sum += e0 + e1;
-                            pk[i] = pack2<T>(e0, e1);
-                        }
-                        tmem_st16(ts + 16 * c, pk);
-                    }
-                    l += sum;
+                    });
+                    const float2 all = add2(sum[0], sum[1]);
+                    l += all.x + all.y;
                     tmem_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(B_PF + b));
+                if (lane == 0) mbar_arrive(bar(B_PF + sb));
             }
             if (!ok) break;
             // the slot's last reader was the epilogue two items ago
-            if (!__all_sync(0xffffffffu, mbar_wait(bar(B_MLE + (item & 1)), (uint32_t)(((item >> 1) & 1) ^ 1), p.status,
-                                                   E2C_ERR_WAIT_ATTN)))
+            if (!wait_warp(bar(B_MLE + (item & 1)), (uint32_t)(((item >> 1) & 1) ^ 1), p.status, E2C_ERR_WAIT_ATTN))
                 break;
             ml[((item & 1) * 2 + group) * TR + row] = make_float2(m, l);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_MLF + (item & 1)));
         }
-    } else if (warp >= 12) {
+    } else {
         // ---------------------------------------------------------------- epilogue
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(EPI_REGS));
         const int quad = warp & 3, row = quad * 32 + lane;
         const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16);
         const float2 *ml = reinterpret_cast<const float2 *>(smem + C::ML);
         const int tok = row / p.G, hd = row - tok * p.G;
-        int n = 0;
         Item it;
-        for (int item = 0; take(n, it); item++) {
+        for (int item = 0; take(item, it); item++) {
             const int ob = item % C::NO;
-            if (!__all_sync(0xffffffffu, mbar_wait(bar(B_MLF + (item & 1)), (uint32_t)((item >> 1) & 1), p.status, E2C_ERR_WAIT_EPI)))
+            if (!wait_warp(bar(B_MLF + (item & 1)), (uint32_t)((item >> 1) & 1), p.status, E2C_ERR_WAIT_EPI))
                 break;
             const float2 a = ml[(item & 1) * 2 * TR + row], b = ml[((item & 1) * 2 + 1) * TR + row];
             __syncwarp();
@@ -964,7 +977,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             if (b.x > -INFINITY) l += b.y * exp2f(b.x - m);
             const bool some = l > 0.f;
             const float inv = some ? __fdiv_rn(1.0f, l) : 0.f;
-            if (!__all_sync(0xffffffffu, mbar_wait(bar(B_OF + ob), (uint32_t)((item / C::NO) & 1), p.status, E2C_ERR_WAIT_EPI))) break;
+            if (!wait_warp(bar(B_OF + ob), (uint32_t)((item / C::NO) & 1), p.status, E2C_ERR_WAIT_EPI)) break;
             tc_fence_after();
             const bool live = tok < it.ntok;
             const int64_t t = it.t0 + tok;
@@ -987,7 +1000,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll 1
                 for (int c = 0; c < D / 32; c++) {
                     uint32_t o[32];
-                    tmem_ld32(ta + 256u + (uint32_t)(ob * D + 32 * c), o);
+                    tmem_ld32(ta + (uint32_t)(C::O_COL + ob * D + 32 * c), o);
                     tmem_wait_ld();
                     // a row that saw nothing may have met a page's NaN: its zeros are not a product
 #pragma unroll
@@ -1160,6 +1173,13 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
             cudaSuccess) {
             cudaGetLastError();
             e2c_set_msg("pages_attention: cannot reserve %d bytes of shared memory", smem_bytes<D>());
+            return -2;
+        }
+        // the softmax warps' registers come out of what the block was launched with
+        cudaFuncAttributes fa;
+        if (cudaFuncGetAttributes(&fa, k_attention_pages<T, D>) != cudaSuccess || fa.numRegs != LAUNCH_REGS) {
+            cudaGetLastError();
+            e2c_set_msg("pages_attention: built with %d registers a thread, not %d", fa.numRegs, LAUNCH_REGS);
             return -2;
         }
         attr.set(dev, 1);
