@@ -25,7 +25,8 @@
 // are zeroed in shared memory up to the product's 16-key granularity: what a page holds there is
 // arbitrary, and 0 x NaN would not vanish. Keys past it are masked in S by a select.
 //
-// Warps: 0 = items and TMA, 1 = MMA issue (and zeroing), 4..11 = softmax, 12..15 = epilogue.
+// Warps: 0 = items and Q loads, 1 = MMA issue, 2 and 3 = K and V loads, 4..11 = softmax (and zeroing),
+// 12..15 = epilogue.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -600,140 +601,138 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             for (int i = n - C::NQ < 0 ? 0 : n - C::NQ; i < n; i++)
                 wait_warp(bar(B_QF + i % C::NQ), (uint32_t)((i / C::NQ) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
         } else if (warp == 1) {
-            // ------------------------------------------------------------ MMA issue
+            // ------------------------------------------------------------ MMA issue (one thread)
             // QK runs LOOK tiles ahead of PV; each has a cursor over the items
-            constexpr int LOOK = C::NS - 1;
-            const uint32_t idesc = (1u << 4) | type_bits<T>() | ((uint32_t)(128 >> 4) << 24);
-            Item iq = {}, iv = {};
-            int nq = 0, nv = 0, jq = 0, jv = 0;  // items taken; tile of the item
-            int ks = 0, vs = 0;                  // stages, and the parity of their round
-            uint32_t kp = 0, vp = 0;
-            int sq = 0, sv = 0;                  // S buffers
-            uint32_t pp = 0;                     // parity of P in S buffer sv
-            int gq = 0, gv = 0;
-            bool more = true, ok = true;         // more: QK has tiles left
-            auto qk = [&]() -> bool {
-                if (jq == iq.nt) {
-                    if (!take(nq, iq)) {
-                        more = false;
-                        return iq.ntok < 0;
-                    }
-                    jq = 0;
-                    const int qb = nq % C::NQ;
-                    if (!wait_warp(bar(B_QF + qb), (uint32_t)((nq / C::NQ) & 1), p.status, E2C_ERR_WAIT_MMA)) return false;
-                    nq++;
-                }
-                const int qb = (nq - 1) % C::NQ, nk = min(TK, iq.klim - iq.k0 - jq * TK);
-                const uint32_t id = idesc | (p.neg << 13) | (uint32_t)(((nk + 15) >> 4) << 1) << 17;
-                const uint32_t d = tmem + (uint32_t)(sq * 128);
-                jq++;
-                uint64_t qd = smem_desc_sw128(sbase + qb * C::Q_BYTES);
+            if (elect_one()) {
+                constexpr int LOOK = C::NS - 1;
+                constexpr uint32_t idesc = (1u << 4) | type_bits<T>() | ((uint32_t)(128 >> 4) << 24);
+                constexpr uint32_t id_pv = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // B: N contiguous
+                const uint32_t id_qk = idesc | (p.neg << 13);
+                auto wait1 = [&](int b, uint32_t parity) -> bool {
+#pragma unroll 1
+                    for (uint32_t i = 0; i < kTries; i++)
+                        if (mbar_try_wait_sleep(bar(b), parity, kTryNs)) return true;
+                    record_status(p.status, E2C_ERR_WAIT_MMA);
+                    return false;
+                };
+                // the keys and tiles of item n; no tiles: the last one
+                auto item = [&](int n, int &left, int &keys) -> bool {
+                    const int s = n & (NI - 1);
+                    if (!wait1(B_ITF + s, (uint32_t)((n / NI) & 1))) return false;
+                    left = items[s].ntok < 0 ? 0 : items[s].nt;
+                    keys = items[s].klim - items[s].k0;
+                    mbar_arrive(bar(B_ITE + s));
+                    return true;
+                };
+                int nq = 0, nv = 0;          // items taken
+                int lq = 0, lv = 0;          // tiles of the item left
+                int kq = 0, kv = 0;          // keys left
+                int ks = 0, vs = 0;          // stages, and the parity of their round
+                uint32_t kp = 0, vp = 0;
+                int sq = 0, sv = 0;          // S buffers
+                uint32_t pp = 0;             // parity of P in S buffer sv
+                int ahead = 0, odd = 0;      // QK products not yet used; parity of PV's tile
+                bool more = true, ok = true; // more: QK has tiles left
+                int qb = 0, ob = 0;          // Q and O buffers, and their parities
+                uint32_t qp = 0, op = 1;
+                bool first = false;
+#pragma unroll 1
+                while (ok && (more || ahead > 0)) {
+                    // with one Q buffer an item's first QK waits for the last PV before it
+                    const bool qk_now = more && (C::CROSS || lq > 0 || ahead == 0);
+                    if (qk_now) {
+                        if (lq == 0) {
+                            if (!(ok = item(nq, lq, kq))) break;
+                            if (lq == 0) {
+                                more = false;
+                                continue;
+                            }
+                            qb = nq % C::NQ;
+                            qp = (uint32_t)((nq / C::NQ) & 1);
+                            nq++;
+                            if (!(ok = wait1(B_QF + qb, qp))) break;
+                        }
+                        const uint32_t id = id_qk | (uint32_t)(((min(TK, kq) + 15) >> 4) << 1) << 17;
+                        const uint32_t d = tmem + (uint32_t)(sq * 128);
+                        lq--;
+                        kq -= TK;
+                        uint64_t qd = smem_desc_sw128(sbase + qb * C::Q_BYTES);
 #pragma unroll
-                for (int h = 0; h < C::KPARTS; h++) {
-                    if (!wait_warp(bar(B_KF + ks), kp, p.status, E2C_ERR_WAIT_MMA)) return false;
-                    tc_fence_after();
-                    if (elect_one()) {
-                        uint64_t kd = smem_desc_sw128(sbase + C::K_OFF + ks * C::STAGE);
-                        constexpr int PP = C::PANELS / C::KPARTS;
+                        for (int h = 0; h < C::KPARTS; h++) {
+                            if (!(ok = wait1(B_KF + ks, kp))) break;
+                            const uint64_t kd = smem_desc_sw128(sbase + C::K_OFF + ks * C::STAGE);
 #pragma unroll
-                        for (int k = 0; k < PP * 4; k++) {
-                            const int off = ((k >> 2) * (TR * 128) + (k & 3) * 32) >> 4;
-                            mma_bf16(d, qd + off, kd + off, id, h != 0 || k != 0);
+                            for (int k = 0; k < C::PANELS / C::KPARTS * 4; k++) {
+                                const int off = ((k >> 2) * (TR * 128) + (k & 3) * 32) >> 4;
+                                mma_bf16(d, qd + off, kd + off, id, h != 0 || k != 0);
+                            }
+                            mma_commit(bar(B_KE + ks));
+                            qd += (C::PANELS / C::KPARTS * TR * 128) >> 4;
+                            if (++ks == C::NST) {
+                                ks = 0;
+                                kp ^= 1;
+                            }
                         }
-                        mma_commit(bar(B_KE + ks));
-                        if (h == C::KPARTS - 1) {
-                            mma_commit(bar(B_SF + sq));
-                            if (jq == iq.nt) mma_commit(bar(B_QE + qb));
+                        if (!ok) break;
+                        mma_commit(bar(B_SF + sq));
+                        if (lq == 0) mma_commit(bar(B_QE + qb));
+                        if (++sq == C::NS) sq = 0;
+                        ahead++;
+                    }
+                    if (ahead > LOOK || (ahead > 0 && !qk_now) || (ahead > 0 && !more)) {
+                        if (lv == 0) {
+                            if (!(ok = item(nv, lv, kv))) break;  // QK has taken it: it is there
+                            ob = nv % C::NO;
+                            op = (uint32_t)(((nv / C::NO) & 1) ^ 1);
+                            nv++;
+                            first = true;
                         }
-                    }
-                    __syncwarp();
-                    qd += (C::PANELS / C::KPARTS * TR * 128) >> 4;
-                    if (++ks == C::NST) {
-                        ks = 0;
-                        kp ^= 1;
-                    }
-                }
-                if (++sq == C::NS) sq = 0;
-                gq++;
-                return true;
-            };
-            auto pv = [&]() -> bool {
-                if (jv == iv.nt) {
-                    if (!take(nv, iv)) return false;  // QK has taken it: it is there
-                    jv = 0;
-                    nv++;
-                }
-                const int ob = (nv - 1) % C::NO, nk = min(TK, iv.klim - iv.k0 - jv * TK), nk16 = (nk + 15) & ~15;
-                const bool first = jv == 0;
-                const uint32_t id = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // B: N contiguous
-                const uint32_t d = tmem + (uint32_t)(C::O_COL + ob * D);
-                uint32_t a = tmem + (uint32_t)(sv * 128);
-                jv++;
-#pragma unroll 1
-                for (int r0 = 0; r0 < nk; r0 += C::VROWS) {
-                    if (!wait_warp(bar(B_VF + vs), vp, p.status, E2C_ERR_WAIT_MMA)) return false;
-                    const int here = min(C::VROWS, nk16 - r0), rows = r0 + here - nk;
-                    if (rows > 0) {  // rows nk .. nk16 - 1 of every panel are zeroed, 16 bytes a lane
-                        uint8_t *v = smem + C::V_OFF + vs * C::STAGE + (nk - r0) * 128;
-                        for (int x = lane; x < C::PANELS * rows * 8; x += 32) {
-                            const int panel = x / (rows * 8), y = x - panel * (rows * 8);
-                            *reinterpret_cast<uint4 *>(v + panel * (C::VROWS * 128) + y * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    if (r0 == 0) {
-                        if (!wait_warp(bar(B_PF + sv), pp, p.status, E2C_ERR_WAIT_MMA)) return false;
-                        if (first && !wait_warp(bar(B_OE + ob), (uint32_t)((((nv - 1) / C::NO) & 1) ^ 1), p.status, E2C_ERR_WAIT_MMA))
-                            return false;
-                    }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        uint64_t vd = smem_desc_sw128_mn(sbase + C::V_OFF + vs * C::STAGE, C::VROWS * 128);
-                        if (here == C::VROWS) {
+                        const int nk16 = (min(TK, kv) + 15) & ~15;
+                        const uint32_t d = tmem + (uint32_t)(C::O_COL + ob * D);
+                        uint32_t a = tmem + (uint32_t)(sv * 128);
+                        lv--;
+                        kv -= TK;
+                        if (!(ok = wait1(B_PF + sv, pp))) break;
+                        if (first && !(ok = wait1(B_OE + ob, op))) break;
+                        tc_fence_after();
 #pragma unroll
-                            for (int k = 0; k < C::VROWS / 16; k++)
-                                mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id, !first || r0 != 0 || k != 0);
-                        } else {
+                        for (int h = 0; h < C::KPARTS; h++) {
+                            if (!(ok = wait1(B_VF + vs, vp))) break;
+                            const uint64_t vd = smem_desc_sw128_mn(sbase + C::V_OFF + vs * C::STAGE, C::VROWS * 128);
+                            const int here = min(C::VROWS, nk16 - h * C::VROWS);
+                            if (here == C::VROWS) {
+#pragma unroll
+                                for (int k = 0; k < C::VROWS / 16; k++)
+                                    mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id_pv, !first || h != 0 || k != 0);
+                            } else {
 #pragma unroll 1
-                            for (int k = 0; k < here / 16; k++) mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id, !first || r0 != 0 || k != 0);
+                                for (int k = 0; k < here / 16; k++)
+                                    mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id_pv, !first || h != 0 || k != 0);
+                            }
+                            mma_commit(bar(B_VE + vs));
+                            a += C::VROWS / 2;
+                            if (++vs == C::NST) {
+                                vs = 0;
+                                vp ^= 1;
+                            }
                         }
-                        mma_commit(bar(B_VE + vs));
-                        if (r0 + C::VROWS >= nk) {
-                            mma_commit(bar(B_PV + (gv & 1)));
-                            if (jv == iv.nt) mma_commit(bar(B_OF + ob));
+                        if (!ok) break;
+                        mma_commit(bar(B_PV + odd));
+                        odd ^= 1;
+                        if (lv == 0) mma_commit(bar(B_OF + ob));
+                        first = false;
+                        if (++sv == C::NS) {
+                            sv = 0;
+                            pp ^= 1;
                         }
-                    }
-                    __syncwarp();
-                    a += C::VROWS / 2;
-                    if (++vs == C::NST) {
-                        vs = 0;
-                        vp ^= 1;
+                        ahead--;
                     }
                 }
-                if (++sv == C::NS) {
-                    sv = 0;
-                    pp ^= 1;
-                }
-                gv++;
-                return true;
-            };
-#pragma unroll 1
-            while (ok && (more || gv < gq)) {
-                const bool early = C::CROSS || jq != iq.nt;
-#pragma unroll 1
-                for (int half = 0; ok && half < 2; half++) {
-                    if ((half == 0) == early) {
-                        if (more) ok = qk();
-                    } else if (gv < gq && (gq - gv > LOOK || !more || !early)) {
-                        ok = pv();
-                    }
-                }
+                // all products are done before the block frees tensor memory or ends
+                mma_commit(bar(B_DRAIN));
+                wait1(B_DRAIN, 0);
             }
-            // all products are done before the block frees tensor memory or ends
-            if (elect_one()) mma_commit(bar(B_DRAIN));
             __syncwarp();
-            wait_warp(bar(B_DRAIN), 0, nullptr, E2C_ERR_WAIT_DRAIN);
         } else {
             // ------------------------------------------------------------ K loads (warp 2), V loads (warp 3)
             const bool is_v = warp == 3;
@@ -771,12 +770,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 if (have) {
                     const int nb = (nk + PB - 1) / PB;
                     // a K stage holds PANELS / KPARTS panels of every key, a V stage every panel of VROWS keys
-                    const int parts = is_v ? (nk + C::VROWS - 1) / C::VROWS : C::KPARTS;
                     const int np = is_v ? C::PANELS : C::PANELS / C::KPARTS;
                     const int pitch = (is_v ? C::VROWS : TK) * 128;
 #pragma unroll 1
-                    for (int h = 0; h < parts; h++) {
-                        const int b0 = is_v ? h * C::VROWS / PB : 0, b1 = is_v ? min(nb, (h + 1) * C::VROWS / PB) : nb;
+                    for (int h = 0; h < C::KPARTS; h++) {
+                        const int b0 = is_v ? min(nb, h * C::VROWS / PB) : 0, b1 = is_v ? min(nb, (h + 1) * C::VROWS / PB) : nb;
                         const int x = kvh * D + (is_v ? 0 : h * np * 64);
                         if (!(ok = wait_warp(bar(E + st), par, p.status, E2C_ERR_WAIT_PRODUCER))) break;
                         if (elect_one()) mbar_arrive_expect_tx(bar(F + st), (uint32_t)((b1 - b0) * PB * 128 * np));
@@ -943,6 +941,20 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     const float2 all = add2(sum[0], sum[1]);
                     l += all.x + all.y;
                     tmem_wait_st();
+                }
+                if (nk & 15) {
+                    // V's rows past the last key, up to the product's 16: this group's four warps zero a
+                    // quarter of the 16-byte pieces each
+                    const int part = nk / C::VROWS, vt = g * C::KPARTS + part, vs = vt % C::NST;
+                    if (!wait_warp(bar(B_VF + vs), (uint32_t)((vt / C::NST) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *v = smem + C::V_OFF + vs * C::STAGE + (nk - part * C::VROWS) * 128;
+                    const int pieces = (16 - (nk & 15)) * 8;  // of one panel
+                    for (int x = quad * 32 + lane; x < C::PANELS * pieces; x += 128)
+                        *reinterpret_cast<uint4 *>(v + x / pieces * (C::VROWS * 128) + x % pieces * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async_smem();
                 }
                 tc_fence_before();
                 __syncwarp();
