@@ -25,8 +25,6 @@
 // are zeroed in shared memory up to the product's 16-key granularity: what a page holds there is
 // arbitrary, and 0 x NaN would not vanish. Keys past it are masked in S by a select.
 //
-// Warps: 0 = items and Q loads, 1 = MMA issue, 2 and 3 = K and V loads, 4..11 = softmax (and zeroing),
-// 12..15 = epilogue.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -45,7 +43,9 @@ namespace {
 
 constexpr int TR = 128;  // rows of an item
 constexpr int TK = 128;  // keys of a tile
-constexpr int NTHREADS = 512;
+// warps: 0..7 softmax (two groups of four), 8..11 epilogue, then one each
+enum { W_EPI = 8, W_ITEMS = 12, W_MMA, W_K, W_V, W_Q, WARPS };
+constexpr int NTHREADS = 32 * WARPS;
 constexpr int NI = 8;  // item descriptors in flight
 constexpr float kRescaleLog2 = 8.0f;
 
@@ -67,23 +67,23 @@ constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 template <int D>
 struct Cfg {
     static constexpr int PANELS = D / 64;  // 64 of the head's dimensions each, 128 bytes a row
-    static constexpr int NQ = D == 256 ? 1 : 2;  // Q buffers
-    // K and V have a ring of NST stages each: of a tile, or for D = 256 of half a one (K: half of the
+    static constexpr int NQ = D == 64 ? 2 : 1;  // Q buffers
+    // K and V have a ring of stages each: of a tile, or for D = 256 of half a one (K: half of the
     // head's dimensions, V: half of the keys)
     static constexpr int KPARTS = D == 256 ? 2 : 1, VROWS = TK / KPARTS;
     static constexpr int STAGE = TK * D * 2 / KPARTS;
-    static constexpr int NST = D == 64 ? 5 : 2;
+    static constexpr int NKS = D == 64 ? 5 : D == 128 ? 3 : 2, NVS = D == 64 ? 5 : 2;
     // tensor memory: NS buffers of S (128 columns each), then NO of O (D columns each), 512 columns
     static constexpr int NS = D == 256 ? 2 : 3;
     static constexpr int NO = D == 64 ? 2 : 1;
     static constexpr int O_COL = NS * 128;
-    // QK runs NS - 1 tiles ahead of PV; with two Q buffers across items too, with one an item's first
-    // QK follows the last PV of the item before
-    static constexpr bool CROSS = NQ == 2;
+    // QK runs NS - 1 tiles ahead of PV, across items too; with half tiles in the rings an item's first QK
+    // follows the last PV of the item before
+    static constexpr bool CROSS = KPARTS == 1;
     static constexpr int Q_BYTES = TR * D * 2;
     static constexpr int K_OFF = NQ * Q_BYTES;
-    static constexpr int V_OFF = K_OFF + NST * STAGE;
-    static constexpr int XM = V_OFF + NST * STAGE;              // running maxima handed on [2][128]
+    static constexpr int V_OFF = K_OFF + NKS * STAGE;
+    static constexpr int XM = V_OFF + NVS * STAGE;              // running maxima handed on [2][128]
     static constexpr int ML = XM + 2 * TR * 4;                  // item's (m, l) [2 items][2 groups][128] x 2
     static constexpr int ITEMS = ML + 2 * 2 * TR * 8;
     static constexpr int SCAN = ITEMS + NI * 64;
@@ -128,7 +128,7 @@ struct Args {
     float *lse;
     // workspace
     int4 *split;       // [blocks][2]: the item a block's first part belongs to, if the block is to report it
-    int64_t *before;   // [n + 1] tiles of the sequence items before entry i; [n]: of the prefix items
+    int *before;       // [n + 1] tiles of the sequence items before entry i; [n]: of the prefix items
     float *po, *pl;    // parts: [2 * blocks][128][D], [2 * blocks][128]
     float *dpo, *dpl;  // undivided parts with a prefix: [2][T][H][D], [2][T][H] (0: prefix, 1: own)
     int *status;
@@ -148,10 +148,21 @@ struct __align__(16) Item {
 };
 static_assert(sizeof(Item) == 64, "descriptor");
 
-// What one block of a grid of `blocks` does: tiles [begin(c), begin(c + 1)) of W. The number of blocks
-// at work is at most W, so every one of them has a tile.
-E2C_DEV int64_t begin_of(int64_t c, int64_t W, int64_t blocks) { return c * W / blocks; }
-E2C_DEV int block_of(int64_t x, int64_t W, int64_t blocks) { return (int)(((x + 1) * blocks - 1) / W); }
+// Equal shares of W tiles for up to `grid` blocks: block c does tiles [begin(c), begin(c + 1)).
+struct Share {
+    int W, blocks, each, rest;
+    E2C_DEV void set(int w, int grid) {
+        W = w;
+        blocks = min(w, grid);
+        each = blocks ? w / blocks : 0;
+        rest = w - each * blocks;  // the first `rest` blocks do one tile more
+    }
+    E2C_DEV int begin(int c) const { return c >= blocks ? W : c * each + min(c, rest); }
+    E2C_DEV int block(int x) const {
+        const int c = (int)((unsigned)x / (unsigned)(each + 1));
+        return c < rest ? c : rest + (int)((unsigned)(x - rest * (each + 1)) / (unsigned)each);
+    }
+};
 
 struct Entry {
     int seq, len, q0, nq;
@@ -216,19 +227,21 @@ E2C_DEV int64_t tiles_of(const Args &p, int len, int nq, int base) {
 
 // the batch's totals, the same in every block
 struct Plan {
-    int64_t W, Wp;   // tiles in all; of prefix items
+    Share share;
+    int Wp;          // tiles of prefix items
     int ptiles, plo; // tiles of a prefix item, its first key
     int pseq, pmax;  // the sequence whose table maps the prefix, and its tokens there
     int masked;      // some row does not see every key of the prefix
     int npt;         // row tiles of the batch
     int first;       // the entry of this block's first sequence item,
-    int64_t first_before;  // and the tiles before it
+    int first_before;  // and the tiles before it
 };
 
 // Every thread of the block. Pass 0 sums over the entries and finds the longest; pass 1 finds the entry in
 // which this block's share begins (and leaves the joining kernel the tiles before each entry).
 struct PlanScratch {
-    int64_t sum[16], at;  // by warp; tiles before the block's first entry
+    int64_t sum[WARPS];  // by warp
+    int at;           // tiles before the block's first entry
     int longest, least, masked, first, seq;
 };
 E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
@@ -284,16 +297,16 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
             __syncthreads();
             int64_t before = run + x - mine;
 #pragma unroll 4
-            for (int k = 0; k < 16; k++) {
+            for (int k = 0; k < WARPS; k++) {
                 if (k < w) before += s.sum[k];
                 run += s.sum[k];
             }
             if (pass == 1 && i < p.n) {
                 if (at >= before && at < before + mine) {
                     s.first = i;
-                    s.at = before;
+                    s.at = (int)before;
                 }
-                if (blockIdx.x == 0 && p.shared > 0) p.before[i] = before;
+                if (blockIdx.x == 0 && p.shared > 0) p.before[i] = (int)before;
             }
         }
         if (pass == 0) {
@@ -302,10 +315,12 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
             pl.masked = s.masked || p.window >= 0;
             if (p.window >= 0) pl.plo = max(0, s.least - p.window) / TK * TK;
             pl.ptiles = pl.plo < pl.pmax ? (pl.pmax - pl.plo + TK - 1) / TK : 0;
-            pl.Wp = (int64_t)pl.ptiles * pl.npt * p.pc.KV;
-            pl.W = pl.Wp + run;
-            const int64_t blocks = min((int64_t)gridDim.x, pl.W);
-            if ((int64_t)blockIdx.x < blocks) at = max((int64_t)0, begin_of(blockIdx.x, pl.W, blocks) - pl.Wp);
+            const int64_t Wp = (int64_t)pl.ptiles * pl.npt * p.pc.KV;
+            const bool fits = Wp + run < 1ll << 31;
+            if (!fits && tid == 0) record_status(p.status, E2C_ERR_BAD_SEQ);
+            pl.Wp = fits ? (int)Wp : 0;
+            pl.share.set(fits ? (int)(Wp + run) : 0, gridDim.x);
+            if ((int)blockIdx.x < pl.share.blocks) at = max(0, pl.share.begin(blockIdx.x) - pl.Wp);
         }
     }
     __syncthreads();
@@ -314,7 +329,7 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
     pl.pseq = s.seq;
     if (blockIdx.x == 0 && tid == 0) {
         p.before[p.n] = pl.Wp;
-        p.before[p.n + 1] = pl.W;
+        p.before[p.n + 1] = pl.share.W;
         p.before[p.n + 2] = pl.ptiles;
     }
 }
@@ -345,17 +360,25 @@ E2C_DEV float2 add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
     return y;
 }
-// f(0), f(1), .. with the index a constant expression
-template <int V>
-struct Const {
-    E2C_DEV constexpr operator int() const { return V; }
-};
-template <int N, int I = 0, typename F>
-E2C_DEV void static_for(F &&f) {
-    if constexpr (I < N) {
-        f(Const<I>());
-        static_for<N, I + 1>(f);
-    }
+// 2^x of two values on the FMA pipe, for x <= 125: x = n + f with |f| <= 1/2 (adding 1.5 * 2^23 rounds to
+// the whole number n and leaves it in the low bits), a polynomial of degree 4 in f fitted to the
+// least relative error (2.6e-6), and n added to the exponent. Below 2^-125 the result stays there.
+// One exponential in kPoly pairs takes this way: the exponential unit's 16 a cycle are what
+// bounds 64-wide heads, and nearly bound 128-wide ones.
+constexpr int kPoly = 4;
+E2C_DEV float2 ex2_poly(float2 x) {
+    const float2 big = make_float2(12582912.f, 12582912.f), less = make_float2(-12582912.f, -12582912.f);
+    x.x = fmaxf(x.x, -125.f);
+    x.y = fmaxf(x.y, -125.f);
+    const float2 r = add2(x, big), n = add2(r, less);
+    const float2 f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 y = fma2(make_float2(9.5701e-3f, 9.5701e-3f), f, make_float2(5.591786e-2f, 5.591786e-2f));
+    y = fma2(y, f, make_float2(2.4024745e-1f, 2.4024745e-1f));
+    y = fma2(y, f, make_float2(6.9312181e-1f, 6.9312181e-1f));
+    y = fma2(y, f, make_float2(9.9999926e-1f, 9.9999926e-1f));
+    y.x = __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(r.x) << 23));
+    y.y = __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(r.y) << 23));
+    return y;
 }
 // 32 columns of tensor memory into r[B] .. r[B + 31]
 template <int B, int N>
@@ -408,7 +431,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     Item *items = reinterpret_cast<Item *>(smem + C::ITEMS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == W_ITEMS && lane == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(bar(B_QF + i), 1);
             mbar_init(bar(B_QE + i), 1);
@@ -425,9 +448,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         for (int i = 0; i < 8; i++) mbar_init(bar(B_MX + i), 1);
         for (int i = 0; i < NI; i++) {
             mbar_init(bar(B_ITF + i), 1);
-            mbar_init(bar(B_ITE + i), 16);  // K, V, QK, PV, 8 softmax and 4 epilogue warps
+            mbar_init(bar(B_ITE + i), 17);  // Q, K, V, QK, PV, 8 softmax and 4 epilogue warps
         }
-        for (int i = 0; i < C::NST; i++) {
+        for (int i = 0; i < 5; i++) {
             mbar_init(bar(B_KF + i), 1);
             mbar_init(bar(B_KE + i), 1);
             mbar_init(bar(B_VF + i), 1);
@@ -439,7 +462,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
-    if (warp == 1) {
+    if (warp == W_MMA) {
         tmem_alloc(sbase + C::BARS + B_NUM * 8, 512);
         tmem_relinquish();
     }
@@ -465,113 +488,34 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         return it.ntok >= 0;
     };
 
-    if (warp < 4) {
-        if (warp == 0) {
-            // ------------------------------------------------------------ items and Q loads
-            const int64_t blocks = min((int64_t)gridDim.x, pl.W);
-            const bool at_work = (int64_t)blockIdx.x < blocks;
-            const int64_t L0 = at_work ? begin_of(blockIdx.x, pl.W, blocks) : 0;
-            const int64_t L1 = at_work ? begin_of(blockIdx.x + 1, pl.W, blocks) : 0;
-            // where a part of the item of tiles [s, end) goes: `whole` where it lies in this block
-            auto destination = [&](Item &it, int64_t s, int64_t end, int whole) {
+    if (warp >= W_ITEMS) {
+        if (warp == W_ITEMS) {
+            // ------------------------------------------------------------ items
+            const int L0 = pl.share.begin(blockIdx.x), L1 = pl.share.begin(blockIdx.x + 1);
+            if (p.shared == 0 && lane == 0 && L0 < L1) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+            __syncwarp();
+            int pos = L0, n = 0;
+            bool ok = true;
+            Item it = {};
+            // Publishes the part of the item of tiles [s, s + nt) that begins at pos. It goes to `whole` where it
+            // is not divided.
+            auto emit = [&](int s, int nt, int whole) {
+                const int end = s + nt;
+                it.nt = min(end, L1) - pos;
                 it.dst = whole;
                 it.slot = 0;
-                if (s >= L0 && end <= L1) return;
-                it.dst = TO_SLOT;
-                it.slot = 2 * blockIdx.x + (s > L0 ? 1 : 0);
-                // an item's second block reports it to the joining kernel
-                if (p.shared == 0 && s < L0 && block_of(s, pl.W, blocks) == (int)blockIdx.x - 1 && lane == 0) {
-                    const int c0 = blockIdx.x - 1, c1 = block_of(end - 1, pl.W, blocks);
-                    p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, it.kvh, 2 * c0 + (s > begin_of(c0, pl.W, blocks) ? 1 : 0));
-                    p.split[2 * blockIdx.x + 1] = make_int4(c1, 0, 0, 0);
-                }
-            };
-            if (p.shared == 0 && lane == 0 && at_work) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
-            __syncwarp();
-            // sequence entries, 32 at a time, one per lane
-            int ebase = -1, ei = pl.first, kvh = 0, r = 0;
-            bool placed = false;  // kvh and r are valid for entry ei
-            Entry e = {};
-            int64_t etiles = 0, pos = L0;
-            Item it = {};
-            int n = 0;
-            bool ok = true;
-#pragma unroll 1
-            for (bool more = true; more && ok; n++) {
-                more = pos < L1;
-                if (!more) {
-                    it.ntok = -1;
-                } else if (pos < pl.Wp) {
-                    const int64_t q = pos / pl.ptiles;
-                    const int j0 = (int)(pos - q * pl.ptiles);
-                    it.prefix = 1;
-                    it.kvh = (int)(q / pl.npt);
-                    it.t0 = (int)(q - (int64_t)it.kvh * pl.npt) * p.tpt;
-                    it.ntok = min(p.tpt, p.T - it.t0);
-                    it.nt = (int)(min((q + 1) * pl.ptiles, L1) - pos);
-                    it.k0 = pl.plo + j0 * TK;
-                    it.klim = pl.pmax;
-                    it.masked = pl.masked;
-                    it.seq = pl.pseq;
-                    destination(it, q * pl.ptiles, (q + 1) * pl.ptiles, TO_DENSE);
-                } else {
-                    int nq;
-                    int64_t skip = 0;  // tiles of the item before this block's share
-                    for (;;) {  // to the next row tile: of this key head, of the next, of the next entry
-                        if (ebase < 0 || ei >= ebase + 32) {
-                            ebase = ei;
-                            e = {};
-                            etiles = 0;
-                            if (ei + lane < p.n) {
-                                e = entry_of(p, ei + lane, false);
-                                etiles = tiles_of(p, e.len, e.nq, p.shared);
-                            }
-                        }
-                        nq = __shfl_sync(0xffffffffu, e.nq, ei - ebase);
-                        if (!placed) {
-                            const int64_t c = __shfl_sync(0xffffffffu, etiles, ei - ebase), off = pos - pl.Wp - pl.first_before;
-                            kvh = (int)(off / c);
-                            skip = off - kvh * c;
-                            placed = true;
-                        }
-                        if (r * p.tpt < nq) break;
-                        r = 0;
-                        if (nq > 0 && ++kvh < p.pc.KV) break;
-                        kvh = 0;
-                        if (++ei >= p.n) break;  // cannot happen: pos < L1 <= W
+                if (s < L0 || end > L1) {
+                    it.dst = TO_SLOT;
+                    it.slot = 2 * blockIdx.x + (s > L0 ? 1 : 0);
+                    // an item's second block reports it to the joining kernel
+                    const int c0 = pl.share.block(s);
+                    if (p.shared == 0 && s < L0 && c0 == (int)blockIdx.x - 1 && lane == 0) {
+                        p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, it.kvh, 2 * c0 + (s > pl.share.begin(c0) ? 1 : 0));
+                        p.split[2 * blockIdx.x + 1] = make_int4(pl.share.block(end - 1), 0, 0, 0);
                     }
-                    if (ei >= p.n) {
-                        ok = false;
-                        break;
-                    }
-                    const int src = ei - ebase;
-                    const int len = __shfl_sync(0xffffffffu, e.len, src), q0 = __shfl_sync(0xffffffffu, e.q0, src);
-                    int k0, klim, nt;
-#pragma unroll 1
-                    for (;; r++) {
-                        nt = span_of(p, len, nq, r, p.shared, k0, klim);
-                        if (skip < nt) break;
-                        skip -= nt;
-                    }
-                    const int64_t s = pos - skip;
-                    it.seq = __shfl_sync(0xffffffffu, e.seq, src);
-                    if (len == 0) it.seq = -1;  // its table says nothing
-                    it.prefix = 0;
-                    it.kvh = kvh;
-                    it.t0 = q0 + r * p.tpt;
-                    it.ntok = min(p.tpt, nq - r * p.tpt);
-                    it.nt = (int)(min(s + nt, L1) - pos);
-                    it.k0 = k0 + (int)skip * TK;
-                    it.klim = klim;
-                    it.base = p.shared;
-                    it.len = len;
-                    it.pos0 = len - nq + r * p.tpt;
-                    it.masked = 1;
-                    destination(it, s, s + nt, p.shared > 0 ? TO_DENSE : TO_OUT);
-                    r++;
                 }
                 const int sl = n & (NI - 1);
-                if (!(ok = wait_warp(bar(B_ITE + sl), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) break;
+                if (!(ok = wait_warp(bar(B_ITE + sl), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) return;
                 if (lane == 0) {
                     const int4 *d = reinterpret_cast<const int4 *>(&it);
                     int4 *o = reinterpret_cast<int4 *>(items + sl);
@@ -580,23 +524,110 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     mbar_arrive(bar(B_ITF + sl));
                 }
                 __syncwarp();
-                if (!more) break;
                 pos += it.nt;
+                n++;
+            };
+            if (pos < pl.Wp) {
+                int q = pos / pl.ptiles, j0 = pos - q * pl.ptiles, kvh = q / pl.npt, rt = q - kvh * pl.npt;
+                it.prefix = 1;
+                it.klim = pl.pmax;
+                it.masked = pl.masked;
+                it.seq = pl.pseq;
+#pragma unroll 1
+                for (; ok && pos < min(L1, pl.Wp); q++) {
+                    it.kvh = kvh;
+                    it.t0 = rt * p.tpt;
+                    it.ntok = min(p.tpt, p.T - it.t0);
+                    it.k0 = pl.plo + j0 * TK;
+                    j0 = 0;
+                    if (++rt == pl.npt) {
+                        rt = 0;
+                        kvh++;
+                    }
+                    emit(q * pl.ptiles, pl.ptiles, TO_DENSE);
+                }
+            }
+            if (ok && pos < L1) {
+                // sequence entries, 32 at a time, one per lane
+                int off = pos - pl.Wp - pl.first_before, ebase = -32;  // off: tiles before pos of the entry
+                Entry e = {};
+                int etiles = 0;
+                it.prefix = 0;
+                it.base = p.shared;
+                it.masked = 1;
+#pragma unroll 1
+                for (int i = pl.first; ok && pos < L1 && i < p.n; i++) {
+                    if (i >= ebase + 32) {
+                        ebase = i;
+                        e = {};
+                        etiles = 0;
+                        if (i + lane < p.n) {
+                            e = entry_of(p, i + lane, false);
+                            etiles = (int)tiles_of(p, e.len, e.nq, p.shared);
+                        }
+                    }
+                    const int src = i - ebase, nq = __shfl_sync(0xffffffffu, e.nq, src), c = __shfl_sync(0xffffffffu, etiles, src);
+                    if (nq == 0) continue;
+                    const int len = __shfl_sync(0xffffffffu, e.len, src), q0 = __shfl_sync(0xffffffffu, e.q0, src);
+                    it.seq = __shfl_sync(0xffffffffu, e.seq, src);
+                    if (len == 0) it.seq = -1;  // its table says nothing
+                    it.len = len;
+                    int kvh = 0;
+                    if (off >= c) {
+                        kvh = off / c;
+                        off -= kvh * c;
+                    }
+#pragma unroll 1
+                    for (int r = 0; ok && pos < L1 && kvh < p.pc.KV;) {
+                        int k0, klim;
+                        const int nt = span_of(p, len, nq, r, p.shared, k0, klim);
+                        if (off >= nt) {
+                            off -= nt;
+                        } else {
+                            it.kvh = kvh;
+                            it.t0 = q0 + r * p.tpt;
+                            it.ntok = min(p.tpt, nq - r * p.tpt);
+                            it.k0 = k0 + off * TK;
+                            it.klim = klim;
+                            it.pos0 = len - nq + r * p.tpt;
+                            const int s = pos - off;
+                            off = 0;
+                            emit(s, nt, p.shared > 0 ? TO_DENSE : TO_OUT);
+                        }
+                        if (++r * p.tpt >= nq) {
+                            r = 0;
+                            kvh++;
+                        }
+                    }
+                }
+            }
+            if (ok && wait_warp(bar(B_ITE + (n & (NI - 1))), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER) &&
+                lane == 0) {
+                items[n & (NI - 1)].ntok = -1;
+                mbar_arrive(bar(B_ITF + (n & (NI - 1))));
+            }
+            __syncwarp();
+        } else if (warp == W_Q) {
+            // ------------------------------------------------------------ Q loads
+            int n = 0;
+            Item it;
+#pragma unroll 1
+            for (; take(n, it); n++) {
                 const int qb = n % C::NQ;
-                if (!(ok = wait_warp(bar(B_QE + qb), (uint32_t)(((n / C::NQ) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) break;
+                if (!wait_warp(bar(B_QE + qb), (uint32_t)(((n / C::NQ) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) break;
                 if (elect_one()) {
-                    const int box = it.prefix ? qp_box : q_box;
-                    mbar_arrive_expect_tx(bar(B_QF + qb), (uint32_t)(C::PANELS * box * p.G * 128));
+                    const CUtensorMap *tm = it.prefix ? &tmQp : &tmQ;
+                    mbar_arrive_expect_tx(bar(B_QF + qb), (uint32_t)(C::PANELS * (it.prefix ? qp_box : q_box) * p.G * 128));
+#pragma unroll
                     for (int i = 0; i < C::PANELS; i++)
-                        tma_load_3d(sbase + qb * C::Q_BYTES + i * (TR * 128), it.prefix ? &tmQp : &tmQ, 64 * i, it.kvh * p.G, it.t0,
-                                    bar(B_QF + qb));
+                        tma_load_3d(sbase + qb * C::Q_BYTES + i * (TR * 128), tm, 64 * i, it.kvh * p.G, it.t0, bar(B_QF + qb));
                 }
                 __syncwarp();
             }
             // every load that was issued has landed before the block may end
             for (int i = n - C::NQ < 0 ? 0 : n - C::NQ; i < n; i++)
                 wait_warp(bar(B_QF + i % C::NQ), (uint32_t)((i / C::NQ) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
-        } else if (warp == 1) {
+        } else if (warp == W_MMA) {
             // ------------------------------------------------------------ MMA issue (one thread)
             // QK runs LOOK tiles ahead of PV; each has a cursor over the items
             if (elect_one()) {
@@ -664,7 +695,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                             }
                             mma_commit(bar(B_KE + ks));
                             qd += (C::PANELS / C::KPARTS * TR * 128) >> 4;
-                            if (++ks == C::NST) {
+                            if (++ks == C::NKS) {
                                 ks = 0;
                                 kp ^= 1;
                             }
@@ -707,7 +738,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                             }
                             mma_commit(bar(B_VE + vs));
                             a += C::VROWS / 2;
-                            if (++vs == C::NST) {
+                            if (++vs == C::NVS) {
                                 vs = 0;
                                 vp ^= 1;
                             }
@@ -730,10 +761,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             }
             __syncwarp();
         } else {
-            // ------------------------------------------------------------ K loads (warp 2), V loads (warp 3)
-            const bool is_v = warp == 3;
+            // ------------------------------------------------------------ K loads, V loads
+            const bool is_v = warp == W_V;
             const CUtensorMap *tm = is_v ? &tmV : &tmK;
-            const int F = is_v ? B_VF : B_KF, E = is_v ? B_VE : B_KE;
+            const int F = is_v ? B_VF : B_KF, E = is_v ? B_VE : B_KE, NST = is_v ? C::NVS : C::NKS;
             const uint32_t ring = sbase + (is_v ? C::V_OFF : C::K_OFF);
             const int PB = min(p.pc.page, C::VROWS), shift = 31 - __clz(p.pc.page);
             Item it = {};
@@ -772,20 +803,31 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     for (int h = 0; h < C::KPARTS; h++) {
                         const int b0 = is_v ? min(nb, h * C::VROWS / PB) : 0, b1 = is_v ? min(nb, (h + 1) * C::VROWS / PB) : nb;
                         const int x = kvh * D + (is_v ? 0 : h * np * 64);
-                        if (!(ok = wait_warp(bar(E + st), par, p.status, E2C_ERR_WAIT_PRODUCER))) break;
-                        if (elect_one()) mbar_arrive_expect_tx(bar(F + st), (uint32_t)((b1 - b0) * PB * 128 * np));
-                        __syncwarp();
-                        uint32_t dst = ring + st * C::STAGE;
-#pragma unroll 1
-                        for (int b = b0; b < b1; b++, dst += PB * 128) {
-                            const int y = __shfl_sync(0xffffffffu, row, b);
-                            if (elect_one()) {
+                        // the first rows are in every lane before the wait: from a free stage to its loads is the
+                        // shortest way
+                        int y[4];
 #pragma unroll
-                                for (int i = 0; i < C::PANELS; i++)
-                                    if (i < np) tma_load_2d(dst + i * pitch, tm, x + 64 * i, y, bar(F + st));
-                            }
+                        for (int i = 0; i < 4; i++) y[i] = __shfl_sync(0xffffffffu, row, min(b0 + i, 31));
+                        if (!(ok = wait_warp(bar(E + st), par, p.status, E2C_ERR_WAIT_PRODUCER))) break;
+                        const uint32_t dst = ring + st * C::STAGE, full = bar(F + st);
+                        auto box = [&](int b, int y) {
+#pragma unroll
+                            for (int i = 0; i < C::PANELS; i++)
+                                if (i < np) tma_load_2d(dst + (b - b0) * (PB * 128) + i * pitch, tm, x + 64 * i, y, full);
+                        };
+                        if (elect_one()) {
+                            mbar_arrive_expect_tx(full, (uint32_t)((b1 - b0) * PB * 128 * np));
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (b0 + i < b1) box(b0 + i, y[i]);
                         }
-                        if (++st == C::NST) {
+                        __syncwarp();
+#pragma unroll 1
+                        for (int b = b0 + 4; b < b1; b++) {
+                            const int yb = __shfl_sync(0xffffffffu, row, b);
+                            if (elect_one()) box(b, yb);
+                        }
+                        if (++st == NST) {
                             st = 0;
                             par ^= 1;
                         }
@@ -799,12 +841,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 nk = nk2;
                 have = have2;
             }
-            for (int i = total - C::NST < 0 ? 0 : total - C::NST; i < total; i++)
-                wait_warp(bar(F + i % C::NST), (uint32_t)((i / C::NST) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
+            for (int i = total - NST < 0 ? 0 : total - NST; i < total; i++)
+                wait_warp(bar(F + i % NST), (uint32_t)((i / NST) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
         }
-    } else if (warp < 12) {
+    } else if (warp < W_EPI) {
         // ---------------------------------------------------------------- softmax
-        const int quad = warp & 3, group = (warp - 4) >> 2, row = quad * 32 + lane;
+        const int quad = warp & 3, group = warp >> 2, row = quad * 32 + lane;
         const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16);
         float *xm = reinterpret_cast<float *>(smem + C::XM);
         float2 *ml = reinterpret_cast<float2 *>(smem + C::ML);
@@ -840,49 +882,52 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             for (int j = 0; j < it.nt; j++, g++) {
                 if ((g & 1) != group) continue;
                 const int b = g & 1, sb = g % C::NS, kk = it.k0 + j * TK, nk = min(TK, it.klim - kk);
+                // the running maximum, from the tile before (its wait runs while this tile's products do)
+                if (g > 0 && !wait_warp(bar(B_MX + (b ^ 1) * 4 + quad), (uint32_t)(((g - 1) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                    ok = false;
+                    break;
+                }
+                const float before = j > 0 ? xm[(b ^ 1) * TR + row] : -INFINITY;
                 if (!wait_warp(bar(B_SF + sb), (uint32_t)((g / C::NS) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
                 const uint32_t ts = ta + (uint32_t)(sb * 128);
-                // Columns read at once, twice over: for the maximum and for the exponentials. A loop of 64
-                // columns' code beats a row of 128 held in registers, whose straight code does not stay in
-                // the instruction cache (16 heads of 128, 4096 tokens: 370 against 443 us)
-                constexpr int W = 64;
-                float mx = -INFINITY;
                 const int ra = lo - kk, rb = max(hi - kk, ra);  // columns [ra, rb) are seen
                 const bool masked = __any_sync(0xffffffffu, live && (ra > 0 || rb < TK));
-                auto part = [&](int c0, uint32_t (&s)[W]) {
-                    static_for<W / 32>([&](auto c) { tmem_ld32_to<32 * c>(ts + c0 + 32 * c, s); });
-                    tmem_wait_ld();
-                    if (masked) {
+                // The columns are read twice, for the maximum and for the exponentials, in loops short enough
+                // for the instruction cache: a row of 128 logits held in registers is straight code that does
+                // not stay in it (16 heads of 128, 4096 tokens: 443 us, against 370 with loops of 64 columns)
+                auto hide = [&](int c0, uint32_t (&s)[32]) {
 #pragma unroll
-                        for (int i = 0; i < W; i++)
-                            if ((unsigned)(c0 + i - ra) >= (unsigned)(rb - ra)) s[i] = 0xff800000u;
-                    }
+                    for (int i = 0; i < 32; i++)
+                        if ((unsigned)(c0 + i - ra) >= (unsigned)(rb - ra)) s[i] = 0xff800000u;
                 };
+                float mx = -INFINITY;
                 if (busy) {
                     float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (!masked) {
 #pragma unroll 1
-                    for (int c0 = 0; c0 < nk; c0 += W) {
-                        uint32_t s[W];
-                        part(c0, s);
+                        for (int c0 = 0; c0 < TK; c0 += 32) {
+                            uint32_t s[32];
+                            tmem_ld32(ts + c0, s);
+                            tmem_wait_ld();
 #pragma unroll
-                        for (int i = 0; i < W; i += 8)
+                            for (int i = 0; i < 32; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < nk; c0 += 32) {
+                            uint32_t s[32];
+                            tmem_ld32(ts + c0, s);
+                            tmem_wait_ld();
+                            hide(c0, s);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) mm[k] = max3(mm[k], __uint_as_float(s[i + 2 * k]), __uint_as_float(s[i + 2 * k + 1]));
+                            for (int i = 0; i < 32; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        }
                     }
                     mx = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])) * p.c;
-                }
-                // the running maximum, from the tile before
-                float before = -INFINITY;
-                if (g > 0) {
-                    if (!wait_warp(bar(B_MX + (b ^ 1) * 4 + quad), (uint32_t)(((g - 1) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
-                        ok = false;
-                        break;
-                    }
-                    if (j > 0) before = xm[(b ^ 1) * TR + row];
                 }
                 float now = before, alpha = 1.f;
                 if (live && (mx > before + kRescaleLog2 || (before == -INFINITY && mx > -INFINITY))) {
@@ -921,22 +966,37 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     const float mneg = m == -INFINITY ? 0.f : -m;
                     const float2 mm = make_float2(mneg, mneg);
                     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+                    if (!masked) {
 #pragma unroll 1
-                    for (int c0 = 0; c0 < nk; c0 += W) {
-                        uint32_t s[W];
-                        part(c0, s);
-                        static_for<W / 32>([&](auto c) {
-                            uint32_t pk[16];
+                        for (int c0 = 0; c0 < TK; c0 += 32) {
+                            uint32_t s[32], pk[16];
+                            tmem_ld32(ts + c0, s);
+                            tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
-                                float2 x = fma2(make_float2(__uint_as_float(s[32 * c + 2 * i]), __uint_as_float(s[32 * c + 2 * i + 1])), cc, mm);
-                                x.x = ex2_approx(x.x);
-                                x.y = ex2_approx(x.y);
+                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, mm);
+                                x = i % kPoly == kPoly - 1 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
                                 pk[i] = pack2<T>(x.x, x.y);
                             }
-                            tmem_st16(ts + c0 / 2 + 16 * c, pk);
-                        });
+                            tmem_st16(ts + c0 / 2, pk);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < nk; c0 += 32) {
+                            uint32_t s[32], pk[16];
+                            tmem_ld32(ts + c0, s);
+                            tmem_wait_ld();
+                            hide(c0, s);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, mm);
+                                x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                                sum[i & 1] = add2(sum[i & 1], x);
+                                pk[i] = pack2<T>(x.x, x.y);
+                            }
+                            tmem_st16(ts + c0 / 2, pk);
+                        }
                     }
                     const float2 all = add2(sum[0], sum[1]);
                     l += all.x + all.y;
@@ -945,8 +1005,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 if (nk & 15) {
                     // V's rows past the last key, up to the product's 16: this group's four warps zero a
                     // quarter of the 16-byte pieces each
-                    const int part = nk / C::VROWS, vt = g * C::KPARTS + part, vs = vt % C::NST;
-                    if (!wait_warp(bar(B_VF + vs), (uint32_t)((vt / C::NST) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                    const int part = nk / C::VROWS, vt = g * C::KPARTS + part, vs = vt % C::NVS;
+                    if (!wait_warp(bar(B_VF + vs), (uint32_t)((vt / C::NVS) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                         ok = false;
                         break;
                     }
@@ -982,67 +1042,73 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             const float2 a = ml[(item & 1) * 2 * TR + row], b = ml[((item & 1) * 2 + 1) * TR + row];
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_MLE + (item & 1)));
-            const float m = fmaxf(a.x, b.x);
-            float l = 0.f;
-            if (a.x > -INFINITY) l += a.y * exp2f(a.x - m);
-            if (b.x > -INFINITY) l += b.y * exp2f(b.x - m);
-            const bool some = l > 0.f;
-            const float inv = some ? __fdiv_rn(1.0f, l) : 0.f;
-            if (!wait_warp(bar(B_OF + ob), (uint32_t)((item / C::NO) & 1), p.status, E2C_ERR_WAIT_EPI)) break;
-            tc_fence_after();
-            const bool live = tok < it.ntok;
+            // the groups' sums, to the larger maximum; a row that neither saw a key of has l = 0
+            const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.f : m;
+            const float l = a.y * ex2_approx(a.x - ref) + b.y * ex2_approx(b.x - ref);
+            const bool live = tok < it.ntok, some = l > 0.f;
+            const float inv = some ? __fdividef(1.0f, l) : 0.f;
+            const bool blank = __any_sync(0xffffffffu, live && !some);
             const int64_t t = it.t0 + tok;
             const int h = it.kvh * p.G + hd;
-            if (quad * 32 < it.ntok * p.G) {
+            const bool busy = quad * 32 < it.ntok * p.G;
+            T *out = nullptr;
+            float *part = nullptr;
+            if (busy) {
                 const float sums = some ? m + log2f(l) : -INFINITY;
-                T *out = nullptr;
-                float *part = nullptr;
                 if (it.dst == TO_OUT) {
-                    out = static_cast<T *>(p.out) + t * p.ldo + (int64_t)h * D;
+                    out = static_cast<T *>(p.out) + t * p.ldo + h * D;
                     if (live && p.lse) p.lse[t * p.H + h] = sums * LN2;
-                } else if (it.dst == TO_SLOT) {
-                    part = p.po + ((int64_t)it.slot * TR + row) * D;
-                    if (live) p.pl[(int64_t)it.slot * TR + row] = sums;
                 } else {
-                    const int64_t at = ((int64_t)(it.prefix ? 0 : 1) * p.T + t) * p.H + h;
-                    part = p.dpo + at * D;
-                    if (live) p.dpl[at] = sums;
-                }
-#pragma unroll 1
-                for (int c = 0; c < D / 32; c++) {
-                    uint32_t o[32];
-                    tmem_ld32(ta + (uint32_t)(C::O_COL + ob * D + 32 * c), o);
-                    tmem_wait_ld();
-                    // a row that saw nothing may have met a page's NaN: its zeros are not a product
-#pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = some ? __float_as_uint(__uint_as_float(o[i]) * inv) : 0u;
-                    if (live && out) {
-                        uint4 *y = reinterpret_cast<uint4 *>(out + 32 * c);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            uint4 v;
-                            v.x = pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1]));
-                            v.y = pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3]));
-                            v.z = pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5]));
-                            v.w = pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7]));
-                            y[i] = v;
-                        }
-                    } else if (live) {
-                        uint4 *y = reinterpret_cast<uint4 *>(part + 32 * c);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) y[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                    }
+                    const int64_t at = it.dst == TO_SLOT ? (int64_t)it.slot * TR + row : ((int64_t)(it.prefix ? 0 : 1) * p.T + t) * p.H + h;
+                    part = (it.dst == TO_SLOT ? p.po : p.dpo) + at * D;
+                    if (live) (it.dst == TO_SLOT ? p.pl : p.dpl)[at] = sums;
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(B_OE + ob));
+            if (!wait_warp(bar(B_OF + ob), (uint32_t)((item / C::NO) & 1), p.status, E2C_ERR_WAIT_EPI)) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                if (busy) {
+                    tmem_ld32(ta + (uint32_t)(C::O_COL + ob * D + c), o);
+                    tmem_wait_ld();
+                }
+                if (c == D - 32) {  // O has been read: the next item may use it while this one is stored
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(B_OE + ob));
+                }
+                if (!busy) continue;
+                if (blank && !some) {  // such a row may have met a page's NaN: its zeros are not a product
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = 0u;
+                }
+                if (live && out) {
+                    uint4 *y = reinterpret_cast<uint4 *>(out + c);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint4 v;
+                        v.x = pack2<T>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
+                        v.y = pack2<T>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
+                        v.z = pack2<T>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
+                        v.w = pack2<T>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
+                        y[i] = v;
+                    }
+                } else if (live) {
+                    float4 *y = reinterpret_cast<float4 *>(part + c);
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        y[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                           __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+                }
+                __syncwarp();
+            }
         }
     }
 
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) {
+    if (warp == W_MMA) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -1083,8 +1149,7 @@ __global__ void __launch_bounds__(JOIN) k_join_split(const Args p, int grid) {
     using J = Join<T, D>;
     griddep_launch_dependents();
     griddep_wait();
-    const int64_t W = p.before[p.n + 1];
-    if ((int64_t)blockIdx.x >= min((int64_t)grid, W)) return;
+    if ((int)blockIdx.x >= min(grid, p.before[p.n + 1])) return;
     const int4 a = p.split[2 * blockIdx.x];
     if (a.y == 0) return;
     const int c1 = p.split[2 * blockIdx.x + 1].x;
@@ -1108,25 +1173,25 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     const int64_t t = u / p.H;
     if (t >= p.T) return;
     const int h = (int)(u - t * p.H), kvh = h / p.G, hd = h - kvh * p.G, x = threadIdx.x % J::LANES;
-    const int64_t Wp = p.before[p.n], W = p.before[p.n + 1];
-    const int ptiles = (int)p.before[p.n + 2];
-    const int64_t blocks = min((int64_t)grid, W);
+    const int Wp = p.before[p.n], ptiles = p.before[p.n + 2];
+    Share share;
+    share.set(p.before[p.n + 1], grid);
     J j;
-    auto parts = [&](int64_t s, int64_t end, int which, int row) {
-        const int c0 = block_of(s, W, blocks), c1 = block_of(end - 1, W, blocks);
+    auto parts = [&](int s, int end, int which, int row) {
+        const int c0 = share.block(s), c1 = share.block(end - 1);
         if (c0 == c1) {
             const int64_t at = ((int64_t)which * p.T + t) * p.H + h;
             j.add(p.dpo + at * D, p.dpl[at], x);
             return;
         }
         for (int c = c0; c <= c1; c++) {
-            const int slot = 2 * c + (c == c0 && s > begin_of(c0, W, blocks) ? 1 : 0);
+            const int slot = 2 * c + (c == c0 && s > share.begin(c0) ? 1 : 0);
             j.add(p.po + ((int64_t)slot * TR + row) * D, p.pl[(int64_t)slot * TR + row], x);
         }
     };
     if (ptiles) {
         const int npt = (p.T + p.tpt - 1) / p.tpt, rt = (int)(t / p.tpt);
-        const int64_t s = ((int64_t)kvh * npt + rt) * ptiles;
+        const int s = (kvh * npt + rt) * ptiles;
         parts(s, s + ptiles, 0, (int)(t - (int64_t)rt * p.tpt) * p.G + hd);
     }
     int last;
@@ -1137,7 +1202,7 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     // an entry has one row tile here
     int k0, klim;
     const int nt = span_of(p, e.len, e.nq, 0, p.shared, k0, klim);
-    const int64_t s = Wp + p.before[i] + (int64_t)kvh * nt;
+    const int s = Wp + p.before[i] + kvh * nt;
     parts(s, s + nt, 1, (int)(t - e.q0) * p.G + hd);
     j.put(p, t, h, x);
 }
@@ -1158,7 +1223,7 @@ Layout layout(int blocks, int n, int T, int H, int D, bool prefix) {
         return here;
     };
     l.split = take(sizeof(int4) * 2 * blocks);
-    l.before = take(sizeof(int64_t) * (prefix ? (size_t)n + 3 : (size_t)n + 3));
+    l.before = take(sizeof(int) * ((size_t)n + 3));
     l.pl = take(sizeof(float) * 2 * blocks * TR);
     l.po = take(sizeof(float) * 2 * blocks * TR * D);
     l.dpl = take(prefix ? sizeof(float) * 2 * (size_t)T * H : 0);
@@ -1202,9 +1267,9 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
     if (launch_error("pages_attention")) return -2;
     using J = Join<T, D>;
     if (prefix)
-        e2c_launch(k_join_prefix<T, D>, dim3((unsigned)(((int64_t)a.T * a.H + J::ROWS - 1) / J::ROWS)), dim3(JOIN), 0, st, a, sms);
+        e2c_launch_as(true, k_join_prefix<T, D>, dim3((unsigned)(((int64_t)a.T * a.H + J::ROWS - 1) / J::ROWS)), dim3(JOIN), 0, st, a, sms);
     else
-        e2c_launch(k_join_split<T, D>, dim3(sms, 8), dim3(JOIN), 0, st, a, sms);
+        e2c_launch_as(true, k_join_split<T, D>, dim3(sms, 8), dim3(JOIN), 0, st, a, sms);
     return launch_error("pages_attention join");
 }
 
@@ -1251,7 +1316,7 @@ extern "C" int e2c_pages_attention(const e2c_pages *pc, const void *q, int64_t l
     a.lse = lse;
     uint8_t *w = static_cast<uint8_t *>(ws);
     a.split = reinterpret_cast<int4 *>(w + l.split);
-    a.before = reinterpret_cast<int64_t *>(w + l.before);
+    a.before = reinterpret_cast<int *>(w + l.before);
     a.po = reinterpret_cast<float *>(w + l.po);
     a.pl = reinterpret_cast<float *>(w + l.pl);
     a.dpo = reinterpret_cast<float *>(w + l.dpo);
