@@ -47,6 +47,8 @@ constexpr int TK = 128;  // keys of a tile
 enum { W_EPI = 8, W_ITEMS = 12, W_MMA, W_K, W_V, W_Q, WARPS };
 constexpr int NTHREADS = 32 * WARPS;
 constexpr int NI = 8;  // item descriptors in flight
+// What a sequence item costs beside its tiles, in tiles: its set-up and its output
+constexpr int ITEM_COST = 1;
 constexpr float kRescaleLog2 = 8.0f;
 
 // A wait of a whole warp, bounded by its number of (sleeping) tries: up to 1.3 s. It is small on
@@ -128,9 +130,9 @@ struct Args {
     float *lse;
     // workspace
     int4 *split;       // [blocks][2]: the item a block's first part belongs to, if the block is to report it
-    int *before;       // [n + 1] tiles of the sequence items before entry i; [n]: of the prefix items
-    float *po, *pl;    // parts: [2 * blocks][128][D], [2 * blocks][128]
-    float *dpo, *dpl;  // undivided parts with a prefix: [2][T][H][D], [2][T][H] (0: prefix, 1: own)
+    int *before;       // [n + 2] the cost of the sequence items before entry i; of all; tiles of the prefix
+    float *po, *pl;    // parts: [slots][128][D], [slots][128]; two a block, then one a prefix item
+    float *dpo, *dpl;  // with a prefix, the undivided sequence items: [T][H][D], [T][H]
     int *status;
 };
 
@@ -148,20 +150,47 @@ struct __align__(16) Item {
 };
 static_assert(sizeof(Item) == 64, "descriptor");
 
-// Equal shares of W tiles for up to `grid` blocks: block c does tiles [begin(c), begin(c + 1)).
+// What each of `grid` blocks does.
+//
+// Prefix items: a key head's prefix is cut into as many runs of `chunk` tiles as there are blocks for its row
+// tiles, and the row tiles of one run go to neighbouring blocks, which read its keys at the same time: then one
+// of them fetches a tile from memory and the others find it near in the L2 cache. (Shares that divide
+// items anywhere had each row tile read the prefix at a time of its own, and took twice as long.) Item
+// i goes to block i mod grid, whole.
+//
+// Sequence items: their tiles, in order, are divided so that all blocks have about the same to do; block
+// c does tiles [begin(c), begin(c + 1)), and items are divided where a share ends.
 struct Share {
-    int W, blocks, each, rest;
-    E2C_DEV void set(int w, int grid) {
-        W = w;
-        blocks = min(w, grid);
-        each = blocks ? w / blocks : 0;
-        rest = w - each * blocks;  // the first `rest` blocks do one tile more
+    int items, splits, chunk;  // prefix items, runs of a key head's prefix, tiles of a run
+    int n1, s1, each1, rest1;  // the first n1 blocks have a prefix item more; s1 tiles are theirs
+    int each2, rest2;          // the other blocks' shares: each2, the first rest2 of them one more
+    E2C_DEV void set(int rows, int ptiles, int tiles, int grid) {
+        items = splits = chunk = 0;
+        if (ptiles > 0) {
+            const int s = max(1, grid / rows);
+            chunk = (ptiles + s - 1) / s;
+            splits = (ptiles + chunk - 1) / chunk;
+            items = rows * splits;
+        }
+        const int cost = chunk + 2 * ITEM_COST, k = items / grid;
+        n1 = items - k * grid;
+        const int64_t target = ((int64_t)items * cost + tiles) / grid;
+        const int64_t room = target - (int64_t)(k + 1) * cost;  // for a block with k + 1 prefix items
+        s1 = room > 0 ? (int)min((int64_t)tiles, room * n1) : 0;
+        each1 = n1 > 0 ? s1 / n1 : 0;
+        rest1 = s1 - each1 * n1;
+        const int n2 = grid - n1;
+        each2 = (tiles - s1) / n2;
+        rest2 = tiles - s1 - each2 * n2;
     }
-    E2C_DEV int begin(int c) const { return c >= blocks ? W : c * each + min(c, rest); }
-    E2C_DEV int block(int x) const {
+    E2C_DEV int begin(int c) const {
+        return c <= n1 ? c * each1 + min(c, rest1) : s1 + (c - n1) * each2 + min(c - n1, rest2);
+    }
+    static E2C_DEV int part(int x, int each, int rest) {
         const int c = (int)((unsigned)x / (unsigned)(each + 1));
         return c < rest ? c : rest + (int)((unsigned)(x - rest * (each + 1)) / (unsigned)each);
     }
+    E2C_DEV int block(int x) const { return x < s1 ? part(x, each1, rest1) : n1 + part(x - s1, each2, rest2); }
 };
 
 struct Entry {
@@ -210,7 +239,7 @@ E2C_DEV int span_of(const Args &p, int len, int nq, int r, int base, int &k0, in
     klim = hi;
     return (hi - k0 + TK - 1) / TK;
 }
-// tiles of all of an entry's row tiles, for one key head
+// the cost of all of an entry's row tiles, for one key head
 E2C_DEV int64_t tiles_of(const Args &p, int len, int nq, int base) {
     if (nq <= 0) return 0;
     const int nr = (nq + p.tpt - 1) / p.tpt;
@@ -219,7 +248,7 @@ E2C_DEV int64_t tiles_of(const Args &p, int len, int nq, int base) {
     int64_t s = 0;
 #pragma unroll 1
     for (int r = 0; r < nr; r++) {
-        s += span_of(p, len, nq, r, base, k0, klim);
+        s += span_of(p, len, nq, r, base, k0, klim) + ITEM_COST;
         if (same) return s * nr;
     }
     return s;
@@ -228,8 +257,7 @@ E2C_DEV int64_t tiles_of(const Args &p, int len, int nq, int base) {
 // the batch's totals, the same in every block
 struct Plan {
     Share share;
-    int Wp;          // tiles of prefix items
-    int ptiles, plo; // tiles of a prefix item, its first key
+    int ptiles, plo; // tiles of the prefix, its first key
     int pseq, pmax;  // the sequence whose table maps the prefix, and its tokens there
     int masked;      // some row does not see every key of the prefix
     int npt;         // row tiles of the batch
@@ -257,7 +285,8 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
     pl.npt = (p.T + p.tpt - 1) / p.tpt;
     pl.plo = 0;
     Entry e = {};
-    int64_t mine = 0, at = -1;
+    int64_t mine = 0;
+    int at = -1, tiles = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 2; pass++) {
         int64_t run = 0;
@@ -315,12 +344,11 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
             pl.masked = s.masked || p.window >= 0;
             if (p.window >= 0) pl.plo = max(0, s.least - p.window) / TK * TK;
             pl.ptiles = pl.plo < pl.pmax ? (pl.pmax - pl.plo + TK - 1) / TK : 0;
-            const int64_t Wp = (int64_t)pl.ptiles * pl.npt * p.pc.KV;
-            const bool fits = Wp + run < 1ll << 31;
+            const bool fits = run < 1ll << 30;
             if (!fits && tid == 0) record_status(p.status, E2C_ERR_BAD_SEQ);
-            pl.Wp = fits ? (int)Wp : 0;
-            pl.share.set(fits ? (int)(Wp + run) : 0, gridDim.x);
-            if ((int)blockIdx.x < pl.share.blocks) at = max(0, pl.share.begin(blockIdx.x) - pl.Wp);
+            tiles = fits ? (int)run : 0;
+            pl.share.set(p.pc.KV * pl.npt, pl.ptiles, tiles, gridDim.x);
+            at = pl.share.begin(blockIdx.x);
         }
     }
     __syncthreads();
@@ -328,9 +356,8 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
     pl.first_before = s.at;
     pl.pseq = s.seq;
     if (blockIdx.x == 0 && tid == 0) {
-        p.before[p.n] = pl.Wp;
-        p.before[p.n + 1] = pl.share.W;
-        p.before[p.n + 2] = pl.ptiles;
+        p.before[p.n] = tiles;
+        p.before[p.n + 1] = pl.ptiles;
     }
 }
 
@@ -497,23 +524,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             int pos = L0, n = 0;
             bool ok = true;
             Item it = {};
-            // Publishes the part of the item of tiles [s, s + nt) that begins at pos. It goes to `whole` where it
-            // is not divided.
-            auto emit = [&](int s, int nt, int whole) {
-                const int end = s + nt;
-                it.nt = min(end, L1) - pos;
-                it.dst = whole;
-                it.slot = 0;
-                if (s < L0 || end > L1) {
-                    it.dst = TO_SLOT;
-                    it.slot = 2 * blockIdx.x + (s > L0 ? 1 : 0);
-                    // an item's second block reports it to the joining kernel
-                    const int c0 = pl.share.block(s);
-                    if (p.shared == 0 && s < L0 && c0 == (int)blockIdx.x - 1 && lane == 0) {
-                        p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, it.kvh, 2 * c0 + (s > pl.share.begin(c0) ? 1 : 0));
-                        p.split[2 * blockIdx.x + 1] = make_int4(pl.share.block(end - 1), 0, 0, 0);
-                    }
-                }
+            auto publish = [&]() {
                 const int sl = n & (NI - 1);
                 if (!(ok = wait_warp(bar(B_ITE + sl), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) return;
                 if (lane == 0) {
@@ -524,32 +535,34 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     mbar_arrive(bar(B_ITF + sl));
                 }
                 __syncwarp();
-                pos += it.nt;
                 n++;
             };
-            if (pos < pl.Wp) {
-                int q = pos / pl.ptiles, j0 = pos - q * pl.ptiles, kvh = q / pl.npt, rt = q - kvh * pl.npt;
-                it.prefix = 1;
-                it.klim = pl.pmax;
-                it.masked = pl.masked;
-                it.seq = pl.pseq;
+            // Neighbours share a run of the prefix; every other group of them begins with its sequence items, so
+            // that products (the prefix) and loads (the sequences) go on side by side.
+            const bool late = pl.share.items > 0 && (blockIdx.x / pl.npt & 1);
 #pragma unroll 1
-                for (; ok && pos < min(L1, pl.Wp); q++) {
-                    it.kvh = kvh;
-                    it.t0 = rt * p.tpt;
-                    it.ntok = min(p.tpt, p.T - it.t0);
-                    it.k0 = pl.plo + j0 * TK;
-                    j0 = 0;
-                    if (++rt == pl.npt) {
-                        rt = 0;
-                        kvh++;
+            for (int half = 0; half < 2; half++) {
+                if ((half == 1) == late) {
+                    it.prefix = 1;
+                    it.masked = pl.masked;
+                    it.seq = pl.pseq;
+                    it.dst = TO_SLOT;
+#pragma unroll 1
+                    for (int q = blockIdx.x; ok && q < pl.share.items; q += gridDim.x) {
+                        const int u = q / pl.npt, rt = q - u * pl.npt, kvh = u / pl.share.splits, s = u - kvh * pl.share.splits;
+                        it.kvh = kvh;
+                        it.t0 = rt * p.tpt;
+                        it.ntok = min(p.tpt, p.T - it.t0);
+                        it.nt = min(pl.share.chunk, pl.ptiles - s * pl.share.chunk);
+                        it.k0 = pl.plo + s * pl.share.chunk * TK;
+                        it.klim = min(pl.pmax, it.k0 + it.nt * TK);
+                        it.slot = 2 * gridDim.x + q;
+                        publish();
                     }
-                    emit(q * pl.ptiles, pl.ptiles, TO_DENSE);
+                    continue;
                 }
-            }
-            if (ok && pos < L1) {
                 // sequence entries, 32 at a time, one per lane
-                int off = pos - pl.Wp - pl.first_before, ebase = -32;  // off: tiles before pos of the entry
+                int off = pos - pl.first_before, ebase = -32;  // off: tiles before pos of the entry
                 Entry e = {};
                 int etiles = 0;
                 it.prefix = 0;
@@ -580,19 +593,35 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll 1
                     for (int r = 0; ok && pos < L1 && kvh < p.pc.KV;) {
                         int k0, klim;
-                        const int nt = span_of(p, len, nq, r, p.shared, k0, klim);
-                        if (off >= nt) {
-                            off -= nt;
+                        const int nt = span_of(p, len, nq, r, p.shared, k0, klim), cost = nt + ITEM_COST;
+                        if (off >= cost) {
+                            off -= cost;
+                        } else if (off >= nt) {  // the share begins past the item's tiles
+                            pos = min(pos + cost - off, L1);
+                            off = 0;
                         } else {
+                            const int s = pos - off, end = s + nt;
                             it.kvh = kvh;
                             it.t0 = q0 + r * p.tpt;
                             it.ntok = min(p.tpt, nq - r * p.tpt);
+                            it.nt = min(end, L1) - pos;
                             it.k0 = k0 + off * TK;
                             it.klim = klim;
                             it.pos0 = len - nq + r * p.tpt;
-                            const int s = pos - off;
+                            it.dst = p.shared > 0 ? TO_DENSE : TO_OUT;
+                            if (off > 0 || end > L1) {  // a part of an item
+                                it.dst = TO_SLOT;
+                                it.slot = 2 * blockIdx.x + (s > L0 ? 1 : 0);
+                                // an item's second block reports it to the joining kernel
+                                const int c0 = pl.share.block(s);
+                                if (p.shared == 0 && off > 0 && c0 == (int)blockIdx.x - 1 && lane == 0) {
+                                    p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, kvh, 2 * c0 + (s > pl.share.begin(c0) ? 1 : 0));
+                                    p.split[2 * blockIdx.x + 1] = make_int4(pl.share.block(end - 1), 0, 0, 0);
+                                }
+                            }
+                            publish();
+                            pos = min(s + cost, L1);
                             off = 0;
-                            emit(s, nt, p.shared > 0 ? TO_DENSE : TO_OUT);
                         }
                         if (++r * p.tpt >= nq) {
                             r = 0;
@@ -900,9 +929,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 // for the instruction cache: a row of 128 logits held in registers is straight code that does
                 // not stay in it (16 heads of 128, 4096 tokens: 443 us, against 370 with loops of 64 columns)
                 auto hide = [&](int c0, uint32_t (&s)[32]) {
+                    // bit i: column c0 + i is seen
+                    const int a = min(max(ra - c0, 0), 32), b = min(max(rb - c0, 0), 32);
+                    const uint32_t seen = (uint32_t)((1ull << b) - (1ull << a));
 #pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if ((unsigned)(c0 + i - ra) >= (unsigned)(rb - ra)) s[i] = 0xff800000u;
+                    for (int i = 0; i < 32; i++) s[i] = seen & (1u << i) ? s[i] : 0xff800000u;
                 };
                 float mx = -INFINITY;
                 if (busy) {
@@ -1003,17 +1034,19 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     tmem_wait_st();
                 }
                 if (nk & 15) {
-                    // V's rows past the last key, up to the product's 16: this group's four warps zero a
-                    // quarter of the 16-byte pieces each
+                    // V's rows past the last key, up to the product's 16: each of the group's warps zeroes panels
                     const int part = nk / C::VROWS, vt = g * C::KPARTS + part, vs = vt % C::NVS;
                     if (!wait_warp(bar(B_VF + vs), (uint32_t)((vt / C::NVS) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                         ok = false;
                         break;
                     }
-                    uint8_t *v = smem + C::V_OFF + vs * C::STAGE + (nk - part * C::VROWS) * 128;
-                    const int pieces = (16 - (nk & 15)) * 8;  // of one panel
-                    for (int x = quad * 32 + lane; x < C::PANELS * pieces; x += 128)
-                        *reinterpret_cast<uint4 *>(v + x / pieces * (C::VROWS * 128) + x % pieces * 16) = make_uint4(0, 0, 0, 0);
+                    const int pieces = (16 - (nk & 15)) * 8;  // of 16 bytes, in one panel
+#pragma unroll 1
+                    for (int panel = quad; panel < C::PANELS; panel += 4) {
+                        uint8_t *v = smem + C::V_OFF + vs * C::STAGE + panel * (C::VROWS * 128) + (nk - part * C::VROWS) * 128;
+#pragma unroll 1
+                        for (int x = lane; x < pieces; x += 32) *reinterpret_cast<uint4 *>(v + x * 16) = make_uint4(0, 0, 0, 0);
+                    }
                     fence_proxy_async_smem();
                 }
                 tc_fence_before();
@@ -1059,7 +1092,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     out = static_cast<T *>(p.out) + t * p.ldo + h * D;
                     if (live && p.lse) p.lse[t * p.H + h] = sums * LN2;
                 } else {
-                    const int64_t at = it.dst == TO_SLOT ? (int64_t)it.slot * TR + row : ((int64_t)(it.prefix ? 0 : 1) * p.T + t) * p.H + h;
+                    const int64_t at = it.dst == TO_SLOT ? (int64_t)it.slot * TR + row : t * p.H + h;
                     part = (it.dst == TO_SLOT ? p.po : p.dpo) + at * D;
                     if (live) (it.dst == TO_SLOT ? p.pl : p.dpl)[at] = sums;
                 }
@@ -1067,26 +1100,27 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             if (!wait_warp(bar(B_OF + ob), (uint32_t)((item / C::NO) & 1), p.status, E2C_ERR_WAIT_EPI)) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
+            for (int c = 0; c < D; c += 64) {
+                uint32_t o[64];
                 if (busy) {
-                    tmem_ld32(ta + (uint32_t)(C::O_COL + ob * D + c), o);
+                    const uint32_t to = ta + (uint32_t)(C::O_COL + ob * D + c);
+                    tmem_ld32_to<0>(to, o);
+                    tmem_ld32_to<32>(to + 32, o);
                     tmem_wait_ld();
                 }
-                if (c == D - 32) {  // O has been read: the next item may use it while this one is stored
+                if (c == D - 64) {  // O has been read: the next item may use it while this one is stored
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(B_OE + ob));
                 }
-                if (!busy) continue;
                 if (blank && !some) {  // such a row may have met a page's NaN: its zeros are not a product
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = 0u;
+                    for (int i = 0; i < 64; i++) o[i] = 0u;
                 }
                 if (live && out) {
                     uint4 *y = reinterpret_cast<uint4 *>(out + c);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
+                    for (int i = 0; i < 8; i++) {
                         uint4 v;
                         v.x = pack2<T>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
                         v.y = pack2<T>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
@@ -1097,7 +1131,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 } else if (live) {
                     float4 *y = reinterpret_cast<float4 *>(part + c);
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
+                    for (int i = 0; i < 16; i++)
                         y[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
                                            __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
                 }
@@ -1149,7 +1183,9 @@ __global__ void __launch_bounds__(JOIN) k_join_split(const Args p, int grid) {
     using J = Join<T, D>;
     griddep_launch_dependents();
     griddep_wait();
-    if ((int)blockIdx.x >= min(grid, p.before[p.n + 1])) return;
+    Share share;
+    share.set(1, 0, p.before[p.n], grid);
+    if (share.begin(blockIdx.x) == share.begin(blockIdx.x + 1)) return;
     const int4 a = p.split[2 * blockIdx.x];
     if (a.y == 0) return;
     const int c1 = p.split[2 * blockIdx.x + 1].x;
@@ -1173,26 +1209,14 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     const int64_t t = u / p.H;
     if (t >= p.T) return;
     const int h = (int)(u - t * p.H), kvh = h / p.G, hd = h - kvh * p.G, x = threadIdx.x % J::LANES;
-    const int Wp = p.before[p.n], ptiles = p.before[p.n + 2];
+    const int npt = (p.T + p.tpt - 1) / p.tpt;
     Share share;
-    share.set(p.before[p.n + 1], grid);
+    share.set(p.pc.KV * npt, p.before[p.n + 1], p.before[p.n], grid);
     J j;
-    auto parts = [&](int s, int end, int which, int row) {
-        const int c0 = share.block(s), c1 = share.block(end - 1);
-        if (c0 == c1) {
-            const int64_t at = ((int64_t)which * p.T + t) * p.H + h;
-            j.add(p.dpo + at * D, p.dpl[at], x);
-            return;
-        }
-        for (int c = c0; c <= c1; c++) {
-            const int slot = 2 * c + (c == c0 && s > share.begin(c0) ? 1 : 0);
-            j.add(p.po + ((int64_t)slot * TR + row) * D, p.pl[(int64_t)slot * TR + row], x);
-        }
-    };
-    if (ptiles) {
-        const int npt = (p.T + p.tpt - 1) / p.tpt, rt = (int)(t / p.tpt);
-        const int s = (kvh * npt + rt) * ptiles;
-        parts(s, s + ptiles, 0, (int)(t - (int64_t)rt * p.tpt) * p.G + hd);
+    auto slot = [&](int k, int row) { j.add(p.po + ((int64_t)k * TR + row) * D, p.pl[(int64_t)k * TR + row], x); };
+    if (share.items) {
+        const int rt = (int)(t / p.tpt), row = (int)(t - (int64_t)rt * p.tpt) * p.G + hd;
+        for (int s = 0; s < share.splits; s++) slot(2 * grid + (kvh * share.splits + s) * npt + rt, row);
     }
     int last;
     const int i = e2c_token_seq(p.q_start, p.n, p.T, (int)t, last);
@@ -1202,8 +1226,13 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     // an entry has one row tile here
     int k0, klim;
     const int nt = span_of(p, e.len, e.nq, 0, p.shared, k0, klim);
-    const int s = Wp + p.before[i] + kvh * nt;
-    parts(s, s + nt, 1, (int)(t - e.q0) * p.G + hd);
+    const int s = p.before[i] + kvh * (nt + ITEM_COST), c0 = share.block(s), c1 = share.block(s + nt - 1);
+    if (c0 == c1) {
+        j.add(p.dpo + (t * p.H + h) * D, p.dpl[t * p.H + h], x);
+    } else {
+        const int row = (int)(t - e.q0) * p.G + hd;
+        for (int c = c0; c <= c1; c++) slot(2 * c + (c == c0 && s > share.begin(c0) ? 1 : 0), row);
+    }
     j.put(p, t, h, x);
 }
 
@@ -1214,7 +1243,7 @@ bool use_prefix(int max_q, int G, int shared) { return shared > 0 && 2 * max_q *
 struct Layout {
     size_t split, before, po, pl, dpo, dpl, bytes;
 };
-Layout layout(int blocks, int n, int T, int H, int D, bool prefix) {
+Layout layout(int blocks, int n, int T, int H, int KV, int D, bool prefix) {
     Layout l;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -1222,12 +1251,15 @@ Layout layout(int blocks, int n, int T, int H, int D, bool prefix) {
         at += (bytes + 255) & ~(size_t)255;
         return here;
     };
+    // a prefix has at most one item a block, or one for each row tile of each key head if those are more
+    const size_t tpt = TR / (H / KV), rows = KV * ((T + tpt - 1) / tpt);
+    const size_t slots = 2 * (size_t)blocks + (prefix ? (rows > (size_t)blocks ? rows : (size_t)blocks) : 0);
     l.split = take(sizeof(int4) * 2 * blocks);
-    l.before = take(sizeof(int) * ((size_t)n + 3));
-    l.pl = take(sizeof(float) * 2 * blocks * TR);
-    l.po = take(sizeof(float) * 2 * blocks * TR * D);
-    l.dpl = take(prefix ? sizeof(float) * 2 * (size_t)T * H : 0);
-    l.dpo = take(prefix ? sizeof(float) * 2 * (size_t)T * H * D : 0);
+    l.before = take(sizeof(int) * ((size_t)n + 2));
+    l.pl = take(sizeof(float) * slots * TR);
+    l.po = take(sizeof(float) * slots * TR * D);
+    l.dpl = take(prefix ? sizeof(float) * (size_t)T * H : 0);
+    l.dpo = take(prefix ? sizeof(float) * (size_t)T * H * D : 0);
     l.bytes = at;
     return l;
 }
@@ -1277,7 +1309,7 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
 
 extern "C" size_t e2c_pages_attention_ws_bytes(int n, int T, int max_q, int H, int KV, int D, int shared) {
     const int sms = e2c_sm_count(e2c_device());
-    return sms ? layout(sms, n, T, H, D, use_prefix(max_q, H / KV, shared)).bytes : 0;
+    return sms ? layout(sms, n, T, H, KV, D, use_prefix(max_q, H / KV, shared)).bytes : 0;
 }
 
 extern "C" int e2c_pages_attention(const e2c_pages *pc, const void *q, int64_t ldq, const int32_t *seqs, const int32_t *q_start, int n,
@@ -1290,7 +1322,7 @@ extern "C" int e2c_pages_attention(const e2c_pages *pc, const void *q, int64_t l
     }
     const int G = H / pc->KV;
     const bool prefix = use_prefix(max_q, G, shared);
-    const Layout l = layout(sms, n, T, H, pc->D, prefix);
+    const Layout l = layout(sms, n, T, H, pc->KV, pc->D, prefix);
     if (ws_bytes < l.bytes) {
         e2c_set_msg("pages_attention: workspace");
         return -1;
