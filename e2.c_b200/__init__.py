@@ -218,12 +218,18 @@ def _ok(rc: int, what: str) -> None:
         raise E2CudaError(f"{what}: {last_error()}")
 
 
-def _torch():
-    import torch
+_torch_mod = None
 
-    if not torch.cuda.is_available():
-        raise E2CudaError("no CUDA device: the e2cuda ops have no CPU path")
-    return torch
+
+def _torch():
+    global _torch_mod
+    if _torch_mod is None:
+        import torch
+
+        if not torch.cuda.is_available():
+            raise E2CudaError("no CUDA device: the e2cuda ops have no CPU path")
+        _torch_mod = torch
+    return _torch_mod
 
 
 def _ptr(t) -> int:
@@ -232,8 +238,10 @@ def _ptr(t) -> int:
 
 def _stream(stream) -> int | None:
     torch = _torch()
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    if stream is not None:
+        return stream.cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without a Stream object (3 us a call)
+    return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
 
 
 def check(stream=None) -> None:
@@ -368,14 +376,17 @@ def _type(t) -> int:
 def _rows(t, what: str) -> int:
     """Elements between the rows of a [rows][heads][head_dim] tensor whose heads lie side by side."""
     s = t.stride()
-    if len(s) != 3 or (s[2] != 1 and t.shape[2] > 1) or (s[1] != t.shape[2] and t.shape[1] > 1):
+    if len(s) != 3:
+        raise E2CudaError(f"{what}: [rows][heads][head_dim], got {tuple(t.shape)}")
+    rows, heads, dim = t.shape
+    if (s[2] != 1 and dim > 1) or (s[1] != dim and heads > 1):
         raise E2CudaError(f"{what}: [rows][heads][head_dim] with the heads of a row side by side, got strides {tuple(s)}")
-    return s[0] if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return s[0] if rows > 1 else heads * dim
 
 
 def _ints(t, count: int, what: str) -> int:
     """The address of a device int32 list of `count` entries."""
-    if t.dtype != _torch().int32 or t.dim() != 1 or t.shape[0] != count or not t.is_cuda or (count > 1 and t.stride(0) != 1):
+    if t.dtype is not _torch().int32 or t.shape != (count,) or not t.is_cuda or not t.is_contiguous():
         raise E2CudaError(f"{what}: a contiguous device int32 list of {count}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
@@ -408,7 +419,7 @@ def rope(x, cos, sin, pos=None, interleaved: bool = False, backward: bool = Fals
     T, H, D = x.shape
     positions, rot = _table(cos, sin)
     if out is None:
-        out = torch.empty((T, H, D), dtype=dtype or x.dtype, device=x.device)
+        out = torch.empty_like(x) if dtype is None and x.is_contiguous() else x.new_empty((T, H, D), dtype=dtype or x.dtype)
     elif out.shape != x.shape:
         raise E2CudaError(f"rope: out {tuple(out.shape)} for x {tuple(x.shape)}")
     _ok(lib().e2cuda_rope(x.data_ptr(), _rows(x, "rope"), _type(x), out.data_ptr(), _rows(out, "rope out"), _type(out),
@@ -436,7 +447,8 @@ class PageCache:
         self.k, self.v, self.table, self.length, self.refs = k, v, table, length, refs
         layers, n_pages, page, kv, dim = k.shape
         self.ws = torch.empty(lib().e2cuda_pages_ws_bytes(n_pages, length.shape[0]) // 4, dtype=torch.int32, device=k.device)
-        self._scratch: dict = {}  # the attention's, by stream
+        self._scratch: dict = {}  # the attention's workspace and its size, by stream
+        self._needs: dict = {}    # workspace bytes by batch
         self.pages = Pages(k.data_ptr(), v.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.ws.data_ptr(),
                            _type(k), layers, n_pages, page, kv, dim, table.shape[0], table.shape[1])
         self._p = C.addressof(self.pages)
@@ -505,20 +517,27 @@ class PageCache:
         if D != p.head_dim or q.dtype != self.k.dtype:
             raise E2CudaError(f"attention: q {tuple(q.shape)} {q.dtype} for a cache of heads of {p.head_dim} {self.k.dtype}")
         if out is None:
-            out = q.new_empty((T, H, D))
+            out = _torch().empty_like(q) if q.is_contiguous() else q.new_empty((T, H, D))
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise E2CudaError(f"attention: out {tuple(out.shape)} {out.dtype}")
         sums = q.new_empty((T, H), dtype=_torch().float32) if lse else None
         st = _stream(stream)
-        need = lib().e2cuda_pages_attention_ws_bytes(self._p, n, T, max_q, H, shared)
-        ws = self._scratch.get(st)
-        if ws is None or ws.numel() < need:
+        batch = (n, T, max_q, H, shared)
+        need = self._needs.get(batch)
+        if need is None:
+            if len(self._needs) > 4096:
+                self._needs.clear()
+            need = self._needs[batch] = lib().e2cuda_pages_attention_ws_bytes(self._p, *batch)
+        ws, size = self._scratch.get(st, (None, 0))
+        if size < need or ws is None:
+            size = max(need, 16)
             with _torch().cuda.stream(stream):  # its memory is reused in that stream's order
-                ws = self._scratch[st] = q.new_empty(max(need, 16), dtype=_torch().uint8)
+                ws = q.new_empty(size, dtype=_torch().uint8)
+            self._scratch[st] = ws, size
         _ok(lib().e2cuda_pages_attention(self._p, layer, q.data_ptr(), _rows(q, "attention q"), _ints(seqs, n, "attention seqs"),
                                          _ints(q_start, n + 1, "attention q_start"), n, T, max_q, H, shared, causal, window,
                                          1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(),
-                                         _rows(out, "attention out"), _ptr(sums), ws.data_ptr(), ws.numel(), st), "attention")
+                                         _rows(out, "attention out"), _ptr(sums), ws.data_ptr(), size, st), "attention")
         return (out, sums) if lse else out
 
 

@@ -49,6 +49,7 @@ constexpr int NTHREADS = 32 * WARPS;
 constexpr int NI = 8;  // item descriptors in flight
 // What a sequence item costs beside its tiles, in tiles: its set-up and its output
 constexpr int ITEM_COST = 1;
+constexpr int PREFIX_TILES = 13;
 constexpr float kRescaleLog2 = 8.0f;
 
 // A wait of a whole warp, bounded by its number of (sleeping) tries: up to 1.3 s. It is small on
@@ -1036,6 +1037,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 if (nk & 15) {
                     // V's rows past the last key, up to the product's 16: each of the group's warps zeroes panels
                     const int part = nk / C::VROWS, vt = g * C::KPARTS + part, vs = vt % C::NVS;
+                    // Parities tell only neighbouring phases apart: the stage's load before this one, of tile
+                    // g - BACK, must be known to have landed. S(g) says so of tile g - NS; for a shorter ring its
+                    // product is waited for.
+                    constexpr int BACK = C::NVS / C::KPARTS;
+                    if (BACK < C::NS && g >= BACK &&
+                        !wait_warp(bar(B_PV + ((g - BACK) & 1)), (uint32_t)(((g - BACK) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                        ok = false;
+                        break;
+                    }
                     if (!wait_warp(bar(B_VF + vs), (uint32_t)((vt / C::NVS) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                         ok = false;
                         break;
@@ -1236,9 +1246,15 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     j.put(p, t, h, x);
 }
 
-// Sequences of few query tokens fill a small part of a 128-row tile each; packed, the batch reads the
-// prefix once per 128 rows instead of once per sequence. From half a tile on they gain nothing.
-bool use_prefix(int max_q, int G, int shared) { return shared > 0 && 2 * max_q * G <= TR; }
+// Sequences of few query tokens fill a small part of a 128-row tile each; packed, the batch reads the prefix
+// once per 128 rows instead of once per sequence. From half a tile on they gain nothing, and where
+// all sequences' own passes over the prefix are a dozen tiles a block, joining two parts of every row
+// costs more than it saves (8 key heads of 128, 300 tokens past the prefix, us a call, packed and not: 16
+// sequences behind 1024 tokens, 6.5 tiles a block, 28.4 and 23.8; 32 behind 1024, 13.4 tiles, 31.2 and 32.7;
+// 64 behind 512, 13.6 tiles, 35.2 and 38.5).
+bool use_prefix(int n, int max_q, int KV, int G, int shared, int sms) {
+    return shared > 0 && 2 * max_q * G <= TR && (int64_t)(n - 1) * KV * ((shared + TK - 1) / TK) > PREFIX_TILES * sms;
+}
 
 struct Layout {
     size_t split, before, po, pl, dpo, dpl, bytes;
@@ -1291,11 +1307,12 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
     const uint32_t box = a.pc.page < C::VROWS ? a.pc.page : C::VROWS;
     CUtensorMap tq, tqp, tk, tv;
     if (e2c_tmap_3d(&tq, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, q_box) ||
-        e2c_tmap_3d(&tqp, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, qp_box) ||
+        (prefix && e2c_tmap_3d(&tqp, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, qp_box)) ||
         e2c_tmap_2d(&tk, a.pc.k, dt, 2, width, rows, width * 2, 64, box) ||
         e2c_tmap_2d(&tv, a.pc.v, dt, 2, width, rows, width * 2, 64, box))
         return -3;
-    e2c_launch(k_attention_pages<T, D>, dim3(sms), dim3(NTHREADS), smem_bytes<D>(), st, tq, tqp, tk, tv, a, q_box, qp_box);
+    if (!prefix) tqp = tq;
+    e2c_launch_as(true, k_attention_pages<T, D>, dim3(sms), dim3(NTHREADS), smem_bytes<D>(), st, tq, tqp, tk, tv, a, q_box, qp_box);
     if (launch_error("pages_attention")) return -2;
     using J = Join<T, D>;
     if (prefix)
@@ -1309,7 +1326,7 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
 
 extern "C" size_t e2c_pages_attention_ws_bytes(int n, int T, int max_q, int H, int KV, int D, int shared) {
     const int sms = e2c_sm_count(e2c_device());
-    return sms ? layout(sms, n, T, H, KV, D, use_prefix(max_q, H / KV, shared)).bytes : 0;
+    return sms ? layout(sms, n, T, H, KV, D, use_prefix(n, max_q, KV, H / KV, shared, sms)).bytes : 0;
 }
 
 extern "C" int e2c_pages_attention(const e2c_pages *pc, const void *q, int64_t ldq, const int32_t *seqs, const int32_t *q_start, int n,
@@ -1321,7 +1338,7 @@ extern "C" int e2c_pages_attention(const e2c_pages *pc, const void *q, int64_t l
         return -2;
     }
     const int G = H / pc->KV;
-    const bool prefix = use_prefix(max_q, G, shared);
+    const bool prefix = use_prefix(n, max_q, pc->KV, G, shared, sms);
     const Layout l = layout(sms, n, T, H, pc->KV, pc->D, prefix);
     if (ws_bytes < l.bytes) {
         e2c_set_msg("pages_attention: workspace");

@@ -319,7 +319,7 @@ int move_pages(const e2c_pages *pc, const int32_t *src, const int32_t *dst, int 
     const int pieces = (vecs + (UNROLL << shift) - 1) / (UNROLL << shift);
     const int64_t blocks = ((int64_t)n * 2 * pc->layers * pieces * (1 << shift) + 255) / 256;
     const unsigned grid = (unsigned)(blocks < (int64_t)sms * 8 ? blocks : (int64_t)sms * 8);
-    e2c_launch(k_move, dim3(grid), dim3(256), 0, (cudaStream_t)stream, *pc, src, dst, n, count, vecs, pieces, shift,
+    e2c_launch_as(true, k_move, dim3(grid), dim3(256), 0, (cudaStream_t)stream, *pc, src, dst, n, count, vecs, pieces, shift,
                status);
     return launched(what);
 }
@@ -338,27 +338,27 @@ extern "C" int e2c_pages_copy(const e2c_pages *pc, const int32_t *src, const int
 
 extern "C" int e2c_pages_fork(const e2c_pages *pc, const int32_t *parents, const int32_t *children, int n, int *status, void *stream) {
     if (n <= 0) return 0;
-    e2c_launch(k_fork, dim3(n), dim3(256), 0, (cudaStream_t)stream, *pc, parents, children, status);
+    e2c_launch_as(true, k_fork, dim3(n), dim3(256), 0, (cudaStream_t)stream, *pc, parents, children, status);
     return launched("pages_fork");
 }
 
 extern "C" int e2c_pages_append(const e2c_pages *pc, const int32_t *seqs, const int32_t *counts, int n, int *status, void *stream) {
     if (n <= 0) return 0;
-    e2c_launch(k_append, dim3(1), dim3(PLAN), 0, (cudaStream_t)stream, *pc, seqs, counts, n, status);
+    e2c_launch_as(true, k_append, dim3(1), dim3(PLAN), 0, (cudaStream_t)stream, *pc, seqs, counts, n, status);
     if (launched("pages_append")) return -2;
     return move_pages(pc, ws_at(pc, pc->max_seqs), ws_at(pc, 2 * (int64_t)pc->max_seqs), n, nullptr, status, stream, "pages_append");
 }
 
 extern "C" int e2c_pages_free(const e2c_pages *pc, const int32_t *seqs, int n, int *status, void *stream) {
     if (n <= 0) return 0;
-    e2c_launch(k_free, dim3(n), dim3(256), 0, (cudaStream_t)stream, *pc, seqs, status);
+    e2c_launch_as(true, k_free, dim3(n), dim3(256), 0, (cudaStream_t)stream, *pc, seqs, status);
     return launched("pages_free");
 }
 
 extern "C" int e2c_pages_compact(const e2c_pages *pc, int32_t *used, int *status, void *stream) {
-    e2c_launch(k_compact, dim3(1), dim3(PLAN), 0, (cudaStream_t)stream, *pc, used);
+    e2c_launch_as(true, k_compact, dim3(1), dim3(PLAN), 0, (cudaStream_t)stream, *pc, used);
     if (launched("pages_compact")) return -2;
-    e2c_launch(k_remap, dim3(pc->max_seqs), dim3(256), 0, (cudaStream_t)stream, *pc);
+    e2c_launch_as(true, k_remap, dim3(pc->max_seqs), dim3(256), 0, (cudaStream_t)stream, *pc);
     if (launched("pages_compact")) return -2;
     const int64_t list = 3 * (int64_t)pc->max_seqs;
     return move_pages(pc, ws_at(pc, list + pc->n_pages), ws_at(pc, list), pc->n_pages / 2 + 1, pc->ws + W_MOVES, status, stream,

@@ -8,7 +8,8 @@
 // order unless E2C_PDL=1 is set in the environment. The GEMMs for a few rows against a short weight
 // are the exception: there the attribute lets the next GEMM's CTAs become resident and fetch their
 // weight while the previous one finishes, which a chain of such launches gains 20-25% from; they
-// carry it unless E2C_PDL_SMALL=0.
+// carry it unless E2C_PDL_SMALL=0. So do the prompt cache's kernels (rope.cu, pages.cu,
+// attention_pages.cu), which a decode step runs in short chains.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdlib.h>
@@ -25,7 +26,8 @@ inline bool e2c_pdl_on() {
     return on != 0;
 }
 
-// the co-resident small-row GEMMs launch with the attribute (E2C_PDL_SMALL=0: only with E2C_PDL=1)
+// the co-resident small-row GEMMs and the prompt cache's kernels launch with the attribute
+// (E2C_PDL_SMALL=0: only with E2C_PDL=1)
 inline bool e2c_pdl_small_on() {
     static int on = -1;
     if (on < 0) {

@@ -16,6 +16,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "launch.h"
 #include "pages.cuh"
 #include "pdl.h"
@@ -88,6 +90,32 @@ E2C_DEV void store(T *p, const float (&r)[N]) {
     }
 }
 
+// N values from x to y: as they are where the types are the same
+template <typename TI, typename TO, int N>
+struct Copy {
+    float f[N];
+    uint4 w[N * sizeof(TI) / 16 ? N * sizeof(TI) / 16 : 1];
+    static constexpr bool raw = std::is_same<TI, TO>::value && N > 1;
+    E2C_DEV void get(const TI *x) {
+        if constexpr (raw)
+            w[0] = *reinterpret_cast<const uint4 *>(x);
+        else
+            load<TI, N>(x, f);
+    }
+    E2C_DEV void put(TO *y) const {
+        if constexpr (raw)
+            *reinterpret_cast<uint4 *>(y) = w[0];
+        else
+            store<TO, N>(y, f);
+    }
+};
+
+// u / d for u < 2^31 by a multiplication
+struct Div {
+    uint32_t d, mul, shift;
+};
+E2C_DEV uint32_t div_by(uint32_t u, const Div &v) { return v.d == 1 ? u : (uint32_t)(__umulhi(u, v.mul) >> v.shift); }
+
 // V pairs of one head: the raw values at the two places, and the rotation
 template <typename TI, typename TO, int V>
 struct Pairs {
@@ -147,16 +175,16 @@ struct RopeArgs {
     int *status;
 };
 
-// one thread: rotation unit j (V pairs, or V pass-through elements past them) of heads 4 hg .. 4 hg + 3
+// One thread: unit j of heads 4 hg .. 4 hg + 3, of V pairs, or past them of 2 V elements passed through
 template <typename TI, typename TO, int V>
-__global__ void __launch_bounds__(BLOCK) k_rope(const RopeArgs p, int units, int hgroups) {
+__global__ void __launch_bounds__(BLOCK) k_rope(const RopeArgs p, const Div per_token, const Div units) {
     griddep_launch_dependents();
     griddep_wait();
-    const int64_t u = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
-    const int t = (int)(u / (units * hgroups));
+    const uint32_t u = blockIdx.x * BLOCK + threadIdx.x;
+    const int t = (int)div_by(u, per_token);
     if (t >= p.T) return;
-    const int rem = (int)(u - (int64_t)t * (units * hgroups));
-    const int hg = rem / units, j = rem - hg * units;
+    const uint32_t rem = u - t * per_token.d;
+    const int hg = (int)div_by(rem, units), j = (int)(rem - hg * units.d);
     const int h0 = hg * HPT, nh = min(HPT, p.H - h0);
     const TI *x = static_cast<const TI *>(p.x) + t * p.ldx + (int64_t)h0 * p.D;
     TO *y = static_cast<TO *>(p.y) + t * p.ldy + (int64_t)h0 * p.D;
@@ -180,14 +208,21 @@ __global__ void __launch_bounds__(BLOCK) k_rope(const RopeArgs p, int units, int
         for (int h = 0; h < HPT; h++)
             if (h < nh) r[h].put(y + h * p.D, j, p.half, p.inter, c, s);
     } else {
-        const int e = 2 * p.half + (j - nrot) * V;
-        float a[HPT][V];
+        const int e = 2 * p.half + (j - nrot) * 2 * V;
+        const bool two = e + V < p.D;
+        Copy<TI, TO, V> a[HPT], b[HPT];
 #pragma unroll
         for (int h = 0; h < HPT; h++)
-            if (h < nh) load<TI, V>(x + h * p.D + e, a[h]);
+            if (h < nh) {
+                a[h].get(x + h * p.D + e);
+                if (two) b[h].get(x + h * p.D + e + V);
+            }
 #pragma unroll
         for (int h = 0; h < HPT; h++)
-            if (h < nh) store<TO, V>(y + h * p.D + e, a[h]);
+            if (h < nh) {
+                a[h].put(y + h * p.D + e);
+                if (two) b[h].put(y + h * p.D + e + V);
+            }
     }
 }
 
@@ -208,19 +243,18 @@ struct StoreArgs {
 // key heads (rotated) and KV value heads (passed through). The input loads are issued before the
 // chain of lookups (token -> sequence -> length -> page) that the stores wait for.
 template <typename TI, typename TO, int V>
-__global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, int units, int qgroups, int kgroups, int vunits) {
+__global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, const Div per_token, const Div units, const Div vunits, int qgroups, int kgroups) {
     griddep_launch_dependents();
     griddep_wait();
-    const int rot_units = units * (qgroups + kgroups), per_token = rot_units + vunits * kgroups;
-    const int64_t u = (int64_t)blockIdx.x * BLOCK + threadIdx.x;
-    const int t = (int)(u / per_token);
+    const uint32_t u = blockIdx.x * BLOCK + threadIdx.x;
+    const int t = (int)div_by(u, per_token);
     if (t >= p.T) return;
-    const int rem = (int)(u - (int64_t)t * per_token);
+    const uint32_t rem = u - t * per_token.d, rot_units = units.d * (qgroups + kgroups);
     const int D = p.pc.D, KV = p.pc.KV;
     const bool is_v = rem >= rot_units;
-    const int r2 = is_v ? rem - rot_units : rem, per = is_v ? vunits : units;
-    int hg = r2 / per;
-    const int j = r2 - hg * per;
+    const uint32_t r2 = is_v ? rem - rot_units : rem;
+    int hg = (int)div_by(r2, is_v ? vunits : units);
+    const int j = (int)(r2 - hg * (is_v ? vunits.d : units.d));
     const bool is_q = !is_v && hg < qgroups;
     if (!is_v && !is_q) hg -= qgroups;
     const int h0 = hg * HPT, nh = min(HPT, (is_q ? p.H : KV) - h0);
@@ -229,15 +263,18 @@ __global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, int un
     x += (int64_t)h0 * D;
     const int nrot = p.half / V;
     const bool turn = !is_v && j < nrot;
-    const int e = is_v ? j * V : 2 * p.half + (j - nrot) * V;  // the first element passed through
+    const int e = is_v ? j * 2 * V : 2 * p.half + (j - nrot) * 2 * V;  // the first element passed through
+    const bool two = e + V < D;
     Pairs<TI, TO, V> r[HPT];
 #pragma unroll
     for (int h = 0; h < HPT; h++)
         if (h < nh) {
-            if (turn)
+            if (turn) {
                 r[h].get(x + h * D, j, p.half, p.inter);
-            else
+            } else {
                 load<TI, V>(x + h * D + e, r[h].a);
+                if (two) load<TI, V>(x + h * D + e + V, r[h].b);
+            }
         }
     int last;
     const int i = e2c_token_seq(p.q_start, p.n, p.T, t, last);
@@ -273,7 +310,10 @@ __global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, int un
     } else {
 #pragma unroll
         for (int h = 0; h < HPT; h++)
-            if (h < nh) store<TO, V>(y + h * D + e, r[h].a);
+            if (h < nh) {
+                store<TO, V>(y + h * D + e, r[h].a);
+                if (two) store<TO, V>(y + h * D + e + V, r[h].b);
+            }
     }
 }
 
@@ -303,24 +343,33 @@ int launched(const char *what) {
     return -2;
 }
 
+Div divide_by(int d) {
+    int s = 0;
+    while ((1ll << s) < d) s++;
+    // ceil(2^(31 + s) / d) < 2^32: right for every u < 2^31
+    return {(uint32_t)d, (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), (uint32_t)(s ? s - 1 : 0)};
+}
+
 bool fits16(const void *p, int64_t ld, int bytes) { return ((uintptr_t)p & 15) == 0 && (ld * bytes) % 16 == 0; }
 
 template <typename TI, typename TO>
 int rope_as(const RopeArgs &a, bool vec, cudaStream_t st) {
     constexpr int VV = 16 / sizeof(TO);
     const int V = vec ? VV : 1;
-    const int units = a.half / V + (a.copy_rest ? (a.D - 2 * a.half) / V : 0), hgroups = (a.H + HPT - 1) / HPT;
+    const int rest = a.copy_rest ? (a.D - 2 * a.half) / V : 0;
+    const int units = a.half / V + (rest + 1) / 2, hgroups = (a.H + HPT - 1) / HPT;
     const int64_t total = (int64_t)a.T * units * hgroups;
     if (total == 0) return 0;
     const int64_t blocks = (total + BLOCK - 1) / BLOCK;
-    if (blocks > 0x7fffffff) {
-        e2c_set_msg("rope: too many tokens for one call");
+    if (total > 0x7fffffff - BLOCK) {
+        e2c_set_msg("rope: %d tokens of %d heads are too many for one call", a.T, a.H);
         return -1;
     }
+    const Div per = divide_by(units * hgroups), by = divide_by(units);
     if (vec)
-        e2c_launch(k_rope<TI, TO, VV>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, hgroups);
+        e2c_launch_as(true, k_rope<TI, TO, VV>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, per, by);
     else
-        e2c_launch(k_rope<TI, TO, 1>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, hgroups);
+        e2c_launch_as(true, k_rope<TI, TO, 1>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, per, by);
     return launched("rope");
 }
 
@@ -328,17 +377,18 @@ template <typename TI, typename TO>
 int store_as(const StoreArgs &a, bool vec, cudaStream_t st) {
     constexpr int VV = 16 / sizeof(TO);
     const int V = vec ? VV : 1, D = a.pc.D;
-    const int units = a.half / V + (D - 2 * a.half) / V, vunits = D / V;
-    const int qg = (a.H + HPT - 1) / HPT, kg = (a.pc.KV + HPT - 1) / HPT;
-    const int64_t blocks = ((int64_t)a.T * (units * (qg + kg) + vunits * kg) + BLOCK - 1) / BLOCK;
-    if (blocks > 0x7fffffff) {
-        e2c_set_msg("pages_store: too many tokens for one call");
+    const int units = a.half / V + ((D - 2 * a.half) / V + 1) / 2, vunits = (D / V + 1) / 2;
+    const int qg = (a.H + HPT - 1) / HPT, kg = (a.pc.KV + HPT - 1) / HPT, per_token = units * (qg + kg) + vunits * kg;
+    const int64_t total = (int64_t)a.T * per_token, blocks = (total + BLOCK - 1) / BLOCK;
+    if (total > 0x7fffffff - BLOCK) {
+        e2c_set_msg("pages_store: %d tokens of %d heads are too many for one call", a.T, a.H);
         return -1;
     }
+    const Div per = divide_by(per_token), by = divide_by(units), vby = divide_by(vunits);
     if (vec)
-        e2c_launch(k_pages_store<TI, TO, VV>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, qg, kg, vunits);
+        e2c_launch_as(true, k_pages_store<TI, TO, VV>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, per, by, vby, qg, kg);
     else
-        e2c_launch(k_pages_store<TI, TO, 1>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, units, qg, kg, vunits);
+        e2c_launch_as(true, k_pages_store<TI, TO, 1>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, a, per, by, vby, qg, kg);
     return launched("pages_store");
 }
 
@@ -348,7 +398,7 @@ extern "C" int e2c_rope_table(float *cs, float *sn, int positions, int half, con
     Freqs fr;
     for (int i = 0; i < half; i++) fr.f[i] = freq[i];
     const int64_t total = (int64_t)positions * half;
-    e2c_launch(k_rope_table, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, cs, sn, total, half, fr,
+    e2c_launch_as(true, k_rope_table, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (cudaStream_t)stream, cs, sn, total, half, fr,
                gain);
     return launched("rope_table");
 }

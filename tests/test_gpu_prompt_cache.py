@@ -469,6 +469,16 @@ CASES = {
     "group of 48": ([513, 40], [4, 9], 0, 96, 2, 128, 8),
     "one key head each": ([600], [600], 0, 12, 12, 64, 256),
     "large pages": ([1500, 1024, 2048], [5, 1, 64], 1024, 4, 2, 64, 1024),
+    # as many sequences as make the shared tokens worth one pass for the batch
+    "packed prefix": ([640 + 3 * (i % 90) for i in range(220)], [1 + i % 3 for i in range(220)], 640, 4, 2, 256, 32),
+    "packed prefix, heads of 128": ([512 + (7 * i) % 130 for i in range(160)], [1 + (i % 5 == 0) for i in range(160)], 512, 10, 5, 128, 16),
+    "packed prefix, small heads": ([1024 + i for i in range(70)], [2] * 70, 1024, 8, 4, 64, 128),
+    "packed prefix, more row tiles than blocks": ([256 + i % 9 for i in range(500)], [1] * 500, 256, 64, 8, 64, 64),
+    "packed prefix, shorter sequences": ([384, 100, 0, 390] * 90, [1] * 360, 384, 4, 2, 128, 128),
+    "packed prefix, queries reach into it": ([640 + i % 4 for i in range(200)], [6] * 200, 640, 4, 2, 128, 64),
+    "one item a block": ([33] * 150, [1] * 150, 0, 8, 2, 256, 32),
+    "short tails, heads of 128": ([1 + (i * 11) % 300 for i in range(190)], [1 + i % 2 for i in range(190)], 0, 8, 2, 128, 8),
+    "short tails, heads of 256": ([1 + (i * 13) % 400 for i in range(140)], [1 + i % 3 for i in range(140)], 0, 4, 2, 256, 16),
     "many sequences": ([1 + (i * 37) % 90 for i in range(700)], [1] * 700, 0, 2, 1, 64, 8),
 }
 
