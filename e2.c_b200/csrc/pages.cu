@@ -290,10 +290,10 @@ __global__ void __launch_bounds__(256) k_move(const e2c_pages p, const int32_t *
         uint4 r[UNROLL];
 #pragma unroll
         for (int j = 0; j < UNROLL; j++)
-            if (v0 + width * j < vecs) r[j] = __ldcs(a + v0 + width * j);
+            if (v0 + width * j < vecs) r[j] = a[v0 + width * j];
 #pragma unroll
         for (int j = 0; j < UNROLL; j++)
-            if (v0 + width * j < vecs) __stcs(b + v0 + width * j, r[j]);
+            if (v0 + width * j < vecs) b[v0 + width * j] = r[j];
     }
 }
 
@@ -318,7 +318,11 @@ int move_pages(const e2c_pages *pc, const int32_t *src, const int32_t *dst, int 
     while (shift < 8 && (UNROLL << shift) < vecs) shift++;
     const int pieces = (vecs + (UNROLL << shift) - 1) / (UNROLL << shift);
     const int64_t blocks = ((int64_t)n * 2 * pc->layers * pieces * (1 << shift) + 255) / 256;
-    const unsigned grid = (unsigned)(blocks < (int64_t)sms * 8 ? blocks : (int64_t)sms * 8);
+    // A block a piece where the host knows how many there are (1021 pages of 16 layers, 32 KB a run: 326 us,
+    // the rate of a plain copy; 373 us with 8 blocks an SM that go round); where only the device does,
+    // enough of them that go round.
+    const int64_t most = (int64_t)sms * (count ? 64 : 1 << 20);
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
     e2c_launch_as(true, k_move, dim3(grid), dim3(256), 0, (cudaStream_t)stream, *pc, src, dst, n, count, vecs, pieces, shift,
                status);
     return launched(what);

@@ -681,3 +681,20 @@ def test_fork_append_store_attend_in_a_graph_and_on_another_stream(e2c, torch_cu
         got = torch.stack([w[b] for w in want])
         assert_attention(torch, got, None, [r[prompt:] for r in ref], "bf16", prompt + steps)
         alone.free(dev([0]))
+
+
+def test_example_shared_and_recomputed_agree(e2c, torch_cuda):
+    """The example's two ways to the same embeddings. Both round activations to int8 and attention operands to
+    bf16; the difference is bf16's in attention (2^-8 of a row) carried through two layers, far below
+    the 1e-3 asked of the cosine."""
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parent.parent / "examples" / "prompt_cache.py"
+    spec = importlib.util.spec_from_file_location("prompt_cache_example", path)
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    for texts, instruction, text in ((5, 70, 9), (90, 1030, 12)):
+        one, other, _ = ex.embed(e2c, texts, instruction, text, 2)
+        assert torch_cuda.isfinite(one).all()
+        assert (one * other).sum(1).min().item() > 0.999
