@@ -929,12 +929,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 // The columns are read twice, for the maximum and for the exponentials, in loops short enough
                 // for the instruction cache: a row of 128 logits held in registers is straight code that does
                 // not stay in it (16 heads of 128, 4096 tokens: 443 us, against 370 with loops of 64 columns)
-                auto hide = [&](int c0, uint32_t (&s)[32]) {
+                auto hide = [&](int c0, uint32_t (&s)[16]) {
                     // bit i: column c0 + i is seen
-                    const int a = min(max(ra - c0, 0), 32), b = min(max(rb - c0, 0), 32);
-                    const uint32_t seen = (uint32_t)((1ull << b) - (1ull << a));
+                    const int a = min(max(ra - c0, 0), 16), b = min(max(rb - c0, 0), 16);
+                    const uint32_t seen = (1u << b) - (1u << a);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) s[i] = seen & (1u << i) ? s[i] : 0xff800000u;
+                    for (int i = 0; i < 16; i++) s[i] = seen & (1u << i) ? s[i] : 0xff800000u;
                 };
                 float mx = -INFINITY;
                 if (busy) {
@@ -950,13 +950,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                         }
                     } else {
 #pragma unroll 1
-                        for (int c0 = 0; c0 < nk; c0 += 32) {
-                            uint32_t s[32];
-                            tmem_ld32(ts + c0, s);
+                        for (int c0 = 0; c0 < nk; c0 += 16) {
+                            uint32_t s[16];
+                            tmem_ld16(ts + c0, s);
                             tmem_wait_ld();
                             hide(c0, s);
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                            for (int i = 0; i < 16; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
                     }
                     mx = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])) * p.c;
@@ -1015,19 +1015,19 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                         }
                     } else {
 #pragma unroll 1
-                        for (int c0 = 0; c0 < nk; c0 += 32) {
-                            uint32_t s[32], pk[16];
-                            tmem_ld32(ts + c0, s);
+                        for (int c0 = 0; c0 < nk; c0 += 16) {
+                            uint32_t s[16], pk[8];
+                            tmem_ld16(ts + c0, s);
                             tmem_wait_ld();
                             hide(c0, s);
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
+                            for (int i = 0; i < 8; i++) {
                                 float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, mm);
                                 x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
                                 pk[i] = pack2<T>(x.x, x.y);
                             }
-                            tmem_st16(ts + c0 / 2, pk);
+                            tmem_st8(ts + c0 / 2, pk);
                         }
                     }
                     const float2 all = add2(sum[0], sum[1]);
@@ -1090,7 +1090,6 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             const float l = a.y * ex2_approx(a.x - ref) + b.y * ex2_approx(b.x - ref);
             const bool live = tok < it.ntok, some = l > 0.f;
             const float inv = some ? __fdividef(1.0f, l) : 0.f;
-            const bool blank = __any_sync(0xffffffffu, live && !some);
             const int64_t t = it.t0 + tok;
             const int h = it.kvh * p.G + hd;
             const bool busy = quad * 32 < it.ntok * p.G;
@@ -1109,41 +1108,36 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             }
             if (!wait_warp(bar(B_OF + ob), (uint32_t)((item / C::NO) & 1), p.status, E2C_ERR_WAIT_EPI)) break;
             tc_fence_after();
+            // 16 columns a step, the next ones on their way: short code, which an item runs through only once
+            const uint32_t to = ta + (uint32_t)(C::O_COL + ob * D);
+            uint32_t nx[16];
+            if (busy) tmem_ld16(to, nx);
 #pragma unroll 1
-            for (int c = 0; c < D; c += 64) {
-                uint32_t o[64];
+            for (int c = 0; c < D; c += 16) {
+                float o[16];
                 if (busy) {
-                    const uint32_t to = ta + (uint32_t)(C::O_COL + ob * D + c);
-                    tmem_ld32_to<0>(to, o);
-                    tmem_ld32_to<32>(to + 32, o);
                     tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[i] = __uint_as_float(nx[i]) * inv;
+                    if (c + 16 < D) tmem_ld16(to + c + 16, nx);
                 }
-                if (c == D - 64) {  // O has been read: the next item may use it while this one is stored
+                if (c + 16 == D) {  // O has been read: the next item may use it while this one is stored
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(B_OE + ob));
                 }
-                if (blank && !some) {  // such a row may have met a page's NaN: its zeros are not a product
+                if (live && !some) {  // such a row may have met a page's NaN: its zeros are not a product
 #pragma unroll
-                    for (int i = 0; i < 64; i++) o[i] = 0u;
+                    for (int i = 0; i < 16; i++) o[i] = 0.f;
                 }
                 if (live && out) {
                     uint4 *y = reinterpret_cast<uint4 *>(out + c);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        uint4 v;
-                        v.x = pack2<T>(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv);
-                        v.y = pack2<T>(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv);
-                        v.z = pack2<T>(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv);
-                        v.w = pack2<T>(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv);
-                        y[i] = v;
-                    }
+                    y[0] = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+                    y[1] = make_uint4(pack2<T>(o[8], o[9]), pack2<T>(o[10], o[11]), pack2<T>(o[12], o[13]), pack2<T>(o[14], o[15]));
                 } else if (live) {
                     float4 *y = reinterpret_cast<float4 *>(part + c);
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        y[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                           __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+                    for (int i = 0; i < 4; i++) y[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                 }
                 __syncwarp();
             }
