@@ -166,13 +166,16 @@ struct Share {
     int n1, s1, each1, rest1;  // the first n1 blocks have a prefix item more; s1 tiles are theirs
     int each2, rest2;          // the other blocks' shares: each2, the first rest2 of them one more
     E2C_DEV void set(int rows, int ptiles, int tiles, int grid) {
-        items = splits = chunk = 0;
-        if (ptiles > 0) {
-            const int s = max(1, grid / rows);
-            chunk = (ptiles + s - 1) / s;
-            splits = (ptiles + chunk - 1) / chunk;
-            items = rows * splits;
+        items = splits = chunk = n1 = s1 = each1 = rest1 = 0;
+        if (ptiles <= 0) {
+            each2 = tiles / grid;
+            rest2 = tiles - each2 * grid;
+            return;
         }
+        const int s = max(1, grid / rows);
+        chunk = (ptiles + s - 1) / s;
+        splits = (ptiles + chunk - 1) / chunk;
+        items = rows * splits;
         const int cost = chunk + 2 * ITEM_COST, k = items / grid;
         n1 = items - k * grid;
         const int64_t target = ((int64_t)items * cost + tiles) / grid;
@@ -262,19 +265,22 @@ struct Plan {
     int pseq, pmax;  // the sequence whose table maps the prefix, and its tokens there
     int masked;      // some row does not see every key of the prefix
     int npt;         // row tiles of the batch
+    int tiles;       // cost of the sequence items
     int first;       // the entry of this block's first sequence item,
     int first_before;  // and the tiles before it
 };
 
-// Every thread of the block. Pass 0 sums over the entries and finds the longest; pass 1 finds the entry in
-// which this block's share begins (and leaves the joining kernel the tiles before each entry).
+// Every thread of the block: sums over the entries, the longest of them, and the entry in which this
+// block's share begins (block 0 leaves the joining kernel the cost before each entry). Up to NTHREADS
+// entries are read once, more of them twice.
 struct PlanScratch {
     int64_t sum[WARPS];  // by warp
-    int at;           // tiles before the block's first entry
+    int at;              // cost before the block's first entry
     int longest, least, masked, first, seq;
 };
 E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+    constexpr int MOST = 1 << 24;  // of one entry; with more, or 2^30 in all, the call does nothing
     if (tid == 0) {
         s.longest = -1;
         s.least = 0x7fffffff;
@@ -282,74 +288,74 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
         s.first = -1;
         s.seq = 0x7fffffff;
     }
-    __syncthreads();
     pl.npt = (p.T + p.tpt - 1) / p.tpt;
     pl.plo = 0;
-    Entry e = {};
-    int64_t mine = 0;
-    int at = -1, tiles = 0;
+    const int rounds = p.n > NTHREADS ? 2 : 1;
+    int at = -1;
 #pragma unroll 1
-    for (int pass = 0; pass < 2; pass++) {
+    for (int round = 0; round < rounds; round++) {
+        const bool last = round == rounds - 1;
         int64_t run = 0;
 #pragma unroll 1
         for (int base = 0; base < p.n; base += NTHREADS) {
             const int i = base + tid;
-            if (pass == 0 || p.n > NTHREADS) {
-                e = {};
-                mine = 0;
-                if (i < p.n) {
-                    e = entry_of(p, i, pass == 0 && blockIdx.x == 0);
-                    mine = tiles_of(p, e.len, e.nq, p.shared) * p.pc.KV;
-                }
+            Entry e = {};
+            int mine = 0;
+            if (i < p.n) {
+                e = entry_of(p, i, round == 0 && blockIdx.x == 0);
+                mine = (int)min(tiles_of(p, e.len, e.nq, p.shared) * p.pc.KV, (int64_t)MOST);
             }
-            int64_t x = mine;
+            int x = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
+                const int y = __shfl_up_sync(0xffffffffu, x, d);
                 if (lane >= d) x += y;
             }
-            __syncthreads();  // the sums of the step before have been read
-            if (lane == 31) s.sum[w] = x;
-            if (pass == 0) {
-                if (p.shared > 0) {
-                    const int longest = __reduce_max_sync(0xffffffffu, e.nq > 0 ? e.len : -1);
-                    const int least = __reduce_min_sync(0xffffffffu, e.nq > 0 ? e.len - e.nq : 0x7fffffff);
-                    const bool masked = __any_sync(0xffffffffu, e.nq > 0 && (e.len < p.shared || (p.causal && e.len - e.nq < p.shared - 1)));
-                    if (lane == 0) {
-                        atomicMax(&s.longest, longest);
-                        atomicMin(&s.least, least);
-                        if (masked) s.masked = 1;
-                    }
+            const bool too_long = __any_sync(0xffffffffu, mine == MOST);
+            __syncthreads();  // the scratch is set, the sums of the step before have been read
+            if (lane == 31) s.sum[w] = too_long ? 1ll << 40 : x;
+            if (p.shared > 0 && round == 0) {
+                const int longest = __reduce_max_sync(0xffffffffu, e.nq > 0 ? e.len : -1);
+                const int least = __reduce_min_sync(0xffffffffu, e.nq > 0 ? e.len - e.nq : 0x7fffffff);
+                const bool masked = __any_sync(0xffffffffu, e.nq > 0 && (e.len < p.shared || (p.causal && e.len - e.nq < p.shared - 1)));
+                if (lane == 0) {
+                    atomicMax(&s.longest, longest);
+                    atomicMin(&s.least, least);
+                    if (masked) s.masked = 1;
                 }
-            } else if (e.nq > 0 && e.len == s.longest) {
-                atomicMin(&s.seq, e.seq);
             }
             __syncthreads();
-            int64_t before = run + x - mine;
-#pragma unroll 4
-            for (int k = 0; k < WARPS; k++) {
-                if (k < w) before += s.sum[k];
-                run += s.sum[k];
+            // every warp adds up the warps' sums
+            int64_t y = lane < WARPS ? s.sum[lane] : 0;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t z = __shfl_up_sync(0xffffffffu, y, d);
+                if (lane >= d) y += z;
             }
-            if (pass == 1 && i < p.n) {
+            const int64_t all = __shfl_sync(0xffffffffu, y, 31), here = __shfl_sync(0xffffffffu, y, w > 0 ? w - 1 : 0);
+            const int64_t before = run + (w > 0 ? here : 0) + x - mine;
+            run += all;
+            if (round == 0 && base + NTHREADS >= p.n) {
+                pl.pmax = min(p.shared, max(s.longest, 0));
+                pl.masked = s.masked || p.window >= 0;
+                if (p.window >= 0) pl.plo = max(0, s.least - p.window) / TK * TK;
+                pl.ptiles = pl.plo < pl.pmax ? (pl.pmax - pl.plo + TK - 1) / TK : 0;
+                const bool fits = run < 1ll << 30;
+                if (!fits && tid == 0) record_status(p.status, E2C_ERR_BAD_SEQ);
+                pl.tiles = fits ? (int)run : 0;
+                pl.share.set(p.pc.KV * pl.npt, pl.ptiles, pl.tiles, gridDim.x);
+                at = pl.share.begin(blockIdx.x);
+            }
+            if (last && i < p.n) {
                 if (at >= before && at < before + mine) {
                     s.first = i;
                     s.at = (int)before;
                 }
-                if (blockIdx.x == 0 && p.shared > 0) p.before[i] = (int)before;
+                if (p.shared > 0) {
+                    if (e.nq > 0 && e.len == s.longest) atomicMin(&s.seq, e.seq);
+                    if (blockIdx.x == 0) p.before[i] = (int)before;
+                }
             }
-        }
-        if (pass == 0) {
-            const int longest = s.longest;
-            pl.pmax = min(p.shared, max(longest, 0));
-            pl.masked = s.masked || p.window >= 0;
-            if (p.window >= 0) pl.plo = max(0, s.least - p.window) / TK * TK;
-            pl.ptiles = pl.plo < pl.pmax ? (pl.pmax - pl.plo + TK - 1) / TK : 0;
-            const bool fits = run < 1ll << 30;
-            if (!fits && tid == 0) record_status(p.status, E2C_ERR_BAD_SEQ);
-            tiles = fits ? (int)run : 0;
-            pl.share.set(p.pc.KV * pl.npt, pl.ptiles, tiles, gridDim.x);
-            at = pl.share.begin(blockIdx.x);
         }
     }
     __syncthreads();
@@ -357,7 +363,7 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
     pl.first_before = s.at;
     pl.pseq = s.seq;
     if (blockIdx.x == 0 && tid == 0) {
-        p.before[p.n] = tiles;
+        p.before[p.n] = pl.tiles;
         p.before[p.n + 1] = pl.ptiles;
     }
 }
@@ -1159,10 +1165,11 @@ struct Join {
     static constexpr int LANES = D / 4, ROWS = JOIN / LANES;
     float4 acc = {0, 0, 0, 0};
     float m = -INFINITY, l = 0.f;
-    E2C_DEV void add(const float *o, float s, int x) {
-        if (s == -INFINITY) return;
+    // a part's sums and its log-sum-exp; -infinity: it saw nothing
+    E2C_DEV void add(const float *o, const float *sums, int x) {
         const float4 v = *reinterpret_cast<const float4 *>(o + 4 * x);
-        const float mn = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - mn);
+        const float s = *sums, mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
+        const float a = exp2f(m - ref), w = exp2f(s - ref);
         acc.x = acc.x * a + w * v.x;
         acc.y = acc.y * a + w * v.y;
         acc.z = acc.z * a + w * v.z;
@@ -1196,8 +1203,9 @@ __global__ void __launch_bounds__(JOIN) k_join_split(const Args p, int grid) {
     const int x = threadIdx.x % J::LANES, rows = a.y * p.G;
     for (int row = blockIdx.y * J::ROWS + threadIdx.x / J::LANES; row < rows; row += gridDim.y * J::ROWS) {
         J j;
-        j.add(p.po + ((int64_t)a.w * TR + row) * D, p.pl[(int64_t)a.w * TR + row], x);
-        for (int c = blockIdx.x; c <= c1; c++) j.add(p.po + ((int64_t)(2 * c) * TR + row) * D, p.pl[(int64_t)(2 * c) * TR + row], x);
+        j.add(p.po + ((int64_t)a.w * TR + row) * D, p.pl + (int64_t)a.w * TR + row, x);
+#pragma unroll 4
+        for (int c = blockIdx.x; c <= c1; c++) j.add(p.po + ((int64_t)(2 * c) * TR + row) * D, p.pl + (int64_t)(2 * c) * TR + row, x);
         const int tok = row / p.G;
         j.put(p, a.x + tok, a.z * p.G + (row - tok * p.G), x);
     }
@@ -1217,9 +1225,10 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     Share share;
     share.set(p.pc.KV * npt, p.before[p.n + 1], p.before[p.n], grid);
     J j;
-    auto slot = [&](int k, int row) { j.add(p.po + ((int64_t)k * TR + row) * D, p.pl[(int64_t)k * TR + row], x); };
+    auto slot = [&](int k, int row) { j.add(p.po + ((int64_t)k * TR + row) * D, p.pl + (int64_t)k * TR + row, x); };
     if (share.items) {
         const int rt = (int)(t / p.tpt), row = (int)(t - (int64_t)rt * p.tpt) * p.G + hd;
+#pragma unroll 4
         for (int s = 0; s < share.splits; s++) slot(2 * grid + (kvh * share.splits + s) * npt + rt, row);
     }
     int last;
@@ -1232,7 +1241,7 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     const int nt = span_of(p, e.len, e.nq, 0, p.shared, k0, klim);
     const int s = p.before[i] + kvh * (nt + ITEM_COST), c0 = share.block(s), c1 = share.block(s + nt - 1);
     if (c0 == c1) {
-        j.add(p.dpo + (t * p.H + h) * D, p.dpl[t * p.H + h], x);
+        j.add(p.dpo + (t * p.H + h) * D, p.dpl + t * p.H + h, x);
     } else {
         const int row = (int)(t - e.q0) * p.G + hd;
         for (int c = c0; c <= c1; c++) slot(2 * c + (c == c0 && s > share.begin(c0) ? 1 : 0), row);
@@ -1312,7 +1321,7 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
     if (prefix)
         e2c_launch_as(true, k_join_prefix<T, D>, dim3((unsigned)(((int64_t)a.T * a.H + J::ROWS - 1) / J::ROWS)), dim3(JOIN), 0, st, a, sms);
     else
-        e2c_launch_as(true, k_join_split<T, D>, dim3(sms, 8), dim3(JOIN), 0, st, a, sms);
+        e2c_launch_as(true, k_join_split<T, D>, dim3(sms, (unsigned)((a.G * (a.max_q < a.tpt ? a.max_q : a.tpt) + J::ROWS - 1) / J::ROWS)), dim3(JOIN), 0, st, a, sms);
     return launch_error("pages_attention join");
 }
 
