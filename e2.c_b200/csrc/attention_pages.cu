@@ -44,7 +44,7 @@ namespace {
 constexpr int TR = 128;  // rows of an item
 constexpr int TK = 128;  // keys of a tile
 // warps: 0..7 softmax (two groups of four), 8..11 epilogue, then one each
-enum { W_EPI = 8, W_ITEMS = 12, W_MMA, W_K, W_V, W_Q, WARPS };
+enum { W_EPI = 8, W_ITEMS = 12, W_MMA, W_K, W_V, WARPS };
 constexpr int NTHREADS = 32 * WARPS;
 constexpr int NI = 8;  // item descriptors in flight
 // What a sequence item costs beside its tiles, in tiles: its set-up and its output
@@ -482,7 +482,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         for (int i = 0; i < 8; i++) mbar_init(bar(B_MX + i), 1);
         for (int i = 0; i < NI; i++) {
             mbar_init(bar(B_ITF + i), 1);
-            mbar_init(bar(B_ITE + i), 17);  // Q, K, V, QK, PV, 8 softmax and 4 epilogue warps
+            mbar_init(bar(B_ITE + i), 16);  // K, V, QK, PV, 8 softmax and 4 epilogue warps
         }
         for (int i = 0; i < 5; i++) {
             mbar_init(bar(B_KF + i), 1);
@@ -524,13 +524,29 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
     if (warp >= W_ITEMS) {
         if (warp == W_ITEMS) {
-            // ------------------------------------------------------------ items
+            // ------------------------------------------------------------ items and Q loads
             const int L0 = pl.share.begin(blockIdx.x), L1 = pl.share.begin(blockIdx.x + 1);
             if (p.shared == 0 && lane == 0 && L0 < L1) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
             __syncwarp();
             int pos = L0, n = 0;
             bool ok = true;
             Item it = {};
+            // Q of an item is loaded once the next one is published: the K and V loads then know of an item more
+            // than Q's buffers hold
+            int q_t0 = 0, q_kvh = 0, q_prefix = 0, loaded = 0;
+            auto load_q = [&]() {
+                const int qb = loaded % C::NQ;
+                if (!(ok = wait_warp(bar(B_QE + qb), (uint32_t)(((loaded / C::NQ) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) return;
+                if (elect_one()) {
+                    const CUtensorMap *tm = q_prefix ? &tmQp : &tmQ;
+                    mbar_arrive_expect_tx(bar(B_QF + qb), (uint32_t)(C::PANELS * (q_prefix ? qp_box : q_box) * p.G * 128));
+#pragma unroll
+                    for (int i = 0; i < C::PANELS; i++)
+                        tma_load_3d(sbase + qb * C::Q_BYTES + i * (TR * 128), tm, 64 * i, q_kvh * p.G, q_t0, bar(B_QF + qb));
+                }
+                __syncwarp();
+                loaded++;
+            };
             auto publish = [&]() {
                 const int sl = n & (NI - 1);
                 if (!(ok = wait_warp(bar(B_ITE + sl), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) return;
@@ -542,7 +558,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     mbar_arrive(bar(B_ITF + sl));
                 }
                 __syncwarp();
-                n++;
+                if (n++ > 0) load_q();
+                q_t0 = it.t0;
+                q_kvh = it.kvh;
+                q_prefix = it.prefix;
             };
             // Neighbours share a run of the prefix; every other group of them begins with its sequence items, so
             // that products (the prefix) and loads (the sequences) go on side by side.
@@ -637,31 +656,20 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     }
                 }
             }
-            if (ok && wait_warp(bar(B_ITE + (n & (NI - 1))), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER) &&
-                lane == 0) {
-                items[n & (NI - 1)].ntok = -1;
-                mbar_arrive(bar(B_ITF + (n & (NI - 1))));
-            }
-            __syncwarp();
-        } else if (warp == W_Q) {
-            // ------------------------------------------------------------ Q loads
-            int n = 0;
-            Item it;
-#pragma unroll 1
-            for (; take(n, it); n++) {
-                const int qb = n % C::NQ;
-                if (!wait_warp(bar(B_QE + qb), (uint32_t)(((n / C::NQ) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) break;
-                if (elect_one()) {
-                    const CUtensorMap *tm = it.prefix ? &tmQp : &tmQ;
-                    mbar_arrive_expect_tx(bar(B_QF + qb), (uint32_t)(C::PANELS * (it.prefix ? qp_box : q_box) * p.G * 128));
-#pragma unroll
-                    for (int i = 0; i < C::PANELS; i++)
-                        tma_load_3d(sbase + qb * C::Q_BYTES + i * (TR * 128), tm, 64 * i, it.kvh * p.G, it.t0, bar(B_QF + qb));
+            // the last one, after which Q of the last item follows
+            if (ok) {
+                const bool any = n > 0;
+                if (wait_warp(bar(B_ITE + (n & (NI - 1))), (uint32_t)(((n / NI) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) {
+                    if (lane == 0) {
+                        items[n & (NI - 1)].ntok = -1;
+                        mbar_arrive(bar(B_ITF + (n & (NI - 1))));
+                    }
+                    __syncwarp();
+                    if (any) load_q();
                 }
-                __syncwarp();
             }
             // every load that was issued has landed before the block may end
-            for (int i = n - C::NQ < 0 ? 0 : n - C::NQ; i < n; i++)
+            for (int i = loaded - C::NQ < 0 ? 0 : loaded - C::NQ; i < loaded; i++)
                 wait_warp(bar(B_QF + i % C::NQ), (uint32_t)((i / C::NQ) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
         } else if (warp == W_MMA) {
             // ------------------------------------------------------------ MMA issue (one thread)
