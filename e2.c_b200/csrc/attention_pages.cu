@@ -767,19 +767,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                         if (first && !(ok = wait1(B_OE + ob, op))) break;
                         tc_fence_after();
 #pragma unroll
-                        for (int h = 0; h < C::KPARTS; h++) {
+                        for (int h = 0; h < C::KPARTS; h++) {  // half tiles of V
                             if (!(ok = wait1(B_VF + vs, vp))) break;
                             const uint64_t vd = smem_desc_sw128_mn(sbase + C::V_OFF + vs * C::STAGE, C::VROWS * 128);
                             const int here = min(C::VROWS, nk16 - h * C::VROWS);
-                            if (here == C::VROWS) {
-#pragma unroll
-                                for (int k = 0; k < C::VROWS / 16; k++)
-                                    mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id_pv, !first || h != 0 || k != 0);
-                            } else {
-#pragma unroll 1
-                                for (int k = 0; k < here / 16; k++)
-                                    mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id_pv, !first || h != 0 || k != 0);
-                            }
+#pragma unroll 2
+                            for (int k = 0; k < here / 16; k++)
+                                mma_bf16_ts(d, a + 8 * k, vd + 128 * k, id_pv, !first || h != 0 || k != 0);
                             mma_commit(bar(B_VE + vs));
                             a += C::VROWS / 2;
                             if (++vs == C::NVS) {
@@ -849,27 +843,21 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                         const int x = kvh * D + (is_v ? 0 : h * np * 64);
                         // the first rows are in every lane before the wait: from a free stage to its loads is the
                         // shortest way
-                        int y[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) y[i] = __shfl_sync(0xffffffffu, row, min(b0 + i, 31));
+                        int y = __shfl_sync(0xffffffffu, row, b0), y2 = __shfl_sync(0xffffffffu, row, min(b0 + 1, 31));
                         if (!(ok = wait_warp(bar(E + st), par, p.status, E2C_ERR_WAIT_PRODUCER))) break;
-                        const uint32_t dst = ring + st * C::STAGE, full = bar(F + st);
-                        auto box = [&](int b, int y) {
-#pragma unroll
-                            for (int i = 0; i < C::PANELS; i++)
-                                if (i < np) tma_load_2d(dst + (b - b0) * (PB * 128) + i * pitch, tm, x + 64 * i, y, full);
-                        };
-                        if (elect_one()) {
-                            mbar_arrive_expect_tx(full, (uint32_t)((b1 - b0) * PB * 128 * np));
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                if (b0 + i < b1) box(b0 + i, y[i]);
-                        }
+                        const uint32_t full = bar(F + st);
+                        uint32_t dst = ring + st * C::STAGE;
+                        if (elect_one()) mbar_arrive_expect_tx(full, (uint32_t)((b1 - b0) * PB * 128 * np));
                         __syncwarp();
 #pragma unroll 1
-                        for (int b = b0 + 4; b < b1; b++) {
-                            const int yb = __shfl_sync(0xffffffffu, row, b);
-                            if (elect_one()) box(b, yb);
+                        for (int b = b0; b < b1; b++, dst += PB * 128) {
+                            if (elect_one()) {
+#pragma unroll
+                                for (int i = 0; i < C::PANELS; i++)
+                                    if (i < np) tma_load_2d(dst + i * pitch, tm, x + 64 * i, y, full);
+                            }
+                            y = y2;
+                            y2 = __shfl_sync(0xffffffffu, row, min(b + 2, 31));
                         }
                         if (++st == NST) {
                             st = 0;
@@ -978,14 +966,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 float now = before, alpha = 1.f;
                 if (live && (mx > before + kRescaleLog2 || (before == -INFINITY && mx > -INFINITY))) {
                     now = mx;
-                    alpha = before == -INFINITY ? 0.f : exp2f(before - mx);
+                    alpha = ex2_approx(before - mx);
                 }
                 xm[b * TR + row] = now;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(B_MX + b * 4 + quad));
                 if (busy) {
                     if (now != m) {
-                        l = m == -INFINITY ? 0.f : l * exp2f(m - now);
+                        l *= ex2_approx(m - now);
                         m = now;
                     }
                     if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
@@ -1110,7 +1098,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             T *out = nullptr;
             float *part = nullptr;
             if (busy) {
-                const float sums = some ? m + log2f(l) : -INFINITY;
+                const float sums = some ? m + __log2f(l) : -INFINITY;
                 if (it.dst == TO_OUT) {
                     out = static_cast<T *>(p.out) + t * p.ldo + h * D;
                     if (live && p.lse) p.lse[t * p.H + h] = sums * LN2;
