@@ -7,24 +7,30 @@
 //   - A sequence item has the rows of one sequence's tokens and reads that sequence's pages.
 //   - With a shared prefix, a prefix item packs the rows of the whole batch, whatever their sequence,
 //     and reads the prefix's pages once for all of them; sequence items then begin past the prefix.
-// All lengths are on the device: every block adds up the items' tiles itself and takes an equal share
-// of the tiles, in order (its first and last item may be parts of one). An item that lies in one block
-// and has no prefix is written to the output; other parts leave their normalised sums and log-sum-exps in
-// the workspace, and a second kernel joins them in a fixed order. No atomics: results do not depend
-// on timing.
+// All lengths are on the device: every block adds up the items' tiles itself and takes its share (Share).
+// A sequence item that lies in one block and has no prefix is written to the output; other parts leave
+// their normalised sums and log-sum-exps in the workspace, and a second kernel joins them in a fixed
+// order. No floating-point atomics: results do not depend on timing.
 //
 // Per key tile j of an item, with the online softmax of attention.cu:
 //   S = Q K_j^T     fp32 in tensor memory, N rounded up to 16 keys in an item's last tile
 //   P = exp2(S scale log2 e - m)  16 bits over S's columns; m moves only when it grows by 2^8, then O is rescaled
 //   O += P V_j      fp32 in tensor memory; V is read as it lies in the cache (its head dim contiguous)
-// Two S buffers: the two softmax warpgroups take alternate tiles, handing the running maximum on as
-// soon as a tile's maximum is known, so their exponentials overlap.
+// P is rounded to the cache's type, the tensor cores' operand; its sum, m and O are held in 32 bits. The two softmax
+// warpgroups take alternate tiles, handing the running maximum on as soon as a tile's is known, so
+// that their exponentials overlap.
 //
-// K and V tiles share one ring of stages in the order the products need them; pages arrive one TMA box
-// each (a page's rows land as consecutive rows of the tile). Rows of V past the sequence's last key
-// are zeroed in shared memory up to the product's 16-key granularity: what a page holds there is
-// arbitrary, and 0 x NaN would not vanish. Keys past it are masked in S by a select.
+// K and V have a ring of stages and a loading warp each; pages arrive one TMA box each (a page's rows land as
+// consecutive rows of the tile). Rows of V past the sequence's last key are zeroed in shared memory up
+// to the product's 16-key granularity: what a page holds there is arbitrary, and 0 x NaN would not
+// vanish. Keys past it are masked in S by a select.
 //
+// What bounds it (one B200, CUDA events): long single-token batches the memory (64 sequences of 8192
+// tokens, 32 heads of 128 over 8 key heads: 270 us, 6.5 TB/s); whole prompts the issue and softmax of a
+// tile, some 1500 cycles for 128 rows by 128 keys (4 x 4096 tokens, 16 heads of 128 over 4: 390 us, 63% of
+// the measured bf16 rate; 8 heads of 256: 335 us, 73%; 16 heads of 64: 350 us); short sequences an item's
+// set-up and output, some 3500 cycles (512 x 16 tokens, 8 key heads: 60 us). A tile's time does not
+// depend on the rings' depth (2 or 5 stages) nor on a third softmax group by more than 5%.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -280,7 +286,6 @@ struct PlanScratch {
 };
 E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-    constexpr int MOST = 1 << 24;  // of one entry; with more, or 2^30 in all, the call does nothing
     if (tid == 0) {
         s.longest = -1;
         s.least = 0x7fffffff;
@@ -300,20 +305,19 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
         for (int base = 0; base < p.n; base += NTHREADS) {
             const int i = base + tid;
             Entry e = {};
-            int mine = 0;
+            int64_t mine = 0;
             if (i < p.n) {
                 e = entry_of(p, i, round == 0 && blockIdx.x == 0);
-                mine = (int)min(tiles_of(p, e.len, e.nq, p.shared) * p.pc.KV, (int64_t)MOST);
+                mine = tiles_of(p, e.len, e.nq, p.shared) * p.pc.KV;
             }
-            int x = mine;
+            int64_t x = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, d);
+                const int64_t y = __shfl_up_sync(0xffffffffu, x, d);
                 if (lane >= d) x += y;
             }
-            const bool too_long = __any_sync(0xffffffffu, mine == MOST);
             __syncthreads();  // the scratch is set, the sums of the step before have been read
-            if (lane == 31) s.sum[w] = too_long ? 1ll << 40 : x;
+            if (lane == 31) s.sum[w] = x;
             if (p.shared > 0 && round == 0) {
                 const int longest = __reduce_max_sync(0xffffffffu, e.nq > 0 ? e.len : -1);
                 const int least = __reduce_min_sync(0xffffffffu, e.nq > 0 ? e.len - e.nq : 0x7fffffff);
@@ -341,8 +345,9 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
                 if (p.window >= 0) pl.plo = max(0, s.least - p.window) / TK * TK;
                 pl.ptiles = pl.plo < pl.pmax ? (pl.pmax - pl.plo + TK - 1) / TK : 0;
                 const bool fits = run < 1ll << 30;
-                if (!fits && tid == 0) record_status(p.status, E2C_ERR_BAD_SEQ);
+                if (!fits && tid == 0) record_status(p.status, E2C_ERR_TOO_LARGE);
                 pl.tiles = fits ? (int)run : 0;
+                if (!fits) pl.ptiles = 0;
                 pl.share.set(p.pc.KV * pl.npt, pl.ptiles, pl.tiles, gridDim.x);
                 at = pl.share.begin(blockIdx.x);
             }
@@ -930,7 +935,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                 const bool masked = __any_sync(0xffffffffu, live && (ra > 0 || rb < TK));
                 // The columns are read twice, for the maximum and for the exponentials, in loops short enough
                 // for the instruction cache: a row of 128 logits held in registers is straight code that does
-                // not stay in it (16 heads of 128, 4096 tokens: 443 us, against 370 with loops of 64 columns)
+                // not stay in it (4 x 4096 tokens, 16 heads of 128: 443 us, 370 with loops of 64 columns; of 32, 368)
                 auto hide = [&](int c0, uint32_t (&s)[16]) {
                     // bit i: column c0 + i is seen
                     const int a = min(max(ra - c0, 0), 16), b = min(max(rb - c0, 0), 16);
@@ -1215,7 +1220,7 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
     griddep_wait();
     const int64_t u = (int64_t)blockIdx.x * J::ROWS + threadIdx.x / J::LANES;
     const int64_t t = u / p.H;
-    if (t >= p.T) return;
+    if (t >= p.T || p.before[p.n] == 0) return;  // no such row; or a batch that is too large, and was left
     const int h = (int)(u - t * p.H), kvh = h / p.G, hd = h - kvh * p.G, x = threadIdx.x % J::LANES;
     const int npt = (p.T + p.tpt - 1) / p.tpt;
     Share share;

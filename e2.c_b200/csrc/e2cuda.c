@@ -69,6 +69,7 @@ static const char *status_name(int s) {
     case 0x108: return "position outside the rotary table";
     case 0x109: return "not enough free pages (the append did nothing)";
     case 0x10a: return "sequence, count or page outside the cache (that entry was left out)";
+    case 0x10b: return "attention batch too large (the call did nothing)";
     default: return "unknown device failure";
     }
 }

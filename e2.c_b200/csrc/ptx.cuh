@@ -25,7 +25,8 @@ enum {
     E2C_ERR_SMEM_ALIGN = 0x107,     // dynamic shared memory not 1024-byte aligned: the kernel did nothing
     E2C_ERR_BAD_POSITION = 0x108,   // a position outside the rotary table
     E2C_ERR_NO_PAGES = 0x109,       // fewer free pages than an append needs: it did nothing
-    E2C_ERR_BAD_SEQ = 0x10a         // a sequence, count or page outside the cache (that entry is left out)
+    E2C_ERR_BAD_SEQ = 0x10a,        // a sequence, count or page outside the cache (that entry is left out)
+    E2C_ERR_TOO_LARGE = 0x10b       // more key tiles than an attention call can count: it did nothing
 };
 
 E2C_DEV uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }

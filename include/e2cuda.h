@@ -300,6 +300,9 @@ int e2cuda_pages_store(const e2cuda_pages *pc, int layer, int x_type, const void
  * pages, as after a fork; their keys are then read once for the batch instead of once for each
  * sequence. 0 asks for nothing of the tables. max_q: an upper bound of an entry's rows.
  *
+ * A call counts its work in tiles of 128 rows (tokens by the heads that share a key head) by 128 keys, for each
+ * key head; with 2^30 of them or more it does nothing and is reported by e2cuda_check.
+ *
  * ws: e2cuda_pages_attention_ws_bytes() of 16-byte aligned scratch that no other call uses meanwhile. */
 size_t e2cuda_pages_attention_ws_bytes(const e2cuda_pages *pc, int n, int T, int max_q, int heads, int shared);
 int e2cuda_pages_attention(const e2cuda_pages *pc, int layer, const void *q, int ldq, const int32_t *seqs,

@@ -565,6 +565,37 @@ def test_attention_past_32_bit_offsets(e2c, torch_cuda):
     assert_attention(torch, out, lse, attention64(torch, cache, 0, q, seqs, q_start, True, -1, D ** -0.5), "bf16", 320)
 
 
+def test_attention_of_one_long_prompt(e2c, torch_cuda):
+    """131072 tokens in one call, over 2^24 tiles: rows at its ends and between, against 64 bits."""
+    torch = torch_cuda
+    T, H, KV, D = 131072, 32, 2, 64
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 5, [T], [T], 0, H, KV, D, 128, "bf16", spare=0)
+    out, lse = cache.attention(0, q, seqs, q_start, max_q, lse=True)
+    e2c.check()
+    for t in (0, 127, 128, 77777, T - 1):
+        cache.length[0] = t + 1
+        row = torch.tensor([0, 1], device="cuda").int()
+        want = attention64(torch, cache, 0, q[t:t + 1], seqs, row, True, -1, D ** -0.5)
+        assert_attention(torch, out[t:t + 1], lse[t:t + 1], want, "bf16", t + 1)
+
+
+@pytest.mark.parametrize("n,each,shared", [(1, 16384, 0), (1536, 1, 1 << 14)])
+def test_attention_of_too_large_a_batch_does_nothing(e2c, torch_cuda, n, each, shared):
+    """Lengths of 2^24 make over 2^30 tiles; the call is reported and leaves the output as it was."""
+    torch = torch_cuda
+    cache = e2c.PageCache.new(1, 4, 128, 8, 64, n, 1 << 17, torch.bfloat16)
+    cache.length.fill_(1 << 24)
+    q = torch.zeros(n * each, 128, 64, device="cuda", dtype=torch.bfloat16)
+    out = torch.full_like(q, 7)
+    seqs = torch.arange(n, device="cuda").int()
+    q_start = torch.arange(0, n * each + 1, each, device="cuda").int()
+    cache.attention(0, q, seqs, q_start, each, shared=shared, causal=False, out=out)
+    with pytest.raises(e2c.E2CudaError, match="too large"):
+        e2c.check()
+    assert (out == 7).all()
+    e2c.check()
+
+
 # ------------------------------------------------------------------------------------------ the cache write
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("src,dtype", [("bf16", "bf16"), ("f32", "bf16"), ("f16", "f16"), ("f32", "f16")])
