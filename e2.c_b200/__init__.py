@@ -244,6 +244,14 @@ def _stream(stream) -> int | None:
     return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
 
 
+def _result(stream, make):
+    """make()'s tensor in memory of the stream that writes it: memory of another stream's may still be in use there."""
+    if stream is None:
+        return make()
+    with _torch().cuda.stream(stream):
+        return make()
+
+
 def check(stream=None) -> None:
     _ok(lib().e2cuda_check(_stream(stream)), "device check")
 
@@ -403,8 +411,8 @@ def rope_table(positions: int, rot: int, theta: float = 1e4, scaling: RopeScalin
     """cos, sin [positions][rot / 2] fp32 of the angles position * theta^(-2 i / rot), scaled for long
     contexts as `scaling` says."""
     torch = _torch()
-    cos = torch.empty((positions, rot // 2), dtype=torch.float32, device="cuda")
-    sin = torch.empty_like(cos)
+    cos, sin = _result(stream, lambda: tuple(torch.empty((positions, rot // 2), dtype=torch.float32, device="cuda")
+                                             for _ in range(2)))
     _ok(lib().e2cuda_rope_table(cos.data_ptr(), sin.data_ptr(), positions, rot, theta,
                                 None if scaling is None else C.byref(scaling), _stream(stream)), "rope_table")
     return cos, sin
@@ -419,7 +427,8 @@ def rope(x, cos, sin, pos=None, interleaved: bool = False, backward: bool = Fals
     T, H, D = x.shape
     positions, rot = _table(cos, sin)
     if out is None:
-        out = torch.empty_like(x) if dtype is None and x.is_contiguous() else x.new_empty((T, H, D), dtype=dtype or x.dtype)
+        out = _result(stream, lambda: torch.empty_like(x) if dtype is None and x.is_contiguous()
+                      else x.new_empty((T, H, D), dtype=dtype or x.dtype))
     elif out.shape != x.shape:
         raise E2CudaError(f"rope: out {tuple(out.shape)} for x {tuple(x.shape)}")
     _ok(lib().e2cuda_rope(x.data_ptr(), _rows(x, "rope"), _type(x), out.data_ptr(), _rows(out, "rope out"), _type(out),
@@ -448,6 +457,7 @@ class PageCache:
         layers, n_pages, page, kv, dim = k.shape
         self.ws = torch.empty(lib().e2cuda_pages_ws_bytes(n_pages, length.shape[0]) // 4, dtype=torch.int32, device=k.device)
         self._scratch: dict = {}  # the attention's workspace and its size, by stream
+        self._outgrown: list = []  # smaller ones before them; each at least doubles, so all are at most the last one's size
         self._needs: dict = {}    # workspace bytes by batch
         self.pages = Pages(k.data_ptr(), v.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.ws.data_ptr(),
                            _type(k), layers, n_pages, page, kv, dim, table.shape[0], table.shape[1])
@@ -497,7 +507,7 @@ class PageCache:
                               f"{p.kv_heads} heads of {p.head_dim}")
         positions, rot = _table(cos, sin)
         if out is None:
-            out = q.new_empty((T, H, D), dtype=self.k.dtype)
+            out = _result(stream, lambda: q.new_empty((T, H, D), dtype=self.k.dtype))
         elif out.shape != q.shape or out.dtype != self.k.dtype:
             raise E2CudaError(f"store: out {tuple(out.shape)} {out.dtype}")
         _ok(lib().e2cuda_pages_store(self._p, layer, _type(q), q.data_ptr(), _rows(q, "store q"), k.data_ptr(), _rows(k, "store k"),
@@ -517,10 +527,10 @@ class PageCache:
         if D != p.head_dim or q.dtype != self.k.dtype:
             raise E2CudaError(f"attention: q {tuple(q.shape)} {q.dtype} for a cache of heads of {p.head_dim} {self.k.dtype}")
         if out is None:
-            out = _torch().empty_like(q) if q.is_contiguous() else q.new_empty((T, H, D))
+            out = _result(stream, lambda: _torch().empty_like(q) if q.is_contiguous() else q.new_empty((T, H, D)))
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise E2CudaError(f"attention: out {tuple(out.shape)} {out.dtype}")
-        sums = q.new_empty((T, H), dtype=_torch().float32) if lse else None
+        sums = _result(stream, lambda: q.new_empty((T, H), dtype=_torch().float32)) if lse else None
         st = _stream(stream)
         batch = (n, T, max_q, H, shared)
         need = self._needs.get(batch)
@@ -530,9 +540,10 @@ class PageCache:
             need = self._needs[batch] = lib().e2cuda_pages_attention_ws_bytes(self._p, *batch)
         ws, size = self._scratch.get(st, (None, 0))
         if size < need or ws is None:
-            size = max(need, 16)
-            with _torch().cuda.stream(stream):  # its memory is reused in that stream's order
-                ws = q.new_empty(size, dtype=_torch().uint8)
+            if ws is not None:
+                self._outgrown.append(ws)  # a captured graph may still use it
+            size = max(need, 2 * size, 16)
+            ws = _result(stream, lambda: q.new_empty(size, dtype=_torch().uint8))
             self._scratch[st] = ws, size
         _ok(lib().e2cuda_pages_attention(self._p, layer, q.data_ptr(), _rows(q, "attention q"), _ints(seqs, n, "attention seqs"),
                                          _ints(q_start, n + 1, "attention q_start"), n, T, max_q, H, shared, causal, window,

@@ -714,6 +714,51 @@ def test_fork_append_store_attend_in_a_graph_and_on_another_stream(e2c, torch_cu
         alone.free(dev([0]))
 
 
+def test_graph_survives_a_larger_call(e2c, torch_cuda):
+    """A captured call's workspace is not given back when a later call needs a larger one."""
+    torch = torch_cuda
+    n = 300
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 8, [3029] * n, [1] * n, 3024, 8, 2, 128, 16, "bf16")
+    few = q[:2], seqs[:2], q_start[:3], 1
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        want = cache.attention(0, *few)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            got = cache.attention(0, *few)
+        (before, _), = cache._scratch.values()
+        cache.attention(0, q, seqs, q_start, max_q, shared=3024)
+        (after, _), = cache._scratch.values()
+        assert after.numel() > before.numel()
+        del before
+        held = [torch.full((1 << 20,), 7, device="cuda", dtype=torch.uint8) for _ in range(200)]  # what was given back
+        got.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    e2c.check()
+    assert torch.equal(got, want)
+    assert all((x == 7).all() for x in held)
+
+
+def test_results_belong_to_their_stream(e2c, torch_cuda):
+    """Memory freed on torch's stream, where a kernel may still use it, is not what another stream's call writes."""
+    torch = torch_cuda
+    cos, sin = e2c.rope_table(64, 64)
+    x = torch.randn(4096, 16, 64, device="cuda").bfloat16()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    gone = torch.empty_like(x)
+    at = gone.data_ptr()
+    del gone
+    assert torch.empty_like(x).data_ptr() == at  # torch's stream would get it again
+    pos = torch.zeros(4096, device="cuda", dtype=torch.int32)
+    y = e2c.rope(x, cos, sin, pos, stream=st)
+    assert y.data_ptr() != at
+    torch.cuda.synchronize()
+    e2c.check()
+
+
 def test_example_shared_and_recomputed_agree(e2c, torch_cuda):
     """The example's two ways to the same embeddings. Both round activations to int8 and attention operands to
     bf16; the difference is bf16's in attention (2^-8 of a row) carried through two layers, far below
