@@ -49,9 +49,6 @@ namespace {
 
 constexpr int TR = 128;  // rows of an item
 constexpr int TK = 128;  // keys of a tile
-// warps: 0..7 softmax (two groups of four), 8..11 epilogue, then one each
-enum { W_EPI = 8, W_ITEMS = 12, W_MMA, W_K, W_V, WARPS };
-constexpr int NTHREADS = 32 * WARPS;
 constexpr int NI = 8;  // item descriptors in flight
 // What a sequence item costs beside its tiles, in tiles: its set-up and its output
 constexpr int ITEM_COST = 1;
@@ -75,6 +72,10 @@ constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 
 template <int D>
 struct Cfg {
+    // warps: NG softmax groups of four, the epilogue's four, then one each
+    static constexpr int NG = D == 64 ? 3 : 2;
+    static constexpr int W_EPI = 4 * NG, W_ITEMS = W_EPI + 4, W_MMA = W_ITEMS + 1, W_K = W_MMA + 1, W_V = W_K + 1;
+    static constexpr int WARPS = W_V + 1, NTHREADS = 32 * WARPS;
     static constexpr int PANELS = D / 64;  // 64 of the head's dimensions each, 128 bytes a row
     static constexpr int NQ = D == 64 ? 2 : 1;  // Q buffers
     // K and V have a ring of stages each: of a tile, or for D = 256 of half a one (K: half of the
@@ -92,9 +93,9 @@ struct Cfg {
     static constexpr int Q_BYTES = TR * D * 2;
     static constexpr int K_OFF = NQ * Q_BYTES;
     static constexpr int V_OFF = K_OFF + NKS * STAGE;
-    static constexpr int XM = V_OFF + NVS * STAGE;              // running maxima handed on [2][128]
-    static constexpr int ML = XM + 2 * TR * 4;                  // item's (m, l) [2 items][2 groups][128] x 2
-    static constexpr int ITEMS = ML + 2 * 2 * TR * 8;
+    static constexpr int XM = V_OFF + NVS * STAGE;              // running maxima handed on [NG][128]
+    static constexpr int ML = XM + NG * TR * 4;                 // item's (m, l) [2 items][NG][128] x 2
+    static constexpr int ITEMS = ML + 2 * NG * TR * 8;
     static constexpr int SCAN = ITEMS + NI * 64;
     static constexpr int BARS = SCAN + 256;
 };
@@ -105,8 +106,8 @@ enum {
     B_SF = B_QE + 2,
     B_PF = B_SF + 3,
     B_PV = B_PF + 3,
-    B_MX = B_PV + 2,  // [2][4 lane quadrants]
-    B_OF = B_MX + 8,
+    B_MX = B_PV + 2,  // [NG][4 lane quadrants]
+    B_OF = B_MX + 12,
     B_OE = B_OF + 2,
     B_MLF = B_OE + 2,
     B_MLE = B_MLF + 2,
@@ -279,12 +280,15 @@ struct Plan {
 // Every thread of the block: sums over the entries, the longest of them, and the entry in which this
 // block's share begins (block 0 leaves the joining kernel the cost before each entry). Up to NTHREADS
 // entries are read once, more of them twice.
+template <int D>
 struct PlanScratch {
-    int64_t sum[WARPS];  // by warp
+    int64_t sum[Cfg<D>::WARPS];  // by warp
     int at;              // cost before the block's first entry
     int longest, least, masked, first, seq;
 };
-E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch &s) {
+template <int D>
+E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<D> &s) {
+    constexpr int WARPS = Cfg<D>::WARPS, NTHREADS = Cfg<D>::NTHREADS;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     if (tid == 0) {
         s.longest = -1;
@@ -452,7 +456,7 @@ __host__ __device__ constexpr uint32_t type_bits() {  // A and B formats of the 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(NTHREADS, 1)
+__global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
     k_attention_pages(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQp,
                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ Args p, const int q_box, const int qp_box) {
@@ -470,24 +474,24 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     Item *items = reinterpret_cast<Item *>(smem + C::ITEMS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (warp == W_ITEMS && lane == 0) {
+    if (warp == C::W_ITEMS && lane == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(bar(B_QF + i), 1);
             mbar_init(bar(B_QE + i), 1);
             mbar_init(bar(B_PV + i), 1);
             mbar_init(bar(B_OF + i), 1);
             mbar_init(bar(B_OE + i), 4);
-            mbar_init(bar(B_MLF + i), 8);
+            mbar_init(bar(B_MLF + i), 4 * C::NG);
             mbar_init(bar(B_MLE + i), 4);
         }
         for (int i = 0; i < 3; i++) {
             mbar_init(bar(B_SF + i), 1);
             mbar_init(bar(B_PF + i), 4);
         }
-        for (int i = 0; i < 8; i++) mbar_init(bar(B_MX + i), 1);
+        for (int i = 0; i < 4 * C::NG; i++) mbar_init(bar(B_MX + i), 1);
         for (int i = 0; i < NI; i++) {
             mbar_init(bar(B_ITF + i), 1);
-            mbar_init(bar(B_ITE + i), 16);  // K, V, QK, PV, 8 softmax and 4 epilogue warps
+            mbar_init(bar(B_ITE + i), 8 + 4 * C::NG);  // K, V, QK, PV, the epilogue and softmax warps
         }
         for (int i = 0; i < 5; i++) {
             mbar_init(bar(B_KF + i), 1);
@@ -501,7 +505,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         tma_prefetch_desc(&tmK);
         tma_prefetch_desc(&tmV);
     }
-    if (warp == W_MMA) {
+    if (warp == C::W_MMA) {
         tmem_alloc(sbase + C::BARS + B_NUM * 8, 512);
         tmem_relinquish();
     }
@@ -512,7 +516,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     const uint32_t tmem = *tmem_slot;
 
     Plan pl;
-    make_plan(p, pl, *reinterpret_cast<PlanScratch *>(smem + C::SCAN));
+    make_plan<D>(p, pl, *reinterpret_cast<PlanScratch<D> *>(smem + C::SCAN));
 
     // A consumer's copy of item n; false after the last one (or a failure). The slot is released at once.
     auto take = [&](int n, Item &it) -> bool {
@@ -527,8 +531,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         return it.ntok >= 0;
     };
 
-    if (warp >= W_ITEMS) {
-        if (warp == W_ITEMS) {
+    if (warp >= C::W_ITEMS) {
+        if (warp == C::W_ITEMS) {
             // ------------------------------------------------------------ items and Q loads
             const int L0 = pl.share.begin(blockIdx.x), L1 = pl.share.begin(blockIdx.x + 1);
             if (p.shared == 0 && lane == 0 && L0 < L1) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -676,7 +680,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             // every load that was issued has landed before the block may end
             for (int i = loaded - C::NQ < 0 ? 0 : loaded - C::NQ; i < loaded; i++)
                 wait_warp(bar(B_QF + i % C::NQ), (uint32_t)((i / C::NQ) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
-        } else if (warp == W_MMA) {
+        } else if (warp == C::W_MMA) {
             // ------------------------------------------------------------ MMA issue (one thread)
             // QK runs LOOK tiles ahead of PV; each has a cursor over the items
             if (elect_one()) {
@@ -805,7 +809,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             __syncwarp();
         } else {
             // ------------------------------------------------------------ K loads, V loads
-            const bool is_v = warp == W_V;
+            const bool is_v = warp == C::W_V;
             const CUtensorMap *tm = is_v ? &tmV : &tmK;
             const int F = is_v ? B_VF : B_KF, E = is_v ? B_VE : B_KE, NST = is_v ? C::NVS : C::NKS;
             const uint32_t ring = sbase + (is_v ? C::V_OFF : C::K_OFF);
@@ -881,9 +885,10 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             for (int i = total - NST < 0 ? 0 : total - NST; i < total; i++)
                 wait_warp(bar(F + i % NST), (uint32_t)((i / NST) & 1), nullptr, E2C_ERR_WAIT_DRAIN);
         }
-    } else if (warp < W_EPI) {
+    } else if (warp < C::W_EPI) {
         // ---------------------------------------------------------------- softmax
-        const int quad = warp & 3, group = warp >> 2, row = quad * 32 + lane;
+        constexpr int NG = C::NG;
+        const int quad = warp & 3, group = warp >> 2, prev = (group + NG - 1) % NG, row = quad * 32 + lane;
         const uint32_t ta = tmem + ((uint32_t)(quad * 32) << 16);
         float *xm = reinterpret_cast<float *>(smem + C::XM);
         float2 *ml = reinterpret_cast<float2 *>(smem + C::ML);
@@ -917,14 +922,14 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             }
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < it.nt; j++, g++) {
-                if ((g & 1) != group) continue;
-                const int b = g & 1, sb = g % C::NS, kk = it.k0 + j * TK, nk = min(TK, it.klim - kk);
+                if (g % NG != group) continue;
+                const int sb = g % C::NS, kk = it.k0 + j * TK, nk = min(TK, it.klim - kk);
                 // the running maximum, from the tile before (its wait runs while this tile's products do)
-                if (g > 0 && !wait_warp(bar(B_MX + (b ^ 1) * 4 + quad), (uint32_t)(((g - 1) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                if (g > 0 && !wait_warp(bar(B_MX + prev * 4 + quad), (uint32_t)(((g - 1) / NG) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                     ok = false;
                     break;
                 }
-                const float before = j > 0 ? xm[(b ^ 1) * TR + row] : -INFINITY;
+                const float before = j > 0 ? xm[prev * TR + row] : -INFINITY;
                 if (!wait_warp(bar(B_SF + sb), (uint32_t)((g / C::NS) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                     ok = false;
                     break;
@@ -973,9 +978,9 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     now = mx;
                     alpha = ex2_approx(before - mx);
                 }
-                xm[b * TR + row] = now;
+                xm[group * TR + row] = now;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(B_MX + b * 4 + quad));
+                if (lane == 0) mbar_arrive(bar(B_MX + group * 4 + quad));
                 if (busy) {
                     if (now != m) {
                         l *= ex2_approx(m - now);
@@ -983,7 +988,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
                     }
                     if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
                         // O holds the tiles before this one once their products are done
-                        if (!wait_warp(bar(B_PV + (b ^ 1)), (uint32_t)(((g - 1) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                        if (!wait_warp(bar(B_PV + ((g - 1) & 1)), (uint32_t)(((g - 1) >> 1) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
                             ok = false;
                             break;
                         }
@@ -1074,7 +1079,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             // the slot's last reader was the epilogue two items ago
             if (!wait_warp(bar(B_MLE + (item & 1)), (uint32_t)(((item >> 1) & 1) ^ 1), p.status, E2C_ERR_WAIT_ATTN))
                 break;
-            ml[((item & 1) * 2 + group) * TR + row] = make_float2(m, l);
+            ml[((item & 1) * NG + group) * TR + row] = make_float2(m, l);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_MLF + (item & 1)));
         }
@@ -1089,12 +1094,18 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             const int ob = item % C::NO;
             if (!wait_warp(bar(B_MLF + (item & 1)), (uint32_t)((item >> 1) & 1), p.status, E2C_ERR_WAIT_EPI))
                 break;
-            const float2 a = ml[(item & 1) * 2 * TR + row], b = ml[((item & 1) * 2 + 1) * TR + row];
+            float2 a[C::NG];
+#pragma unroll
+            for (int i = 0; i < C::NG; i++) a[i] = ml[((item & 1) * C::NG + i) * TR + row];
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_MLE + (item & 1)));
-            // the groups' sums, to the larger maximum; a row that neither saw a key of has l = 0
-            const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.f : m;
-            const float l = a.y * ex2_approx(a.x - ref) + b.y * ex2_approx(b.x - ref);
+            // the groups' sums, to the largest maximum; a row that none saw a key of has l = 0
+            float m = a[0].x, l = 0.f;
+#pragma unroll
+            for (int i = 1; i < C::NG; i++) m = fmaxf(m, a[i].x);
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int i = 0; i < C::NG; i++) l += a[i].y * ex2_approx(a[i].x - ref);
             const bool live = tok < it.ntok, some = l > 0.f;
             const float inv = some ? __fdividef(1.0f, l) : 0.f;
             const int64_t t = it.t0 + tok;
@@ -1153,7 +1164,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
     tc_fence_before();
     __syncthreads();
-    if (warp == W_MMA) {
+    if (warp == C::W_MMA) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -1316,7 +1327,7 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
         e2c_tmap_2d(&tv, a.pc.v, dt, 2, width, rows, width * 2, 64, box))
         return -3;
     if (!prefix) tqp = tq;
-    e2c_launch_as(true, k_attention_pages<T, D>, dim3(sms), dim3(NTHREADS), smem_bytes<D>(), st, tq, tqp, tk, tv, a, q_box, qp_box);
+    e2c_launch_as(true, k_attention_pages<T, D>, dim3(sms), dim3(Cfg<D>::NTHREADS), smem_bytes<D>(), st, tq, tqp, tk, tv, a, q_box, qp_box);
     if (launch_error("pages_attention")) return -2;
     using J = Join<T, D>;
     if (prefix)
