@@ -16,8 +16,8 @@
 //   S = Q K_j^T     fp32 in tensor memory, N rounded up to 16 keys in an item's last tile
 //   P = exp2(S scale log2 e - m)  16 bits over S's columns; m moves only when it grows by 2^8, then O is rescaled
 //   O += P V_j      fp32 in tensor memory; V is read as it lies in the cache (its head dim contiguous)
-// P is rounded to the cache's type, the tensor cores' operand; its sum, m and O are held in 32 bits. The two softmax
-// warpgroups take alternate tiles, handing the running maximum on as soon as a tile's is known, so
+// P is rounded to the cache's type, the tensor cores' operand; its sum, m and O are held in 32 bits. The
+// softmax warpgroups take the tiles in turn, handing the running maximum on as soon as a tile's is known, so
 // that their exponentials overlap.
 //
 // K and V have a ring of stages and a loading warp each; pages arrive one TMA box each (a page's rows land as
@@ -26,11 +26,12 @@
 // vanish. Keys past it are masked in S by a select.
 //
 // What bounds it (one B200, CUDA events): long single-token batches the memory (64 sequences of 8192
-// tokens, 32 heads of 128 over 8 key heads: 270 us, 6.5 TB/s); whole prompts the issue and softmax of a
-// tile, some 1500 cycles for 128 rows by 128 keys (4 x 4096 tokens, 16 heads of 128 over 4: 390 us, 63% of
-// the measured bf16 rate; 8 heads of 256: 335 us, 73%; 16 heads of 64: 350 us); short sequences an item's
-// set-up and output, some 3500 cycles (512 x 16 tokens, 8 key heads: 60 us). A tile's time does not
-// depend on the rings' depth (2 or 5 stages) nor on a third softmax group by more than 5%.
+// tokens, 32 heads of 128 over 8 key heads: 280 us, 96% of the copy rate); whole prompts the chain from S to P
+// in the softmax warps, some 1500 cycles a tile of 128 rows by 128 keys where the products take 512 to
+// 2048 (4 x 4096 tokens, every key: 16 heads of 128 over 4 388 us, 63% of the measured bf16 rate; 8 heads
+// of 256 over 4 315 us, 78%; 16 heads of 64 over 4 338 us); short sequences an item's set-up and output, some
+// 3500 cycles (512 x 16 tokens, 8 key heads: 60 us). The rings' depth (2 to 5 stages) moves a tile's time by
+// less than 2%; so does a thread for each of the two products, except that heads of 256 lose 10%.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -52,7 +53,7 @@ constexpr int TK = 128;  // keys of a tile
 constexpr int NI = 8;  // item descriptors in flight
 // What a sequence item costs beside its tiles, in tiles: its set-up and its output
 constexpr int ITEM_COST = 1;
-constexpr int PREFIX_TILES = 13;
+constexpr int PREFIX_TILES = 13;  // use_prefix
 constexpr float kRescaleLog2 = 8.0f;
 
 // A wait of a whole warp, bounded by its number of (sleeping) tries: up to 1.3 s. It is small on
@@ -72,7 +73,11 @@ constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 
 template <int D>
 struct Cfg {
-    // warps: NG softmax groups of four, the epilogue's four, then one each
+    // warps: NG softmax groups of four, the epilogue's four, then one each. A third softmax group hides more
+    // of a tile's latencies where its products are shortest (heads of 64, us with two and with three: 4 x 4096
+    // tokens 366 and 338, single tokens behind 700 of their own 55.4 and 52.1, behind 16 42.3 and 43.5); with wider
+    // heads it gives less and costs batches of short items (128: 385 and 374, 92.9 and 94.1 for 128
+    // tokens behind a shared prefix; 256: 312 and 314)
     static constexpr int NG = D == 64 ? 3 : 2;
     static constexpr int W_EPI = 4 * NG, W_ITEMS = W_EPI + 4, W_MMA = W_ITEMS + 1, W_K = W_MMA + 1, W_V = W_K + 1;
     static constexpr int WARPS = W_V + 1, NTHREADS = 32 * WARPS;
@@ -407,7 +412,8 @@ E2C_DEV float2 add2(float2 a, float2 b) {
 // the whole number n and leaves it in the low bits), a polynomial of degree 4 in f fitted to the
 // least relative error (2.6e-6), and n added to the exponent. Below 2^-125 the result stays there.
 // One exponential in kPoly pairs takes this way: the exponential unit's 16 a cycle are what
-// bounds 64-wide heads, and nearly bound 128-wide ones.
+// bounds 64-wide heads, and nearly bound 128-wide ones (us with and without: 4 x 4096 tokens, heads of
+// 128 388 and 392, of 256 314 and 319; ragged prompts in a window, heads of 64 172 and 175).
 constexpr int kPoly = 4;
 E2C_DEV float2 ex2_poly(float2 x) {
     const float2 big = make_float2(12582912.f, 12582912.f), less = make_float2(-12582912.f, -12582912.f);
