@@ -5,12 +5,15 @@
 //   a' = a c - b s,  b' = b c + a s          (its transpose, the gradient: s -> -s)
 // for the rot / 2 pairs (i, i + rot/2), or (2i, 2i+1) interleaved; dimensions past rot pass through.
 //
-// Bound: memory. One thread owns V pairs (V elements = 16 bytes of the output type) of up to four
-// heads of one token, so a pair's cos and sin are read once for four heads and every thread has up to
-// eight 16-byte loads in flight (16384 x 40 heads of 128 in fp32: 100 us, 6.7 TB/s; 24000 rows of 8 heads
-// of 256 from fp32 into pages: 47 us, 5.5 TB/s; a quarter of 24 heads of 64: 36 us, 3.4 TB/s, the
-// rotated and the copied dimensions taking different paths in one warp). Decode-sized calls are bound by
-// their launch (4 to 8 us). All arithmetic is in 32 bits with one rounding at the store. Rows
+// Bound: memory. One thread owns two runs of V elements (16 bytes of the output type) at the same place of up
+// to four heads of one token: the two halves of V pairs, or dimensions that pass through. A pair's cos
+// and sin are read once for four heads; every access of neighbouring threads is contiguous, whatever
+// is rotated in it; and loads come before the branch on what to do with them, as they lie in memory (as
+// floats they took twice the registers, and with a thread's runs side by side half sectors were written:
+// 16384 x 40 heads of 128 in bf16 92 us, now 57; 24000 tokens of 48 heads into pages 160, now 86).
+// Further: fp32, the same heads, 106 us, 97% of the copy rate; 24000 rows of 8 heads of 256 from fp32 into pages
+// 53 us; a quarter of 24 heads of 64 rotated, 20011 tokens, 29 us. Decode-sized calls are bound by
+// their launch (4 us). All arithmetic is in 32 bits with one rounding at the store. Rows
 // that 16-byte accesses do not fit (an odd stride, a rot whose halves are not multiples of V, an
 // unaligned base) take V = 1.
 #include <cuda_bf16.h>
@@ -60,22 +63,7 @@ E2C_DEV __half from_f(float x) {
     return __float2half_rn(x);
 }
 
-// N consecutive values as floats; N * sizeof(T) is a multiple of 16 with 16-byte alignment, or N = 1
-template <typename T, int N>
-E2C_DEV void load(const T *p, float (&r)[N]) {
-    if constexpr (N == 1) {
-        r[0] = to_f<T>(*p);
-    } else {
-        constexpr int PER = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < N; i += PER) {
-            const uint4 w = *reinterpret_cast<const uint4 *>(p + i);
-            const T *e = reinterpret_cast<const T *>(&w);
-#pragma unroll
-            for (int j = 0; j < PER; j++) r[i + j] = to_f<T>(e[j]);
-        }
-    }
-}
+// N consecutive values; N * sizeof(T) is a multiple of 16 with 16-byte alignment, or N = 1
 template <typename T, int N>
 E2C_DEV void store(T *p, const float (&r)[N]) {
     if constexpr (N == 1) {
@@ -93,23 +81,40 @@ E2C_DEV void store(T *p, const float (&r)[N]) {
     }
 }
 
-// N values from x to y: as they are where the types are the same
-template <typename TI, typename TO, int N>
-struct Copy {
-    float f[N];
-    uint4 w[N * sizeof(TI) / 16 ? N * sizeof(TI) / 16 : 1];
-    static constexpr bool raw = std::is_same<TI, TO>::value && N > 1;
-    E2C_DEV void get(const TI *x) {
-        if constexpr (raw)
-            w[0] = *reinterpret_cast<const uint4 *>(x);
-        else
-            load<TI, N>(x, f);
+// N values as they lie in memory
+template <typename T, int N>
+struct Raw {
+    static constexpr int WORDS = N == 1 ? 0 : N * sizeof(T) / 16;
+    uint4 w[WORDS ? WORDS : 1];
+    T one;
+    E2C_DEV void get(const T *p) {
+        if constexpr (N == 1) {
+            one = *p;
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) w[i] = reinterpret_cast<const uint4 *>(p)[i];
+        }
     }
-    E2C_DEV void put(TO *y) const {
-        if constexpr (raw)
-            *reinterpret_cast<uint4 *>(y) = w[0];
-        else
-            store<TO, N>(y, f);
+    E2C_DEV void floats(float (&r)[N]) const {
+        if constexpr (N == 1) {
+            r[0] = to_f<T>(one);
+        } else {
+            const T *e = reinterpret_cast<const T *>(w);
+#pragma unroll
+            for (int i = 0; i < N; i++) r[i] = to_f<T>(e[i]);
+        }
+    }
+    // to y: bit for bit where the types are the same
+    template <typename TO>
+    E2C_DEV void copy(TO *y) const {
+        if constexpr (std::is_same<T, TO>::value && N > 1) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) reinterpret_cast<uint4 *>(y)[i] = w[i];
+        } else {
+            float r[N];
+            floats(r);
+            store<TO, N>(y, r);
+        }
     }
 };
 
@@ -119,53 +124,57 @@ struct Div {
 };
 E2C_DEV uint32_t div_by(uint32_t u, const Div &v) { return v.d == 1 ? u : (uint32_t)(__umulhi(u, v.mul) >> v.shift); }
 
-// V pairs of one head: the raw values at the two places, and the rotation
-template <typename TI, typename TO, int V>
-struct Pairs {
-    float a[V], b[V];
-    // pairs j V .. j V + V - 1 of the head at x
-    E2C_DEV void get(const TI *x, int j, int half, bool inter) {
-        if (!inter) {
-            load<TI, V>(x + j * V, a);
-            load<TI, V>(x + half + j * V, b);
-        } else if constexpr (V == 1) {
-            a[0] = to_f<TI>(x[2 * j]);
-            b[0] = to_f<TI>(x[2 * j + 1]);
-        } else {
-            load<TI, V>(x + 2 * j * V, a);
-            load<TI, V>(x + 2 * j * V + V, b);
-        }
-    }
-    E2C_DEV void put(TO *y, int j, int half, bool inter, const float (&c)[V], const float (&s)[V]) {
-        if (!inter || V == 1) {
-            float u[V], w[V];
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                u[i] = a[i] * c[i] - b[i] * s[i];
-                w[i] = b[i] * c[i] + a[i] * s[i];
-            }
-            if (inter) {
-                y[2 * j] = from_f<TO>(u[0]);
-                y[2 * j + 1] = from_f<TO>(w[0]);
-            } else {
-                store<TO, V>(y + j * V, u);
-                store<TO, V>(y + half + j * V, w);
-            }
-        } else {
-            // a holds elements 0 .. V-1 of the 2 V interleaved ones, b the others
-            float u[V], w[V];
-#pragma unroll
-            for (int i = 0; i < V; i += 2) {
-                u[i] = a[i] * c[i / 2] - a[i + 1] * s[i / 2];
-                u[i + 1] = a[i + 1] * c[i / 2] + a[i] * s[i / 2];
-                w[i] = b[i] * c[(V + i) / 2] - b[i + 1] * s[(V + i) / 2];
-                w[i + 1] = b[i + 1] * c[(V + i) / 2] + b[i] * s[(V + i) / 2];
-            }
-            store<TO, V>(y + 2 * j * V, u);
-            store<TO, V>(y + 2 * j * V + V, w);
-        }
-    }
+// A thread's part of each of its heads: V elements from e0 on and V from e1 on, which neighbouring threads
+// continue; together V pairs, or some of the dimensions that pass through.
+struct Part {
+    int e0, e1;
+    bool two, turn;  // there is a second run; it is rotated
 };
+template <int V>
+E2C_DEV Part part_of(int j, int half, int units, int D, bool inter) {
+    const int nrot = half / V;
+    if (j < nrot && V == 1 && inter) return {2 * j, 2 * j + 1, true, true};
+    if (j < nrot) return {j * V, half + j * V, true, true};
+    const int e0 = 2 * half + (j - nrot) * V, e1 = e0 + (units - nrot) * V;
+    return {e0, e1, e1 < D, false};
+}
+// the angles of unit j's V pairs: those of its first run and those of its second
+template <int V>
+E2C_DEV void angles(const float *t, int j, int half, bool inter, float (&r)[V]) {
+    if constexpr (V == 1) {
+        r[0] = t[j];
+    } else {
+        const float *a = t + (inter ? j * V / 2 : j * V), *b = inter ? a + half / 2 : a + V / 2;
+        using Half = std::conditional_t<V == 8, float4, float2>;
+        static_assert(sizeof(Half) * 2 == sizeof r, "16-bit or 32-bit results");
+        reinterpret_cast<Half *>(r)[0] = *reinterpret_cast<const Half *>(a);
+        reinterpret_cast<Half *>(r)[1] = *reinterpret_cast<const Half *>(b);
+    }
+}
+template <typename TI, typename TO, int V>
+E2C_DEV void turn(const Raw<TI, V> &x0, const Raw<TI, V> &x1, TO *y0, TO *y1, bool inter, const float (&c)[V],
+                  const float (&s)[V]) {
+    float a[V], b[V], u[V], w[V];
+    x0.floats(a);
+    x1.floats(b);
+    if (!inter || V == 1) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            u[i] = a[i] * c[i] - b[i] * s[i];
+            w[i] = b[i] * c[i] + a[i] * s[i];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i + 1 < V; i += 2) {
+            u[i] = a[i] * c[i / 2] - a[i + 1] * s[i / 2];
+            u[i + 1] = a[i + 1] * c[i / 2] + a[i] * s[i / 2];
+            w[i] = b[i] * c[(V + i) / 2] - b[i + 1] * s[(V + i) / 2];
+            w[i + 1] = b[i + 1] * c[(V + i) / 2] + b[i] * s[(V + i) / 2];
+        }
+    }
+    store<TO, V>(y0, u);
+    store<TO, V>(y1, w);
+}
 
 struct RopeArgs {
     const void *x;
@@ -191,40 +200,34 @@ __global__ void __launch_bounds__(BLOCK) k_rope(const RopeArgs p, const Div per_
     const int h0 = hg * HPT, nh = min(HPT, p.H - h0);
     const TI *x = static_cast<const TI *>(p.x) + t * p.ldx + (int64_t)h0 * p.D;
     TO *y = static_cast<TO *>(p.y) + t * p.ldy + (int64_t)h0 * p.D;
-    const int nrot = p.half / V;
-    if (j < nrot) {
-        Pairs<TI, TO, V> r[HPT];
+    const Part at = part_of<V>(j, p.half, (int)units.d, p.D, p.inter);
+    Raw<TI, V> a[HPT], b[HPT];
 #pragma unroll
-        for (int h = 0; h < HPT; h++)
-            if (h < nh) r[h].get(x + h * p.D, j, p.half, p.inter);
-        int at = p.pos ? p.pos[t] : t;
-        if ((unsigned)at >= (unsigned)p.positions) {
-            record_status(p.status, E2C_ERR_BAD_POSITION);
-            at = 0;
+    for (int h = 0; h < HPT; h++)
+        if (h < nh) {
+            a[h].get(x + h * p.D + at.e0);
+            if (at.two) b[h].get(x + h * p.D + at.e1);
         }
-        float c[V], s[V];
-        load<float, V>(p.cs + (int64_t)at * p.half + j * V, c);
-        load<float, V>(p.sn + (int64_t)at * p.half + j * V, s);
+    if (at.turn) {
+        int pos = p.pos ? p.pos[t] : t;
+        if ((unsigned)pos >= (unsigned)p.positions) {
+            record_status(p.status, E2C_ERR_BAD_POSITION);
+            pos = 0;
+        }
+        alignas(16) float c[V], s[V];
+        angles<V>(p.cs + (int64_t)pos * p.half, j, p.half, p.inter, c);
+        angles<V>(p.sn + (int64_t)pos * p.half, j, p.half, p.inter, s);
 #pragma unroll
         for (int i = 0; i < V; i++) s[i] *= p.sign;
 #pragma unroll
         for (int h = 0; h < HPT; h++)
-            if (h < nh) r[h].put(y + h * p.D, j, p.half, p.inter, c, s);
+            if (h < nh) turn<TI, TO, V>(a[h], b[h], y + h * p.D + at.e0, y + h * p.D + at.e1, p.inter, c, s);
     } else {
-        const int e = 2 * p.half + (j - nrot) * 2 * V;
-        const bool two = e + V < p.D;
-        Copy<TI, TO, V> a[HPT], b[HPT];
 #pragma unroll
         for (int h = 0; h < HPT; h++)
             if (h < nh) {
-                a[h].get(x + h * p.D + e);
-                if (two) b[h].get(x + h * p.D + e + V);
-            }
-#pragma unroll
-        for (int h = 0; h < HPT; h++)
-            if (h < nh) {
-                a[h].put(y + h * p.D + e);
-                if (two) b[h].put(y + h * p.D + e + V);
+                a[h].copy(y + h * p.D + at.e0);
+                if (at.two) b[h].copy(y + h * p.D + at.e1);
             }
     }
 }
@@ -264,20 +267,13 @@ __global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, const 
     const TI *x = is_q ? static_cast<const TI *>(p.q) + t * p.ldq
                        : is_v ? static_cast<const TI *>(p.v) + t * p.ldv : static_cast<const TI *>(p.k) + t * p.ldk;
     x += (int64_t)h0 * D;
-    const int nrot = p.half / V;
-    const bool turn = !is_v && j < nrot;
-    const int e = is_v ? j * 2 * V : 2 * p.half + (j - nrot) * 2 * V;  // the first element passed through
-    const bool two = e + V < D;
-    Pairs<TI, TO, V> r[HPT];
+    const Part part = is_v ? part_of<V>(j, 0, (int)vunits.d, D, false) : part_of<V>(j, p.half, (int)units.d, D, p.inter);
+    Raw<TI, V> a[HPT], b[HPT];
 #pragma unroll
     for (int h = 0; h < HPT; h++)
         if (h < nh) {
-            if (turn) {
-                r[h].get(x + h * D, j, p.half, p.inter);
-            } else {
-                load<TI, V>(x + h * D + e, r[h].a);
-                if (two) load<TI, V>(x + h * D + e + V, r[h].b);
-            }
+            a[h].get(x + h * D + part.e0);
+            if (part.two) b[h].get(x + h * D + part.e1);
         }
     int last;
     const int i = e2c_token_seq(p.q_start, p.n, p.T, t, last);
@@ -303,19 +299,19 @@ __global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, const 
         y = static_cast<TO *>(is_v ? p.pc.v : p.pc.k) + row * (KV * D);
     }
     y += (int64_t)h0 * D;
-    if (turn) {
-        float c[V], s[V];
-        load<float, V>(p.cs + (int64_t)at * p.half + j * V, c);
-        load<float, V>(p.sn + (int64_t)at * p.half + j * V, s);
+    if (part.turn) {
+        alignas(16) float c[V], s[V];
+        angles<V>(p.cs + (int64_t)at * p.half, j, p.half, p.inter, c);
+        angles<V>(p.sn + (int64_t)at * p.half, j, p.half, p.inter, s);
 #pragma unroll
         for (int h = 0; h < HPT; h++)
-            if (h < nh) r[h].put(y + h * D, j, p.half, p.inter, c, s);
+            if (h < nh) turn<TI, TO, V>(a[h], b[h], y + h * D + part.e0, y + h * D + part.e1, p.inter, c, s);
     } else {
 #pragma unroll
         for (int h = 0; h < HPT; h++)
             if (h < nh) {
-                store<TO, V>(y + h * D + e, r[h].a);
-                if (two) store<TO, V>(y + h * D + e + V, r[h].b);
+                a[h].copy(y + h * D + part.e0);
+                if (part.two) b[h].copy(y + h * D + part.e1);
             }
     }
 }
