@@ -27,11 +27,12 @@
 //
 // What bounds it (one B200, CUDA events): long single-token batches the memory (64 sequences of 8192
 // tokens, 32 heads of 128 over 8 key heads: 280 us, 96% of the copy rate); whole prompts the chain from S to P
-// in the softmax warps, some 1500 cycles a tile of 128 rows by 128 keys where the products take 512 to
-// 2048 (4 x 4096 tokens, every key: 16 heads of 128 over 4 388 us, 63% of the measured bf16 rate; 8 heads
-// of 256 over 4 315 us, 78%; 16 heads of 64 over 4 338 us); short sequences an item's set-up and output, some
-// 3500 cycles (512 x 16 tokens, 8 key heads: 60 us). The rings' depth (2 to 5 stages) moves a tile's time by
-// less than 2%; so does a thread for each of the two products, except that heads of 256 lose 10%.
+// in the softmax warps and the products' issue, some 1800 (heads of 64) to 3500 cycles (of 256) a tile of
+// 128 rows by 128 keys where the products take 512 to 2048 (4 sequences of up to 4096 tokens, every key: 16
+// heads of 128 over 4 388 us, 63% of the measured bf16 rate; 8 heads of 256 over 4 315 us, 78%; 16 heads of 64
+// over 4 338 us); short sequences an item's set-up and output, some 3500 cycles (512 x 16 tokens, 8 key
+// heads: 60 us). The rings' depth (2 to 5 stages) moves a tile's time by less than 2%; so does a thread
+// for each of the two products, except that heads of 256 lose 10%.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
