@@ -256,6 +256,15 @@ E2C_DEV int span_of(const Args &p, int len, int nq, int r, int base, int &k0, in
     klim = hi;
     return (hi - k0 + TK - 1) / TK;
 }
+// whether a row at position pos of a sequence of len tokens sees any key
+E2C_DEV bool sees_keys(const Args &p, int pos, int len) {
+    int lo = 0, hi = p.causal ? min(len, pos + 1) : len;
+    if (p.window >= 0) {
+        lo = max(lo, pos - p.window);
+        hi = min(hi, pos + p.window + 1);
+    }
+    return lo < hi;
+}
 // the cost of all of an entry's row tiles, for one key head
 E2C_DEV int64_t tiles_of(const Args &p, int len, int nq, int base) {
     if (nq <= 0) return 0;
@@ -389,11 +398,19 @@ E2C_DEV float ex2_approx(float x) {
     return y;
 }
 
+// Maxima that a NaN stays in. A row whose largest logit is NaN or +infinity has no softmax: its running maximum
+// keeps that value to the end, and the result is NaN whatever the sums became meanwhile.
 E2C_DEV float max3(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
+E2C_DEV float max2(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+E2C_DEV bool no_softmax(float m) { return !(m < INFINITY); }
 // two fp32 operations in one instruction
 E2C_DEV float2 fma2(float2 a, float2 b, float2 c) {
     float2 y;
@@ -963,12 +980,12 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                             for (int i = 0; i < 16; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
                     }
-                    mx = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])) * p.c;
+                    mx = max2(max2(mm[0], mm[1]), max2(mm[2], mm[3])) * p.c;
                 }
                 float now = before, alpha = 1.f;
-                if (live && (mx > before + kRescaleLog2 || (before == -INFINITY && mx > -INFINITY))) {
-                    now = mx;
-                    alpha = ex2_approx(before - mx);
+                if (live && !(mx <= before + kRescaleLog2)) {  // so also from -infinity, and for a NaN
+                    now = max2(before, mx);
+                    alpha = ex2_approx(before - now);
                 }
                 xm[group * TR + row] = now;
                 __syncwarp();
@@ -1091,23 +1108,25 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
             for (int i = 0; i < C::NG; i++) a[i] = ml[((item & 1) * C::NG + i) * TR + row];
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_MLE + (item & 1)));
-            // the groups' sums, to the largest maximum; a row that none saw a key of has l = 0
+            // the groups' sums, to the largest maximum; l = 0: every logit was -infinity, or no key was seen
             float m = a[0].x, l = 0.f;
 #pragma unroll
-            for (int i = 1; i < C::NG; i++) m = fmaxf(m, a[i].x);
+            for (int i = 1; i < C::NG; i++) m = max2(m, a[i].x);
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
             for (int i = 0; i < C::NG; i++) l += a[i].y * ex2_approx(a[i].x - ref);
-            const bool live = tok < it.ntok, some = l > 0.f;
-            const float inv = some ? __fdividef(1.0f, l) : 0.f;
+            const bool live = tok < it.ntok, bad = no_softmax(m), some = bad || l > 0.f;
+            const float inv = bad ? NAN : some ? __fdividef(1.0f, l) : 0.f;
+            float none = 0.f;  // the result of a row with l = 0; a part leaves that to the join
             const int64_t t = it.t0 + tok;
             const int h = it.kvh * p.G + hd;
             const bool busy = quad * 32 < it.ntok * p.G;
             T *out = nullptr;
             float *part = nullptr;
             if (busy) {
-                const float sums = some ? m + __log2f(l) : -INFINITY;
+                const float sums = bad ? m : some ? m + __log2f(l) : -INFINITY;
                 if (it.dst == TO_OUT) {
+                    if (!some && sees_keys(p, it.pos0 + tok, it.len)) none = NAN;
                     out = static_cast<T *>(p.out) + t * p.ldo + h * D;
                     if (live && p.lse) p.lse[t * p.H + h] = sums * LN2;
                 } else {
@@ -1138,7 +1157,7 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                 }
                 if (live && !some) {  // such a row may have met a page's NaN: its zeros are not a product
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[i] = 0.f;
+                    for (int i = 0; i < 16; i++) o[i] = none;
                 }
                 if (live && out) {
                     uint4 *y = reinterpret_cast<uint4 *>(out + c);
@@ -1169,10 +1188,10 @@ struct Join {
     static constexpr int LANES = D / 4, ROWS = JOIN / LANES;
     float4 acc = {0, 0, 0, 0};
     float m = -INFINITY, l = 0.f;
-    // a part's sums and its log-sum-exp; -infinity: it saw nothing
+    // a part's sums and its log-sum-exp; -infinity: it adds nothing
     E2C_DEV void add(const float *o, const float *sums, int x) {
         const float4 v = *reinterpret_cast<const float4 *>(o + 4 * x);
-        const float s = *sums, mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
+        const float s = *sums, mn = max2(m, s), ref = mn == -INFINITY ? 0.f : mn;
         const float a = exp2f(m - ref), w = exp2f(s - ref);
         acc.x = acc.x * a + w * v.x;
         acc.y = acc.y * a + w * v.y;
@@ -1181,14 +1200,17 @@ struct Join {
         l = l * a + w;
         m = mn;
     }
-    E2C_DEV void put(const Args &p, int64_t t, int h, int x) {
-        const float inv = l > 0.f ? __fdiv_rn(1.0f, l) : 0.f;
+    // sees(): whether the row sees any key, asked only if its parts add up to nothing
+    template <typename Sees>
+    E2C_DEV void put(const Args &p, int64_t t, int h, int x, Sees sees) {
+        const bool bad = no_softmax(m);
+        const float inv = bad ? NAN : l > 0.f ? __fdiv_rn(1.0f, l) : sees() ? NAN : 0.f;
         T *y = static_cast<T *>(p.out) + t * p.ldo + (int64_t)h * D + 4 * x;
         uint2 v;
         v.x = pack2<T>(acc.x * inv, acc.y * inv);
         v.y = pack2<T>(acc.z * inv, acc.w * inv);
         *reinterpret_cast<uint2 *>(y) = v;
-        if (p.lse && x == 0) p.lse[t * p.H + h] = l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
+        if (p.lse && x == 0) p.lse[t * p.H + h] = bad ? m : l > 0.f ? (m + log2f(l)) * LN2 : -INFINITY;
     }
 };
 
@@ -1211,7 +1233,13 @@ __global__ void __launch_bounds__(JOIN) k_join_split(const Args p, int grid) {
 #pragma unroll 4
         for (int c = blockIdx.x; c <= c1; c++) j.add(p.po + ((int64_t)(2 * c) * TR + row) * D, p.pl + (int64_t)(2 * c) * TR + row, x);
         const int tok = row / p.G;
-        j.put(p, a.x + tok, a.z * p.G + (row - tok * p.G), x);
+        j.put(p, a.x + tok, a.z * p.G + (row - tok * p.G), x, [&]() {
+            int last;
+            const int i = e2c_token_seq(p.q_start, p.n, p.T, a.x + tok, last);
+            if (i < 0) return false;
+            const Entry e = entry_of(p, i, false);
+            return sees_keys(p, e.len - (last - a.x - tok), e.len);
+        });
     }
 }
 
@@ -1250,7 +1278,7 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
         const int row = (int)(t - e.q0) * p.G + hd;
         for (int c = c0; c <= c1; c++) slot(2 * c + (c == c0 && s > share.begin(c0) ? 1 : 0), row);
     }
-    j.put(p, t, h, x);
+    j.put(p, t, h, x, [&]() { return sees_keys(p, e.len - e.nq + (int)t - e.q0, e.len); });
 }
 
 // Sequences of few query tokens fill a small part of a 128-row tile each; packed, the batch reads the prefix

@@ -519,6 +519,108 @@ def test_attention_scales(e2c, torch_cuda, scale):
     assert_attention(torch, out, lse, attention64(torch, cache, 0, q, seqs, q_start, True, -1, scale), "bf16", 400)
 
 
+def same_where_not_finite(torch, got, lse, want, big, name, keys):
+    """NaN and infinite sums exactly where the 64-bit form has them; every other row within the tolerance."""
+    out, mag, ref, _ = want
+    lost = torch.isnan(out)
+    assert torch.equal(torch.isnan(got), lost)
+    assert torch.equal(torch.isnan(lse), torch.isnan(ref)) and torch.equal(torch.isinf(lse), torch.isinf(ref))
+    endless = torch.isinf(ref)
+    assert torch.equal(lse[endless] > 0, ref[endless] > 0)
+
+    def settled(x):
+        return x.masked_fill(lost, 0.0)
+
+    fill = 0.0 if ref.isnan().any() or endless.any() else None
+    sums = [x if fill is None else x.masked_fill(~torch.isfinite(ref), fill) for x in (lse, ref)]
+    assert_attention(torch, settled(got), sums[0], (settled(out), settled(mag), sums[1], big), name, keys)
+
+
+UNSETTLED = {
+    # lens, queries, shared, KV: every item in one block; items that blocks share; a prefix read for the batch
+    "undivided": ([384] * 148, [2] * 148, 0, 1),
+    "divided": ([20011, 15000, 9000], [1, 3, 2], 0, 2),
+    "prefix": ([512 + (7 * i) % 130 + 2 for i in range(160)], [1 + (i % 5 == 0) for i in range(160)], 512, 5),
+}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("what", ["q nan", "k nan", "k inf", "v nan"])
+@pytest.mark.parametrize("form", list(UNSETTLED))
+def test_attention_keeps_nan_and_infinity(e2c, torch_cuda, form, what, D, dtype):
+    """A NaN in a query, a key or a value in sight, and the NaN of an infinite logit, reach the result, in
+    whatever column of a tile the key lies; rows that do not see them are right."""
+    torch = torch_cuda
+    lens, queries, shared, KV = UNSETTLED[form]
+    H = 2 * KV
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 31, lens, queries, shared, H, KV, D, 16, dtype)
+    big = attention64(torch, cache, 0, q, seqs, q_start, False, -1, D ** -0.5)[3]
+    rng = np.random.default_rng(D)
+    if what == "q nan":
+        for t in range(0, q.shape[0], 3):
+            q[t, t % H, t * 5 % D] = float("nan")
+    else:
+        x = cache.v if what == "v nan" else cache.k
+        value = float("nan") if what.endswith("nan") else float("inf")
+        for i in range(1, len(lens), 2):  # one key head of every second sequence, at every column of a tile
+            j = shared + (37 * i) % (lens[i] - shared)
+            x[0, int(cache.table[i, j // 16]), j % 16, i % KV, rng.integers(D)] = value
+        if form == "prefix":  # and of one token that all share, in one key head
+            x[0, int(cache.table[0, 300 // 16]), 300 % 16, 2, 5] = value
+    out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, causal=False, lse=True)
+    e2c.check()
+    want = attention64(torch, cache, 0, q, seqs, q_start, False, -1, D ** -0.5)
+    assert torch.isnan(want[0]).any() and not torch.isnan(want[0]).all()
+    same_where_not_finite(torch, out, lse, want, big, dtype, max(lens))
+
+
+@pytest.mark.parametrize("at", range(0, 128, 3))
+def test_attention_keeps_a_nan_of_every_column(e2c, torch_cuda, at):
+    """One NaN key in the first, whole tile of 300 keys."""
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 32, [300], [3], 0, 4, 2, 128, 64, "bf16")
+    cache.k[0, int(cache.table[0, at // 64]), at % 64, 1, 0] = float("nan")
+    out, lse = cache.attention(0, q, seqs, q_start, max_q, lse=True)
+    e2c.check()
+    assert torch.isnan(out[:, 2:]).all() and torch.isnan(lse[:, 2:]).all()
+    assert torch.isfinite(out[:, :2]).all() and torch.isfinite(lse[:, :2]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("form", list(UNSETTLED))
+def test_attention_of_infinite_logits_only(e2c, torch_cuda, form, D):
+    """Every key infinite in one dimension: logits of +infinity (q > 0 there) or -infinity. No softmax of either
+    exists, the sums are what they are; a row without a key in sight still gets zeros."""
+    torch = torch_cuda
+    lens, queries, shared, KV = UNSETTLED[form]
+    lens = [0 if i == 1 and form != "prefix" else n for i, n in enumerate(lens)]
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 33, lens, queries, shared, 2 * KV, KV, D, 16, "f16")
+    cache.k[..., 0] = float("inf")
+    q[..., 0] = 1.0
+    q[:, 1::2, 0] = -1.0
+    out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, causal=False, lse=True)
+    e2c.check()
+    counts = q_start.long().diff()
+    sees = torch.repeat_interleave(cache.length[seqs.long()] > 0, counts)
+    assert torch.isnan(out[sees]).all() and (out[~sees] == 0).all()
+    assert (lse[sees][:, 0::2] == math.inf).all() and (lse[sees][:, 1::2] == -math.inf).all() and (lse[~sees] == -math.inf).all()
+
+
+def test_attention_hides_nan_keys_out_of_sight(e2c, torch_cuda):
+    """A NaN key that a row's mask leaves out does not reach it."""
+    torch = torch_cuda
+    for D, shared in ((64, 0), (128, 256), (256, 0)):
+        cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 34, [300] * 150, [4] * 150, shared, 2, 1, D, 32, "bf16")
+        for i in range(150):
+            cache.k[0, int(cache.table[i, 298 // 32]), 298 % 32] = float("nan")
+        out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, lse=True)
+        e2c.check()
+        seen = torch.arange(600, device="cuda") % 4 >= 2  # positions 298 and 299
+        assert torch.isnan(out[seen]).all() and torch.isnan(lse[seen]).all()
+        assert torch.isfinite(out[~seen]).all() and torch.isfinite(lse[~seen]).all()
+
+
 def test_attention_strided_rows_and_layers(e2c, torch_cuda):
     """q and out as columns of wider rows, the second layer of the cache; what lies beside out stays."""
     torch = torch_cuda
