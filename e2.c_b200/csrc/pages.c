@@ -189,9 +189,17 @@ int e2cuda_pages_store(const e2cuda_pages *pc, int layer, int x_type, const void
                        "pages_store");
 }
 
+/* what an attention call and the size of its workspace take: a row tile holds 128 (token, head) rows, so one token's
+ * heads over a key head must fit in it */
+static int attention_ok(const e2c_pages *c, int n, int T, int max_q, int heads, int shared) {
+    if (n >= 1 && T >= 1 && max_q >= 1 && heads >= c->KV && heads % c->KV == 0 && heads / c->KV <= 128 && shared >= 0) return 1;
+    e2cu_err("pages_attention: bad batch (n %d, T %d, max_q %d, heads %d over %d, shared %d)", n, T, max_q, heads, c->KV, shared);
+    return 0;
+}
+
 size_t e2cuda_pages_attention_ws_bytes(const e2cuda_pages *pc, int n, int T, int max_q, int heads, int shared) {
     e2c_pages c;
-    if (view(pc, 0, &c, "pages_attention") || n < 1 || T < 1 || max_q < 1 || heads < c.KV || heads % c.KV || shared < 0) return 0;
+    if (view(pc, 0, &c, "pages_attention") || !attention_ok(&c, n, T, max_q, heads, shared)) return 0;
     return e2c_pages_attention_ws_bytes(n, T, max_q, heads, c.KV, c.D, shared);
 }
 
@@ -201,10 +209,10 @@ int e2cuda_pages_attention(const e2cuda_pages *pc, int layer, const void *q, int
     e2c_pages c;
     if (view(pc, layer, &c, "pages_attention")) return -1;
     if (T == 0) return 0;
-    if (!batch_ok(seqs, q_start, n, T, heads, c.KV, "pages_attention")) return -1;
+    if (!batch_ok(seqs, q_start, n, T, heads, c.KV, "pages_attention") || !attention_ok(&c, n, T, max_q, heads, shared)) return -1;
     const int64_t row = (int64_t)heads * c.D;
-    if (!q || !out || ldq < row || ldo < row || max_q < 1 || max_q > T || !isfinite(scale) || heads / c.KV > 128 || shared < 0 ||
-        shared % c.page || shared > (int64_t)c.max_blocks * c.page) {
+    if (!q || !out || ldq < row || ldo < row || max_q > T || !isfinite(scale) || shared % c.page ||
+        shared > (int64_t)c.max_blocks * c.page) {
         e2cu_err("pages_attention: bad arguments (ld %d -> %d, max_q %d, heads %d over %d, shared %d of pages of %d)", ldq, ldo,
                  max_q, heads, c.KV, shared, c.page);
         return -1;

@@ -650,6 +650,16 @@ def test_attention_sequence_outside_the_cache(e2c, torch_cuda):
     assert_attention(torch, out[keep], lse[keep], want, "bf16", 70)
 
 
+def test_attention_refuses_too_many_heads_for_a_key_head(e2c, torch_cuda):
+    torch = torch_cuda
+    cache = e2c.PageCache.new(1, 4, 16, 1, 64, 2, 4, torch.bfloat16)
+    q = torch.zeros(1, 129, 64, device="cuda", dtype=torch.bfloat16)
+    seqs, q_start = torch.tensor([0], device="cuda").int(), torch.tensor([0, 1], device="cuda").int()
+    with pytest.raises(e2c.E2CudaError, match="heads 129 over 1"):
+        cache.attention(0, q, seqs, q_start, 1)
+    e2c.check()
+
+
 def test_attention_past_32_bit_offsets(e2c, torch_cuda):
     """A pool of over 2^32 bytes in one layer: pages at its end are read."""
     torch = torch_cuda

@@ -73,6 +73,19 @@ def test_bad_attention_is_refused(e2c, over):
     assert e2c.last_error().startswith("pages_attention")
 
 
+BAD_SIZES = [dict(n=0), dict(T=0), dict(max_q=0), dict(heads=3), dict(heads=1), dict(heads=258), dict(heads=256 * 129), dict(shared=-16)]
+
+
+@pytest.mark.parametrize("over", BAD_SIZES, ids=[str(o) for o in BAD_SIZES])
+def test_bad_attention_workspace_is_refused(e2c, over):
+    """The size is asked for before the call: what the call refuses has none, and says so."""
+    lib, p = e2c.lib(), pages(e2c)
+    lib.e2cuda_pages_copy(C.addressof(p), None, None, -1, None)  # leaves another message
+    size = lib.e2cuda_pages_attention_ws_bytes(C.addressof(p), *dict(dict(n=2, T=4, max_q=2, heads=4, shared=0), **over).values())
+    assert size == 0
+    assert e2c.last_error().startswith("pages_attention")
+
+
 def test_no_rows_do_nothing(e2c):
     p = pages(e2c)
     assert e2c.lib().e2cuda_pages_attention(C.addressof(p), *dict(ATTENTION, T=0).values(), None) == 0
