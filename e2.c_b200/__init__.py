@@ -381,8 +381,15 @@ def _type(t) -> int:
         raise E2CudaError(f"element type {t.dtype}: fp32, bf16 or fp16") from None
 
 
-def _rows(t, what: str) -> int:
-    """Elements between the rows of a [rows][heads][head_dim] tensor whose heads lie side by side."""
+def _on(t, what: str, device: int) -> None:
+    """Refuses a tensor of the host or of another GPU: its address would go to a kernel on this one."""
+    if t.get_device() != device:  # -1: the host
+        raise E2CudaError(f"{what}: a tensor on cuda:{device}, got {t.device}")
+
+
+def _rows(t, what: str, device: int) -> int:
+    """Elements between the rows of a [rows][heads][head_dim] tensor on the GPU whose heads lie side by side."""
+    _on(t, what, device)
     s = t.stride()
     if len(s) != 3:
         raise E2CudaError(f"{what}: [rows][heads][head_dim], got {tuple(t.shape)}")
@@ -392,17 +399,19 @@ def _rows(t, what: str) -> int:
     return s[0] if rows > 1 else heads * dim
 
 
-def _ints(t, count: int, what: str) -> int:
+def _ints(t, count: int, what: str, device: int) -> int:
     """The address of a device int32 list of `count` entries."""
-    if t.dtype is not _torch().int32 or t.shape != (count,) or not t.is_cuda or not t.is_contiguous():
-        raise E2CudaError(f"{what}: a contiguous device int32 list of {count}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    _on(t, what, device)
+    if t.dtype is not _torch().int32 or t.shape != (count,) or not t.is_contiguous():
+        raise E2CudaError(f"{what}: a contiguous device int32 list of {count}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
-def _table(cos, sin) -> tuple[int, int]:
+def _table(cos, sin, device: int) -> tuple[int, int]:
     """(positions, rot) of a rotary table."""
-    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()) or _type(cos) or _type(sin) \
-            or not (cos.is_cuda and sin.is_cuda):
+    _on(cos, "rotary table", device)
+    _on(sin, "rotary table", device)
+    if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()) or _type(cos) or _type(sin):
         raise E2CudaError("rotary table: contiguous device fp32 cos and sin of the same [positions][rot / 2]")
     return cos.shape[0], 2 * cos.shape[1]
 
@@ -424,16 +433,18 @@ def rope(x, cos, sin, pos=None, interleaved: bool = False, backward: bool = Fals
     with respect to the result to one with respect to x. out may be x; dtype: the result's type
     (x's own, or 16 bits for an fp32 x)."""
     torch = _torch()
+    here = torch.cuda.current_device()
+    ldx = _rows(x, "rope", here)
     T, H, D = x.shape
-    positions, rot = _table(cos, sin)
+    positions, rot = _table(cos, sin, here)
     if out is None:
         out = _result(stream, lambda: torch.empty_like(x) if dtype is None and x.is_contiguous()
                       else x.new_empty((T, H, D), dtype=dtype or x.dtype))
     elif out.shape != x.shape:
         raise E2CudaError(f"rope: out {tuple(out.shape)} for x {tuple(x.shape)}")
-    _ok(lib().e2cuda_rope(x.data_ptr(), _rows(x, "rope"), _type(x), out.data_ptr(), _rows(out, "rope out"), _type(out),
-                          cos.data_ptr(), sin.data_ptr(), positions, rot, None if pos is None else _ints(pos, T, "rope pos"), T, H,
-                          D, (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_TRANSPOSE if backward else 0), _stream(stream)),
+    _ok(lib().e2cuda_rope(x.data_ptr(), ldx, _type(x), out.data_ptr(), _rows(out, "rope out", here), _type(out),
+                          cos.data_ptr(), sin.data_ptr(), positions, rot, None if pos is None else _ints(pos, T, "rope pos", here),
+                          T, H, D, (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_TRANSPOSE if backward else 0), _stream(stream)),
         "rope")
     return out
 
@@ -462,6 +473,7 @@ class PageCache:
         self.pages = Pages(k.data_ptr(), v.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.ws.data_ptr(),
                            _type(k), layers, n_pages, page, kv, dim, table.shape[0], table.shape[1])
         self._p = C.addressof(self.pages)
+        self._device = k.get_device()
 
     @classmethod
     def new(cls, layers: int, n_pages: int, page: int, kv_heads: int, head_dim: int, max_seqs: int, max_blocks: int, dtype):
@@ -471,50 +483,61 @@ class PageCache:
         return cls(torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"),
                    torch.zeros((max_seqs, max_blocks), **ints), torch.zeros(max_seqs, **ints), torch.zeros(n_pages, **ints))
 
+    def _here(self) -> int:
+        """The cache's GPU, on which calls are made."""
+        here = _torch().cuda.current_device()
+        if here != self._device:
+            raise E2CudaError(f"PageCache: a cache on cuda:{self._device}, called on cuda:{here}")
+        return here
+
     def fork(self, parents, children, stream=None) -> None:
         """Each child, a free sequence, maps its parent's pages."""
-        n = children.shape[0]
-        _ok(lib().e2cuda_pages_fork(self._p, _ints(parents, n, "fork"), _ints(children, n, "fork"), n, _stream(stream)), "fork")
+        here, n = self._here(), children.shape[0]
+        _ok(lib().e2cuda_pages_fork(self._p, _ints(parents, n, "fork", here), _ints(children, n, "fork", here), n, _stream(stream)),
+            "fork")
 
     def append(self, seqs, counts, stream=None) -> None:
         """Sequence seqs[i] grows by counts[i] tokens; a partly filled page that others map is copied first."""
-        n = seqs.shape[0]
-        _ok(lib().e2cuda_pages_append(self._p, _ints(seqs, n, "append"), _ints(counts, n, "append"), n, _stream(stream)),
+        here, n = self._here(), seqs.shape[0]
+        _ok(lib().e2cuda_pages_append(self._p, _ints(seqs, n, "append", here), _ints(counts, n, "append", here), n, _stream(stream)),
             "append")
 
     def free(self, seqs, stream=None) -> None:
-        n = seqs.shape[0]
-        _ok(lib().e2cuda_pages_free(self._p, _ints(seqs, n, "free"), n, _stream(stream)), "free")
+        here, n = self._here(), seqs.shape[0]
+        _ok(lib().e2cuda_pages_free(self._p, _ints(seqs, n, "free", here), n, _stream(stream)), "free")
 
     def compact(self, used=None, stream=None) -> None:
         """The pages in use move to the pool's low end; used (device int32 [1]) gets their count."""
-        _ok(lib().e2cuda_pages_compact(self._p, None if used is None else _ints(used, 1, "compact"), _stream(stream)), "compact")
+        here = self._here()
+        _ok(lib().e2cuda_pages_compact(self._p, None if used is None else _ints(used, 1, "compact", here), _stream(stream)),
+            "compact")
 
     def copy(self, src, dst, stream=None) -> None:
         """Page src[i]'s keys and values, in every layer, to page dst[i]."""
-        n = src.shape[0]
-        _ok(lib().e2cuda_pages_copy(self._p, _ints(src, n, "copy"), _ints(dst, n, "copy"), n, _stream(stream)), "copy")
+        here, n = self._here(), src.shape[0]
+        _ok(lib().e2cuda_pages_copy(self._p, _ints(src, n, "copy", here), _ints(dst, n, "copy", here), n, _stream(stream)), "copy")
 
     def store(self, layer: int, q, k, v, cos, sin, seqs, q_start, interleaved: bool = False, out=None, stream=None):
         """The batch's q [T][heads][head_dim] and k, v [T][kv_heads][head_dim] (fp32 or the cache's type) of
         `layer`: q and k rotated at their tokens' positions, k and v written to the cache; returns the
         rotated q in the cache's type. Entry i's rows q_start[i]..q_start[i+1]-1 are the last tokens of
         sequence seqs[i], which append has grown."""
+        here = self._here()
+        ldq, ldk, ldv = _rows(q, "store q", here), _rows(k, "store k", here), _rows(v, "store v", here)
         T, H, D = q.shape
         p, n = self.pages, seqs.shape[0]
         if k.shape != (T, p.kv_heads, p.head_dim) or v.shape != k.shape or D != p.head_dim or not q.dtype == k.dtype == v.dtype:
             raise E2CudaError(f"store: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} of one type for a cache of "
                               f"{p.kv_heads} heads of {p.head_dim}")
-        positions, rot = _table(cos, sin)
+        positions, rot = _table(cos, sin, here)
         if out is None:
             out = _result(stream, lambda: q.new_empty((T, H, D), dtype=self.k.dtype))
         elif out.shape != q.shape or out.dtype != self.k.dtype:
             raise E2CudaError(f"store: out {tuple(out.shape)} {out.dtype}")
-        _ok(lib().e2cuda_pages_store(self._p, layer, _type(q), q.data_ptr(), _rows(q, "store q"), k.data_ptr(), _rows(k, "store k"),
-                                     v.data_ptr(), _rows(v, "store v"), out.data_ptr(), _rows(out, "store out"), cos.data_ptr(),
-                                     sin.data_ptr(), positions, rot, ROPE_INTERLEAVED if interleaved else 0,
-                                     _ints(seqs, n, "store seqs"), _ints(q_start, n + 1, "store q_start"), n, T, H,
-                                     _stream(stream)), "store")
+        _ok(lib().e2cuda_pages_store(self._p, layer, _type(q), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                                     out.data_ptr(), _rows(out, "store out", here), cos.data_ptr(), sin.data_ptr(), positions, rot,
+                                     ROPE_INTERLEAVED if interleaved else 0, _ints(seqs, n, "store seqs", here),
+                                     _ints(q_start, n + 1, "store q_start", here), n, T, H, _stream(stream)), "store")
         return out
 
     def attention(self, layer: int, q, seqs, q_start, max_q: int, shared: int = 0, causal: bool = True, window: int = -1,
@@ -522,6 +545,8 @@ class PageCache:
         """Attention of q [T][heads][head_dim] over the batch's cached tokens (the batch as in store; max_q:
         an upper bound of an entry's rows). The first `shared` tokens of every sequence lie in the same
         pages and are read once for the batch. Returns out, or (out, lse [T][heads])."""
+        here = self._here()
+        ldq = _rows(q, "attention q", here)
         T, H, D = q.shape
         p, n = self.pages, seqs.shape[0]
         if D != p.head_dim or q.dtype != self.k.dtype:
@@ -545,10 +570,10 @@ class PageCache:
             size = max(need, 2 * size, 16)
             ws = _result(stream, lambda: q.new_empty(size, dtype=_torch().uint8))
             self._scratch[st] = ws, size
-        _ok(lib().e2cuda_pages_attention(self._p, layer, q.data_ptr(), _rows(q, "attention q"), _ints(seqs, n, "attention seqs"),
-                                         _ints(q_start, n + 1, "attention q_start"), n, T, max_q, H, shared, causal, window,
+        _ok(lib().e2cuda_pages_attention(self._p, layer, q.data_ptr(), ldq, _ints(seqs, n, "attention seqs", here),
+                                         _ints(q_start, n + 1, "attention q_start", here), n, T, max_q, H, shared, causal, window,
                                          1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(),
-                                         _rows(out, "attention out"), _ptr(sums), ws.data_ptr(), size, st), "attention")
+                                         _rows(out, "attention out", here), _ptr(sums), ws.data_ptr(), size, st), "attention")
         return (out, sums) if lse else out
 
 

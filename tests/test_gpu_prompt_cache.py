@@ -660,6 +660,30 @@ def test_attention_refuses_too_many_heads_for_a_key_head(e2c, torch_cuda):
     e2c.check()
 
 
+def test_host_tensors_are_refused(e2c, torch_cuda):
+    """Refused on the host, whichever argument it is; and nothing of such a call is kept."""
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 41, [50, 60], [1, 2], 0, 4, 2, 64, 16, "bf16")
+    k, (cos, sin) = q[:, :2].contiguous(), e2c.rope_table(64, 64)
+    want = cache.attention(0, q, seqs, q_start, max_q)
+    pos, out = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.empty_like(q)
+    calls = ((e2c.rope, [q, cos, sin], dict(pos=pos, out=out)), (cache.store, [0, q, k, k, cos, sin, seqs, q_start], dict(out=out)),
+             (cache.attention, [0, q, seqs, q_start, max_q], dict(out=out)), (cache.fork, [seqs, seqs], {}),
+             (cache.append, [seqs, seqs], {}), (cache.free, [seqs], {}), (cache.copy, [seqs, seqs], {}), (cache.compact, [seqs[:1]], {}))
+    cache._scratch.clear()
+    for f, args, kw in calls:
+        for at in [*range(len(args)), *kw]:
+            a, b = list(args), dict(kw)
+            where = b if at in b else a
+            if not torch.is_tensor(where[at]):
+                continue
+            where[at] = where[at].cpu()
+            with pytest.raises(e2c.E2CudaError, match="cuda:0, got cpu"):
+                f(*a, **b)
+    assert torch.equal(cache.attention(0, q, seqs, q_start, max_q), want)
+    e2c.check()
+
+
 def test_attention_past_32_bit_offsets(e2c, torch_cuda):
     """A pool of over 2^32 bytes in one layer: pages at its end are read."""
     torch = torch_cuda

@@ -140,3 +140,12 @@ def test_ws_bytes(e2c):
     lib = e2c.lib()
     assert lib.e2cuda_pages_ws_bytes(1000, 10) >= 4 * 3 * 1010
     assert lib.e2cuda_pages_ws_bytes(-1, 10) == 0
+
+
+def test_host_tensors_are_refused(e2c):
+    """Every tensor of a call passes one of these; a host address must not reach a kernel."""
+    torch = pytest.importorskip("torch")
+    rows, ints, table = torch.zeros(3, 2, 64), torch.zeros(3, dtype=torch.int32), torch.zeros(8, 32)
+    for f, args in ((e2c._rows, (rows, "x", 0)), (e2c._ints, (ints, 3, "x", 0)), (e2c._table, (table, table, 0))):
+        with pytest.raises(e2c.E2CudaError, match="cuda:0, got cpu"):
+            f(*args)
