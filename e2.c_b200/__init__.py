@@ -557,6 +557,7 @@ class PageCache:
             raise E2CudaError(f"attention: out {tuple(out.shape)} {out.dtype}")
         sums = _result(stream, lambda: q.new_empty((T, H), dtype=_torch().float32)) if lse else None
         st = _stream(stream)
+        max_q = min(max_q, T)  # a bound kept for batches of any size
         batch = (n, T, max_q, H, shared)
         need = self._needs.get(batch)
         if need is None:

@@ -298,7 +298,7 @@ int e2cuda_pages_store(const e2cuda_pages *pc, int layer, int x_type, const void
  *
  * shared (a multiple of page): the first `shared` tokens of every sequence of the batch lie in the same
  * pages, as after a fork; their keys are then read once for the batch instead of once for each
- * sequence. 0 asks for nothing of the tables. max_q: an upper bound of an entry's rows.
+ * sequence. 0 asks for nothing of the tables. max_q, 1..T: an upper bound of an entry's rows.
  *
  * A call counts its work in tiles of 128 rows (tokens by the heads that share a key head) by 128 keys, for each
  * key head; with 2^30 of them or more it does nothing and is reported by e2cuda_check.

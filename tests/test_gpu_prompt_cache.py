@@ -684,6 +684,19 @@ def test_host_tensors_are_refused(e2c, torch_cuda):
     e2c.check()
 
 
+@pytest.mark.parametrize("case", ["ragged decode", "prefix decode", "packed prefix, small heads", "prompts"])
+def test_attention_bound_above_the_rows(e2c, torch_cuda, case):
+    """max_q is an upper bound: one above an entry's rows, and above all rows there are, gives the same."""
+    torch = torch_cuda
+    lens, queries, shared, H, KV, D, page = CASES[case]
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 12, lens, queries, shared, H, KV, D, page, "bf16")
+    want = attention64(torch, cache, 0, q, seqs, q_start, True, -1, D ** -0.5)
+    for bound in (max_q + 1, q.shape[0], q.shape[0] + 1, 1 << 20):
+        out, lse = cache.attention(0, q, seqs, q_start, bound, shared=shared, lse=True)
+        e2c.check()
+        assert_attention(torch, out, lse, want, "bf16", max(lens))
+
+
 def test_attention_past_32_bit_offsets(e2c, torch_cuda):
     """A pool of over 2^32 bytes in one layer: pages at its end are read."""
     torch = torch_cuda
