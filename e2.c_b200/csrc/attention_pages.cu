@@ -844,7 +844,11 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                     int page = 0;
                     if (it.seq >= 0 && key < min(it.klim, kk + TK))
                         page = p.pc.table[(int64_t)it.seq * p.pc.max_blocks + (key >> shift)];
-                    row2 = ((unsigned)page < (unsigned)p.pc.n_pages ? page << shift : 0) + (key & (p.pc.page - 1));
+                    if ((unsigned)page >= (unsigned)p.pc.n_pages) {  // page 0 instead, reported
+                        record_status(p.status, E2C_ERR_BAD_SEQ);
+                        page = 0;
+                    }
+                    row2 = (page << shift) + (key & (p.pc.page - 1));
                     nk2 = min(TK, it.klim - kk);
                     kvh2 = it.kvh;
                     have2 = true;

@@ -244,7 +244,8 @@ int e2cuda_rope(const void *x, int ldx, int x_type, void *y, int ldy, int y_type
  *
  * Calls on one cache must be ordered (one stream, or events). The calls take device lists of sequences;
  * no sequence may be named twice in one call (except as a parent). An entry that is outside the cache is
- * left out and reported by e2cuda_check. */
+ * left out and reported by e2cuda_check; so is a page of a table that is not in the pool, in whose place
+ * attention reads page 0. */
 typedef struct e2cuda_pages {
     void *k, *v;    /* [layers][n_pages][page][kv_heads][head_dim], 16-byte aligned                */
     int32_t *table; /* [max_seqs][max_blocks]                                                      */

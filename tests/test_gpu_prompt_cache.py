@@ -697,6 +697,26 @@ def test_attention_bound_above_the_rows(e2c, torch_cuda, case):
         assert_attention(torch, out, lse, want, "bf16", max(lens))
 
 
+@pytest.mark.parametrize("wild", [-1, 1 << 20, 2 ** 31 - 1])
+@pytest.mark.parametrize("D,shared", [(64, 0), (128, 0), (256, 0), (128, 512)])
+def test_attention_page_outside_the_pool(e2c, torch_cuda, D, shared, wild):
+    """A page that a sequence holds but the pool does not is reported, and other sequences are right."""
+    torch = torch_cuda
+    n = 160
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 42, [shared + 90 + i for i in range(n)], [1] * n, shared, 8, 4, D, 16, "bf16")
+    for x in (cache.k, cache.v):
+        x.nan_to_num_(0.0)
+    bad = int(seqs[5])
+    cache.table[bad, shared // 16 + 2] = wild
+    out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, lse=True)
+    with pytest.raises(e2c.E2CudaError, match="page outside the cache"):
+        e2c.check()
+    keep = torch.tensor([i for i in range(n) if i != 5], device="cuda")
+    starts = torch.arange(n, device="cuda")
+    want = attention64(torch, cache, 0, q[keep], seqs[keep], starts, True, -1, D ** -0.5)
+    assert_attention(torch, out[keep], lse[keep], want, "bf16", shared + 90 + n)
+
+
 def test_attention_past_32_bit_offsets(e2c, torch_cuda):
     """A pool of over 2^32 bytes in one layer: pages at its end are read."""
     torch = torch_cuda
