@@ -101,6 +101,7 @@ class Pages(C.Structure):
 F32, BF16, F16 = 0, 1, 2
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_BY_ROTATIONS, ROPE_BY_PAIRS = 0, 1, 2, 3, 4
 ROPE_INTERLEAVED, ROPE_TRANSPOSE = 1, 2
+INT_MAX = 2 ** 31 - 1
 
 EPI_F32, EPI_RESID, EPI_I32, EPI_GELU, EPI_QKV, EPI_NORMADD, EPI_GELUQ, EPI_QKVPB = 0, 1, 2, 3, 4, 5, 6, 7
 
@@ -396,7 +397,10 @@ def _rows(t, what: str, device: int) -> int:
     rows, heads, dim = t.shape
     if (s[2] != 1 and dim > 1) or (s[1] != dim and heads > 1):
         raise E2CudaError(f"{what}: [rows][heads][head_dim] with the heads of a row side by side, got strides {tuple(s)}")
-    return s[0] if rows > 1 else heads * dim
+    ld = s[0] if rows > 1 else heads * dim
+    if ld > INT_MAX:  # a C int: ctypes would drop its high bits
+        raise E2CudaError(f"{what}: rows {ld} elements apart, at most {INT_MAX}")
+    return ld
 
 
 def _ints(t, count: int, what: str, device: int) -> int:
@@ -558,6 +562,7 @@ class PageCache:
         sums = _result(stream, lambda: q.new_empty((T, H), dtype=_torch().float32)) if lse else None
         st = _stream(stream)
         max_q = min(max_q, T)  # a bound kept for batches of any size
+        window = max(-1, min(window, INT_MAX))  # none, or wider than any sequence
         batch = (n, T, max_q, H, shared)
         need = self._needs.get(batch)
         if need is None:

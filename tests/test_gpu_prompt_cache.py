@@ -717,6 +717,16 @@ def test_attention_page_outside_the_pool(e2c, torch_cuda, D, shared, wild):
     assert_attention(torch, out[keep], lse[keep], want, "bf16", shared + 90 + n)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 63 - 1, -2 ** 32])
+def test_attention_window_wider_than_any_sequence(e2c, torch_cuda, window):
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 43, [300, 70], [5, 40], 0, 4, 2, 64, 16, "bf16")
+    for causal in (False, True):
+        want = cache.attention(0, q, seqs, q_start, max_q, causal=causal)
+        assert torch.equal(cache.attention(0, q, seqs, q_start, max_q, causal=causal, window=window), want)
+    e2c.check()
+
+
 def test_attention_past_32_bit_offsets(e2c, torch_cuda):
     """A pool of over 2^32 bytes in one layer: pages at its end are read."""
     torch = torch_cuda

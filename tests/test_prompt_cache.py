@@ -149,3 +149,20 @@ def test_host_tensors_are_refused(e2c):
     for f, args in ((e2c._rows, (rows, "x", 0)), (e2c._ints, (ints, 3, "x", 0)), (e2c._table, (table, table, 0))):
         with pytest.raises(e2c.E2CudaError, match="cuda:0, got cpu"):
             f(*args)
+
+
+@pytest.mark.parametrize("ld", [2 ** 31, 2 ** 32, 2 ** 32 + 128])
+def test_rows_further_apart_than_an_int_are_refused(e2c, ld):
+    """The library's row strides are ints; a view of a larger tensor must not be read at another one."""
+    class View:
+        shape = (3, 2, 64)
+        device = "cuda:0"
+
+        def stride(self):
+            return (ld, 64, 1)
+
+        def get_device(self):
+            return 0
+
+    with pytest.raises(e2c.E2CudaError, match="elements apart"):
+        e2c._rows(View(), "q", 0)
