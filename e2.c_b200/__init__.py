@@ -220,16 +220,17 @@ def _ok(rc: int, what: str) -> None:
 
 
 _torch_mod = None
+_raw_stream = None  # a device's current stream without a Stream object (3 us a call)
 
 
 def _torch():
-    global _torch_mod
+    global _torch_mod, _raw_stream
     if _torch_mod is None:
         import torch
 
         if not torch.cuda.is_available():
             raise E2CudaError("no CUDA device: the e2cuda ops have no CPU path")
-        _torch_mod = torch
+        _torch_mod, _raw_stream = torch, getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return _torch_mod
 
 
@@ -237,12 +238,14 @@ def _ptr(t) -> int:
     return t.data_ptr() if t is not None else None
 
 
-def _stream(stream) -> int | None:
+def _stream(stream, device: int | None = None) -> int | None:
+    """The stream's address; device: the current one, where the caller has asked for it."""
     torch = _torch()
     if stream is not None:
         return stream.cuda_stream
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without a Stream object (3 us a call)
-    return raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream
+    if _raw_stream is None:
+        return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(torch.cuda.current_device() if device is None else device)
 
 
 def _result(stream, make):
@@ -382,15 +385,15 @@ def _type(t) -> int:
         raise E2CudaError(f"element type {t.dtype}: fp32, bf16 or fp16") from None
 
 
-def _on(t, what: str, device: int) -> None:
-    """Refuses a tensor of the host or of another GPU: its address would go to a kernel on this one."""
-    if t.get_device() != device:  # -1: the host
-        raise E2CudaError(f"{what}: a tensor on cuda:{device}, got {t.device}")
+def _elsewhere(t, what: str, device: int) -> E2CudaError:
+    """A tensor of the host (get_device() -1) or of another GPU: its address must not reach a kernel on this one."""
+    return E2CudaError(f"{what}: a tensor on cuda:{device}, got {t.device}")
 
 
 def _rows(t, what: str, device: int) -> int:
     """Elements between the rows of a [rows][heads][head_dim] tensor on the GPU whose heads lie side by side."""
-    _on(t, what, device)
+    if t.get_device() != device:
+        raise _elsewhere(t, what, device)
     s = t.stride()
     if len(s) != 3:
         raise E2CudaError(f"{what}: [rows][heads][head_dim], got {tuple(t.shape)}")
@@ -405,16 +408,17 @@ def _rows(t, what: str, device: int) -> int:
 
 def _ints(t, count: int, what: str, device: int) -> int:
     """The address of a device int32 list of `count` entries."""
-    _on(t, what, device)
-    if t.dtype is not _torch().int32 or t.shape != (count,) or not t.is_contiguous():
+    if t.get_device() != device:
+        raise _elsewhere(t, what, device)
+    if t.dtype is not _torch_mod.int32 or t.shape != (count,) or not t.is_contiguous():
         raise E2CudaError(f"{what}: a contiguous device int32 list of {count}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _table(cos, sin, device: int) -> tuple[int, int]:
     """(positions, rot) of a rotary table."""
-    _on(cos, "rotary table", device)
-    _on(sin, "rotary table", device)
+    if cos.get_device() != device or sin.get_device() != device:
+        raise _elsewhere(sin if cos.get_device() == device else cos, "rotary table", device)
     if cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()) or _type(cos) or _type(sin):
         raise E2CudaError("rotary table: contiguous device fp32 cos and sin of the same [positions][rot / 2]")
     return cos.shape[0], 2 * cos.shape[1]
@@ -448,8 +452,8 @@ def rope(x, cos, sin, pos=None, interleaved: bool = False, backward: bool = Fals
         raise E2CudaError(f"rope: out {tuple(out.shape)} for x {tuple(x.shape)}")
     _ok(lib().e2cuda_rope(x.data_ptr(), ldx, _type(x), out.data_ptr(), _rows(out, "rope out", here), _type(out),
                           cos.data_ptr(), sin.data_ptr(), positions, rot, None if pos is None else _ints(pos, T, "rope pos", here),
-                          T, H, D, (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_TRANSPOSE if backward else 0), _stream(stream)),
-        "rope")
+                          T, H, D, (ROPE_INTERLEAVED if interleaved else 0) | (ROPE_TRANSPOSE if backward else 0),
+                          _stream(stream, here)), "rope")
     return out
 
 
@@ -497,29 +501,30 @@ class PageCache:
     def fork(self, parents, children, stream=None) -> None:
         """Each child, a free sequence, maps its parent's pages."""
         here, n = self._here(), children.shape[0]
-        _ok(lib().e2cuda_pages_fork(self._p, _ints(parents, n, "fork", here), _ints(children, n, "fork", here), n, _stream(stream)),
-            "fork")
+        _ok(lib().e2cuda_pages_fork(self._p, _ints(parents, n, "fork", here), _ints(children, n, "fork", here), n,
+                                    _stream(stream, here)), "fork")
 
     def append(self, seqs, counts, stream=None) -> None:
         """Sequence seqs[i] grows by counts[i] tokens; a partly filled page that others map is copied first."""
         here, n = self._here(), seqs.shape[0]
-        _ok(lib().e2cuda_pages_append(self._p, _ints(seqs, n, "append", here), _ints(counts, n, "append", here), n, _stream(stream)),
-            "append")
+        _ok(lib().e2cuda_pages_append(self._p, _ints(seqs, n, "append", here), _ints(counts, n, "append", here), n,
+                                      _stream(stream, here)), "append")
 
     def free(self, seqs, stream=None) -> None:
         here, n = self._here(), seqs.shape[0]
-        _ok(lib().e2cuda_pages_free(self._p, _ints(seqs, n, "free", here), n, _stream(stream)), "free")
+        _ok(lib().e2cuda_pages_free(self._p, _ints(seqs, n, "free", here), n, _stream(stream, here)), "free")
 
     def compact(self, used=None, stream=None) -> None:
         """The pages in use move to the pool's low end; used (device int32 [1]) gets their count."""
         here = self._here()
-        _ok(lib().e2cuda_pages_compact(self._p, None if used is None else _ints(used, 1, "compact", here), _stream(stream)),
+        _ok(lib().e2cuda_pages_compact(self._p, None if used is None else _ints(used, 1, "compact", here), _stream(stream, here)),
             "compact")
 
     def copy(self, src, dst, stream=None) -> None:
         """Page src[i]'s keys and values, in every layer, to page dst[i]."""
         here, n = self._here(), src.shape[0]
-        _ok(lib().e2cuda_pages_copy(self._p, _ints(src, n, "copy", here), _ints(dst, n, "copy", here), n, _stream(stream)), "copy")
+        _ok(lib().e2cuda_pages_copy(self._p, _ints(src, n, "copy", here), _ints(dst, n, "copy", here), n,
+                                    _stream(stream, here)), "copy")
 
     def store(self, layer: int, q, k, v, cos, sin, seqs, q_start, interleaved: bool = False, out=None, stream=None):
         """The batch's q [T][heads][head_dim] and k, v [T][kv_heads][head_dim] (fp32 or the cache's type) of
@@ -541,7 +546,7 @@ class PageCache:
         _ok(lib().e2cuda_pages_store(self._p, layer, _type(q), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
                                      out.data_ptr(), _rows(out, "store out", here), cos.data_ptr(), sin.data_ptr(), positions, rot,
                                      ROPE_INTERLEAVED if interleaved else 0, _ints(seqs, n, "store seqs", here),
-                                     _ints(q_start, n + 1, "store q_start", here), n, T, H, _stream(stream)), "store")
+                                     _ints(q_start, n + 1, "store q_start", here), n, T, H, _stream(stream, here)), "store")
         return out
 
     def attention(self, layer: int, q, seqs, q_start, max_q: int, shared: int = 0, causal: bool = True, window: int = -1,
@@ -560,7 +565,7 @@ class PageCache:
         elif out.shape != q.shape or out.dtype != q.dtype:
             raise E2CudaError(f"attention: out {tuple(out.shape)} {out.dtype}")
         sums = _result(stream, lambda: q.new_empty((T, H), dtype=_torch().float32)) if lse else None
-        st = _stream(stream)
+        st = _stream(stream, here)
         max_q = min(max_q, T)  # a bound kept for batches of any size
         window = max(-1, min(window, INT_MAX))  # none, or wider than any sequence
         batch = (n, T, max_q, H, shared)
