@@ -553,7 +553,8 @@ class PageCache:
                   scale: float | None = None, lse: bool = False, out=None, stream=None):
         """Attention of q [T][heads][head_dim] over the batch's cached tokens (the batch as in store; max_q:
         an upper bound of an entry's rows). The first `shared` tokens of every sequence lie in the same
-        pages and are read once for the batch. Returns out, or (out, lse [T][heads])."""
+        pages and, where that pays, are read once for the batch: with at most 64 rows of max_q tokens by the heads of a
+        key head, so a bound near the true one is worth its while. Returns out, or (out, lse [T][heads])."""
         here = self._here()
         ldq = _rows(q, "attention q", here)
         T, H, D = q.shape

@@ -16,7 +16,9 @@
 //   S = Q K_j^T     fp32 in tensor memory, N rounded up to 16 keys in an item's last tile
 //   P = exp2(S scale log2 e - m)  16 bits over S's columns; m moves only when it grows by 2^8, then O is rescaled
 //   O += P V_j      fp32 in tensor memory; V is read as it lies in the cache (its head dim contiguous)
-// P is rounded to the cache's type, the tensor cores' operand; its sum, m and O are held in 32 bits. The
+// P is rounded to the cache's type, the tensor cores' operand (against 64 bits the output is then off by 0.0018 to
+// 0.0023 of its size in bf16, where 32-bit arithmetic rounded once at the end is off by 0.0017; an fp32 P would
+// take a second product for its low bits); its sum, m and O are held in 32 bits. The
 // softmax warpgroups take the tiles in turn, handing the running maximum on as soon as a tile's is known, so
 // that their exponentials overlap.
 //
@@ -25,13 +27,13 @@
 // to the product's 16-key granularity: what a page holds there is arbitrary, and 0 x NaN would not
 // vanish. Keys past it are masked in S by a select.
 //
-// What bounds it (one B200, CUDA events): long single-token batches the memory (64 sequences of 8192
-// tokens, 32 heads of 128 over 8 key heads: 280 us, 96% of the copy rate); whole prompts the chain from S to P
-// in the softmax warps and the products' issue, some 1800 (heads of 64) to 3500 cycles (of 256) a tile of
-// 128 rows by 128 keys where the products take 512 to 2048 (4 sequences of up to 4096 tokens, every key: 16
-// heads of 128 over 4 388 us, 63% of the measured bf16 rate; 8 heads of 256 over 4 315 us, 78%; 16 heads of 64
-// over 4 338 us); short sequences an item's set-up and output, some 3500 cycles (512 x 16 tokens, 8 key
-// heads: 60 us). The rings' depth (2 to 5 stages) moves a tile's time by less than 2%; so does a thread
+// What bounds it (one B200, CUDA events): long single-token batches the memory (64 sequences of 5470 to 8192
+// tokens, 429425 in all, 32 heads of 128 over 8 key heads, 1.76 GB: 280 us, 96% of the copy rate); whole prompts
+// the chain from S to P in the softmax warps and the products' issue, some 1800 (heads of 64), 1980 (of 128)
+// and 3100 cycles (of 256) a tile of 128 rows by 128 keys where the products take 512, 1024 and 2048 (4 prompts of
+// 4096, 3007, 3284 and 3561 tokens, every key: 16 heads of 128 over 4 388 us, 63% of the measured bf16 rate; 8 heads
+// of 256 over 4 315 us, 78%; 16 heads of 64 over 4 338 us); short sequences an item's set-up and output, some
+// 3500 cycles (512 sequences of 11 to 16 tokens, 8 key heads: 60 us). The rings' depth (2 to 5 stages) moves a tile's time by less than 2%; so does a thread
 // for each of the two products, except that heads of 256 lose 10%.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -57,9 +59,10 @@ constexpr int ITEM_COST = 1;
 constexpr int PREFIX_TILES = 13;  // use_prefix
 constexpr float kRescaleLog2 = 8.0f;
 
-// A wait of a whole warp, bounded by its number of (sleeping) tries: up to 1.3 s. It is small on
+// A wait of a whole warp, bounded by its number of tries, each of which sleeps for kTryNs at most: it gives up
+// after 1.3 s at the latest, sooner where tries return early. It is small on
 // purpose: with ptx.cuh's mbar_wait inlined at every wait the kernel was 234 KB of code, whose
-// instruction fetches took most of a tile's time (128-wide heads, 4096 tokens: 905 us a call).
+// instruction fetches took most of a tile's time (heads of 128, the 4 prompts above: 905 us a call).
 constexpr uint32_t kTryNs = 10000, kTries = 1u << 17;
 E2C_DEV bool wait_warp(uint32_t bar, uint32_t parity, int *status, int code) {
     bool ok = false;
@@ -75,8 +78,8 @@ constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 template <int D>
 struct Cfg {
     // warps: NG softmax groups of four, the epilogue's four, then one each. A third softmax group hides more
-    // of a tile's latencies where its products are shortest (heads of 64, us with two and with three: 4 x 4096
-    // tokens 366 and 338, single tokens behind 700 of their own 55.4 and 52.1, behind 16 42.3 and 43.5); with wider
+    // of a tile's latencies where its products are shortest (heads of 64, us with two and with three: the 4 prompts
+    // above 366 and 338, single tokens behind 700 of their own 55.4 and 52.1, behind 16 42.3 and 43.5); with wider
     // heads it gives less and costs batches of short items (128: 385 and 374, 92.9 and 94.1 for 128
     // tokens behind a shared prefix; 256: 312 and 314)
     static constexpr int NG = D == 64 ? 3 : 2;
@@ -428,9 +431,9 @@ E2C_DEV float2 add2(float2 a, float2 b) {
 }
 // 2^x of two values on the FMA pipe, for x <= 125: x = n + f with |f| <= 1/2 (adding 1.5 * 2^23 rounds to
 // the whole number n and leaves it in the low bits), a polynomial of degree 4 in f fitted to the
-// least relative error (2.6e-6), and n added to the exponent. Below 2^-125 the result stays there.
+// least relative error (2.7e-6 in fp32), and n added to the exponent. Below 2^-125 the result stays there.
 // One exponential in kPoly pairs takes this way: the exponential unit's 16 a cycle are what
-// bounds 64-wide heads, and nearly bound 128-wide ones (us with and without: 4 x 4096 tokens, heads of
+// bounds 64-wide heads, and nearly bound 128-wide ones (us with and without: the 4 prompts above, heads of
 // 128 388 and 392, of 256 314 and 319; ragged prompts in a window, heads of 64 172 and 175).
 constexpr int kPoly = 4;
 E2C_DEV float2 ex2_poly(float2 x) {
@@ -953,7 +956,7 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                 const bool masked = __any_sync(0xffffffffu, live && (ra > 0 || rb < TK));
                 // The columns are read twice, for the maximum and for the exponentials, in loops short enough
                 // for the instruction cache: a row of 128 logits held in registers is straight code that does
-                // not stay in it (4 x 4096 tokens, 16 heads of 128: 443 us, 370 with loops of 64 columns; of 32, 368)
+                // not stay in it (the 4 prompts above, 16 heads of 128: 443 us, 370 with loops of 64 columns; of 32, 368)
                 auto hide = [&](int c0, uint32_t (&s)[16]) {
                     // bit i: column c0 + i is seen
                     const int a = min(max(ra - c0, 0), 16), b = min(max(rb - c0, 0), 16);
@@ -1286,7 +1289,12 @@ __global__ void __launch_bounds__(JOIN) k_join_prefix(const Args p, int grid) {
 }
 
 // Sequences of few query tokens fill a small part of a 128-row tile each; packed, the batch reads the prefix
-// once per 128 rows instead of once per sequence. From half a tile on they gain nothing, and where
+// once per 128 rows instead of once per sequence. It is done up to half a tile of the longest entry's rows (max_q
+// stands for it: the rows themselves are on the device). Past that the gain fades and turns over (us a call,
+// packed and not; 128 sequences behind 16384 tokens, 32 heads of 128 over 8, 68 rows each 632 and 1042, 96 rows 905 and
+// 1045, 112 rows 1050 and 1082, 128 rows 1159 and 1105; 256 behind 6144, 4 heads of 256 over 2, 66 rows 240 and
+// 300, 80 rows 329 and 302, 112 rows 443 and 316; 32 behind 4096, heads of 128, 68 rows 79 and 103, 96 rows 111
+// and 97), and entries of more rows than a tile would need a join that knows their tiles. Where
 // all sequences' own passes over the prefix are a dozen tiles a block, joining two parts of every row
 // costs more than it saves (8 key heads of 128, 300 tokens past the prefix, us a call, packed and not: 16
 // sequences behind 1024 tokens, 6.5 tiles a block, 28.4 and 23.8; 32 behind 1024, 13.4 tiles, 31.2 and 32.7;

@@ -321,7 +321,8 @@ struct Freqs {
 };
 
 // cos and sin of position * frequency, in 64 bits: at position 10^6 a 32-bit product would be off by
-// 0.06 radians
+// 0.06 radians. That arithmetic is what bounds it (32768 positions of 64 pairs 22.5 us, 262144 135 us, where
+// writing them takes 2.6 and 21); a program makes its table once.
 __global__ void __launch_bounds__(256) k_rope_table(float *cs, float *sn, int64_t total, int half, const __grid_constant__ Freqs fr,
                                                     double gain) {
     griddep_launch_dependents();

@@ -260,7 +260,7 @@ typedef struct e2cuda_pages {
 } e2cuda_pages;
 size_t e2cuda_pages_ws_bytes(int n_pages, int max_seqs);
 
-/* Each child (a free sequence) maps its parent's pages: no data moves. */
+/* Each child (a free sequence) maps its parent's pages: no data moves. A child is no parent in the same call. */
 int e2cuda_pages_fork(const e2cuda_pages *pc, const int32_t *parents, const int32_t *children, int n, void *stream);
 /* Sequence seqs[i] grows by counts[i] tokens, whose keys and values are then stored. Blocks past the
  * old ones get the lowest free pages, in the list's order. A partly filled last page that other
@@ -294,12 +294,19 @@ int e2cuda_pages_store(const e2cuda_pages *pc, int layer, int x_type, const void
  * over the tokens j in sight of t's position p: j < len, with `causal` j <= p, with window >= 0
  * |p - j| <= window. Query head h reads key head h / (heads / kv_heads); at most 128 query heads for one key
  * head. q, out: rows of heads of head_dim in the cache's type, 16-byte aligned, ld a multiple of 8. lse: fp32
- * [T][heads] or NULL. A row that sees nothing gets zeros and -infinity. What the cache holds past a sequence's
- * length is never used, whatever its value.
+ * [T][heads] or NULL. Logits, their exponentials' sum and the accumulated output are held in 32 bits; the exponentials
+ * are rounded to the cache's type before their product with v, the output once more.
+ *
+ * A row that sees nothing gets zeros and -infinity. A NaN among the logits in sight, +infinity or only -infinity make
+ * the row NaN, and lse what the sum is. Keys out of sight are never used, whatever their value, nor is what the
+ * cache holds where no sequence of the batch has a token. A token's v counts with weight zero in rows that do not
+ * see it: one that is not finite can make such a row NaN too (0 x infinity).
  *
  * shared (a multiple of page): the first `shared` tokens of every sequence of the batch lie in the same
- * pages, as after a fork; their keys are then read once for the batch instead of once for each
- * sequence. 0 asks for nothing of the tables. max_q, 1..T: an upper bound of an entry's rows.
+ * pages, as after a fork. It is a hint: where that pays, their keys are read once for each 128 rows of the
+ * whole batch instead of once for each sequence, which needs max_q * heads / kv_heads <= 64 and many sequences or
+ * a long prefix; one longer entry, or a looser max_q, and each sequence reads them by itself. 0 asks for nothing of the
+ * tables. max_q, 1..T: an upper bound of an entry's rows.
  *
  * A call counts its work in tiles of 128 rows (tokens by the heads that share a key head) by 128 keys, for each
  * key head; with 2^30 of them or more it does nothing and is reported by e2cuda_check.
