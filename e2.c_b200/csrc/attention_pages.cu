@@ -478,6 +478,7 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
     if (smem_u32(smem) & 1023) {
         griddep_wait();
         if (threadIdx.x == 0) record_status(p.status, E2C_ERR_SMEM_ALIGN);
+        if (blockIdx.x == 0 && threadIdx.x < 2) p.before[p.n + threadIdx.x] = 0;  // the join has nothing to do
         return;
     }
     const uint32_t sbase = smem_u32(smem);
