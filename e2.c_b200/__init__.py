@@ -95,10 +95,16 @@ class Pages(C.Structure):
 
     _fields_ = [("k", vp), ("v", vp), ("table", vp), ("len", vp), ("refs", vp), ("ws", vp), ("type", C.c_int),
                 ("layers", C.c_int), ("n_pages", C.c_int), ("page", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
-                ("max_seqs", C.c_int), ("max_blocks", C.c_int)]
+                ("max_seqs", C.c_int), ("max_blocks", C.c_int), ("k_scale", vp), ("v_scale", vp)]
 
 
-F32, BF16, F16 = 0, 1, 2
+class Sight(C.Structure):
+    """e2cuda_sight: what the rows of an attention call see."""
+
+    _fields_ = [("causal", C.c_int), ("window", C.c_int), ("sinks", C.c_int), ("words", C.c_int), ("tree", vp)]
+
+
+F32, BF16, F16, I8 = 0, 1, 2, 3
 ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_BY_ROTATIONS, ROPE_BY_PAIRS = 0, 1, 2, 3, 4
 ROPE_INTERLEAVED, ROPE_TRANSPOSE = 1, 2
 INT_MAX = 2 ** 31 - 1
@@ -149,9 +155,16 @@ API = [
     ("e2cuda_pages_copy", C.c_int, [vp, vp, vp, C.c_int, vp]),
     ("e2cuda_pages_store", C.c_int, [vp, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, vp, C.c_int,
                                      C.c_int, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, vp]),
+    ("e2cuda_pages_store_at", C.c_int, [vp, C.c_int, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_int, vp, C.c_int, C.c_int, vp, vp,
+                                        C.c_int, C.c_int, C.c_int, vp, vp, vp, C.c_int, C.c_int, C.c_int, vp]),
+    ("e2cuda_pages_load", C.c_int, [vp, C.c_int, vp, vp, vp, C.c_int, C.c_int, vp, vp, C.c_int, vp]),
+    ("e2cuda_pages_tree", C.c_int, [vp, vp, vp, vp, C.c_int, C.c_int, vp, C.c_int, vp, vp]),
+    ("e2cuda_pages_keep", C.c_int, [vp, vp, vp, vp, vp, C.c_int, C.c_int, vp]),
     ("e2cuda_pages_attention_ws_bytes", C.c_size_t, [vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     ("e2cuda_pages_attention", C.c_int, [vp, C.c_int, vp, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                          C.c_int, C.c_float, vp, C.c_int, vp, vp, C.c_size_t, vp]),
+    ("e2cuda_pages_attention_sight", C.c_int, [vp, C.c_int, C.c_int, vp, C.c_int, vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                               vp, C.c_float, vp, C.c_int, vp, vp, C.c_size_t, vp]),
     ("e2cuda_ffn_create", vp, [C.POINTER(Q8W), C.POINTER(Q8W), C.POINTER(Q8W), f32p, C.c_float, C.c_int]),
     ("e2cuda_ffn_destroy", None, [vp]),
     ("e2cuda_ffn_forward", C.c_int, [vp, vp, C.c_int, vp, vp]),
@@ -461,25 +474,36 @@ class PageCache:
     """A paged key/value cache (e2cuda_pages) over the caller's tensors: k, v
     [layers][n_pages][page][kv_heads][head_dim] bf16 or fp16, table [max_seqs][max_blocks], length
     [max_seqs] and refs [n_pages] int32 (length and refs zero when new). PageCache.new makes them.
+    With k and v int8 a token's heads are quantised as they are stored, and k_scale, v_scale [layers][n_pages][kv_heads][page]
+    fp32 hold their scales.
     Sequence and count lists are device int32 tensors; every method only queues work."""
 
-    def __init__(self, k, v, table, length, refs):
+    def __init__(self, k, v, table, length, refs, k_scale=None, v_scale=None):
         torch = _torch()
         if k.dim() != 5 or v.shape != k.shape or v.dtype != k.dtype or not (k.is_contiguous() and v.is_contiguous()):
             raise E2CudaError("PageCache: contiguous k and v of the same [layers][n_pages][page][kv_heads][head_dim] and type")
         for t, shape in ((table, (length.shape[0], table.shape[-1])), (length, (length.shape[0],)), (refs, (k.shape[1],))):
             if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
                 raise E2CudaError(f"PageCache: a contiguous int32 tensor of {shape}, got {t.dtype} {tuple(t.shape)}")
-        if not all(t.is_cuda and t.device == k.device for t in (k, v, table, length, refs)):
+        layers, n_pages, page, kv, dim = k.shape
+        codes = k.dtype == torch.int8
+        scales = [t for t in (k_scale, v_scale) if t is not None]
+        if len(scales) != 2 * codes:
+            raise E2CudaError("PageCache: k_scale and v_scale beside int8 k and v, and only there")
+        for t in scales:
+            if t.dtype != torch.float32 or tuple(t.shape) != (layers, n_pages, kv, page) or not t.is_contiguous():
+                raise E2CudaError(f"PageCache: contiguous fp32 scales of {(layers, n_pages, kv, page)}, got {t.dtype} {tuple(t.shape)}")
+        if not all(t.is_cuda and t.device == k.device for t in (k, v, table, length, refs, *scales)):
             raise E2CudaError("PageCache: all tensors on one CUDA device")
         self.k, self.v, self.table, self.length, self.refs = k, v, table, length, refs
-        layers, n_pages, page, kv, dim = k.shape
+        self.k_scale, self.v_scale = k_scale, v_scale
         self.ws = torch.empty(lib().e2cuda_pages_ws_bytes(n_pages, length.shape[0]) // 4, dtype=torch.int32, device=k.device)
         self._scratch: dict = {}  # the attention's workspace and its size, by stream
         self._outgrown: list = []  # smaller ones before them; each at least doubles, so all are at most the last one's size
         self._needs: dict = {}    # workspace bytes by batch
         self.pages = Pages(k.data_ptr(), v.data_ptr(), table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.ws.data_ptr(),
-                           _type(k), layers, n_pages, page, kv, dim, table.shape[0], table.shape[1])
+                           I8 if codes else _type(k), layers, n_pages, page, kv, dim, table.shape[0], table.shape[1],
+                           _ptr(k_scale), _ptr(v_scale))
         self._p = C.addressof(self.pages)
         self._device = k.get_device()
 
@@ -488,8 +512,10 @@ class PageCache:
         torch = _torch()
         shape = (layers, n_pages, page, kv_heads, head_dim)
         ints = dict(dtype=torch.int32, device="cuda")
+        scales = [torch.empty((layers, n_pages, kv_heads, page), dtype=torch.float32, device="cuda")
+                  for _ in range(2 if dtype == torch.int8 else 0)]
         return cls(torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"),
-                   torch.zeros((max_seqs, max_blocks), **ints), torch.zeros(max_seqs, **ints), torch.zeros(n_pages, **ints))
+                   torch.zeros((max_seqs, max_blocks), **ints), torch.zeros(max_seqs, **ints), torch.zeros(n_pages, **ints), *scales)
 
     def _here(self) -> int:
         """The cache's GPU, on which calls are made."""
@@ -526,11 +552,14 @@ class PageCache:
         _ok(lib().e2cuda_pages_copy(self._p, _ints(src, n, "copy", here), _ints(dst, n, "copy", here), n,
                                     _stream(stream, here)), "copy")
 
-    def store(self, layer: int, q, k, v, cos, sin, seqs, q_start, interleaved: bool = False, out=None, stream=None):
+    def store(self, layer: int, q, k, v, cos, sin, seqs, q_start, interleaved: bool = False, out=None, stream=None, pos=None,
+              dtype=None):
         """The batch's q [T][heads][head_dim] and k, v [T][kv_heads][head_dim] (fp32 or the cache's type) of
         `layer`: q and k rotated at their tokens' positions, k and v written to the cache; returns the
         rotated q in the cache's type. Entry i's rows q_start[i]..q_start[i+1]-1 are the last tokens of
-        sequence seqs[i], which append has grown."""
+        sequence seqs[i], which append has grown.
+        pos (device int32 [T]): the rows' rotary positions, where they are not their places in their sequences.
+        An int8 cache takes fp32, bf16 or fp16 and returns q as `dtype` (default: q's own 16 bits, bf16 for fp32)."""
         here = self._here()
         ldq, ldk, ldv = _rows(q, "store q", here), _rows(k, "store k", here), _rows(v, "store v", here)
         T, H, D = q.shape
@@ -539,27 +568,67 @@ class PageCache:
             raise E2CudaError(f"store: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} of one type for a cache of "
                               f"{p.kv_heads} heads of {p.head_dim}")
         positions, rot = _table(cos, sin, here)
+        if dtype is None:
+            torch = _torch_mod
+            dtype = self.k.dtype if p.type != I8 else out.dtype if out is not None else torch.bfloat16 if q.dtype is torch.float32 else q.dtype
         if out is None:
-            out = _result(stream, lambda: q.new_empty((T, H, D), dtype=self.k.dtype))
-        elif out.shape != q.shape or out.dtype != self.k.dtype:
+            out = _result(stream, lambda: q.new_empty((T, H, D), dtype=dtype))
+        elif out.shape != q.shape or out.dtype != dtype:
             raise E2CudaError(f"store: out {tuple(out.shape)} {out.dtype}")
-        _ok(lib().e2cuda_pages_store(self._p, layer, _type(q), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
-                                     out.data_ptr(), _rows(out, "store out", here), cos.data_ptr(), sin.data_ptr(), positions, rot,
-                                     ROPE_INTERLEAVED if interleaved else 0, _ints(seqs, n, "store seqs", here),
-                                     _ints(q_start, n + 1, "store q_start", here), n, T, H, _stream(stream, here)), "store")
+        _ok(lib().e2cuda_pages_store_at(self._p, layer, _type(q), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
+                                        out.data_ptr(), _type(out), _rows(out, "store out", here), cos.data_ptr(), sin.data_ptr(),
+                                        positions, rot, ROPE_INTERLEAVED if interleaved else 0,
+                                        None if pos is None else _ints(pos, T, "store pos", here), _ints(seqs, n, "store seqs", here),
+                                        _ints(q_start, n + 1, "store q_start", here), n, T, H, _stream(stream, here)), "store")
         return out
 
+    def load(self, layer: int, seqs, q_start, tokens: int, first=None, dtype=None, stream=None):
+        """Keys and values read back: (k, v) [tokens][kv_heads][head_dim] of `dtype` (fp32, bf16, fp16; default: the cache's, bf16
+        for int8). Entry i's rows q_start[i]..q_start[i+1]-1 are the tokens of sequence seqs[i] from first[i] on (None: its last ones)."""
+        here = self._here()
+        torch, p, n = _torch_mod, self.pages, seqs.shape[0]
+        if dtype is None:
+            dtype = torch.bfloat16 if p.type == I8 else self.k.dtype
+        k, v = _result(stream, lambda: tuple(torch.empty((tokens, p.kv_heads, p.head_dim), dtype=dtype, device=self.k.device) for _ in "kv"))
+        _ok(lib().e2cuda_pages_load(self._p, layer, _ints(seqs, n, "load seqs", here), None if first is None else _ints(first, n, "load first", here),
+                                    _ints(q_start, n + 1, "load q_start", here), n, tokens, k.data_ptr(), v.data_ptr(), _type(k),
+                                    _stream(stream, here)), "load")
+        return k, v
+
+    def tree(self, parents, seqs, q_start, max_q: int, stream=None):
+        """The rows' trees, for attention and store: parents [T] int32 (each row's parent among its entry's rows, before it; -1: the text)
+        -> (tree [T][(max_q + 31) / 32] int32, pos [T] int32): the bits of each row's ancestors and its own, and its rotary position."""
+        here = self._here()
+        torch, T, n = _torch_mod, parents.shape[0], seqs.shape[0]
+        words = max(1, (max_q + 31) // 32)
+        tree, pos = _result(stream, lambda: (torch.empty((T, words), dtype=torch.int32, device=self.k.device),
+                                             torch.empty(T, dtype=torch.int32, device=self.k.device)))
+        _ok(lib().e2cuda_pages_tree(self._p, _ints(parents, T, "tree parents", here), _ints(seqs, n, "tree seqs", here),
+                                    _ints(q_start, n + 1, "tree q_start", here), n, T, tree.data_ptr(), words, pos.data_ptr(),
+                                    _stream(stream, here)), "tree")
+        return tree, pos
+
+    def keep(self, seqs, q_start, kept, counts, stream=None) -> None:
+        """Of entry i's rows, the last tokens of sequence seqs[i], the counts[i] ones kept[q_start[i]..] (ascending indices among
+        these rows; kept [T] int32) stay, in every layer, moved up behind the text; the sequence ends with them."""
+        here = self._here()
+        T, n = kept.shape[0], seqs.shape[0]
+        _ok(lib().e2cuda_pages_keep(self._p, _ints(seqs, n, "keep", here), _ints(q_start, n + 1, "keep", here), _ints(kept, T, "keep", here),
+                                    _ints(counts, n, "keep", here), n, T, _stream(stream, here)), "keep")
+
     def attention(self, layer: int, q, seqs, q_start, max_q: int, shared: int = 0, causal: bool = True, window: int = -1,
-                  scale: float | None = None, lse: bool = False, out=None, stream=None):
+                  scale: float | None = None, lse: bool = False, out=None, stream=None, sinks: int = 0, tree=None):
         """Attention of q [T][heads][head_dim] over the batch's cached tokens (the batch as in store; max_q:
         an upper bound of an entry's rows). The first `shared` tokens of every sequence lie in the same
         pages and, where that pays, are read once for the batch: with at most 64 rows of max_q tokens by the heads of a
-        key head, so a bound near the true one is worth its while. Returns out, or (out, lse [T][heads])."""
+        key head, so a bound near the true one is worth its while. Returns out, or (out, lse [T][heads]).
+        sinks: with a window, the first tokens that stay in sight. tree [T][words] int32: the rows are drafted tokens, which see the
+        text before them and the drafted ones whose bits are set (as `tree` makes them). q of an int8 cache: bf16 or fp16."""
         here = self._here()
         ldq = _rows(q, "attention q", here)
         T, H, D = q.shape
         p, n = self.pages, seqs.shape[0]
-        if D != p.head_dim or q.dtype != self.k.dtype:
+        if D != p.head_dim or (q.dtype != self.k.dtype if p.type != I8 else _type(q) == F32):
             raise E2CudaError(f"attention: q {tuple(q.shape)} {q.dtype} for a cache of heads of {p.head_dim} {self.k.dtype}")
         if out is None:
             out = _result(stream, lambda: _torch().empty_like(q) if q.is_contiguous() else q.new_empty((T, H, D)))
@@ -569,6 +638,13 @@ class PageCache:
         st = _stream(stream, here)
         max_q = min(max_q, T)  # a bound kept for batches of any size
         window = max(-1, min(window, INT_MAX))  # none, or wider than any sequence
+        sight = Sight(causal, window, min(sinks, INT_MAX), 0, None)
+        if tree is not None:
+            if tree.get_device() != here:
+                raise _elsewhere(tree, "attention tree", here)
+            if tree.dtype is not _torch_mod.int32 or tree.dim() != 2 or tree.shape[0] != T or not tree.is_contiguous():
+                raise E2CudaError(f"attention: a contiguous int32 tree of {T} rows, got {tree.dtype} {tuple(tree.shape)}")
+            sight.words, sight.tree = tree.shape[1], tree.data_ptr()
         batch = (n, T, max_q, H, shared)
         need = self._needs.get(batch)
         if need is None:
@@ -582,10 +658,10 @@ class PageCache:
             size = max(need, 2 * size, 16)
             ws = _result(stream, lambda: q.new_empty(size, dtype=_torch().uint8))
             self._scratch[st] = ws, size
-        _ok(lib().e2cuda_pages_attention(self._p, layer, q.data_ptr(), ldq, _ints(seqs, n, "attention seqs", here),
-                                         _ints(q_start, n + 1, "attention q_start", here), n, T, max_q, H, shared, causal, window,
-                                         1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(),
-                                         _rows(out, "attention out", here), _ptr(sums), ws.data_ptr(), size, st), "attention")
+        _ok(lib().e2cuda_pages_attention_sight(self._p, layer, _type(q), q.data_ptr(), ldq, _ints(seqs, n, "attention seqs", here),
+                                               _ints(q_start, n + 1, "attention q_start", here), n, T, max_q, H, shared, C.addressof(sight),
+                                               1.0 / math.sqrt(D) if scale is None else scale, out.data_ptr(),
+                                               _rows(out, "attention out", here), _ptr(sums), ws.data_ptr(), size, st), "attention")
         return (out, sums) if lse else out
 
 

@@ -206,7 +206,7 @@ int e2c_attention_wide(const void *q, const void *k, const void *vt, int ldvt, c
                        int B, int S, int H, int KV, float scale, int window, int *status, void *stream);
 
 /* ---- rotary positions (rope.cu) */
-enum { E2C_F32 = 0, E2C_BF16 = 1, E2C_F16 = 2 }; /* element types, E2CUDA_F32.. */
+enum { E2C_F32 = 0, E2C_BF16 = 1, E2C_F16 = 2, E2C_I8 = 3 }; /* element types, E2CUDA_F32.. */
 /* cs/sn [positions][half] = gain * cos/sin(position * freq[i]); freq: host, half <= 256 */
 int e2c_rope_table(float *cs, float *sn, int positions, int half, const double *freq, double gain, void *stream);
 /* x [T] rows of H heads of D (row stride ldx elements) -> y; pos NULL: row t is position t. Types
@@ -217,27 +217,39 @@ int e2c_rope(const void *x, int64_t ldx, int x_type, void *y, int64_t ldy, int y
 
 /* ---- a paged key/value cache (pages.cu, rope.cu, attention_pages.cu). k, v point at one layer for
  * the store and the attention, at layer 0 for the page operations; a layer is
- * [n_pages][page][KV][D] of `type` (16 bits). */
+ * [n_pages][page][KV][D] of `type` (16 bits, or E2C_I8 with scales ks, vs [n_pages][KV][page] a layer). */
 typedef struct {
     void *k, *v;
+    float *ks, *vs;
     int32_t *table;      /* [max_seqs][max_blocks] */
     int32_t *len, *refs; /* [max_seqs], [n_pages] */
     int32_t *ws;         /* e2c_pages_ws_ints() */
     int type, layers, n_pages, page, KV, D, max_seqs, max_blocks;
 } e2c_pages;
+enum { E2C_PAGES_WS_HEAD = 16 }; /* counters, before an entry each of lists [max_seqs] */
 size_t e2c_pages_ws_ints(int n_pages, int max_seqs);
+/* pos NULL: a row's place in its sequence is its rotary position too; q_out of q_type, the cache's type or beside E2C_I8
+ * any of 16 bits */
 int e2c_pages_store(const e2c_pages *pc, int x_type, const void *q, int64_t ldq, const void *k, int64_t ldk, const void *v,
-                    int64_t ldv, void *q_out, int64_t ldo, const float *cs, const float *sn, int positions, int half, int inter,
-                    const int32_t *seqs, const int32_t *q_start, int n, int T, int H, int *status, void *stream);
+                    int64_t ldv, void *q_out, int q_type, int64_t ldo, const float *cs, const float *sn, int positions, int half,
+                    int inter, const int32_t *pos, const int32_t *seqs, const int32_t *q_start, int n, int T, int H, int *status, void *stream);
+/* rows of k and v as y_type, dense; first NULL: an entry's rows are its last tokens */
+int e2c_pages_load(const e2c_pages *pc, const int32_t *seqs, const int32_t *first, const int32_t *q_start, int n, int T, void *k_out,
+                   void *v_out, int y_type, int *status, void *stream);
+/* drafted tokens (drafts.cu) */
+int e2c_pages_tree(const e2c_pages *pc, const int32_t *parents, const int32_t *seqs, const int32_t *q_start, int n, int T,
+                   uint32_t *tree, int words, int32_t *pos, int *status, void *stream);
+int e2c_pages_keep(const e2c_pages *pc, const int32_t *seqs, const int32_t *q_start, const int32_t *kept, const int32_t *counts, int n,
+                   int T, int *status, void *stream);
 int e2c_pages_copy(const e2c_pages *pc, const int32_t *src, const int32_t *dst, int n, int *status, void *stream);
 int e2c_pages_fork(const e2c_pages *pc, const int32_t *parents, const int32_t *children, int n, int *status, void *stream);
 int e2c_pages_append(const e2c_pages *pc, const int32_t *seqs, const int32_t *counts, int n, int *status, void *stream);
 int e2c_pages_free(const e2c_pages *pc, const int32_t *seqs, int n, int *status, void *stream);
 int e2c_pages_compact(const e2c_pages *pc, int32_t *used, int *status, void *stream);
 size_t e2c_pages_attention_ws_bytes(int n, int T, int max_q, int H, int KV, int D, int shared);
-int e2c_pages_attention(const e2c_pages *pc, const void *q, int64_t ldq, const int32_t *seqs, const int32_t *q_start, int n, int T,
-                        int max_q, int H, int shared, int causal, int window, float scale, void *out, int64_t ldo, float *lse,
-                        void *ws, size_t ws_bytes, int *status, void *stream);
+int e2c_pages_attention(const e2c_pages *pc, int q_type, const void *q, int64_t ldq, const int32_t *seqs, const int32_t *q_start, int n,
+                        int T, int max_q, int H, int shared, int causal, int window, int sinks, const uint32_t *tree, int words,
+                        float scale, void *out, int64_t ldo, float *lse, void *ws, size_t ws_bytes, int *status, void *stream);
 
 /* ---- self-test of the bounded wait (selftest.cu): one warp waits on an mbarrier that receives
  * its arrival first (arrive != 0) or never (arrive == 0). *completed is 1 if the wait completed, 0

@@ -7,7 +7,7 @@
 
 #define E2CU_PI 3.14159265358979323846
 
-static int type_ok(int t) { return t == E2CUDA_BF16 || t == E2CUDA_F16; }
+static int bits16(int t) { return t == E2CUDA_BF16 || t == E2CUDA_F16; }
 
 /* ------------------------------------------------------------------ rotary positions */
 /* pair index at which a pair makes `turns` rotations over `original` positions */
@@ -102,7 +102,7 @@ static int view(const e2cuda_pages *p, int layer, e2c_pages *out, const char *wh
         e2cu_err("%s: a cache's k, v, table, len, refs and ws must be given", what);
         return -1;
     }
-    if (!type_ok(p->type) || p->layers < 1 || p->n_pages < 1 || p->page < 8 || p->page > 1024 || (p->page & (p->page - 1)) ||
+    if ((!bits16(p->type) && p->type != E2CUDA_I8) || p->layers < 1 || p->n_pages < 1 || p->page < 8 || p->page > 1024 || (p->page & (p->page - 1)) ||
         p->kv_heads < 1 || p->kv_heads > 1024 || (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) ||
         p->max_seqs < 1 || p->max_blocks < 1 || p->max_blocks > 1 << 20 || (int64_t)p->max_blocks * p->page > 1 << 30 ||
         (int64_t)p->n_pages * p->page > INT32_MAX) {
@@ -114,12 +114,18 @@ static int view(const e2cuda_pages *p, int layer, e2c_pages *out, const char *wh
         e2cu_err("%s: a cache's k, v and refs must be 16-byte aligned", what);
         return -1;
     }
+    const int codes = p->type == E2CUDA_I8;
+    if (codes && (!p->k_scale || !p->v_scale || (((uintptr_t)p->k_scale | (uintptr_t)p->v_scale) & 15))) {
+        e2cu_err("%s: a cache of 8 bits needs k_scale and v_scale, 16-byte aligned", what);
+        return -1;
+    }
     if (layer < 0 || layer >= p->layers) {
         e2cu_err("%s: layer %d of %d", what, layer, p->layers);
         return -1;
     }
-    const size_t at = (size_t)layer * p->n_pages * p->page * p->kv_heads * p->head_dim * 2;
-    *out = (e2c_pages){ .k = (char *)p->k + at, .v = (char *)p->v + at, .table = p->table, .len = p->len, .refs = p->refs,
+    const size_t heads = (size_t)layer * p->n_pages * p->page * p->kv_heads, at = heads * p->head_dim * (codes ? 1 : 2);
+    *out = (e2c_pages){ .k = (char *)p->k + at, .v = (char *)p->v + at, .ks = codes ? p->k_scale + heads : NULL,
+                        .vs = codes ? p->v_scale + heads : NULL, .table = p->table, .len = p->len, .refs = p->refs,
                         .ws = p->ws, .type = p->type, .layers = p->layers, .n_pages = p->n_pages, .page = p->page,
                         .KV = p->kv_heads, .D = p->head_dim, .max_seqs = p->max_seqs, .max_blocks = p->max_blocks };
     return 0;
@@ -172,21 +178,69 @@ static int batch_ok(const int32_t *seqs, const int32_t *q_start, int n, int T, i
 int e2cuda_pages_store(const e2cuda_pages *pc, int layer, int x_type, const void *q, int ldq, const void *k, int ldk,
                        const void *v, int ldv, void *q_out, int ldo, const float *cos_t, const float *sin_t, int positions,
                        int rot, int flags, const int32_t *seqs, const int32_t *q_start, int n, int T, int heads, void *stream) {
+    const int q_type = pc && pc->type != E2CUDA_I8 ? pc->type : x_type;
+    return e2cuda_pages_store_at(pc, layer, x_type, q, ldq, k, ldk, v, ldv, q_out, q_type, ldo, cos_t, sin_t, positions, rot, flags,
+                                 NULL, seqs, q_start, n, T, heads, stream);
+}
+
+int e2cuda_pages_store_at(const e2cuda_pages *pc, int layer, int x_type, const void *q, int ldq, const void *k, int ldk,
+                          const void *v, int ldv, void *q_out, int q_type, int ldo, const float *cos_t, const float *sin_t,
+                          int positions, int rot, int flags, const int32_t *pos, const int32_t *seqs, const int32_t *q_start, int n,
+                          int T, int heads, void *stream) {
     e2c_pages c;
     if (view(pc, layer, &c, "pages_store")) return -1;
     if (T == 0) return 0;
     if (!batch_ok(seqs, q_start, n, T, heads, c.KV, "pages_store")) return -1;
     const int64_t qrow = (int64_t)heads * c.D, krow = (int64_t)c.KV * c.D;
     if (!q || !k || !v || !q_out || !cos_t || !sin_t || ldq < qrow || ldo < qrow || ldk < krow || ldv < krow || positions < 1 ||
-        rot < 2 || rot % 2 || rot > c.D || (flags & ~E2CUDA_ROPE_INTERLEAVED) || (x_type != E2CUDA_F32 && x_type != c.type) ||
-        (q == q_out && (x_type != c.type || ldq != ldo))) {
-        e2cu_err("pages_store: bad arguments (type %d, ld %d %d %d -> %d, rot %d, positions %d, flags %d)", x_type, ldq, ldk, ldv,
-                 ldo, rot, positions, flags);
+        rot < 2 || rot % 2 || rot > c.D || (flags & ~E2CUDA_ROPE_INTERLEAVED) || !bits16(q_type) ||
+        (c.type == E2CUDA_I8 ? x_type != E2CUDA_F32 && !bits16(x_type) : q_type != c.type || (x_type != E2CUDA_F32 && x_type != c.type)) ||
+        (q == q_out && (x_type != q_type || ldq != ldo))) {
+        e2cu_err("pages_store: bad arguments (types %d -> %d, %d, ld %d %d %d -> %d, rot %d, positions %d, flags %d)", x_type, q_type,
+                 c.type, ldq, ldk, ldv, ldo, rot, positions, flags);
         return -1;
     }
-    return e2cu_launch(e2c_pages_store(&c, x_type, q, ldq, k, ldk, v, ldv, q_out, ldo, cos_t, sin_t, positions, rot / 2,
-                                       flags & E2CUDA_ROPE_INTERLEAVED, seqs, q_start, n, T, heads, e2cu_status(), stream),
+    return e2cu_launch(e2c_pages_store(&c, x_type, q, ldq, k, ldk, v, ldv, q_out, q_type, ldo, cos_t, sin_t, positions, rot / 2,
+                                       flags & E2CUDA_ROPE_INTERLEAVED, pos, seqs, q_start, n, T, heads, e2cu_status(), stream),
                        "pages_store");
+}
+
+int e2cuda_pages_load(const e2cuda_pages *pc, int layer, const int32_t *seqs, const int32_t *first, const int32_t *q_start, int n, int T,
+                      void *k_out, void *v_out, int y_type, void *stream) {
+    e2c_pages c;
+    if (view(pc, layer, &c, "pages_load")) return -1;
+    if (T == 0) return 0;
+    if (!seqs || !q_start || n < 1 || T < 1 || !k_out || !v_out || (((uintptr_t)k_out | (uintptr_t)v_out) & 15) ||
+        (y_type != E2CUDA_F32 && !bits16(y_type))) {
+        e2cu_err("pages_load: bad arguments (n %d, T %d, type %d; outputs 16-byte aligned)", n, T, y_type);
+        return -1;
+    }
+    return e2cu_launch(e2c_pages_load(&c, seqs, first, q_start, n, T, k_out, v_out, y_type, e2cu_status(), stream), "pages_load");
+}
+
+/* ------------------------------------------------------------------ drafted tokens */
+int e2cuda_pages_tree(const e2cuda_pages *pc, const int32_t *parents, const int32_t *seqs, const int32_t *q_start, int n, int T,
+                      uint32_t *tree, int words, int32_t *pos, void *stream) {
+    e2c_pages c;
+    if (view(pc, 0, &c, "pages_tree")) return -1;
+    if (T == 0) return 0;
+    if (!parents || !seqs || !q_start || n < 1 || T < 1 || !tree || words < 1 || (int64_t)T * words > INT32_MAX) {
+        e2cu_err("pages_tree: bad arguments (n %d, T %d, words %d)", n, T, words);
+        return -1;
+    }
+    return e2cu_launch(e2c_pages_tree(&c, parents, seqs, q_start, n, T, tree, words, pos, e2cu_status(), stream), "pages_tree");
+}
+
+int e2cuda_pages_keep(const e2cuda_pages *pc, const int32_t *seqs, const int32_t *q_start, const int32_t *kept, const int32_t *counts,
+                      int n, int T, void *stream) {
+    e2c_pages c;
+    if (view(pc, 0, &c, "pages_keep") || !list_ok(seqs, q_start, n, c.max_seqs, "pages_keep")) return -1;
+    if (n == 0 || T == 0) return 0;
+    if (T < 0 || !kept || !counts) {
+        e2cu_err("pages_keep: bad arguments (T %d)", T);
+        return -1;
+    }
+    return e2cu_launch(e2c_pages_keep(&c, seqs, q_start, kept, counts, n, T, e2cu_status(), stream), "pages_keep");
 }
 
 /* what an attention call and the size of its workspace take: a row tile holds 128 (token, head) rows, so one token's
@@ -206,6 +260,14 @@ size_t e2cuda_pages_attention_ws_bytes(const e2cuda_pages *pc, int n, int T, int
 int e2cuda_pages_attention(const e2cuda_pages *pc, int layer, const void *q, int ldq, const int32_t *seqs, const int32_t *q_start,
                            int n, int T, int max_q, int heads, int shared, int causal, int window, float scale, void *out, int ldo,
                            float *lse, void *ws, size_t ws_bytes, void *stream) {
+    const e2cuda_sight s = { .causal = causal, .window = window };
+    return e2cuda_pages_attention_sight(pc, layer, pc ? pc->type : 0, q, ldq, seqs, q_start, n, T, max_q, heads, shared, &s, scale, out,
+                                        ldo, lse, ws, ws_bytes, stream);
+}
+
+int e2cuda_pages_attention_sight(const e2cuda_pages *pc, int layer, int q_type, const void *q, int ldq, const int32_t *seqs,
+                                 const int32_t *q_start, int n, int T, int max_q, int heads, int shared, const e2cuda_sight *sight,
+                                 float scale, void *out, int ldo, float *lse, void *ws, size_t ws_bytes, void *stream) {
     e2c_pages c;
     if (view(pc, layer, &c, "pages_attention")) return -1;
     if (T == 0) return 0;
@@ -221,12 +283,22 @@ int e2cuda_pages_attention(const e2cuda_pages *pc, int layer, const void *q, int
         e2cu_err("pages_attention: q and out must be 16-byte aligned with rows of a multiple of 8 elements");
         return -1;
     }
+    if (!bits16(q_type) || (c.type != E2CUDA_I8 && q_type != c.type)) {
+        e2cu_err("pages_attention: q of type %d for a cache of type %d", q_type, c.type);
+        return -1;
+    }
+    if (!sight || sight->sinks < 0 || (sight->tree && (sight->words < 1 || (int64_t)sight->words * 32 < max_q || ((uintptr_t)sight->tree & 3)))) {
+        e2cu_err("pages_attention: sinks %d, a tree of %d words a row for %d rows", sight ? sight->sinks : 0, sight ? sight->words : 0,
+                 max_q);
+        return -1;
+    }
     const size_t need = e2c_pages_attention_ws_bytes(n, T, max_q, heads, c.KV, c.D, shared);
     if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) {
         e2cu_err("pages_attention: needs %zu bytes of 16-byte aligned workspace, got %zu", need, ws ? ws_bytes : 0);
         return -1;
     }
-    return e2cu_launch(e2c_pages_attention(&c, q, ldq, seqs, q_start, n, T, max_q, heads, shared, causal, window, scale, out, ldo,
-                                           lse, ws, ws_bytes, e2cu_status(), stream),
+    return e2cu_launch(e2c_pages_attention(&c, q_type, q, ldq, seqs, q_start, n, T, max_q, heads, shared, sight->causal, sight->window,
+                                           sight->sinks, sight->tree, sight->words, scale, out, ldo, lse, ws, ws_bytes, e2cu_status(),
+                                           stream),
                        "pages_attention");
 }

@@ -27,7 +27,7 @@ namespace {
 constexpr int PLAN = 1024;  // threads of the planning block
 
 // the workspace: counters, an append's offsets and copies (one per entry), page lists
-enum { W_MOVES = 0, W_HEAD = 16 };
+enum { W_MOVES = 0, W_HEAD = E2C_PAGES_WS_HEAD };
 struct Ws {
     int32_t *off, *src, *dst, *list, *high, *remap;
 };
@@ -314,7 +314,7 @@ int move_pages(const e2c_pages *pc, const int32_t *src, const int32_t *dst, int 
         e2c_set_msg("%s: no CUDA device", what);
         return -2;
     }
-    const int64_t bytes = (int64_t)pc->page * pc->KV * pc->D * 2;
+    const int64_t bytes = (int64_t)pc->page * pc->KV * (pc->type == E2C_F32 ? 4 : pc->D * (pc->type == E2C_I8 ? 1 : 2));
     const int vecs = (int)(bytes / 16);
     int shift = 3;
     while (shift < 8 && (UNROLL << shift) < vecs) shift++;
@@ -327,7 +327,14 @@ int move_pages(const e2c_pages *pc, const int32_t *src, const int32_t *dst, int 
     const unsigned grid = (unsigned)(blocks < most ? blocks : most);
     e2c_launch_as(true, k_move, dim3(grid), dim3(256), 0, (cudaStream_t)stream, *pc, src, dst, n, count, vecs, pieces, shift,
                status);
-    return launched(what);
+    if (launched(what)) return -2;
+    if (pc->type != E2C_I8) return 0;
+    // the scales, page by page, are moved like the codes
+    e2c_pages s = *pc;
+    s.k = pc->ks;
+    s.v = pc->vs;
+    s.type = E2C_F32;
+    return move_pages(&s, src, dst, n, count, status, stream, what);
 }
 
 int32_t *ws_at(const e2c_pages *pc, int64_t ints) { return pc->ws + W_HEAD + ints; }

@@ -22,159 +22,14 @@
 #include <math.h>
 #include <stdint.h>
 
-#include <type_traits>
-
 #include "launch.h"
 #include "pages.cuh"
+#include "pages_codes.h"
 #include "pdl.h"
 #include "ptx.cuh"
+#include "rope.cuh"
 
 namespace {
-
-constexpr int HPT = 4;      // heads per thread
-constexpr int BLOCK = 128;  // threads per block: decode-sized calls spread over more SMs than with 256
-
-template <typename T>
-E2C_DEV float to_f(T x);
-template <>
-E2C_DEV float to_f(float x) {
-    return x;
-}
-template <>
-E2C_DEV float to_f(__nv_bfloat16 x) {
-    return __bfloat162float(x);
-}
-template <>
-E2C_DEV float to_f(__half x) {
-    return __half2float(x);
-}
-template <typename T>
-E2C_DEV T from_f(float x);
-template <>
-E2C_DEV float from_f(float x) {
-    return x;
-}
-template <>
-E2C_DEV __nv_bfloat16 from_f(float x) {
-    return __float2bfloat16_rn(x);
-}
-template <>
-E2C_DEV __half from_f(float x) {
-    return __float2half_rn(x);
-}
-
-// N consecutive values; N * sizeof(T) is a multiple of 16 with 16-byte alignment, or N = 1
-template <typename T, int N>
-E2C_DEV void store(T *p, const float (&r)[N]) {
-    if constexpr (N == 1) {
-        *p = from_f<T>(r[0]);
-    } else {
-        constexpr int PER = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < N; i += PER) {
-            uint4 w;
-            T *e = reinterpret_cast<T *>(&w);
-#pragma unroll
-            for (int j = 0; j < PER; j++) e[j] = from_f<T>(r[i + j]);
-            *reinterpret_cast<uint4 *>(p + i) = w;
-        }
-    }
-}
-
-// N values as they lie in memory
-template <typename T, int N>
-struct Raw {
-    static constexpr int WORDS = N == 1 ? 0 : N * sizeof(T) / 16;
-    uint4 w[WORDS ? WORDS : 1];
-    T one;
-    E2C_DEV void get(const T *p) {
-        if constexpr (N == 1) {
-            one = *p;
-        } else {
-#pragma unroll
-            for (int i = 0; i < WORDS; i++) w[i] = reinterpret_cast<const uint4 *>(p)[i];
-        }
-    }
-    E2C_DEV void floats(float (&r)[N]) const {
-        if constexpr (N == 1) {
-            r[0] = to_f<T>(one);
-        } else {
-            const T *e = reinterpret_cast<const T *>(w);
-#pragma unroll
-            for (int i = 0; i < N; i++) r[i] = to_f<T>(e[i]);
-        }
-    }
-    // to y: bit for bit where the types are the same
-    template <typename TO>
-    E2C_DEV void copy(TO *y) const {
-        if constexpr (std::is_same<T, TO>::value && N > 1) {
-#pragma unroll
-            for (int i = 0; i < WORDS; i++) reinterpret_cast<uint4 *>(y)[i] = w[i];
-        } else {
-            float r[N];
-            floats(r);
-            store<TO, N>(y, r);
-        }
-    }
-};
-
-// u / d for u < 2^31 by a multiplication
-struct Div {
-    uint32_t d, mul, shift;
-};
-E2C_DEV uint32_t div_by(uint32_t u, const Div &v) { return v.d == 1 ? u : (uint32_t)(__umulhi(u, v.mul) >> v.shift); }
-
-// A thread's part of each of its heads: V elements from e0 on and V from e1 on, which neighbouring threads
-// continue; together V pairs, or some of the dimensions that pass through.
-struct Part {
-    int e0, e1;
-    bool two, turn;  // there is a second run; it is rotated
-};
-template <int V>
-E2C_DEV Part part_of(int j, int half, int units, int D, bool inter) {
-    const int nrot = half / V;
-    if (j < nrot && V == 1 && inter) return {2 * j, 2 * j + 1, true, true};
-    if (j < nrot) return {j * V, half + j * V, true, true};
-    const int e0 = 2 * half + (j - nrot) * V, e1 = e0 + (units - nrot) * V;
-    return {e0, e1, e1 < D, false};
-}
-// the angles of unit j's V pairs: those of its first run and those of its second
-template <int V>
-E2C_DEV void angles(const float *t, int j, int half, bool inter, float (&r)[V]) {
-    if constexpr (V == 1) {
-        r[0] = t[j];
-    } else {
-        const float *a = t + (inter ? j * V / 2 : j * V), *b = inter ? a + half / 2 : a + V / 2;
-        using Half = std::conditional_t<V == 8, float4, float2>;
-        static_assert(sizeof(Half) * 2 == sizeof r, "16-bit or 32-bit results");
-        reinterpret_cast<Half *>(r)[0] = *reinterpret_cast<const Half *>(a);
-        reinterpret_cast<Half *>(r)[1] = *reinterpret_cast<const Half *>(b);
-    }
-}
-template <typename TI, typename TO, int V>
-E2C_DEV void turn(const Raw<TI, V> &x0, const Raw<TI, V> &x1, TO *y0, TO *y1, bool inter, const float (&c)[V],
-                  const float (&s)[V]) {
-    float a[V], b[V], u[V], w[V];
-    x0.floats(a);
-    x1.floats(b);
-    if (!inter || V == 1) {
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            u[i] = a[i] * c[i] - b[i] * s[i];
-            w[i] = b[i] * c[i] + a[i] * s[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i + 1 < V; i += 2) {
-            u[i] = a[i] * c[i / 2] - a[i + 1] * s[i / 2];
-            u[i + 1] = a[i + 1] * c[i / 2] + a[i] * s[i / 2];
-            w[i] = b[i] * c[(V + i) / 2] - b[i + 1] * s[(V + i) / 2];
-            w[i + 1] = b[i + 1] * c[(V + i) / 2] + b[i] * s[(V + i) / 2];
-        }
-    }
-    store<TO, V>(y0, u);
-    store<TO, V>(y1, w);
-}
 
 struct RopeArgs {
     const void *x;
@@ -232,24 +87,12 @@ __global__ void __launch_bounds__(BLOCK) k_rope(const RopeArgs p, const Div per_
     }
 }
 
-struct StoreArgs {
-    const void *q, *k, *v;
-    int64_t ldq, ldk, ldv;
-    void *q_out;
-    int64_t ldo;
-    const float *cs, *sn;
-    int positions, half, inter;
-    const int32_t *seqs, *q_start;
-    int n, T, H;
-    e2c_pages pc;  // k and v at the layer
-    int *status;
-};
 
 // One thread: unit j of up to four heads of one token, as k_rope; the heads are H query heads and KV
 // key heads (rotated) and KV value heads (passed through). The input loads are issued before the
 // chain of lookups (token -> sequence -> length -> page) that the stores wait for.
 template <typename TI, typename TO, int V>
-__global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, const Div per_token, const Div units, const Div vunits, int qgroups, int kgroups) {
+__global__ void __launch_bounds__(BLOCK) k_pages_store(const e2c_store_args p, const Div per_token, const Div units, const Div vunits, int qgroups, int kgroups) {
     griddep_launch_dependents();
     griddep_wait();
     const uint32_t u = blockIdx.x * BLOCK + threadIdx.x;
@@ -282,8 +125,9 @@ __global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, const 
     const int at = ok ? p.pc.len[seq] - (last - t) : -1;
     // a token without a place (its sequence is not in the cache, or is shorter than its queries, or
     // longer than the table or the rotary table) is not written
-    if (at < 0 || at >= p.positions) {
-        record_status(p.status, at >= p.positions ? E2C_ERR_BAD_POSITION : E2C_ERR_BAD_SEQ);
+    const int turn_at = p.pos && at >= 0 ? p.pos[t] : at;
+    if (at < 0 || (unsigned)turn_at >= (unsigned)p.positions) {
+        record_status(p.status, at < 0 ? E2C_ERR_BAD_SEQ : E2C_ERR_BAD_POSITION);
         return;
     }
     TO *y;
@@ -301,8 +145,8 @@ __global__ void __launch_bounds__(BLOCK) k_pages_store(const StoreArgs p, const 
     y += (int64_t)h0 * D;
     if (part.turn) {
         alignas(16) float c[V], s[V];
-        angles<V>(p.cs + (int64_t)at * p.half, j, p.half, p.inter, c);
-        angles<V>(p.sn + (int64_t)at * p.half, j, p.half, p.inter, s);
+        angles<V>(p.cs + (int64_t)turn_at * p.half, j, p.half, p.inter, c);
+        angles<V>(p.sn + (int64_t)turn_at * p.half, j, p.half, p.inter, s);
 #pragma unroll
         for (int h = 0; h < HPT; h++)
             if (h < nh) turn<TI, TO, V>(a[h], b[h], y + h * D + part.e0, y + h * D + part.e1, p.inter, c, s);
@@ -336,22 +180,6 @@ __global__ void __launch_bounds__(256) k_rope_table(float *cs, float *sn, int64_
     sn[u] = (float)(s * gain);
 }
 
-int launched(const char *what) {
-    const cudaError_t e = cudaGetLastError();
-    if (e == cudaSuccess) return 0;
-    e2c_set_msg("%s launch: %s", what, cudaGetErrorString(e));
-    return -2;
-}
-
-Div divide_by(int d) {
-    int s = 0;
-    while ((1ll << s) < d) s++;
-    // ceil(2^(31 + s) / d) < 2^32: right for every u < 2^31
-    return {(uint32_t)d, (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d), (uint32_t)(s ? s - 1 : 0)};
-}
-
-bool fits16(const void *p, int64_t ld, int bytes) { return ((uintptr_t)p & 15) == 0 && (ld * bytes) % 16 == 0; }
-
 template <typename TI, typename TO>
 int rope_as(const RopeArgs &a, bool vec, cudaStream_t st) {
     constexpr int VV = 16 / sizeof(TO);
@@ -374,7 +202,7 @@ int rope_as(const RopeArgs &a, bool vec, cudaStream_t st) {
 }
 
 template <typename TI, typename TO>
-int store_as(const StoreArgs &a, bool vec, cudaStream_t st) {
+int store_as(const e2c_store_args &a, bool vec, cudaStream_t st) {
     constexpr int VV = 16 / sizeof(TO);
     const int V = vec ? VV : 1, D = a.pc.D;
     const int units = a.half / V + ((D - 2 * a.half) / V + 1) / 2, vunits = (D / V + 1) / 2;
@@ -420,14 +248,15 @@ extern "C" int e2c_rope(const void *x, int64_t ldx, int x_type, void *y, int64_t
 }
 
 extern "C" int e2c_pages_store(const e2c_pages *pc, int x_type, const void *q, int64_t ldq, const void *k, int64_t ldk,
-                               const void *v, int64_t ldv, void *q_out, int64_t ldo, const float *cs, const float *sn,
-                               int positions, int half, int inter, const int32_t *seqs, const int32_t *q_start, int n, int T, int H,
+                               const void *v, int64_t ldv, void *q_out, int q_type, int64_t ldo, const float *cs,
+                               const float *sn, int positions, int half, int inter, const int32_t *pos, const int32_t *seqs, const int32_t *q_start, int n, int T, int H,
                                int *status, void *stream) {
-    StoreArgs a = {q, k, v, ldq, ldk, ldv, q_out, ldo, cs, sn, positions, half, inter, seqs, q_start, n, T, H, *pc, status};
+    e2c_store_args a = {q, k, v, ldq, ldk, ldv, q_out, ldo, cs, sn, positions, half, inter, pos, seqs, q_start, n, T, H, *pc, status};
     const int xb = x_type == E2C_F32 ? 4 : 2;
     const bool vec = half % 8 == 0 && fits16(q, ldq, xb) && fits16(k, ldk, xb) && fits16(v, ldv, xb) && fits16(q_out, ldo, 2) &&
                      fits16(cs, 0, 4) && fits16(sn, 0, 4);
     cudaStream_t st = (cudaStream_t)stream;
+    if (pc->type == E2C_I8) return e2c_store_codes(a, x_type, q_type, st);
     if (pc->type == E2C_BF16)
         return x_type == E2C_F32 ? store_as<float, __nv_bfloat16>(a, vec, st) : store_as<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
     return x_type == E2C_F32 ? store_as<float, __half>(a, vec, st) : store_as<__half, __half>(a, vec, st);

@@ -196,7 +196,7 @@ int e2cuda_attention_window(const void *q, const void *k, const void *vt, int ld
 
 /* ------------------------------------------------------------------ rotary positions */
 /* Element types of the calls below. */
-enum { E2CUDA_F32 = 0, E2CUDA_BF16 = 1, E2CUDA_F16 = 2 };
+enum { E2CUDA_F32 = 0, E2CUDA_BF16 = 1, E2CUDA_F16 = 2, E2CUDA_I8 = 3 /* a cache's pages only */ };
 
 /* How the frequencies theta^(-2 i / rot) of the rot / 2 pairs are scaled to reach past the length a
  * model was trained on, by `factor` >= 1:
@@ -252,13 +252,19 @@ typedef struct e2cuda_pages {
     int32_t *len;   /* [max_seqs] tokens held; 0: the sequence is free                             */
     int32_t *refs;  /* [n_pages] sequences that map the page; 0: free. 16-byte aligned             */
     int32_t *ws;    /* e2cuda_pages_ws_bytes() of scratch                                          */
-    int type;       /* E2CUDA_BF16 or E2CUDA_F16                                                   */
+    int type;       /* E2CUDA_BF16, E2CUDA_F16 or E2CUDA_I8                                        */
     int layers, n_pages;
     int page;       /* tokens of a page: a power of two, 8..1024                                   */
     int kv_heads, head_dim; /* head_dim 64, 128 or 256                                             */
     int max_seqs, max_blocks;
+    float *k_scale, *v_scale; /* type E2CUDA_I8 alone: [layers][n_pages][kv_heads][page], 16-byte aligned */
 } e2cuda_pages;
 size_t e2cuda_pages_ws_bytes(int n_pages, int max_seqs);
+
+/* Pages of 8 bits. A token's head of k or v is held as signed codes and one scale, quantised as e2cuda_quantize_rows does:
+ * scale = amax / 127 (1 for zeros), code = round(x * 127 / amax), amax the head's largest magnitude. It stands for
+ * code * scale: half the memory of a 16-bit cache less four bytes a head. A head with a NaN or an infinity stands for NaN, one whose
+ * amax is below 2^-100 for zeros. */
 
 /* Each child (a free sequence) maps its parent's pages: no data moves. A child is no parent in the same call. */
 int e2cuda_pages_fork(const e2cuda_pages *pc, const int32_t *parents, const int32_t *children, int n, void *stream);
@@ -288,6 +294,20 @@ int e2cuda_pages_store(const e2cuda_pages *pc, int layer, int x_type, const void
                        const void *v, int ldv, void *q_out, int ldo, const float *cos_t, const float *sin_t, int positions,
                        int rot, int flags, const int32_t *seqs, const int32_t *q_start, int n, int T, int heads,
                        void *stream);
+/* The same with the rotary position of each row given (pos, device [T]; NULL: its place in its sequence), as rows whose order is
+ * not that of their positions need, and with q_out's type: the cache's, or with pages of E2CUDA_I8 either of 16 bits.
+ * Such a cache takes q, k and v of any type, all the same, and e2cuda_pages_store gives q_out x_type, which has 16 bits there.
+ * Rotation and quantisation are in 32 bits. A row whose position is outside the table is left out and reported. */
+int e2cuda_pages_store_at(const e2cuda_pages *pc, int layer, int x_type, const void *q, int ldq, const void *k, int ldk,
+                          const void *v, int ldv, void *q_out, int q_type, int ldo, const float *cos_t, const float *sin_t,
+                          int positions, int rot, int flags, const int32_t *pos, const int32_t *seqs, const int32_t *q_start, int n,
+                          int T, int heads, void *stream);
+/* Keys and values read back: entry i's rows q_start[i].. of k_out and v_out [T][kv_heads][head_dim] (dense, 16-byte aligned,
+ * of y_type: any of fp32 and 16 bits) are the tokens of sequence seqs[i] from first[i] on (first NULL: its last ones). Pages of 16
+ * bits are converted, those of 8 bits give code * scale, rounded once. Rows that are not in the cache are left
+ * as they are and reported. */
+int e2cuda_pages_load(const e2cuda_pages *pc, int layer, const int32_t *seqs, const int32_t *first, const int32_t *q_start, int n, int T,
+                      void *k_out, void *v_out, int y_type, void *stream);
 
 /* Attention of the batch's rows over their sequences' cached tokens:
  *   out[t][h] = sum_j softmax_j(scale * q[t][h] . k_j) v_j,   lse[t][h] = log sum_j exp(scale * q[t][h] . k_j)
@@ -316,6 +336,38 @@ size_t e2cuda_pages_attention_ws_bytes(const e2cuda_pages *pc, int n, int T, int
 int e2cuda_pages_attention(const e2cuda_pages *pc, int layer, const void *q, int ldq, const int32_t *seqs,
                            const int32_t *q_start, int n, int T, int max_q, int heads, int shared, int causal, int window,
                            float scale, void *out, int ldo, float *lse, void *ws, size_t ws_bytes, void *stream);
+
+/* What rows see. Without a tree: causal and window as above, and with a window the first `sinks` tokens of the sequence
+ * too, whatever their distance (with causal, those up to the row). Tiles of keys that no row sees are not read.
+ * With a tree (device [T][words], words * 32 >= max_q), an entry's rows are drafted tokens in an order of their own, behind
+ * the text, the tokens before them: row t sees the text, and the entry's drafted token i if bit i % 32 of tree[t][i / 32] is set
+ * (its own is one of them); causal says nothing. A row's position is that of the text's last token plus the number of
+ * its bits; by it a window and sinks apply to the text, and among the drafted tokens the bits alone decide. */
+typedef struct e2cuda_sight {
+    int causal, window, sinks;
+    int words;
+    const uint32_t *tree;
+} e2cuda_sight;
+/* The same for q and out of q_type: the cache's type, or with pages of E2CUDA_I8 either of 16 bits. Over such pages the logits
+ * are the codes' products times the key's scale, exact up to 32-bit sums; an exponential times its token's scale of v is rounded
+ * to 16 bits before the product with the codes. */
+int e2cuda_pages_attention_sight(const e2cuda_pages *pc, int layer, int q_type, const void *q, int ldq, const int32_t *seqs,
+                                 const int32_t *q_start, int n, int T, int max_q, int heads, int shared, const e2cuda_sight *sight,
+                                 float scale, void *out, int ldo, float *lse, void *ws, size_t ws_bytes, void *stream);
+
+/* ---- trees of drafted tokens: append grows each sequence by its drafted tokens, pages_tree says what they see and where they
+ * stand, pages_store_at and pages_attention_sight take that in every layer, and pages_keep ends the step. */
+/* parents [T]: the index, among its entry's rows, of each row's parent, which comes before it, or -1 for the text. tree [T][words]
+ * (words * 32 >= the longest entry's rows) gets the bits of each row's ancestors and its own, pos [T] (or NULL) its rotary position: the text's
+ * length plus its ancestors. A parent that is not before its row is taken as -1 and reported. */
+int e2cuda_pages_tree(const e2cuda_pages *pc, const int32_t *parents, const int32_t *seqs, const int32_t *q_start, int n, int T,
+                      uint32_t *tree, int words, int32_t *pos, void *stream);
+/* Of the last q_start[i + 1] - q_start[i] tokens of sequence seqs[i], those of kept[q_start[i]..] (counts[i] of them, ascending
+ * indices among these tokens) stay, in every layer, moved up behind the text; the sequence ends with them, and pages past its end
+ * lose its mapping. An entry whose list is not like that, or with a page to be written that other sequences map too, is left
+ * as it is and reported. */
+int e2cuda_pages_keep(const e2cuda_pages *pc, const int32_t *seqs, const int32_t *q_start, const int32_t *kept, const int32_t *counts,
+                      int n, int T, void *stream);
 
 /* ------------------------------------------------------------------ fused FFN block (config 1) */
 typedef struct e2cuda_ffn e2cuda_ffn;
