@@ -72,8 +72,8 @@ struct e2c_attn_args {
     int *status;
 };
 
-// What rows see beside causal order and a window: SIGHT says that a call has sinks or a tree.
-enum { SIGHT = 1 };
+// What a call has beside causal order and a window: sinks or a tree (SIGHT), pages of 8 bits (CODES)
+enum { SIGHT = 1, CODES = 2 };
 // The kernels of one kind over 16-bit pages: launches them for heads of a.pc.D, and their join.
 int e2c_attn_plain(const e2c_attn_args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st);
 int e2c_attn_sight(const e2c_attn_args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st);
@@ -108,23 +108,30 @@ E2C_DEV bool wait_warp(uint32_t bar, uint32_t parity, int *status, int code) {
 
 constexpr float LN2 = 0.6931471805599453f, LOG2E = 1.4426950408889634f;
 
-template <int D>
+template <int D, int KIND>
 struct Cfg {
+    static constexpr bool CODE = KIND & CODES;
     // warps: NG softmax groups of four, the epilogue's four, then one each. A third softmax group hides more
     // of a tile's latencies where its products are shortest (heads of 64, us with two and with three: the 4 prompts
     // above 366 and 338, single tokens behind 700 of their own 55.4 and 52.1, behind 16 42.3 and 43.5); with wider
     // heads it gives less and costs batches of short items (128: 385 and 374, 92.9 and 94.1 for 128
     // tokens behind a shared prefix; 256: 312 and 314)
-    static constexpr int NG = D == 64 ? 3 : 2;
+    static constexpr int NG = D == 64 && !CODE ? 3 : 2;
     static constexpr int W_EPI = 4 * NG, W_ITEMS = W_EPI + 4, W_MMA = W_ITEMS + 1, W_K = W_MMA + 1, W_V = W_K + 1;
-    static constexpr int WARPS = W_V + 1, NTHREADS = 32 * WARPS;
+    static constexpr int W_CONVERT = W_V + 1;  // CODES: four warps for K, then four for V
+    static constexpr int WARPS = W_CONVERT + (CODE ? 8 : 0), NTHREADS = 32 * WARPS;
     static constexpr int PANELS = D / 64;  // 64 of the head's dimensions each, 128 bytes a row
     static constexpr int NQ = D == 64 ? 2 : 1;  // Q buffers
     // K and V have a ring of stages each: of a tile, or for D = 256 of half a one (K: half of the
     // head's dimensions, V: half of the keys)
     static constexpr int KPARTS = D == 256 ? 2 : 1, VROWS = TK / KPARTS;
     static constexpr int STAGE = TK * D * 2 / KPARTS;
-    static constexpr int NKS = D == 64 ? 5 : D == 128 ? 3 : 2, NVS = D == 64 ? 5 : 2;
+    static constexpr int NKS = CODE ? (D == 64 ? 3 : D == 128 ? 2 : 1) : D == 64 ? 5 : D == 128 ? 3 : 2;
+    static constexpr int NVS = CODE ? (D == 64 ? 3 : 1) : D == 64 ? 5 : 2;
+    // CODES: stages as the pages hold them, rows of ROW bytes in panels; K's with the scales of both behind its codes
+    static constexpr int ROW = D == 64 ? 64 : 128, CSTAGE = STAGE / 2, KCSTAGE = CSTAGE + 2 * TK * 4;
+    static constexpr int NKC = !CODE ? 0 : D == 64 ? 4 : 3, NVC = !CODE ? 0 : D == 64 ? 4 : 2;
+    static constexpr int NC = 4;  // tiles whose scales are in shared memory
     // tensor memory: NS buffers of S (128 columns each), then NO of O (D columns each), 512 columns
     static constexpr int NS = D == 256 ? 2 : 3;
     static constexpr int NO = D == 64 ? 2 : 1;
@@ -135,7 +142,9 @@ struct Cfg {
     static constexpr int Q_BYTES = TR * D * 2;
     static constexpr int K_OFF = NQ * Q_BYTES;
     static constexpr int V_OFF = K_OFF + NKS * STAGE;
-    static constexpr int XM = V_OFF + NVS * STAGE;              // running maxima handed on [NG][128]
+    static constexpr int KC_OFF = V_OFF + NVS * STAGE, VC_OFF = KC_OFF + NKC * KCSTAGE;
+    static constexpr int SC_OFF = VC_OFF + NVC * CSTAGE;        // [NC][3][128]: of K times c, log2 of V's, V's
+    static constexpr int XM = SC_OFF + (CODE ? NC * 3 * TK * 4 : 0);  // running maxima handed on [NG][128]
     static constexpr int ML = XM + NG * TR * 4;                 // item's (m, l) [2 items][NG][128] x 2
     static constexpr int ITEMS = ML + 2 * NG * TR * 8;
     static constexpr int SCAN = ITEMS + NI * 64;
@@ -160,13 +169,21 @@ enum {
     B_KE = B_KF + 5,
     B_VF = B_KE + 5,
     B_VE = B_VF + 5,
-    B_NUM = B_VE + 5
+    B_KCF = B_VE + 5,  // CODES: codes of K and V, and scales
+    B_KCE = B_KCF + 4,
+    B_VCF = B_KCE + 4,
+    B_VCE = B_VCF + 4,
+    B_SCF = B_VCE + 4,
+    B_SCE = B_SCF + 4,
+    B_NUM = B_SCE + 4
 };
-template <int D>
+template <int D, int KIND>
 constexpr int smem_bytes() {
-    return Cfg<D>::BARS + B_NUM * 8 + 16;
+    return Cfg<D, KIND>::BARS + B_NUM * 8 + 16;
 }
-static_assert(smem_bytes<64>() <= 232448 && smem_bytes<128>() <= 232448 && smem_bytes<256>() <= 232448, "shared memory");
+template <int KIND>
+constexpr bool fits = smem_bytes<64, KIND>() <= 232448 && smem_bytes<128, KIND>() <= 232448 && smem_bytes<256, KIND>() <= 232448;
+static_assert(fits<0> && fits<SIGHT | CODES>, "shared memory");
 
 enum { TO_OUT = 0, TO_SLOT = 1, TO_DENSE = 2 };
 struct __align__(16) Item {
@@ -416,15 +433,15 @@ struct Plan {
 // Every thread of the block: sums over the entries, the longest of them, and the entry in which this
 // block's share begins (block 0 leaves the joining kernel the cost before each entry). Up to NTHREADS
 // entries are read once, more of them twice.
-template <int D>
+template <int D, int KIND>
 struct PlanScratch {
-    int64_t sum[Cfg<D>::WARPS];  // by warp
+    int64_t sum[Cfg<D, KIND>::WARPS];  // by warp
     int at;              // cost before the block's first entry
     int longest, least, masked, first, seq;
 };
 template <int D, int KIND>
-E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<D> &s) {
-    constexpr int WARPS = Cfg<D>::WARPS, NTHREADS = Cfg<D>::NTHREADS;
+E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<D, KIND> &s) {
+    constexpr int WARPS = Cfg<D, KIND>::WARPS, NTHREADS = Cfg<D, KIND>::NTHREADS;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     if (tid == 0) {
         s.longest = -1;
@@ -556,6 +573,13 @@ E2C_DEV float2 add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
     return y;
 }
+E2C_DEV float2 mul2(float2 a, float2 b) {
+    float2 y;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t &>(y))
+        : "l"(reinterpret_cast<uint64_t &>(a)), "l"(reinterpret_cast<uint64_t &>(b)));
+    return y;
+}
 // 2^x of two values on the FMA pipe, for x <= 125: x = n + f with |f| <= 1/2 (adding 1.5 * 2^23 rounds to
 // the whole number n and leaves it in the low bits), a polynomial of degree 4 in f fitted to the
 // least relative error (2.7e-6 in fp32), and n added to the exponent. Below 2^-125 the result stays there.
@@ -594,12 +618,140 @@ __host__ __device__ constexpr uint32_t type_bits() {  // A and B formats of the 
     return sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? (1u << 7) | (1u << 10) : 0u;
 }
 
+// ---- pages of 8 bits (CODES). A tile's codes become 16-bit numbers (exactly: they are whole and at most 127) on their
+// way from the stages that the loads fill to those that the products read; scales stay out of the products:
+//   logit_j = (q . code_j) kc_j,   kc = K's scale * c
+//   O = sum_j P_j code_j,   P_j = 2^(logit_j - m) vs_j rounded to 16 bits,   m at least the largest logit_j + log2 vs_j (less 2^8)
+// so that P has the size that it has without scales whatever theirs is; l = sum_j 2^(logit_j - m) in 32 bits. A scale of
+// V that is not finite makes P, and the rows with it, NaN.
+
+// four codes as 16-bit floats
+template <typename T>
+E2C_DEV uint2 from_codes(uint32_t w);
+// 128 + the low seven bits, less 128 or, with the sign's bit set, 256: bf16 holds both
+template <>
+E2C_DEV uint2 from_codes<__nv_bfloat16>(uint32_t w) {
+    const uint32_t low = w & 0x7f7f7f7fu, sign = w & 0x80808080u;
+    const uint32_t a = __byte_perm(low, 0x43434343u, 0x4140), b = __byte_perm(low, 0x43434343u, 0x4342);
+    const uint32_t c = __byte_perm(sign, 0x43434343u, 0x4140), d = __byte_perm(sign, 0x43434343u, 0x4342);
+    const __nv_bfloat162 x = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(a), reinterpret_cast<const __nv_bfloat162 &>(c));
+    const __nv_bfloat162 y = __hsub2(reinterpret_cast<const __nv_bfloat162 &>(b), reinterpret_cast<const __nv_bfloat162 &>(d));
+    return make_uint2(reinterpret_cast<const uint32_t &>(x), reinterpret_cast<const uint32_t &>(y));
+}
+// 1024 + (code + 128), less 1152
+template <>
+E2C_DEV uint2 from_codes<__half>(uint32_t w) {
+    const uint32_t u = w ^ 0x80808080u, less = 0x64806480u;
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(reinterpret_cast<const __half2 &>(a), reinterpret_cast<const __half2 &>(less));
+    const __half2 y = __hsub2(reinterpret_cast<const __half2 &>(b), reinterpret_cast<const __half2 &>(less));
+    return make_uint2(reinterpret_cast<const uint32_t &>(x), reinterpret_cast<const uint32_t &>(y));
+}
+
+// logits of N columns with log2 of their scales of V (sc: the columns' kc, 128 further log2 vs)
+template <int N>
+E2C_DEV void scale_logits(uint32_t (&s)[N], const float *sc) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 k = *reinterpret_cast<const float4 *>(sc + i), v = *reinterpret_cast<const float4 *>(sc + TK + i);
+        const float2 a = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y), make_float2(v.x, v.y));
+        const float2 b = fma2(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w), make_float2(v.z, v.w));
+        s[i] = __float_as_uint(a.x), s[i + 1] = __float_as_uint(a.y), s[i + 2] = __float_as_uint(b.x), s[i + 3] = __float_as_uint(b.y);
+    }
+}
+
+// Four warps for K (w < 4) and four for V: every stage's codes, of as many keys as the product takes, into the 128-byte swizzle that
+// it reads; V's rows past the last key become zeros. K's warps also prepare the tile's scales.
+template <typename T, int D, int KIND, typename Bar, typename Take>
+E2C_DEV void convert_codes(const Args &p, uint8_t *smem, int w, int lane, Bar bar, Take take) {
+    using C = Cfg<D, KIND>;
+    constexpr int CHUNKS = C::ROW / 16, PARTS = C::CSTAGE / 16 / 128;  // of a row; of a thread
+    const bool is_v = w >= 4;
+    const int tid = (w & 3) * 32 + lane, rows = is_v ? C::VROWS : TK;
+    const int FULL = is_v ? B_VCF : B_KCF, FREE = is_v ? B_VCE : B_KCE, NST = is_v ? C::NVC : C::NKC;
+    const int OUT = is_v ? B_VF : B_KF, TAKEN = is_v ? B_VE : B_KE, NOUT = is_v ? C::NVS : C::NKS;
+    const int pitch = is_v ? C::CSTAGE : C::KCSTAGE;
+    const uint8_t *ring = smem + (is_v ? C::VC_OFF : C::KC_OFF);
+    uint8_t *to = smem + (is_v ? C::V_OFF : C::K_OFF);
+    int st = 0, out = 0, g = 0;
+    uint32_t sp = 0, op = 1;
+    Item it;
+    for (int n = 0; take(n, it); n++) {
+#pragma unroll 1
+        for (int j = 0; j < it.nt; j++, g++) {
+            const int nk = min(TK, tile_end<KIND>(p, it, j) - tile_key<KIND>(it, j));
+#pragma unroll 1
+            for (int h = 0; h < C::KPARTS; h++) {
+                if (!wait_warp(bar(FULL + st), sp, p.status, E2C_ERR_WAIT_PRODUCER)) return;
+                const uint8_t *x = ring + st * pitch;
+                if (!is_v && h == 0) {
+                    if (!wait_warp(bar(B_SCE + g % C::NC), (uint32_t)(((g / C::NC) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) return;
+                    float *sc = reinterpret_cast<float *>(smem + C::SC_OFF) + (g % C::NC) * (3 * TK);
+                    const float *from = reinterpret_cast<const float *>(x + C::CSTAGE);
+                    const float k = tid < nk ? from[tid] : 0.f, v = tid < nk ? from[TK + tid] : 0.f;
+                    const bool fine = fabsf(v) < INFINITY;
+                    sc[tid] = k * p.c;
+                    // 2^100 either way is far from where l or P would leave fp32's range
+                    sc[TK + tid] = fine ? fminf(fmaxf(__log2f(fabsf(v)), -100.f), 100.f) : 0.f;
+                    sc[2 * TK + tid] = fine ? v : NAN;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(B_SCF + g % C::NC));
+                }
+                if (!wait_warp(bar(TAKEN + out), op, p.status, E2C_ERR_WAIT_PRODUCER)) return;
+                const int here = is_v ? min(nk - h * C::VROWS, C::VROWS) : nk, up = (here + 15) & ~15;
+                uint8_t *y = to + out * C::STAGE;
+#pragma unroll
+                for (int i0 = 0; i0 < PARTS; i0 += 4) {
+                    uint4 c[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int e = tid + 128 * (i0 + i), r = e / CHUNKS & (rows - 1);
+                        if (r < here) c[i] = *reinterpret_cast<const uint4 *>(x + e * 16);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int e = tid + 128 * (i0 + i), r = e / CHUNKS & (rows - 1), panel = e / CHUNKS / rows;
+                        if (r >= up) continue;
+                        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+                        if (r < here) {
+                            const uint2 s0 = from_codes<T>(c[i].x), s1 = from_codes<T>(c[i].y), s2 = from_codes<T>(c[i].z), s3 = from_codes<T>(c[i].w);
+                            a = make_uint4(s0.x, s0.y, s1.x, s1.y);
+                            b = make_uint4(s2.x, s2.y, s3.x, s3.y);
+                        }
+                        // 16 codes are two 16-byte pieces of a panel of 64; which one a thread writes first
+                        // alternates, so that eight neighbours write to all banks
+                        const int ch = e & (CHUNKS - 1), pan = panel * (C::ROW / 64) + (ch >> 2), piece = (ch & 3) * 2;
+                        uint8_t *row = y + pan * (rows * 128) + r * 128;
+                        const int odd = D == 64 ? 0 : ch >> 2;
+                        *reinterpret_cast<uint4 *>(row + (((piece + odd) ^ (r & 7)) << 4)) = odd ? b : a;
+                        *reinterpret_cast<uint4 *>(row + (((piece + 1 - odd) ^ (r & 7)) << 4)) = odd ? a : b;
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(OUT + out));
+                    mbar_arrive(bar(FREE + st));
+                }
+                if (++st == NST) {
+                    st = 0;
+                    sp ^= 1;
+                }
+                if (++out == NOUT) {
+                    out = 0;
+                    op ^= 1;
+                }
+            }
+        }
+    }
+}
+
 template <typename T, int D, int KIND>
-__global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
+__global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
     k_attention_pages(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQp,
                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ Args p, const int q_box, const int qp_box) {
-    using C = Cfg<D>;
+    using C = Cfg<D, KIND>;
     extern __shared__ __align__(1024) uint8_t smem[];
     griddep_launch_dependents();
     if (smem_u32(smem) & 1023) {
@@ -631,13 +783,21 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
         for (int i = 0; i < 4 * C::NG; i++) mbar_init(bar(B_MX + i), 1);
         for (int i = 0; i < NI; i++) {
             mbar_init(bar(B_ITF + i), 1);
-            mbar_init(bar(B_ITE + i), 8 + 4 * C::NG);  // K, V, QK, PV, the epilogue and softmax warps
+            mbar_init(bar(B_ITE + i), 8 + 4 * C::NG + (C::CODE ? 8 : 0));  // K, V, QK, PV, the epilogue, softmax and converting warps
         }
         for (int i = 0; i < 5; i++) {
-            mbar_init(bar(B_KF + i), 1);
+            mbar_init(bar(B_KF + i), C::CODE ? 4 : 1);
             mbar_init(bar(B_KE + i), 1);
-            mbar_init(bar(B_VF + i), 1);
+            mbar_init(bar(B_VF + i), C::CODE ? 4 : 1);
             mbar_init(bar(B_VE + i), 1);
+        }
+        for (int i = 0; C::CODE && i < 4; i++) {
+            mbar_init(bar(B_KCF + i), 1);
+            mbar_init(bar(B_KCE + i), 4);
+            mbar_init(bar(B_VCF + i), 1);
+            mbar_init(bar(B_VCE + i), 4);
+            mbar_init(bar(B_SCF + i), 4);
+            mbar_init(bar(B_SCE + i), 4);
         }
         mbar_init(bar(B_DRAIN), 1);
         fence_mbar_init();
@@ -656,7 +816,7 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
     const uint32_t tmem = *tmem_slot;
 
     Plan pl;
-    make_plan<D, KIND>(p, pl, *reinterpret_cast<PlanScratch<D> *>(smem + C::SCAN));
+    make_plan<D, KIND>(p, pl, *reinterpret_cast<PlanScratch<D, KIND> *>(smem + C::SCAN));
 
     // A consumer's copy of item n; false after the last one (or a failure). The slot is released at once.
     auto take = [&](int n, Item &it) -> bool {
@@ -671,7 +831,9 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
         return it.ntok >= 0;
     };
 
-    if (warp >= C::W_ITEMS) {
+    if (C::CODE && warp >= C::W_CONVERT) {
+        convert_codes<T, D, KIND>(p, smem, warp - C::W_CONVERT, lane, bar, take);
+    } else if (warp >= C::W_ITEMS) {
         if (warp == C::W_ITEMS) {
             // ------------------------------------------------------------ items and Q loads
             const int L0 = pl.share.begin(blockIdx.x), L1 = pl.share.begin(blockIdx.x + 1);
@@ -958,8 +1120,9 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
             // ------------------------------------------------------------ K loads, V loads
             const bool is_v = warp == C::W_V;
             const CUtensorMap *tm = is_v ? &tmV : &tmK;
-            const int F = is_v ? B_VF : B_KF, E = is_v ? B_VE : B_KE, NST = is_v ? C::NVS : C::NKS;
-            const uint32_t ring = sbase + (is_v ? C::V_OFF : C::K_OFF);
+            const int F = C::CODE ? (is_v ? B_VCF : B_KCF) : is_v ? B_VF : B_KF, E = C::CODE ? (is_v ? B_VCE : B_KCE) : is_v ? B_VE : B_KE;
+            const int NST = C::CODE ? (is_v ? C::NVC : C::NKC) : is_v ? C::NVS : C::NKS;
+            const uint32_t ring = sbase + (C::CODE ? (is_v ? C::VC_OFF : C::KC_OFF) : is_v ? C::V_OFF : C::K_OFF);
             const int PB = min(p.pc.page, C::VROWS), shift = 31 - __clz(p.pc.page);
             Item it = {};
             int n = 0, j = 0, st = 0, total = 0;
@@ -1006,6 +1169,36 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                         int y = __shfl_sync(0xffffffffu, row, b0), y2 = __shfl_sync(0xffffffffu, row, min(b0 + 1, 31));
                         if (!(ok = wait_warp(bar(E + st), par, p.status, E2C_ERR_WAIT_PRODUCER))) break;
                         const uint32_t full = bar(F + st);
+                        if constexpr (C::CODE) {
+                            // panels of ROW bytes a key, and with a tile's first codes of K the scales of both
+                            constexpr int WIDE = D == 256 ? 2 : 1;
+                            const int panels = is_v ? WIDE : 1;
+                            const bool scales = !is_v && h == 0;
+                            uint32_t dst = ring + st * (is_v ? C::CSTAGE : C::KCSTAGE), sd = ring + st * C::KCSTAGE + C::CSTAGE;
+                            const int x8 = kvh * D + (is_v ? 0 : h * C::ROW);
+                            if (elect_one()) mbar_arrive_expect_tx(full, (uint32_t)((b1 - b0) * PB * (panels * C::ROW + (scales ? 8 : 0))));
+                            __syncwarp();
+#pragma unroll 1
+                            for (int b = b0; b < b1; b++, dst += PB * C::ROW, sd += PB * 4) {
+                                if (elect_one()) {
+                                    tma_load_2d(dst, tm, x8, y, full);
+                                    if (WIDE == 2 && is_v) tma_load_2d(dst + C::VROWS * C::ROW, tm, x8 + C::ROW, y, full);
+                                    if (scales) {
+                                        const int64_t at = ((int64_t)(y >> shift) * p.pc.KV + kvh) * p.pc.page + (y & (p.pc.page - 1));
+                                        bulk_load(sd, p.pc.ks + at, (uint32_t)PB * 4, full);
+                                        bulk_load(sd + TK * 4, p.pc.vs + at, (uint32_t)PB * 4, full);
+                                    }
+                                }
+                                y = y2;
+                                y2 = __shfl_sync(0xffffffffu, row, min(b + 2, 31));
+                            }
+                            if (++st == NST) {
+                                st = 0;
+                                par ^= 1;
+                            }
+                            total++;
+                            continue;
+                        }
                         uint32_t dst = ring + st * C::STAGE;
                         if (elect_one()) mbar_arrive_expect_tx(full, (uint32_t)((b1 - b0) * PB * 128 * np));
                         __syncwarp();
@@ -1130,6 +1323,12 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
 #pragma unroll
                     for (int i = 0; i < 16; i++) s[i] = seen & (1u << i) ? s[i] : 0xff800000u;
                 };
+                // CODES: a tile's scales; y(i) is what a logit and the log2 of V's scale come to
+                const float *sc = reinterpret_cast<const float *>(smem + C::SC_OFF) + (g % C::NC) * (3 * TK);
+                if (C::CODE && !wait_warp(bar(B_SCF + g % C::NC), (uint32_t)((g / C::NC) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                    ok = false;
+                    break;
+                }
                 float mx = -INFINITY;
                 if (busy) {
                     float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -1139,6 +1338,7 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                             uint32_t s[32];
                             tmem_ld32(ts + c0, s);
                             tmem_wait_ld();
+                            if constexpr (C::CODE) scale_logits<32>(s, sc + c0);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
@@ -1149,12 +1349,13 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                             uint32_t s[16];
                             tmem_ld16(ts + c0, s);
                             tmem_wait_ld();
+                            if constexpr (C::CODE) scale_logits<16>(s, sc + c0);
                             hide(c0, s, row4c);
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
                     }
-                    mx = max2(max2(mm[0], mm[1]), max2(mm[2], mm[3])) * p.c;
+                    mx = max2(max2(mm[0], mm[1]), max2(mm[2], mm[3])) * (C::CODE ? 1.f : p.c);
                 }
                 float now = before, alpha = 1.f;
                 if (live && !(mx <= before + kRescaleLog2)) {  // so also from -infinity, and for a NaN
@@ -1201,9 +1402,11 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
-                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, mm);
+                                const float2 k2 = C::CODE ? *reinterpret_cast<const float2 *>(sc + c0 + 2 * i) : cc;
+                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k2, mm);
                                 x = i % kPoly == kPoly - 1 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
+                                if constexpr (C::CODE) x = mul2(x, *reinterpret_cast<const float2 *>(sc + 2 * TK + c0 + 2 * i));
                                 pk[i] = pack2<T>(x.x, x.y);
                             }
                             tmem_st16(ts + c0 / 2, pk);
@@ -1214,12 +1417,22 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                             uint32_t s[16], pk[8];
                             tmem_ld16(ts + c0, s);
                             tmem_wait_ld();
+                            if constexpr (C::CODE) {  // before what is hidden becomes -infinity: a scale may be zero
+#pragma unroll
+                                for (int i = 0; i < 8; i++) {
+                                    const float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
+                                                          *reinterpret_cast<const float2 *>(sc + c0 + 2 * i), mm);
+                                    s[2 * i] = __float_as_uint(x.x), s[2 * i + 1] = __float_as_uint(x.y);
+                                }
+                            }
                             hide(c0, s, row4);
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
-                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, mm);
+                                float2 x = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+                                if constexpr (!C::CODE) x = fma2(x, cc, mm);
                                 x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
+                                if constexpr (C::CODE) x = mul2(x, *reinterpret_cast<const float2 *>(sc + 2 * TK + c0 + 2 * i));
                                 pk[i] = pack2<T>(x.x, x.y);
                             }
                             tmem_st8(ts + c0 / 2, pk);
@@ -1229,7 +1442,10 @@ __global__ void __launch_bounds__(Cfg<D>::NTHREADS, 1)
                     l += all.x + all.y;
                     tmem_wait_st();
                 }
-                if (nk & 15) {
+                if (C::CODE) {  // the tile's scales have been read
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(B_SCE + g % C::NC));
+                } else if (nk & 15) {
                     // V's rows past the last key, up to the product's 16: each of the group's warps zeroes panels
                     const int part = nk / C::VROWS, vt = g * C::KPARTS + part, vs = vt % C::NVS;
                     // Parities tell only neighbouring phases apart: the stage's load before this one, of tile
@@ -1463,14 +1679,14 @@ int launch_error(const char *what) {
 
 template <typename T, int D, int KIND>
 int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st) {
-    using C = Cfg<D>;
+    using C = Cfg<D, KIND>;
     static E2cPerDev attr;
     const int dev = e2c_device();
     if (!attr.get(dev)) {
-        if (cudaFuncSetAttribute(k_attention_pages<T, D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>()) !=
+        if (cudaFuncSetAttribute(k_attention_pages<T, D, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D, KIND>()) !=
             cudaSuccess) {
             cudaGetLastError();
-            e2c_set_msg("pages_attention: cannot reserve %d bytes of shared memory", smem_bytes<D>());
+            e2c_set_msg("pages_attention: cannot reserve %d bytes of shared memory", smem_bytes<D, KIND>());
             return -2;
         }
         attr.set(dev, 1);
@@ -1482,11 +1698,13 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
     CUtensorMap tq, tqp, tk, tv;
     if (e2c_tmap_3d(&tq, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, q_box) ||
         (prefix && e2c_tmap_3d(&tqp, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, qp_box)) ||
-        e2c_tmap_2d(&tk, a.pc.k, dt, 2, width, rows, width * 2, 64, box) ||
-        e2c_tmap_2d(&tv, a.pc.v, dt, 2, width, rows, width * 2, 64, box))
+        (C::CODE ? e2c_tmap_2d_plain(&tk, a.pc.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, width, rows, width, C::ROW, box)
+                 : e2c_tmap_2d(&tk, a.pc.k, dt, 2, width, rows, width * 2, 64, box)) ||
+        (C::CODE ? e2c_tmap_2d_plain(&tv, a.pc.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, width, rows, width, C::ROW, box)
+                 : e2c_tmap_2d(&tv, a.pc.v, dt, 2, width, rows, width * 2, 64, box)))
         return -3;
     if (!prefix) tqp = tq;
-    e2c_launch_as(true, k_attention_pages<T, D, KIND>, dim3(sms), dim3(Cfg<D>::NTHREADS), smem_bytes<D>(), st, tq, tqp, tk, tv, a, q_box, qp_box);
+    e2c_launch_as(true, k_attention_pages<T, D, KIND>, dim3(sms), dim3(C::NTHREADS), smem_bytes<D, KIND>(), st, tq, tqp, tk, tv, a, q_box, qp_box);
     if (launch_error("pages_attention")) return -2;
     using J = Join<T, D>;
     if (prefix)

@@ -135,6 +135,12 @@ E2C_DEV void tma_load_3d(uint32_t dst, const CUtensorMap *m, int x, int y, int z
         "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y), "r"(z), "r"(bar)
         : "memory");
 }
+// `bytes` contiguous bytes into this CTA's shared memory: both addresses 16-byte aligned, a multiple of 16
+E2C_DEV void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 // 2D tile store from this CTA's shared memory (bulk-group completion). Rows / columns outside the
 // tensor are not written.
 E2C_DEV void tma_store_2d(const CUtensorMap *m, uint32_t src, int x, int y) {

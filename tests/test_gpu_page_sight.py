@@ -340,3 +340,57 @@ def test_store_at_positions(e2c, torch_cuda, dtype):
     want, _ = turn64(torch, k[good], cos, sin, pos[good], False, False)
     step = want.abs().amax(-1, keepdim=True) * (2.0 ** -8 if dtype == "bfloat16" else 0.5 / 127)
     assert ((k2[good].double() - want).abs() <= step * (1 + 2.0 ** -10)).all()
+
+
+# ------------------------------------------------------------------------------------------ pages of 8 bits
+def quantised(torch, x):
+    """Codes and scales of heads, in the 32-bit arithmetic of the engine's activation quantiser."""
+    amax = x.float().abs().amax(-1, keepdim=True)
+    some = amax > 0
+    codes = (x.float() * torch.where(some, 127.0 / amax, 1.0)).round().to(torch.int8)
+    return codes, torch.where(some, amax * float(np.float32(1 / 127)), 1.0)[..., 0]
+
+
+def make_codes(e2c, torch, seed, lens, queries, shared, H, KV, D, page, dtype, spread=1.0, layers=1):
+    """make_batch's cache in 8 bits; tokens' sizes differ by e^spread, and scales are NaN wherever nothing is held."""
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, seed, lens, queries, shared, H, KV, D, page, dtype, layers=layers)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    parts = []
+    for x in (cache.k, cache.v):
+        held = ~torch.isnan(x[..., 0])
+        size = (torch.randn(held.shape, generator=g, device="cuda") * spread).exp()
+        codes, scale = quantised(torch, torch.nan_to_num(x).float() * size[..., None])
+        wild = torch.randint(-128, 128, codes.shape, generator=g, device="cuda").to(torch.int8)
+        parts.append((torch.where(held[..., None], codes, wild), torch.where(held, scale, float("nan")).transpose(-1, -2).contiguous()))
+    (k, ks), (v, vs) = parts
+    return e2c.PageCache(k, v, cache.table, cache.length, cache.refs, ks, vs), q, seqs, q_start, max_q
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("causal,window,sinks", [(True, -1, 0), (False, 37, 0), (True, 130, 4), (False, 0, 129)])
+@pytest.mark.parametrize("case", list(CASES))
+def test_codes_attention(e2c, torch_cuda, case, causal, window, sinks, dtype):
+    torch = torch_cuda
+    lens, queries, shared, H, KV, D, page = CASES[case]
+    cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 14, lens, queries, shared, H, KV, D, page, dtype, spread=0.3)
+    out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, causal=causal, window=window, sinks=sinks, lse=True)
+    e2c.check()
+    assert_attention(torch, out, lse, sight64(torch, cache, 0, q, seqs, q_start, causal, window, D ** -0.5, sinks), dtype, max(lens))
+    again = cache.attention(0, q, seqs, q_start, max_q, shared=shared, causal=causal, window=window, sinks=sinks)
+    assert torch.equal(again, out), "two calls differ"
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", list(TREES))
+def test_codes_tree_attention(e2c, torch_cuda, case, dtype):
+    torch = torch_cuda
+    lens, rows, shared, H, KV, D, page = TREES[case]
+    rng = np.random.default_rng(len(case))
+    cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 15, lens, rows, shared, H, KV, D, page, dtype, spread=0.3)
+    parents = [random_parents(rng, rows[s]) for s in seqs.tolist()]
+    tree, _ = cache.tree(dev(torch, sum(parents, [])), seqs, q_start, max_q)
+    for window, sinks in ((-1, 0), (40, 3)):
+        out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, window=window, sinks=sinks, tree=tree, lse=True)
+        e2c.check()
+        want = sight64(torch, cache, 0, q, seqs, q_start, True, window, D ** -0.5, sinks, [tree_mask(p) for p in parents])
+        assert_attention(torch, out, lse, want, dtype, max(lens))
