@@ -19,9 +19,14 @@ bool use_prefix(int n, int max_q, int KV, int G, int shared, int sms) {
     return shared > 0 && 2 * max_q * G <= TR && (int64_t)(n - 1) * KV * ((shared + TK - 1) / TK) > PREFIX_TILES * sms;
 }
 
+bool few_rows(bool here, bool prefix, int max_q, int G) { return here && !prefix && (int64_t)max_q * G <= FEW_ROWS; }
+
 struct Layout {
     size_t split, before, po, pl, dpo, dpl, bytes;
 };
+// Blocks an SM and rows of a part that a call for few rows has at most: its parts take no more than the others' (16 of 128 rows, twice)
+constexpr int FEW_BLOCKS = 2;
+static_assert(FEW_BLOCKS * FEW_ROWS <= 128, "workspace");
 Layout layout(int blocks, int n, int T, int H, int KV, int D, bool prefix) {
     Layout l;
     size_t at = 0;
@@ -33,7 +38,7 @@ Layout layout(int blocks, int n, int T, int H, int KV, int D, bool prefix) {
     // a prefix has at most one item a block, or one for each row tile of each key head if those are more
     const size_t tpt = TR / (H / KV), rows = KV * ((T + tpt - 1) / tpt);
     const size_t slots = 2 * (size_t)blocks + (prefix ? (rows > (size_t)blocks ? rows : (size_t)blocks) : 0);
-    l.split = take(sizeof(int4) * 2 * blocks);
+    l.split = take(sizeof(int4) * 2 * FEW_BLOCKS * blocks);
     l.before = take(sizeof(int) * ((size_t)n + 2));
     l.pl = take(sizeof(float) * slots * TR);
     l.po = take(sizeof(float) * slots * TR * D);
@@ -83,6 +88,7 @@ extern "C" int e2c_pages_attention(const e2c_pages *pc, int q_type, const void *
     a.sinks = a.window >= 0 ? sinks : 0;
     a.tree = tree;
     a.words = words;
+    a.align = pc->page < 16 ? 16 : pc->page < 128 ? pc->page : 128;
     // a scale of zero keeps masked logits (-inf) apart from the others (0)
     a.c = scale == 0.f ? 1e-30f : fabsf(scale) * LOG2E;
     a.neg = scale < 0.f;
@@ -98,7 +104,9 @@ extern "C" int e2c_pages_attention(const e2c_pages *pc, int q_type, const void *
     a.dpl = reinterpret_cast<float *>(w + l.dpl);
     a.status = status;
     cudaStream_t st = (cudaStream_t)stream;
-    if (pc->type == E2C_I8) return e2c_attn_codes(a, q, ldq, prefix, sms, st);
+    const bool codes = pc->type == E2C_I8;
+    if (few_rows(codes || a.sinks || a.tree, prefix, max_q, G)) return codes ? e2c_attn_few_codes(a, q, ldq, sms, st) : e2c_attn_few(a, q, ldq, sms, st);
+    if (codes) return e2c_attn_codes(a, q, ldq, prefix, sms, st);
     return a.sinks || a.tree ? e2c_attn_sight(a, q, ldq, prefix, sms, st) : e2c_attn_plain(a, q, ldq, prefix, sms, st);
 }
 

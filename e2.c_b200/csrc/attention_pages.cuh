@@ -58,6 +58,7 @@ struct e2c_attn_args {
     int n, T, max_q, H, G, tpt;  // tpt: tokens of an item
     int shared, causal, window;
     int sinks, words;            // SIGHT: first tokens that a window leaves visible (0 without a window);
+    int align;                   // FEW: what a window's first key is rounded down to
     const uint32_t *tree;        // rows' bits among their entry's drafted tokens [T][words], or null
     float c;                     // |scale| log2 e
     uint32_t neg;                // scale < 0: the products negate Q
@@ -72,13 +73,18 @@ struct e2c_attn_args {
     int *status;
 };
 
-// What a call has beside causal order and a window: sinks or a tree (SIGHT), pages of 8 bits (CODES)
-enum { SIGHT = 1, CODES = 2 };
+// What a call has beside causal order and a window: sinks or a tree (SIGHT), pages of 8 bits (CODES), few rows an
+// entry (FEW, attention_few.cuh)
+enum { SIGHT = 1, CODES = 2, FEW = 4 };
 // The kernels of one kind over 16-bit pages: launches them for heads of a.pc.D, and their join.
 int e2c_attn_plain(const e2c_attn_args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st);
 int e2c_attn_sight(const e2c_attn_args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st);
 // The same over pages of 8 bits, with SIGHT.
 int e2c_attn_codes(const e2c_attn_args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st);
+// The same over pages of 16 and of 8 bits, for entries of at most FEW_ROWS rows (tokens by the heads of a key head), without a prefix.
+constexpr int FEW_ROWS = 16;
+int e2c_attn_few(const e2c_attn_args &a, const void *q, int64_t ldq, int sms, cudaStream_t st);
+int e2c_attn_few_codes(const e2c_attn_args &a, const void *q, int64_t ldq, int sms, cudaStream_t st);
 
 namespace {
 
@@ -274,6 +280,13 @@ E2C_DEV Entry entry_of(const Args &p, int i, bool report) {
 }
 
 // A run of key tiles: nt of them from k0 on, keys before klim; gap keys are skipped after the first ns.
+// a window's first tile begins at a multiple of it (past the prefix): of what one load brings, at least
+template <int KIND>
+E2C_DEV int aligned(const Args &p, int x) {
+    return KIND & FEW ? x & -p.align : x / TK * TK;
+}
+template <int KIND>
+constexpr int SLOT = KIND & FEW ? FEW_ROWS : TR;  // rows of a part in the workspace
 struct Span {
     int nt, k0, klim, ns, gap;
     // the part of nt tiles from tile off on, in an item's fields
@@ -296,13 +309,14 @@ E2C_DEV int tile_end(const Args &p, const Item &it, int j) {
     return KIND & SIGHT && j < it.ns ? p.sinks : it.klim;
 }
 // the sinks [base, se) and a window's keys [lo, hi) as one run of tiles from base on; those in neither are skipped
-E2C_DEV Span with_sinks(int base, int se, int lo, int hi) {
+template <int KIND>
+E2C_DEV Span with_sinks(const Args &p, int base, int se, int lo, int hi) {
     const int ns = se > base ? (se - base + TK - 1) / TK : 0;
     if (hi <= lo) {
         if (ns == 0) return {1, 0, 1, 0, 0};
         return {ns, base, se, 0, 0};
     }
-    const int kw = base + (lo - base) / TK * TK, end = base + ns * TK;
+    const int kw = base + aligned<KIND>(p, lo - base), end = base + ns * TK;
     if (ns > 0 && kw > end) return {ns + (hi - kw + TK - 1) / TK, base, hi, ns, kw - end};
     const int k0 = ns > 0 ? base : kw, klim = max(hi, se);
     return {(klim - k0 + TK - 1) / TK, k0, klim, 0, 0};
@@ -326,7 +340,7 @@ E2C_DEV Span span_of(const Args &p, int len, int nq, int r, int base) {
             lo = max(lo, pa - p.window);
             if (!p.tree) hi = min(hi, pb + p.window + 1);
         }
-        return with_sinks(base, min(p.sinks, text), lo, hi);
+        return with_sinks<KIND>(p, base, min(p.sinks, text), lo, hi);
     }
     int lo = base, hi = p.causal ? min(len, pb + 1) : len;
     if (p.window >= 0) {
@@ -433,15 +447,15 @@ struct Plan {
 // Every thread of the block: sums over the entries, the longest of them, and the entry in which this
 // block's share begins (block 0 leaves the joining kernel the cost before each entry). Up to NTHREADS
 // entries are read once, more of them twice.
-template <int D, int KIND>
+template <int WARPS>
 struct PlanScratch {
-    int64_t sum[Cfg<D, KIND>::WARPS];  // by warp
+    int64_t sum[WARPS];  // by warp
     int at;              // cost before the block's first entry
     int longest, least, masked, first, seq;
 };
-template <int D, int KIND>
-E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<D, KIND> &s) {
-    constexpr int WARPS = Cfg<D, KIND>::WARPS, NTHREADS = Cfg<D, KIND>::NTHREADS;
+template <int WARPS, int KIND>
+E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<WARPS> &s) {
+    constexpr int NTHREADS = 32 * WARPS;
     const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
     if (tid == 0) {
         s.longest = -1;
@@ -503,7 +517,7 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<D, KIND> &s) {
                 if (p.window >= 0) lo = max(0, s.least - (KIND & SIGHT && p.tree ? 1 : 0) - p.window);
                 if (KIND & SIGHT) {
                     const int se = min(p.sinks, pmax);
-                    pl.pspan = with_sinks(0, se, lo, pmax);
+                    pl.pspan = with_sinks<KIND>(p, 0, se, lo, pmax);
                     pl.ptiles = lo < pmax || se > 0 ? pl.pspan.nt : 0;
                 } else {
                     const int k0 = lo / TK * TK;
@@ -538,6 +552,101 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<D, KIND> &s) {
         p.before[p.n + 1] = pl.ptiles;
     }
 }
+
+// One warp: the parts of sequence items in a block's share, in order. Entries are read 32 at a time, one a lane.
+template <int KIND>
+struct Walk {
+    int pos, end, off;      // the share left; tiles before pos of the entry
+    int i, base, kvh, r;    // the entry, the first of those read; the next key head and row tile
+    Entry e;                // the lane's entry and its tiles for one key head
+    int etiles;
+    bool inside;            // an entry has been begun: its tokens, rows and first row
+    int len, nq, q0, seq;
+    E2C_DEV void begin(const Plan &pl, int L0, int L1) {
+        pos = L0;
+        end = L1;
+        off = L0 - pl.first_before;
+        i = pl.first;
+        base = -32;
+        inside = false;
+    }
+    // the next part, in the fields of `it` that do not hold for all of them; false after the last
+    E2C_DEV bool next(const Args &p, const Plan &pl, Item &it, int lane) {
+        for (;;) {
+            if (!inside) {
+                if (pos >= end || i >= p.n) return false;
+                if (i >= base + 32) {
+                    base = i;
+                    e = {};
+                    etiles = 0;
+                    if (i + lane < p.n) {
+                        e = entry_of(p, i + lane, false);
+                        etiles = (int)tiles_of<KIND>(p, e.len, e.nq, p.shared);
+                    }
+                }
+                const int src = i - base, c = __shfl_sync(0xffffffffu, etiles, src);
+                nq = __shfl_sync(0xffffffffu, e.nq, src);
+                if (nq == 0) {
+                    i++;
+                    continue;
+                }
+                len = __shfl_sync(0xffffffffu, e.len, src);
+                q0 = __shfl_sync(0xffffffffu, e.q0, src);
+                seq = __shfl_sync(0xffffffffu, e.seq, src);
+                if (len == 0) seq = -1;  // its table says nothing
+                kvh = r = 0;
+                if (off >= c) {
+                    kvh = off / c;
+                    off -= kvh * c;
+                }
+                inside = true;
+            }
+#pragma unroll 1
+            while (pos < end && kvh < p.pc.KV) {
+                const Span sp = span_of<KIND>(p, len, nq, r, p.shared);
+                const int nt = sp.nt, cost = nt + ITEM_COST;
+                bool found = false;
+                if (off >= cost) {
+                    off -= cost;
+                } else if (off >= nt) {  // the share begins past the item's tiles
+                    pos = min(pos + cost - off, end);
+                    off = 0;
+                } else {
+                    const int s = pos - off, stop = s + nt, first = pl.share.begin(blockIdx.x);
+                    it.seq = seq;
+                    it.len = len;
+                    if (KIND & SIGHT) it.base = len - nq;
+                    it.kvh = kvh;
+                    it.t0 = q0 + r * p.tpt;
+                    it.ntok = min(p.tpt, nq - r * p.tpt);
+                    sp.cut(p, off, min(stop, end) - pos, it);
+                    it.pos0 = len - nq + r * p.tpt;
+                    it.dst = p.shared > 0 ? TO_DENSE : TO_OUT;
+                    if (off > 0 || stop > end) {  // a part of an item
+                        it.dst = TO_SLOT;
+                        it.slot = 2 * blockIdx.x + (s > first ? 1 : 0);
+                        // an item's second block reports it to the joining kernel
+                        const int c0 = pl.share.block(s);
+                        if (p.shared == 0 && off > 0 && c0 == (int)blockIdx.x - 1 && lane == 0) {
+                            p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, kvh, 2 * c0 + (s > pl.share.begin(c0) ? 1 : 0));
+                            p.split[2 * blockIdx.x + 1] = make_int4(pl.share.block(stop - 1), 0, 0, 0);
+                        }
+                    }
+                    pos = min(s + cost, end);
+                    off = 0;
+                    found = true;
+                }
+                if (++r * p.tpt >= nq) {
+                    r = 0;
+                    kvh++;
+                }
+                if (found) return true;
+            }
+            inside = false;
+            i++;
+        }
+    }
+};
 
 E2C_DEV float ex2_approx(float x) {
     float y;
@@ -816,7 +925,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
     const uint32_t tmem = *tmem_slot;
 
     Plan pl;
-    make_plan<D, KIND>(p, pl, *reinterpret_cast<PlanScratch<D, KIND> *>(smem + C::SCAN));
+    make_plan<C::WARPS, KIND>(p, pl, *reinterpret_cast<PlanScratch<C::WARPS> *>(smem + C::SCAN));
 
     // A consumer's copy of item n; false after the last one (or a failure). The slot is released at once.
     auto take = [&](int n, Item &it) -> bool {
@@ -839,7 +948,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
             const int L0 = pl.share.begin(blockIdx.x), L1 = pl.share.begin(blockIdx.x + 1);
             if (p.shared == 0 && lane == 0 && L0 < L1) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
             __syncwarp();
-            int pos = L0, n = 0;
+            int n = 0;
             bool ok = true;
             Item it = {};
             // Q of an item is loaded once the next one is published: the K and V loads then know of an item more
@@ -897,73 +1006,13 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                     }
                     continue;
                 }
-                // sequence entries, 32 at a time, one per lane
-                int off = pos - pl.first_before, ebase = -32;  // off: tiles before pos of the entry
-                Entry e = {};
-                int etiles = 0;
                 it.prefix = 0;
                 it.base = p.shared;
                 it.masked = 1;
+                Walk<KIND> walk;
+                walk.begin(pl, L0, L1);
 #pragma unroll 1
-                for (int i = pl.first; ok && pos < L1 && i < p.n; i++) {
-                    if (i >= ebase + 32) {
-                        ebase = i;
-                        e = {};
-                        etiles = 0;
-                        if (i + lane < p.n) {
-                            e = entry_of(p, i + lane, false);
-                            etiles = (int)tiles_of<KIND>(p, e.len, e.nq, p.shared);
-                        }
-                    }
-                    const int src = i - ebase, nq = __shfl_sync(0xffffffffu, e.nq, src), c = __shfl_sync(0xffffffffu, etiles, src);
-                    if (nq == 0) continue;
-                    const int len = __shfl_sync(0xffffffffu, e.len, src), q0 = __shfl_sync(0xffffffffu, e.q0, src);
-                    it.seq = __shfl_sync(0xffffffffu, e.seq, src);
-                    if (len == 0) it.seq = -1;  // its table says nothing
-                    it.len = len;
-                    if (KIND & SIGHT) it.base = len - nq;
-                    int kvh = 0;
-                    if (off >= c) {
-                        kvh = off / c;
-                        off -= kvh * c;
-                    }
-#pragma unroll 1
-                    for (int r = 0; ok && pos < L1 && kvh < p.pc.KV;) {
-                        const Span sp = span_of<KIND>(p, len, nq, r, p.shared);
-                        const int nt = sp.nt, cost = nt + ITEM_COST;
-                        if (off >= cost) {
-                            off -= cost;
-                        } else if (off >= nt) {  // the share begins past the item's tiles
-                            pos = min(pos + cost - off, L1);
-                            off = 0;
-                        } else {
-                            const int s = pos - off, end = s + nt;
-                            it.kvh = kvh;
-                            it.t0 = q0 + r * p.tpt;
-                            it.ntok = min(p.tpt, nq - r * p.tpt);
-                            sp.cut(p, off, min(end, L1) - pos, it);
-                            it.pos0 = len - nq + r * p.tpt;
-                            it.dst = p.shared > 0 ? TO_DENSE : TO_OUT;
-                            if (off > 0 || end > L1) {  // a part of an item
-                                it.dst = TO_SLOT;
-                                it.slot = 2 * blockIdx.x + (s > L0 ? 1 : 0);
-                                // an item's second block reports it to the joining kernel
-                                const int c0 = pl.share.block(s);
-                                if (p.shared == 0 && off > 0 && c0 == (int)blockIdx.x - 1 && lane == 0) {
-                                    p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, kvh, 2 * c0 + (s > pl.share.begin(c0) ? 1 : 0));
-                                    p.split[2 * blockIdx.x + 1] = make_int4(pl.share.block(end - 1), 0, 0, 0);
-                                }
-                            }
-                            publish();
-                            pos = min(s + cost, L1);
-                            off = 0;
-                        }
-                        if (++r * p.tpt >= nq) {
-                            r = 0;
-                            kvh++;
-                        }
-                    }
-                }
+                while (ok && walk.next(p, pl, it, lane)) publish();
             }
             // the last one, after which Q of the last item follows
             if (ok) {
@@ -1520,7 +1569,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                     out = static_cast<T *>(p.out) + t * p.ldo + h * D;
                     if (live && p.lse) p.lse[t * p.H + h] = sums * LN2;
                 } else {
-                    const int64_t at = it.dst == TO_SLOT ? (int64_t)it.slot * TR + row : t * p.H + h;
+                    const int64_t at = it.dst == TO_SLOT ? (int64_t)it.slot * SLOT<KIND> + row : t * p.H + h;
                     part = (it.dst == TO_SLOT ? p.po : p.dpo) + at * D;
                     if (live) (it.dst == TO_SLOT ? p.pl : p.dpl)[at] = sums;
                 }
@@ -1619,9 +1668,10 @@ __global__ void __launch_bounds__(JOIN) k_join_split(const Args p, int grid) {
     const int x = threadIdx.x % J::LANES, rows = a.y * p.G;
     for (int row = blockIdx.y * J::ROWS + threadIdx.x / J::LANES; row < rows; row += gridDim.y * J::ROWS) {
         J j;
-        j.add(p.po + ((int64_t)a.w * TR + row) * D, p.pl + (int64_t)a.w * TR + row, x);
+        constexpr int64_t R = SLOT<KIND>;
+        j.add(p.po + (a.w * R + row) * D, p.pl + a.w * R + row, x);
 #pragma unroll 4
-        for (int c = blockIdx.x; c <= c1; c++) j.add(p.po + ((int64_t)(2 * c) * TR + row) * D, p.pl + (int64_t)(2 * c) * TR + row, x);
+        for (int c = blockIdx.x; c <= c1; c++) j.add(p.po + (2 * c * R + row) * D, p.pl + 2 * c * R + row, x);
         const int tok = row / p.G;
         j.put(p, a.x + tok, a.z * p.G + (row - tok * p.G), x, [&]() {
             int last;
