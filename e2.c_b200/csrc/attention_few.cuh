@@ -9,12 +9,17 @@
 //   P' = 2^(S' - m) in 16 bits, transposed in registers (movmatrix) into the second product's operand
 //   O' += V' P'    head dim x 8 rows, fp32
 // One more warp walks the block's share of items (those of attention_pages.cuh, as are the joins) and loads their keys by TMA, 16 for
-// each warp at once, a lane for each page; at an item's end the warps' sums are added up in a fixed order. Head dimensions are
-// contracted, and put out, in the order in which 16-byte loads from shared memory hold them.
+// each warp at once, a lane for each page; at an item's end the warps' sums are added up pair by pair, in a fixed order. Head
+// dimensions are contracted in the order in which 16-byte loads from shared memory hold them.
+//
+// Where blocks suffice, the key heads of a share go to neighbouring blocks, which read the heads of a token at the same time: a
+// head's 64 to 128 bytes of a token alone make short bursts (64 x 8192 tokens of 8 bits above: 184 us with a block's share going
+// through one head after the other). Calls of few and short items (a window, or a short table) take a block an item: no
+// plan, and no join.
 //
 // Codes (8 bits) become fp16, exactly, in registers; scales are factors of a lane's own keys, applied as in attention_pages.cuh.
-// Q in bf16 is scaled by a power of two for each row, so that fp16 holds it: exact but for values below 2^-28 of the row's
-// largest.
+// Q in bf16 is scaled by a power of two, one for an item, so that fp16 holds it: exact but for values below 2^-28 of the item's
+// largest, which lose 2^-39 of that at most.
 #pragma once
 #include "attention_pages.cuh"
 
@@ -36,13 +41,10 @@ struct Runs {
 };
 
 // an item for the warps that use it
-template <int ROWS>
 struct __align__(16) FewItem {
     Item it;
     Runs runs;
-    int all_lo, all_hi;  // keys that every row sees
     int pad[2];
-    Seen seen[ROWS];
 };
 
 template <bool CODE, int D, int NT>
@@ -53,16 +55,19 @@ struct Few {
     static constexpr int WIDE = ROW < 128 ? ROW : 128, PANELS = ROW / WIDE, PANEL = KEYS * WIDE;
     static constexpr int UNIT = KEYS * ROW, STAGE = 2 * UNIT;       // K and V of a tile
     static constexpr int CTAS = NT == 1 && STAGE <= 32768 ? 2 : 1;
-    static constexpr int MOST = (CTAS == 2 ? 100 : 192) * 1024 / STAGE, NS = MOST > 5 ? 5 : MOST;
-    static constexpr int NQ = 4;             // items
-    static constexpr int MT = CTAS == 2 || NT == 2 ? 2 : 4;  // tiles of 16 head dimensions added up at once
+    static constexpr int MOST = (CTAS == 2 ? 98 : NT == 1 ? 192 : 184) * 1024 / STAGE, NS = MOST > 5 ? 5 : MOST;
+    static constexpr int NQ = 2;             // items
+    // Adding up: with `a` warps left the last b = min(SLOTS, a / 2) of them give their sums to the b before them. Warp w writes
+    // in slot GIVES[w] (four bits each): the one that it read itself in the step before, at first in order.
+    static constexpr int SLOTS = WARPS == 8 && CODE && NT == 1 && D >= 128 ? 3 : WARPS / 2, SLOT_BYTES = D * ROWS * 4;
+    static constexpr uint32_t GIVES = WARPS == 4 ? 0x1010u : SLOTS == 3 ? 0x21021220u : 0x32103230u;
     static constexpr int SCALES = NS * STAGE;                       // [NS][2][KEYS]
     static constexpr int MERGE = SCALES + (CODE ? NS * 2 * KEYS * 4 : 0);
-    static constexpr int ML = MERGE + WARPS * MT * 16 * ROWS * 4;   // [WARPS][ROWS] (m, l)
-    static constexpr int INV = ML + WARPS * ROWS * 8;               // [ROWS] (1 / l, what a row without sums gets)
-    static constexpr int QUEUE = INV + ROWS * 8;
-    static constexpr int BARS = QUEUE + NQ * (int)sizeof(FewItem<ROWS>);
-    static constexpr int NBARS = 2 * NS + 2 * NQ + 1;
+    static constexpr int ML = MERGE + SLOTS * SLOT_BYTES;           // [SLOTS][ROWS] (m, l)
+    static constexpr int SEEN = ML + SLOTS * ROWS * 8;              // [WARPS][ROWS]: lo, hi and se of Seen
+    static constexpr int QUEUE = SEEN + WARPS * ROWS * 16;
+    static constexpr int BARS = QUEUE + NQ * (int)sizeof(FewItem);
+    static constexpr int NBARS = 2 * NS + 2 * NQ + WARPS;
     static constexpr int SCAN = BARS + NBARS * 8;
     static constexpr int BYTES = SCAN + 256;
     static_assert(NS >= 2 && BYTES <= (CTAS == 2 ? 115712 : 232448) && sizeof(PlanScratch<WARPS + 1>) <= 256, "shared memory");
@@ -88,6 +93,11 @@ E2C_DEV void mma_16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+E2C_DEV float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // the transpose of an 8 x 8 matrix of 16-bit values, a row's pair in each lane
 E2C_DEV uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -106,7 +116,7 @@ E2C_DEV void plan_of_few(const Args &p, Plan &pl, Walk<KIND> &walk, int lane) {
     Entry e = {};
     if (lane < p.n) e = entry_of(p, lane, blockIdx.x == 0);
     const int etiles = (int)min((int64_t)1 << 30, tiles_of<KIND>(p, e.len, e.nq, 0));
-    const int64_t mine = (int64_t)etiles * p.pc.KV;
+    const int64_t mine = (int64_t)etiles * (p.pc.KV / p.hs);
     int64_t x = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -118,12 +128,12 @@ E2C_DEV void plan_of_few(const Args &p, Plan &pl, Walk<KIND> &walk, int lane) {
     if (!fits && lane == 0) record_status(p.status, E2C_ERR_TOO_LARGE);
     pl.tiles = fits ? (int)all : 0;
     pl.ptiles = 0;
-    pl.share.set(1, 0, pl.tiles, gridDim.x);
-    const int at = pl.share.begin(blockIdx.x);
+    pl.share.set(1, 0, pl.tiles, gridDim.x / p.hs);
+    const int at = pl.share.begin(blockIdx.x / p.hs);
     const uint32_t here = __ballot_sync(0xffffffffu, at >= x - mine && at < x);
     pl.first = here ? __ffs(here) - 1 : p.n;
     pl.first_before = (int)__shfl_sync(0xffffffffu, x - mine, pl.first & 31);
-    walk.begin(pl, at, pl.share.begin(blockIdx.x + 1));
+    walk.begin(pl, at, pl.share.begin(blockIdx.x / p.hs + 1));
     walk.base = 0;
     walk.e = e;
     walk.etiles = etiles;
@@ -146,7 +156,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
     if (smem_u32(smem) & 1023) {
         griddep_wait();
         if (threadIdx.x == 0) record_status(p.status, E2C_ERR_SMEM_ALIGN);
-        if (blockIdx.x == 0 && threadIdx.x < 2) p.before[p.n + threadIdx.x] = 0;  // the join has nothing to do
+        if (blockIdx.x == 0 && threadIdx.x < 2) p.before[p.n + threadIdx.x] = 0;  // a join has nothing to do
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -155,11 +165,13 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
     auto empty = [&](int st) { return bars + 8u * (C::NS + st); };
     auto item_full = [&](int i) { return bars + 8u * (2 * C::NS + i); };
     auto item_empty = [&](int i) { return bars + 8u * (2 * C::NS + C::NQ + i); };
-    const uint32_t merged = bars + 8u * (2 * C::NS + 2 * C::NQ);
-    FewItem<C::ROWS> *queue = reinterpret_cast<FewItem<C::ROWS> *>(smem + C::QUEUE);
+    // sums that warp w has handed on, w > 0; those of the item before have all been taken
+    auto given = [&](int w) { return bars + 8u * (2 * C::NS + 2 * C::NQ + w); };
+    const uint32_t taken = bars + 8u * (2 * C::NS + 2 * C::NQ);
+    FewItem *queue = reinterpret_cast<FewItem *>(smem + C::QUEUE);
     if (threadIdx.x < C::NBARS) {
         const int b = threadIdx.x;
-        mbar_init(bars + 8u * b, b < C::NS || (b >= 2 * C::NS && b < 2 * C::NS + C::NQ) ? 1 : W);
+        mbar_init(bars + 8u * b, (b >= C::NS && b < 2 * C::NS) || (b >= 2 * C::NS + C::NQ && b < 2 * C::NS + 2 * C::NQ) ? W : 1);
         fence_mbar_init();
     }
     if (warp == W && lane == 0) {
@@ -169,16 +181,20 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
     __syncthreads();
     griddep_wait();
     Plan pl;
-    if (p.n > 32) make_plan<W + 1, KIND>(p, pl, *reinterpret_cast<PlanScratch<W + 1> *>(smem + C::SCAN));
+    const bool whole = p.whole, wide = !whole && p.n > 32;
+    if (wide) make_plan<W + 1, KIND>(p, pl, *reinterpret_cast<PlanScratch<W + 1> *>(smem + C::SCAN));
 
     if (warp == W) {
         // ------------------------------------------------------------ items, and loads of their slices
         Walk<KIND> walk;
-        if (p.n > 32)
-            walk.begin(pl, pl.share.begin(blockIdx.x), pl.share.begin(blockIdx.x + 1));
-        else
+        Entry e = {};
+        if (wide)
+            walk.begin(pl, pl.share.begin(blockIdx.x / p.hs), pl.share.begin(blockIdx.x / p.hs + 1));
+        else if (!whole)
             plan_of_few<KIND>(p, pl, walk, lane);
-        if (lane == 0 && walk.pos < walk.end) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+        else
+            e = entry_of(p, blockIdx.x / p.pc.KV, blockIdx.x % p.pc.KV == 0 && lane == 0);
+        if (!whole && lane == 0 && walk.pos < walk.end) p.split[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
         __syncwarp();
         const int PB = min(p.pc.page, C::KEYS), shift = 31 - __clz(p.pc.page);
         Item it = {};
@@ -187,8 +203,22 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
         bool ok = true;
 #pragma unroll 1
         for (;; n++) {
-            const bool more = walk.next(p, pl, it, lane);
-            FewItem<C::ROWS> &to = queue[n % C::NQ];
+            bool more;
+            if (whole) {
+                more = n == 0 && e.nq > 0;
+                it.seq = e.len > 0 ? e.seq : -1;
+                it.len = e.len;
+                it.base = it.pos0 = e.len - e.nq;
+                it.kvh = blockIdx.x % p.pc.KV;
+                it.t0 = e.q0;
+                it.ntok = e.nq;
+                const Span sp = span_of<KIND>(p, e.len, e.nq, 0, 0);
+                sp.cut(p, 0, sp.nt, it);
+                it.dst = TO_OUT;
+            } else {
+                more = walk.next(p, pl, it, lane);
+            }
+            FewItem &to = queue[n % C::NQ];
             if (!(ok = wait_warp(item_empty(n % C::NQ), (uint32_t)((n / C::NQ & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER))) break;
             if (!more) {
                 if (lane == 0) {
@@ -206,22 +236,9 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                            ? p.pc.table[(int64_t)it.seq * p.pc.max_blocks + (key >> shift)] : 0;
             };
             int page = page_of(0);
-            int lo = 0, hi = it.klim;
-            if (lane < it.ntok * p.G) {
-                const int tok = lane / p.G;
-                Seen x;
-                x.set(p, it.t0 + tok, it.pos0 + tok, it.len, it.base);
-                to.seen[lane] = x;
-                lo = x.lo;
-                hi = x.hi;
-            }
-            lo = __reduce_max_sync(0xffffffffu, lo);
-            hi = __reduce_min_sync(0xffffffffu, hi);
             if (lane == 0) {
                 to.it = it;
                 to.runs = runs;
-                to.all_lo = lo;
-                to.all_hi = hi;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(item_full(n % C::NQ));
@@ -265,69 +282,76 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
 
     // ---------------------------------------------------------------- products
     const int quad = lane & 3, oct = lane >> 2;
-    float2 *ml = reinterpret_cast<float2 *>(smem + C::ML), *fin = reinterpret_cast<float2 *>(smem + C::INV);
-    float *merge = reinterpret_cast<float *>(smem + C::MERGE);
+    float2 *ml = reinterpret_cast<float2 *>(smem + C::ML);
     uint32_t qf[D / 16][NT][2];
     float o[D / 16][NT][4];
-    float m[NT][2], l[NT][2], cr[NT][2];
-    uint32_t turn = 0;
-    auto together = [&]() -> bool {  // the block's other warps have come here too
-        __syncwarp();
-        if (lane == 0) mbar_arrive(merged);
-        const bool ok = wait_warp(merged, turn, p.status, E2C_ERR_WAIT_ATTN);
-        turn ^= 1;
-        return ok;
-    };
-
+    float m[NT][2], l[NT][2], less[NT][2];  // less: -m, or 0 for a row that has only seen -infinity
+    int4 *seen = reinterpret_cast<int4 *>(smem + C::SEEN) + warp * C::ROWS;
+    int all_lo = 0, all_hi = 0;             // keys that every row sees
+    float cu;                               // what a product times its key's scale is multiplied by
     auto begin = [&](const Item &it) {
         const int rows = it.ntok * p.G;
         // Q: a lane's 16 (8 bits) or 8 neighbouring dimensions of each 64 or 32, of row `oct`
-        float up[NT];
+        constexpr int PER = CODE ? 16 : 8;
+        uint4 w[NT][D / 32];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const int row = nt * 8 + oct, tok = row / p.G, hd = row - tok * p.G;
             const T *q = static_cast<const T *>(q_rows) + (int64_t)(it.t0 + tok) * ldq + (it.kvh * p.G + hd) * D;
-            constexpr int PER = CODE ? 16 : 8;
-            uint4 w[D / 32];
 #pragma unroll
             for (int j = 0; j < D / (4 * PER); j++)
 #pragma unroll
                 for (int k = 0; k < PER / 8; k++)
-                    w[j * (PER / 8) + k] = row < rows ? *reinterpret_cast<const uint4 *>(q + j * 4 * PER + quad * PER + k * 8) : make_uint4(0, 0, 0, 0);
-            up[nt] = 1.f;
-            if constexpr (CODE && !std::is_same<T, __half>::value) {
-                const __nv_bfloat162 *x = reinterpret_cast<const __nv_bfloat162 *>(w);
-                uint32_t top = 0;  // the largest finite magnitude
+                    w[nt][j * (PER / 8) + k] = row < rows ? *reinterpret_cast<const uint4 *>(q + j * 4 * PER + quad * PER + k * 8) : make_uint4(0, 0, 0, 0);
+        }
+        float up = 1.f;
+        if constexpr (CODE && !std::is_same<T, __half>::value) {
+            uint32_t top = 0;  // the largest finite magnitude
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int k = 0; k < D / 8; k++) {
-                    const uint32_t b = reinterpret_cast<const uint32_t *>(w)[k], b0 = b << 16 & 0x7fffffffu, b1 = b & 0x7fff0000u;
+                    const uint32_t b = reinterpret_cast<const uint32_t *>(w[nt])[k], b0 = b << 16 & 0x7fffffffu, b1 = b & 0x7fff0000u;
                     top = max(top, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
                 }
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const uint32_t ex = max(top >> 23, 15u);  // its exponent becomes 14
-                const float scale = __uint_as_float((268u - ex) << 23);
-                up[nt] = __uint_as_float((ex - 14u) << 23);
+            top = __reduce_max_sync(0xffffffffu, top);
+            const uint32_t ex = max(top >> 23, 15u);  // its exponent becomes 14
+            const float scale = __uint_as_float((268u - ex) << 23);
+            up = __uint_as_float((ex - 14u) << 23);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int k = 0; k < D / 8; k++) {
-                    const float2 f = __bfloat1622float2(x[k]);
-                    reinterpret_cast<uint32_t *>(w)[k] = pack2<__half>(f.x * scale, f.y * scale);
+                    const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 *>(w[nt])[k]);
+                    reinterpret_cast<uint32_t *>(w[nt])[k] = pack2<__half>(f.x * scale, f.y * scale);
                 }
-            }
-            const uint32_t *b = reinterpret_cast<const uint32_t *>(w);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
-                qf[k][nt][0] = b[2 * k];
-                qf[k][nt][1] = b[2 * k + 1];
+                qf[k][nt][0] = reinterpret_cast<const uint32_t *>(w[nt])[2 * k];
+                qf[k][nt][1] = reinterpret_cast<const uint32_t *>(w[nt])[2 * k + 1];
             }
+        cu = (p.neg ? -p.c : p.c) * up;
+        int lo = 0, hi = it.klim;
+        if (lane < rows) {
+            const int tok = lane / p.G;
+            Seen x;
+            x.set(p, it.t0 + tok, it.pos0 + tok, it.len, it.base);
+            seen[lane] = make_int4(x.lo, x.hi, x.se, 0);
+            lo = x.lo;
+            hi = x.hi;
         }
-        const float c = p.neg ? -p.c : p.c;
+        all_lo = __reduce_max_sync(0xffffffffu, lo);
+        all_hi = __reduce_min_sync(0xffffffffu, hi);
+        __syncwarp();
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                cr[nt][i] = c * __shfl_sync(0xffffffffu, up[nt], (2 * quad + i) * 4);
                 m[nt][i] = -INFINITY;
+                less[nt][i] = 0.f;
                 l[nt][i] = 0.f;
             }
 #pragma unroll
@@ -339,7 +363,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
     };
 
     // keys [kk, kk + 16) before `end`, of which stage st holds K and V from its row r0 on
-    auto use = [&](const FewItem<C::ROWS> &fi, int st, int r0, int kk, int end) {
+    auto use = [&](const Item &it, int st, int r0, int kk, int end) {
         const uint8_t *k = smem + st * C::STAGE + r0 * C::WIDE, *v = k + C::UNIT;
         float s[NT][4] = {}, s2[NT][4] = {};  // two sums, so that products need not wait for one another
         if constexpr (CODE) {
@@ -367,39 +391,48 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
             }
         }
         // s[nt][2 h + i]: key oct + 8 h, row 8 nt + 2 quad + i
-        float lv[2] = {0.f, 0.f}, vs[2] = {1.f, 1.f}, ks[2] = {1.f, 1.f};
+        float lv[2] = {0.f, 0.f}, vs[2] = {1.f, 1.f}, kc[2] = {cu, cu};
         if constexpr (CODE) {
-            const float *sc = reinterpret_cast<const float *>(smem + C::SCALES) + st * (2 * C::KEYS) + r0;
+            const float *sc = reinterpret_cast<const float *>(smem + C::SCALES) + st * (2 * C::KEYS) + r0 + oct;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                ks[h] = sc[oct + 8 * h];
-                const float x = sc[C::KEYS + oct + 8 * h];
+                kc[h] = sc[8 * h] * cu;
+                const float x = sc[C::KEYS + 8 * h];
                 const bool fine = fabsf(x) < INFINITY;
-                lv[h] = fine ? fminf(fmaxf(__log2f(fabsf(x)), -100.f), 100.f) : 0.f;
+                lv[h] = fine ? fminf(fmaxf(lg2_approx(fabsf(x)), -100.f), 100.f) : 0.f;
                 vs[h] = fine ? x : NAN;
             }
         }
+        // the logits, and, as y, with the log2 of their weights' scale
+        float y[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[nt][e] = (s[nt][e] + s2[nt][e]) * (CODE ? ks[e >> 1] * cr[nt][e & 1] : cr[nt][e & 1]);
-        if (kk < fi.all_lo || kk + 16 > min(end, fi.all_hi)) {  // some row does not see some of them
+            for (int e = 0; e < 4; e++) {
+                s[nt][e] = (s[nt][e] + s2[nt][e]) * kc[e >> 1];
+                y[nt][e] = CODE ? s[nt][e] + lv[e >> 1] : s[nt][e];
+            }
+        if (kk < all_lo || kk + 16 > min(end, all_hi)) {  // some row does not see some of them
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     const int row = 8 * nt + 2 * quad + i;
                     uint32_t bits = Seen::below(end - kk);
-                    if (row < fi.it.ntok * p.G) bits &= fi.seen[row].keys(p, kk);
+                    if (row < it.ntok * p.G) {
+                        const int4 x = seen[row];
+                        const Seen sight = {x.x, x.y, x.z, it.base, it.len, p.tree ? p.tree + (int64_t)(it.t0 + row / p.G) * p.words : nullptr};
+                        bits &= sight.keys(p, kk);
+                    }
 #pragma unroll
                     for (int h = 0; h < 2; h++)
-                        if (!(bits >> (oct + 8 * h) & 1)) s[nt][2 * h + i] = -INFINITY;
+                        if (!(bits >> (oct + 8 * h) & 1)) s[nt][2 * h + i] = y[nt][2 * h + i] = -INFINITY;
                 }
             if (end - kk < 16) {  // past the last key a stage holds anything
                 if constexpr (CODE) {
 #pragma unroll
                     for (int h = 0; h < 2; h++)
-                        if (oct + 8 * h >= end - kk) lv[h] = vs[h] = 0.f;
+                        if (oct + 8 * h >= end - kk) vs[h] = 0.f;
                 } else {
                     uint8_t *y = const_cast<uint8_t *>(v);
                     for (int e = lane; e < (16 - (end - kk)) * (C::ROW / 16); e += 32) {
@@ -411,42 +444,39 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                 }
             }
         }
-        bool moved = false;
-        float alpha[NT][2];
+        // m is the rows' own in all lanes, and moves when some lane's logit is more than 2^8 above it (so also from
+        // -infinity, and for a NaN)
+        bool over = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                float x = max2(s[nt][i] + lv[0], s[nt][2 + i] + lv[1]);
-                x = max2(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                x = max2(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                x = max2(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                alpha[nt][i] = 1.f;
-                if (!(x <= m[nt][i] + kRescaleLog2)) {  // so also from -infinity, and for a NaN
-                    const float now = max2(m[nt][i], x);
-                    alpha[nt][i] = ex2_approx(m[nt][i] - now);
+            for (int i = 0; i < 2; i++) over |= !(max2(y[nt][i], y[nt][2 + i]) <= m[nt][i] + kRescaleLog2);
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    float x = max2(y[nt][i], y[nt][2 + i]);
+                    x = max2(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = max2(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = max2(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    if (x <= m[nt][i] + kRescaleLog2) continue;
+                    const float now = max2(m[nt][i], x), alpha = ex2_approx(m[nt][i] - now);
                     m[nt][i] = now;
-                    l[nt][i] *= alpha[nt][i];
-                    moved = true;
+                    less[nt][i] = now == -INFINITY ? 0.f : -now;
+                    l[nt][i] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < D / 16; d++) o[d][nt][i] *= alpha, o[d][nt][2 + i] *= alpha;
                 }
-            }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[i][nt][e] *= alpha[nt][e & 1];
         }
         uint32_t pb[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float ref = m[nt][i] == -INFINITY ? 0.f : m[nt][i];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float x = ex2_approx(s[nt][2 * h + i] - ref);
+                    const float x = ex2_approx(s[nt][2 * h + i] + less[nt][i]);
                     l[nt][i] += x;
                     s[nt][2 * h + i] = CODE ? x * vs[h] : x;
                 }
@@ -493,7 +523,8 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
         }
     };
 
-    auto finish = [&](const Item &it) -> bool {  // the item's sums from all warps, in their order
+    // the n-th item's sums from all warps; false if a wait ran out
+    auto finish = [&](const Item &it, int n) -> bool {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -502,110 +533,158 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                 x += __shfl_xor_sync(0xffffffffu, x, 4);
                 x += __shfl_xor_sync(0xffffffffu, x, 8);
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
-                if (oct == 0) ml[warp * C::ROWS + 8 * nt + 2 * quad + i] = make_float2(m[nt][i], x);
+                l[nt][i] = x;
             }
-        if (!together()) return false;
-        float f[NT][2];
+        // (a loop, not its steps one after the other: this code runs once an item, and for short ones fetching it is
+        // what it takes)
+        auto slot = [&](int w) { return reinterpret_cast<float4 *>(smem + C::MERGE + (C::GIVES >> 4 * w & 15) * C::SLOT_BYTES) + lane; };
+        auto slot_rows = [&](int w) { return ml + (C::GIVES >> 4 * w & 15) * C::ROWS + 2 * quad; };
+#pragma unroll 1
+        for (int a = W, b; a > 1; a -= b) {
+            b = min(C::SLOTS, a >> 1);
+            if (warp >= a - b) break;
+            if (warp < a - 2 * b) continue;
+            const int w = warp + b;
+            if (!wait_warp(given(w), (uint32_t)(n & 1), p.status, E2C_ERR_WAIT_ATTN)) return false;
+            const float4 *sums = slot(w);
+            const float2 *rows = slot_rows(w);
+            float f[NT][2], g[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const float2 x = rows[8 * nt + i];
+                    const float top = max2(m[nt][i], x.x), ref = top == -INFINITY ? 0.f : top;
+                    f[nt][i] = ex2_approx(m[nt][i] - ref);
+                    g[nt][i] = ex2_approx(x.x - ref);
+                    m[nt][i] = top;
+                    l[nt][i] = l[nt][i] * f[nt][i] + x.y * g[nt][i];
+                }
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float4 x = sums[(i * NT + nt) * 32];
+                    o[i][nt][0] = o[i][nt][0] * f[nt][0] + x.x * g[nt][0];
+                    o[i][nt][1] = o[i][nt][1] * f[nt][1] + x.y * g[nt][1];
+                    o[i][nt][2] = o[i][nt][2] * f[nt][0] + x.z * g[nt][0];
+                    o[i][nt][3] = o[i][nt][3] * f[nt][1] + x.w * g[nt][1];
+                }
+            __syncwarp();
+        }
+        if (warp > 0) {
+            // slots are free once the first warp has the sums of the item before
+            if (warp >= W - C::SLOTS && !wait_warp(taken, (uint32_t)(n & 1) ^ 1, p.status, E2C_ERR_WAIT_ATTN)) return false;
+            float4 *sums = slot(warp);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) sums[(i * NT + nt) * 32] = make_float4(o[i][nt][0], o[i][nt][1], o[i][nt][2], o[i][nt][3]);
+            if (oct == 0)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) slot_rows(warp)[8 * nt + i] = make_float2(m[nt][i], l[nt][i]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(given(warp));
+            return true;
+        }
+        if (lane == 0) mbar_arrive(taken);
+        const int rows = it.ntok * p.G;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                float top = -INFINITY;
-#pragma unroll
-                for (int k = 0; k < W; k++) top = max2(top, ml[k * C::ROWS + 8 * nt + 2 * quad + i].x);
-                f[nt][i] = ex2_approx(m[nt][i] - (top == -INFINITY ? 0.f : top));
-            }
-        const int rows = it.ntok * p.G;
-        if (threadIdx.x < rows) {
-            const int row = threadIdx.x, tok = row / p.G, hd = row - tok * p.G;
-            float top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int k = 0; k < W; k++) top = max2(top, ml[k * C::ROWS + row].x);
-            const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-            for (int k = 0; k < W; k++) {
-                const float2 x = ml[k * C::ROWS + row];
-                sum += x.y * ex2_approx(x.x - ref);
-            }
-            // sum = 0: every logit was -infinity, or no key was seen; a part leaves that to the join
-            const bool bad = no_softmax(top), some = bad || sum > 0.f;
-            const float sums = bad ? top : some ? top + __log2f(sum) : -INFINITY;
-            const int64_t t = it.t0 + tok, h = it.kvh * p.G + hd;
-            float none = 0.f;
-            if (it.dst == TO_OUT) {
-                if (!some && sees_keys<KIND>(p, t, it.pos0 + tok, it.len, it.base)) none = NAN;
-                if (p.lse) p.lse[t * p.H + h] = sums * LN2;
-            } else {
-                p.pl[(int64_t)it.slot * SLOT<KIND> + row] = sums;
-            }
-            fin[row] = make_float2(bad ? NAN : some ? __fdividef(1.f, sum) : 0.f, some ? 0.f : none);
-        }
-#pragma unroll
-        for (int i0 = 0; i0 < D / 16; i0 += C::MT) {
-#pragma unroll
-            for (int i = 0; i < C::MT; i++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        float *y = merge + ((warp * C::MT + i) * C::ROWS + 8 * nt + 2 * quad + k) * 16;
-                        const float a = o[i0 + i][nt][k] * f[nt][k], b = o[i0 + i][nt][2 + k] * f[nt][k];
-                        if constexpr (CODE)
-                            *reinterpret_cast<float2 *>(y + 2 * oct) = make_float2(a, b);
-                        else
-                            y[oct] = a, y[oct + 8] = b;
-                    }
-            if (!together()) return false;
-            for (int e = threadIdx.x; e < C::MT * 8 * C::ROWS; e += 32 * W) {
-                const int pair = e & 7, row = (e >> 3) % C::ROWS, i = (e >> 3) / C::ROWS;
-                float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-                for (int k = 0; k < W; k++) sum = add2(sum, *reinterpret_cast<const float2 *>(merge + ((k * C::MT + i) * C::ROWS + row) * 16 + 2 * pair));
+                const int row = 8 * nt + 2 * quad + i, tok = row / p.G, hd = row - tok * p.G;
+                const int64_t t = it.t0 + tok, h = it.kvh * p.G + hd;
                 if (row >= rows) continue;
-                const int dim = CODE ? pair * (D / 8) + 2 * (i0 + i) : 16 * (i0 + i) + 2 * pair;
-                const float2 u = fin[row];
-                // a row without sums may have met a page's NaN: its zeros are not a product
-                const float2 y = u.x == 0.f ? make_float2(u.y, u.y) : make_float2(sum.x * u.x, sum.y * u.x);
-                if (it.dst == TO_OUT) {
-                    const int tok = row / p.G, hd = row - tok * p.G;
-                    *reinterpret_cast<uint32_t *>(static_cast<T *>(p.out) + (it.t0 + tok) * p.ldo + (it.kvh * p.G + hd) * D + dim) = pack2<T>(y.x, y.y);
+                // l = 0: every logit was -infinity, or no key was seen; a part leaves that to the join
+                const bool bad = no_softmax(m[nt][i]), some = bad || l[nt][i] > 0.f, part = it.dst != TO_OUT;
+                const float sums = bad ? m[nt][i] : some ? m[nt][i] + __log2f(l[nt][i]) : -INFINITY;
+                const float inv = bad ? NAN : __fdividef(1.f, l[nt][i]);
+                if (oct == 0) {
+                    if (part)
+                        p.pl[(int64_t)it.slot * SLOT<KIND> + row] = sums;
+                    else if (p.lse)
+                        p.lse[t * p.H + h] = sums * LN2;
+                }
+                float none = 0.f;
+                if (!some && !part && sees_keys<KIND>(p, t, it.pos0 + tok, it.len, it.base)) none = NAN;
+                float y[D / 8];
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {  // (a row without sums may have met a page's NaN)
+                    y[2 * k] = some ? o[k][nt][i] * inv : none;
+                    y[2 * k + 1] = some ? o[k][nt][2 + i] * inv : none;
+                }
+                // codes: a lane's neighbouring dimensions; otherwise every eighth
+                const int64_t at = CODE ? oct * (D / 8) : oct;
+                if (part) {
+                    float *to = p.po + ((int64_t)it.slot * SLOT<KIND> + row) * D + at;
+#pragma unroll
+                    for (int k = 0; k < D / 8; k += CODE ? 4 : 1) {
+                        if constexpr (CODE)
+                            *reinterpret_cast<float4 *>(to + k) = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+                        else
+                            to[8 * k] = y[k];
+                    }
                 } else {
-                    *reinterpret_cast<float2 *>(p.po + ((int64_t)it.slot * SLOT<KIND> + row) * D + dim) = y;
+                    T *to = static_cast<T *>(p.out) + t * p.ldo + h * D + at;
+#pragma unroll
+                    for (int k = 0; k < D / 8; k += CODE ? 8 : 1) {
+                        if constexpr (CODE)
+                            *reinterpret_cast<uint4 *>(to + k) = make_uint4(pack2<T>(y[k], y[k + 1]), pack2<T>(y[k + 2], y[k + 3]), pack2<T>(y[k + 4], y[k + 5]), pack2<T>(y[k + 6], y[k + 7]));
+                        else
+                            reinterpret_cast<uint16_t *>(to)[8 * k] = (uint16_t)pack2<T>(y[k], 0.f);
+                    }
                 }
             }
-            if (!together()) return false;
-        }
         return true;
     };
 
+    int st = 0, slice = warp;  // stage, and the warp's keys in it: tiles that are not full fall to other warps each time
+    uint32_t parity = 0;
 #pragma unroll 1
-    for (int n = 0, g = 0;; n++) {
+    for (int n = 0;; n++) {
         if (!wait_warp(item_full(n % C::NQ), (uint32_t)(n / C::NQ & 1), p.status, E2C_ERR_WAIT_ATTN)) return;
-        const FewItem<C::ROWS> &fi = queue[n % C::NQ];
+        const FewItem &fi = queue[n % C::NQ];
         if (fi.it.ntok < 0) return;
         begin(fi.it);
-        const int count = fi.runs.count;
+        const Runs runs = fi.runs;
+        int key = runs.key(0, C::KEYS), end = runs.end(0);
 #pragma unroll 1
-        for (int j = 0; j < count; j++, g++) {
-            const int st = g % C::NS, key = fi.runs.key(j, C::KEYS), end = fi.runs.end(j);
-            const int r0 = ((warp + g) % W) * 16;  // tiles that are not full fall to other warps each time
+        for (int j = 1; j <= runs.count; j++) {
             // (also without keys of its own: a warp that ran ahead would count twice in the stage's barrier)
-            if (!wait_warp(full(st), (uint32_t)(g / C::NS & 1), p.status, E2C_ERR_WAIT_ATTN)) return;
-            if (key + r0 < end) use(fi, st, r0, key + r0, end);
+            if (!wait_warp(full(st), parity, p.status, E2C_ERR_WAIT_ATTN)) return;
+            const int kk = key + 16 * slice;
+            if (kk < end) use(fi.it, st, 16 * slice, kk, end);
             __syncwarp();
             if (lane == 0) mbar_arrive(empty(st));
+            if (++st == C::NS) {
+                st = 0;
+                parity ^= 1;
+            }
+            slice = (slice + 1) % W;
+            key += C::KEYS;
+            if (j == runs.first) {
+                key = runs.k2;
+                end = runs.end2;
+            }
         }
-        if (!finish(fi.it)) return;
+        if (!finish(fi.it, n)) return;
+        __syncwarp();
         if (lane == 0) mbar_arrive(item_empty(n % C::NQ));
     }
 }
 
+// Items of which a block can take one each, and the keys of which are few enough that reading them takes no longer than a join of
+// their parts would
+constexpr int WHOLE_BYTES = 512 << 10;
 template <typename T, bool CODE, int D, int NT>
-int run_few(const Args &a, const void *q, int64_t ldq, int sms, cudaStream_t st) {
+int run_few(Args a, const void *q, int64_t ldq, int sms, cudaStream_t st) {
     using C = Few<CODE, D, NT>;
     constexpr int KIND = SIGHT | FEW | (CODE ? CODES : 0);
     static E2cPerDev attr;
-    const int dev = e2c_device(), grid = sms * C::CTAS;
+    const int dev = e2c_device(), KV = a.pc.KV;
     if (!attr.get(dev)) {
         if (cudaFuncSetAttribute(k_attention_few<T, CODE, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::BYTES) != cudaSuccess) {
             cudaGetLastError();
@@ -614,18 +693,27 @@ int run_few(const Args &a, const void *q, int64_t ldq, int sms, cudaStream_t st)
         }
         attr.set(dev, 1);
     }
-    const CUtensorMapDataType dt = CODE ? CU_TENSOR_MAP_DATA_TYPE_UINT8
-                                   : __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const int es = CODE ? 1 : 2;
-    const uint64_t rows = (uint64_t)a.pc.n_pages * a.pc.page, width = (uint64_t)a.pc.KV * D;
+    // the most keys that an item can have: the table's, or those of a window on both sides of its rows and the sinks
+    int64_t keys = (int64_t)a.pc.max_blocks * a.pc.page;
+    if (a.window >= 0) {
+        const int64_t seen = 2 * (int64_t)a.window + 1 + a.max_q + a.sinks + 2 * a.align;
+        keys = keys < seen ? keys : seen;
+    }
+    int grid = sms * C::CTAS;
+    a.whole = (int64_t)a.n * KV <= grid && keys * 2 * C::ROW <= WHOLE_BYTES;
+    // a head for each of KV neighbouring blocks, if that leaves no more than one in twenty without work
+    a.hs = !a.whole && grid / KV * KV * 20 >= grid * 19 ? KV : 1;
+    grid = a.whole ? a.n * KV : grid / a.hs * a.hs;
+    const CUtensorMapDataType dt = __is_same(T, __nv_bfloat16) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const uint64_t rows = (uint64_t)a.pc.n_pages * a.pc.page, width = (uint64_t)KV * D;
     const uint32_t box = a.pc.page < C::KEYS ? a.pc.page : C::KEYS;
-    const auto map = C::WIDE == 64 ? e2c_tmap_2d_sw64 : e2c_tmap_2d;
     CUtensorMap tk, tv;
-    if (map(&tk, a.pc.k, dt, es, width, rows, width * es, C::WIDE / es, box) ||
-        map(&tv, a.pc.v, dt, es, width, rows, width * es, C::WIDE / es, box))
+    if (CODE ? e2c_tmap_bytes(&tk, a.pc.k, width, rows, C::WIDE, box, 1) || e2c_tmap_bytes(&tv, a.pc.v, width, rows, C::WIDE, box, 1)
+             : e2c_tmap_2d(&tk, a.pc.k, dt, 2, width, rows, width * 2, 64, box) || e2c_tmap_2d(&tv, a.pc.v, dt, 2, width, rows, width * 2, 64, box))
         return -3;
     e2c_launch_as(true, k_attention_few<T, CODE, D, NT>, dim3(grid), dim3(32 * (C::WARPS + 1)), C::BYTES, st, tk, tv, a, q, ldq);
     if (launch_error("pages_attention")) return -2;
+    if (a.whole) return 0;
     using J = Join<T, D>;
     e2c_launch_as(true, k_join_split<T, D, KIND>, dim3(grid, (unsigned)((a.G * a.max_q + J::ROWS - 1) / J::ROWS)), dim3(JOIN), 0, st, a, grid);
     return launch_error("pages_attention join");

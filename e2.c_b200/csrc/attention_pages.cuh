@@ -58,7 +58,9 @@ struct e2c_attn_args {
     int n, T, max_q, H, G, tpt;  // tpt: tokens of an item
     int shared, causal, window;
     int sinks, words;            // SIGHT: first tokens that a window leaves visible (0 without a window);
-    int align;                   // FEW: what a window's first key is rounded down to
+    int align;                   // FEW: what a window's first key is rounded down to,
+    int hs;                      // blocks side by side that take a share's items of one key head each (1: all of them),
+    int whole;                   // an item a block, undivided
     const uint32_t *tree;        // rows' bits among their entry's drafted tokens [T][words], or null
     float c;                     // |scale| log2 e
     uint32_t neg;                // scale < 0: the products negate Q
@@ -285,6 +287,11 @@ template <int KIND>
 E2C_DEV int aligned(const Args &p, int x) {
     return KIND & FEW ? x & -p.align : x / TK * TK;
 }
+// The block's share and key head among `hs` blocks that have the same share of the entries' tiles, and those blocks' number
+template <int KIND>
+E2C_DEV int hs_of(const Args &p) {
+    return KIND & FEW ? p.hs : 1;
+}
 template <int KIND>
 constexpr int SLOT = KIND & FEW ? FEW_ROWS : TR;  // rows of a part in the workspace
 struct Span {
@@ -478,7 +485,7 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<WARPS> &s) {
             int64_t mine = 0;
             if (i < p.n) {
                 e = entry_of(p, i, round == 0 && blockIdx.x == 0);
-                mine = tiles_of<KIND>(p, e.len, e.nq, p.shared) * p.pc.KV;
+                mine = tiles_of<KIND>(p, e.len, e.nq, p.shared) * (p.pc.KV / hs_of<KIND>(p));
             }
             int64_t x = mine;
 #pragma unroll
@@ -528,8 +535,8 @@ E2C_DEV void make_plan(const Args &p, Plan &pl, PlanScratch<WARPS> &s) {
                 if (!fits && tid == 0) record_status(p.status, E2C_ERR_TOO_LARGE);
                 pl.tiles = fits ? (int)run : 0;
                 if (!fits) pl.ptiles = 0;
-                pl.share.set(p.pc.KV * pl.npt, pl.ptiles, pl.tiles, gridDim.x);
-                at = pl.share.begin(blockIdx.x);
+                pl.share.set(p.pc.KV * pl.npt, pl.ptiles, pl.tiles, gridDim.x / hs_of<KIND>(p));
+                at = pl.share.begin(blockIdx.x / hs_of<KIND>(p));
             }
             if (last && i < p.n) {
                 if (at >= before && at < before + mine) {
@@ -572,6 +579,7 @@ struct Walk {
     }
     // the next part, in the fields of `it` that do not hold for all of them; false after the last
     E2C_DEV bool next(const Args &p, const Plan &pl, Item &it, int lane) {
+        const int hs = hs_of<KIND>(p), share = blockIdx.x / hs, head = blockIdx.x - share * hs, heads = p.pc.KV / hs;
         for (;;) {
             if (!inside) {
                 if (pos >= end || i >= p.n) return false;
@@ -602,7 +610,7 @@ struct Walk {
                 inside = true;
             }
 #pragma unroll 1
-            while (pos < end && kvh < p.pc.KV) {
+            while (pos < end && kvh < heads) {
                 const Span sp = span_of<KIND>(p, len, nq, r, p.shared);
                 const int nt = sp.nt, cost = nt + ITEM_COST;
                 bool found = false;
@@ -612,11 +620,11 @@ struct Walk {
                     pos = min(pos + cost - off, end);
                     off = 0;
                 } else {
-                    const int s = pos - off, stop = s + nt, first = pl.share.begin(blockIdx.x);
+                    const int s = pos - off, stop = s + nt, first = pl.share.begin(share);
                     it.seq = seq;
                     it.len = len;
                     if (KIND & SIGHT) it.base = len - nq;
-                    it.kvh = kvh;
+                    it.kvh = kvh + head;
                     it.t0 = q0 + r * p.tpt;
                     it.ntok = min(p.tpt, nq - r * p.tpt);
                     sp.cut(p, off, min(stop, end) - pos, it);
@@ -627,8 +635,8 @@ struct Walk {
                         it.slot = 2 * blockIdx.x + (s > first ? 1 : 0);
                         // an item's second block reports it to the joining kernel
                         const int c0 = pl.share.block(s);
-                        if (p.shared == 0 && off > 0 && c0 == (int)blockIdx.x - 1 && lane == 0) {
-                            p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, kvh, 2 * c0 + (s > pl.share.begin(c0) ? 1 : 0));
+                        if (p.shared == 0 && off > 0 && c0 == share - 1 && lane == 0) {
+                            p.split[2 * blockIdx.x] = make_int4(it.t0, it.ntok, it.kvh, 2 * (c0 * hs + head) + (s > pl.share.begin(c0) ? 1 : 0));
                             p.split[2 * blockIdx.x + 1] = make_int4(pl.share.block(stop - 1), 0, 0, 0);
                         }
                     }
@@ -1659,19 +1667,23 @@ __global__ void __launch_bounds__(JOIN) k_join_split(const Args p, int grid) {
     using J = Join<T, D>;
     griddep_launch_dependents();
     griddep_wait();
-    Share share;
-    share.set(1, 0, p.before[p.n], grid);
-    if (share.begin(blockIdx.x) == share.begin(blockIdx.x + 1)) return;
+    // asked for at once; what a block without a share holds there means nothing
+    const int tiles = p.before[p.n], c1 = p.split[2 * blockIdx.x + 1].x;
     const int4 a = p.split[2 * blockIdx.x];
-    if (a.y == 0) return;
-    const int c1 = p.split[2 * blockIdx.x + 1].x;
+    const int hs = hs_of<KIND>(p), c0 = blockIdx.x / hs, head = blockIdx.x - c0 * hs;
+    Share share;
+    share.set(1, 0, tiles, grid / hs);
+    if (share.begin(c0) == share.begin(c0 + 1) || a.y == 0) return;
     const int x = threadIdx.x % J::LANES, rows = a.y * p.G;
     for (int row = blockIdx.y * J::ROWS + threadIdx.x / J::LANES; row < rows; row += gridDim.y * J::ROWS) {
         J j;
         constexpr int64_t R = SLOT<KIND>;
         j.add(p.po + (a.w * R + row) * D, p.pl + a.w * R + row, x);
 #pragma unroll 4
-        for (int c = blockIdx.x; c <= c1; c++) j.add(p.po + (2 * c * R + row) * D, p.pl + 2 * c * R + row, x);
+        for (int c = c0; c <= c1; c++) {
+            const int64_t at = 2 * (c * hs + head) * R + row;
+            j.add(p.po + at * D, p.pl + at, x);
+        }
         const int tok = row / p.G;
         j.put(p, a.x + tok, a.z * p.G + (row - tok * p.G), x, [&]() {
             int last;
@@ -1748,9 +1760,9 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
     CUtensorMap tq, tqp, tk, tv;
     if (e2c_tmap_3d(&tq, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, q_box) ||
         (prefix && e2c_tmap_3d(&tqp, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, qp_box)) ||
-        (C::CODE ? e2c_tmap_2d_plain(&tk, a.pc.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, width, rows, width, C::ROW, box)
+        (C::CODE ? e2c_tmap_bytes(&tk, a.pc.k, width, rows, C::ROW, box, 0)
                  : e2c_tmap_2d(&tk, a.pc.k, dt, 2, width, rows, width * 2, 64, box)) ||
-        (C::CODE ? e2c_tmap_2d_plain(&tv, a.pc.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, width, rows, width, C::ROW, box)
+        (C::CODE ? e2c_tmap_bytes(&tv, a.pc.v, width, rows, C::ROW, box, 0)
                  : e2c_tmap_2d(&tv, a.pc.v, dt, 2, width, rows, width * 2, 64, box)))
         return -3;
     if (!prefix) tqp = tq;

@@ -41,7 +41,8 @@ static encode_tiled_fn get_encode(void) {
 }
 
 static int tmap_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
-                   uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer, uint32_t swz) {
+                   uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer, uint32_t swz,
+                   CUtensorMapL2promotion fetch) {
     encode_tiled_fn enc = get_encode();
     if (!enc) {
         e2c_set_msg("tensor map: cuTensorMapEncodeTiled unavailable");
@@ -62,7 +63,7 @@ static int tmap_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int
                            : swz == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                            : swz == 32 ? CU_TENSOR_MAP_SWIZZLE_32B
                                        : CU_TENSOR_MAP_SWIZZLE_NONE,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           fetch, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         e2c_set_msg("tensor map: encode failed (%d) for %llu x %llu, stride %llu, box %u x %u", (int)r,
                     (unsigned long long)inner, (unsigned long long)outer, (unsigned long long)row_stride, box_inner,
@@ -103,20 +104,25 @@ int e2c_tmap_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int el
 
 int e2c_tmap_2d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
                 uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer) {
-    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 128);
+    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 128, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 int e2c_tmap_2d_sw64(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
                      uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer) {
-    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 64);
+    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 64, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 int e2c_tmap_2d_sw32(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
                      uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer) {
-    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 32);
+    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 32, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 int e2c_tmap_2d_plain(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
                       uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer) {
-    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 0);
+    return tmap_2d(m, base, dt, elem_bytes, inner, outer, row_stride, box_inner, box_outer, 0, CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
+}
+
+int e2c_tmap_bytes(CUtensorMap *m, const void *base, uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer, int swizzled) {
+    return tmap_2d(m, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, inner, outer, inner, box_inner, box_outer, swizzled ? box_inner : 0,
+                   box_inner <= 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
 }

@@ -26,6 +26,10 @@ int e2c_tmap_3d(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int el
 // Without swizzle: row-major boxes (box_inner * elem a multiple of 16 bytes).
 int e2c_tmap_2d_plain(CUtensorMap *m, const void *base, CUtensorMapDataType dt, int elem_bytes, uint64_t inner,
                       uint64_t outer, uint64_t row_stride, uint32_t box_inner, uint32_t box_outer);
+/* dense rows of bytes, boxes of 64 or 128 of them (swizzled in those units, or not at all); the L2 cache fetches no more than a
+ * box's bytes of a row, whose neighbours belong to other heads that are read at other times (a cache of 8 bits, heads of 128: 37% more
+ * DRAM bytes with the 256 of the maps above) */
+int e2c_tmap_bytes(CUtensorMap *m, const void *base, uint64_t inner, uint64_t outer, uint32_t box_inner, uint32_t box_outer, int swizzled);
 
 #ifdef __cplusplus
 }
