@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                 const uint4 y = *reinterpret_cast<const uint4 *>(k + C::piece(oct + 8, 4 * j + quad));
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
-                    const uint2 a = from_codes<X>((&x.x)[t]), b = from_codes<X>((&y.x)[t]);
+                    const uint2 a = from_codes<__half>((&x.x)[t]), b = from_codes<__half>((&y.x)[t]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) mma_16816<X>(t & 1 ? s2[nt] : s[nt], a.x, b.x, a.y, b.y, qf[4 * j + t][nt][0], qf[4 * j + t][nt][1]);
                 }
@@ -506,7 +506,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
 #pragma unroll
                     for (int t = 0; t < 2; t++) {  // two dimensions of a word: rows oct and oct + 8 of a tile
                         const int pick = t ? 0x7362 : 0x5140, tile = 2 * (part * WORDS + d) + t;
-                        const uint2 a = from_codes<X>(__byte_perm(w[0][d], w[1][d], pick)), b = from_codes<X>(__byte_perm(w[2][d], w[3][d], pick));
+                        const uint2 a = from_codes<__half>(__byte_perm(w[0][d], w[1][d], pick)), b = from_codes<__half>(__byte_perm(w[2][d], w[3][d], pick));
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) mma_16816<X>(o[tile][nt], a.x, a.y, b.x, b.y, pb[nt][0], pb[nt][1]);
                     }

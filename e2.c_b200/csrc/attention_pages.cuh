@@ -43,6 +43,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "devstate.cuh"
 #include "launch.h"
 #include "pages.cuh"
@@ -137,7 +139,7 @@ struct Cfg {
     static constexpr int NKS = CODE ? (D == 64 ? 3 : D == 128 ? 2 : 1) : D == 64 ? 5 : D == 128 ? 3 : 2;
     static constexpr int NVS = CODE ? (D == 64 ? 3 : 1) : D == 64 ? 5 : 2;
     // CODES: stages as the pages hold them, rows of ROW bytes in panels; K's with the scales of both behind its codes
-    static constexpr int ROW = D == 64 ? 64 : 128, CSTAGE = STAGE / 2, KCSTAGE = CSTAGE + 2 * TK * 4;
+    static constexpr int ROW = D == 64 ? 64 : 128, CSTAGE = STAGE / 2, KCSTAGE = CSTAGE + 1024;  // (swizzled: multiples of 1024)
     static constexpr int NKC = !CODE ? 0 : D == 64 ? 4 : 3, NVC = !CODE ? 0 : D == 64 ? 4 : 2;
     static constexpr int NC = 4;  // tiles whose scales are in shared memory
     // tensor memory: NS buffers of S (128 columns each), then NO of O (D columns each), 512 columns
@@ -151,8 +153,9 @@ struct Cfg {
     static constexpr int K_OFF = NQ * Q_BYTES;
     static constexpr int V_OFF = K_OFF + NKS * STAGE;
     static constexpr int KC_OFF = V_OFF + NVS * STAGE, VC_OFF = KC_OFF + NKC * KCSTAGE;
-    static constexpr int SC_OFF = VC_OFF + NVC * CSTAGE;        // [NC][3][128]: of K times c, log2 of V's, V's
-    static constexpr int XM = SC_OFF + (CODE ? NC * 3 * TK * 4 : 0);  // running maxima handed on [NG][128]
+    static constexpr int SC_OFF = VC_OFF + NVC * CSTAGE;        // [NC]: K's times c, V's, and the tile's powers
+    static constexpr int SC = 2 * TK + 4;
+    static constexpr int XM = SC_OFF + (CODE ? NC * SC * 4 : 0);  // running maxima handed on [NG][128]
     static constexpr int ML = XM + NG * TR * 4;                 // item's (m, l) [2 items][NG][128] x 2
     static constexpr int ITEMS = ML + 2 * NG * TR * 8;
     static constexpr int SCAN = ITEMS + NI * 64;
@@ -735,12 +738,14 @@ __host__ __device__ constexpr uint32_t type_bits() {  // A and B formats of the 
     return sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? (1u << 7) | (1u << 10) : 0u;
 }
 
-// ---- pages of 8 bits (CODES). A tile's codes become 16-bit numbers (exactly: they are whole and at most 127) on their
-// way from the stages that the loads fill to those that the products read; scales stay out of the products:
-//   logit_j = (q . code_j) kc_j,   kc = K's scale * c
-//   O = sum_j P_j code_j,   P_j = 2^(logit_j - m) vs_j rounded to 16 bits,   m at least the largest logit_j + log2 vs_j (less 2^8)
-// so that P has the size that it has without scales whatever theirs is; l = sum_j 2^(logit_j - m) in 32 bits. A scale of
-// V that is not finite makes P, and the rows with it, NaN.
+// ---- pages of 8 bits (CODES). Codes become 16-bit numbers on their way from the stages that the loads fill to those that the
+// products read, exactly (they are whole and at most 127): K's in q's type, V's in fp16. Scales stay out of the products; the
+// softmax applies them, column by column. With kc = K's scale * c and a power of two for each tile, 2^F, near its largest
+// scale of V:
+//   logit_j = (q . code_j) kc_j,   w_j = 2^(logit_j + F - m),   m the largest logit_j + F (less 2^8 at most)
+//   out = sum_j P_j code_j / l,    P_j = w_j (vs_j 2^-F) in fp16,   l = sum_j 2^(logit_j - m) = sum over tiles of 2^-F sum_j w_j
+// so that P has the size that it has without scales, whatever theirs is. A scale that is not finite makes its key, or the rows that
+// meet its value, NaN.
 
 // four codes as 16-bit floats
 template <typename T>
@@ -764,27 +769,72 @@ E2C_DEV uint2 from_codes<__half>(uint32_t w) {
     const __half2 y = __hsub2(reinterpret_cast<const __half2 &>(b), reinterpret_cast<const __half2 &>(less));
     return make_uint2(reinterpret_cast<const uint32_t &>(x), reinterpret_cast<const uint32_t &>(y));
 }
-
-// logits of N columns with log2 of their scales of V (sc: the columns' kc, 128 further log2 vs)
-template <int N>
-E2C_DEV void scale_logits(uint32_t (&s)[N], const float *sc) {
+// 2^(e - 127) for 1 <= e <= 254
+E2C_DEV float power(int e) { return __uint_as_float((uint32_t)e << 23); }
+E2C_DEV uint32_t finite_bits(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+// sixteen columns' numbers, in registers
+struct Columns {
+    float4 x[4];
+    E2C_DEV Columns(const float *p) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        const float4 k = *reinterpret_cast<const float4 *>(sc + i), v = *reinterpret_cast<const float4 *>(sc + TK + i);
-        const float2 a = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k.x, k.y), make_float2(v.x, v.y));
-        const float2 b = fma2(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k.z, k.w), make_float2(v.z, v.w));
-        s[i] = __float_as_uint(a.x), s[i + 1] = __float_as_uint(a.y), s[i + 2] = __float_as_uint(b.x), s[i + 3] = __float_as_uint(b.y);
+        for (int i = 0; i < 4; i++) x[i] = reinterpret_cast<const float4 *>(p)[i];
+    }
+    E2C_DEV float2 operator[](int i) const { return i & 1 ? make_float2(x[i / 2].z, x[i / 2].w) : make_float2(x[i / 2].x, x[i / 2].y); }
+};
+// the products of sixteen columns times their kc
+E2C_DEV void scale_logits(uint32_t *s, const Columns &k) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float2 y = mul2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k[i]);
+        s[2 * i] = __float_as_uint(y.x), s[2 * i + 1] = __float_as_uint(y.y);
+    }
+}
+
+// One stage: codes x of keys before `here` to y, zeros from there to `upto`. Eight neighbouring lanes
+// take four pieces of 16 codes of row r and of row r ^ 5: with the loads' and the products' 128-byte swizzles these reads and both
+// writes of each are in all banks. A thread's rows are 32 apart, which no swizzle tells apart, so that their addresses are constants
+// away from one another: worked out for each piece they took half of this code.
+template <typename T, int D, int KIND, bool IS_V>
+E2C_DEV void convert_stage(const uint8_t *x, uint8_t *y, int here, int upto, int tid) {
+    using C = Cfg<D, KIND>;
+    using X = std::conditional_t<IS_V, __half, T>;
+    // a panel of codes has ROWS rows of ROW bytes; the four warps take 32 rows by 64 bytes at a time
+    constexpr int ROWS = IS_V ? C::VROWS : TK, HALVES = C::ROW / 64, EACH = ROWS / 32, PARTS = C::CSTAGE / (ROWS * 64);
+    const int pair = tid >> 3 & 3, r0 = (tid >> 5) * 8 + (tid & 4 ? pair ^ 5 : pair), piece = tid & 3;
+    const uint32_t from = r0 * C::ROW + ((HALVES == 2 ? piece ^ (r0 & 7) : piece ^ (r0 >> 1 & 3)) << 4);
+    y += r0 * 128;
+    const int first = ((2 * piece) ^ (r0 & 7)) << 4;
+#pragma unroll 1
+    for (int part = 0; part < PARTS; part++, y += ROWS * 128) {  // of a panel's halves
+        const uint8_t *p = x + (HALVES == 2 ? (part >> 1) * (ROWS * C::ROW) + (from ^ (part & 1) << 6) : from);
+        uint4 c[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; i++) c[i] = *reinterpret_cast<const uint4 *>(p + i * (32 * C::ROW));
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            uint2 s[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) s[k] = from_codes<X>((&c[i].x)[k]);
+            if (here < ROWS) {  // the last keys' tile
+                if (r0 + 32 * i >= here) s[0] = s[1] = s[2] = s[3] = make_uint2(0, 0);
+                if (r0 + 32 * i >= upto) continue;
+            }
+            *reinterpret_cast<uint4 *>(y + i * (32 * 128) + first) = make_uint4(s[0].x, s[0].y, s[1].x, s[1].y);
+            *reinterpret_cast<uint4 *>(y + i * (32 * 128) + (first ^ 16)) = make_uint4(s[2].x, s[2].y, s[3].x, s[3].y);
+        }
     }
 }
 
 // Four warps for K (w < 4) and four for V: every stage's codes, of as many keys as the product takes, into the 128-byte swizzle that
-// it reads; V's rows past the last key become zeros. K's warps also prepare the tile's scales.
+// it reads; rows past the last key become zeros. K's warps also prepare the tile's scales.
 template <typename T, int D, int KIND, typename Bar, typename Take>
 E2C_DEV void convert_codes(const Args &p, uint8_t *smem, int w, int lane, Bar bar, Take take) {
     using C = Cfg<D, KIND>;
-    constexpr int CHUNKS = C::ROW / 16, PARTS = C::CSTAGE / 16 / 128;  // of a row; of a thread
     const bool is_v = w >= 4;
-    const int tid = (w & 3) * 32 + lane, rows = is_v ? C::VROWS : TK;
+    const int tid = (w & 3) * 32 + lane;
     const int FULL = is_v ? B_VCF : B_KCF, FREE = is_v ? B_VCE : B_KCE, NST = is_v ? C::NVC : C::NKC;
     const int OUT = is_v ? B_VF : B_KF, TAKEN = is_v ? B_VE : B_KE, NOUT = is_v ? C::NVS : C::NKS;
     const int pitch = is_v ? C::CSTAGE : C::KCSTAGE;
@@ -796,54 +846,34 @@ E2C_DEV void convert_codes(const Args &p, uint8_t *smem, int w, int lane, Bar ba
     for (int n = 0; take(n, it); n++) {
 #pragma unroll 1
         for (int j = 0; j < it.nt; j++, g++) {
-            const int nk = min(TK, tile_end<KIND>(p, it, j) - tile_key<KIND>(it, j));
+            const int nk = min(TK, tile_end<KIND>(p, it, j) - tile_key<KIND>(it, j)), sb = g % C::NC;
+            float *sc = reinterpret_cast<float *>(smem + C::SC_OFF) + sb * C::SC;
 #pragma unroll 1
             for (int h = 0; h < C::KPARTS; h++) {
                 if (!wait_warp(bar(FULL + st), sp, p.status, E2C_ERR_WAIT_PRODUCER)) return;
                 const uint8_t *x = ring + st * pitch;
-                if (!is_v && h == 0) {
-                    if (!wait_warp(bar(B_SCE + g % C::NC), (uint32_t)(((g / C::NC) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) return;
-                    float *sc = reinterpret_cast<float *>(smem + C::SC_OFF) + (g % C::NC) * (3 * TK);
+                if (h == 0 && !is_v) {
                     const float *from = reinterpret_cast<const float *>(x + C::CSTAGE);
-                    const float k = tid < nk ? from[tid] : 0.f, v = tid < nk ? from[TK + tid] : 0.f;
-                    const bool fine = fabsf(v) < INFINITY;
-                    sc[tid] = k * p.c;
-                    // 2^100 either way is far from where l or P would leave fp32's range
-                    sc[TK + tid] = fine ? fminf(fmaxf(__log2f(fabsf(v)), -100.f), 100.f) : 0.f;
-                    sc[2 * TK + tid] = fine ? v : NAN;
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int i = 0; i < TK; i += 32)
+                        if (i + lane < nk) top = max(top, finite_bits(from[TK + i + lane]));
+                    // the largest's exponent, from 2^-100 to 2^126: l does not leave fp32's range
+                    const int e = min(max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), 27), 253);
+                    if (!wait_warp(bar(B_SCE + sb), (uint32_t)(((g / C::NC) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) return;
+                    sc[tid] = tid < nk ? from[tid] * p.c : 0.f;
+                    sc[TK + tid] = tid < nk ? from[TK + tid] * power(254 - e) : 0.f;
+                    if (tid == 0) *reinterpret_cast<float2 *>(sc + 2 * TK) = make_float2((float)(e - 127), power(254 - e));
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(B_SCF + g % C::NC));
+                    if (lane == 0) mbar_arrive(bar(B_SCF + sb));
                 }
                 if (!wait_warp(bar(TAKEN + out), op, p.status, E2C_ERR_WAIT_PRODUCER)) return;
-                const int here = is_v ? min(nk - h * C::VROWS, C::VROWS) : nk, up = (here + 15) & ~15;
+                const int here = is_v ? min(nk - h * C::VROWS, C::VROWS) : nk, upto = (here + 15) & ~15;
                 uint8_t *y = to + out * C::STAGE;
-#pragma unroll
-                for (int i0 = 0; i0 < PARTS; i0 += 4) {
-                    uint4 c[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int e = tid + 128 * (i0 + i), r = e / CHUNKS & (rows - 1);
-                        if (r < here) c[i] = *reinterpret_cast<const uint4 *>(x + e * 16);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int e = tid + 128 * (i0 + i), r = e / CHUNKS & (rows - 1), panel = e / CHUNKS / rows;
-                        if (r >= up) continue;
-                        uint4 a = make_uint4(0, 0, 0, 0), b = a;
-                        if (r < here) {
-                            const uint2 s0 = from_codes<T>(c[i].x), s1 = from_codes<T>(c[i].y), s2 = from_codes<T>(c[i].z), s3 = from_codes<T>(c[i].w);
-                            a = make_uint4(s0.x, s0.y, s1.x, s1.y);
-                            b = make_uint4(s2.x, s2.y, s3.x, s3.y);
-                        }
-                        // 16 codes are two 16-byte pieces of a panel of 64; which one a thread writes first
-                        // alternates, so that eight neighbours write to all banks
-                        const int ch = e & (CHUNKS - 1), pan = panel * (C::ROW / 64) + (ch >> 2), piece = (ch & 3) * 2;
-                        uint8_t *row = y + pan * (rows * 128) + r * 128;
-                        const int odd = D == 64 ? 0 : ch >> 2;
-                        *reinterpret_cast<uint4 *>(row + (((piece + odd) ^ (r & 7)) << 4)) = odd ? b : a;
-                        *reinterpret_cast<uint4 *>(row + (((piece + 1 - odd) ^ (r & 7)) << 4)) = odd ? a : b;
-                    }
-                }
+                if (is_v)
+                    convert_stage<T, D, KIND, true>(x, y, here, upto, tid);
+                else
+                    convert_stage<T, D, KIND, false>(x, y, here, upto, tid);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
@@ -869,6 +899,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                       const __grid_constant__ Args p, const int q_box, const int qp_box) {
     using C = Cfg<D, KIND>;
+    using X = std::conditional_t<C::CODE, __half, T>;  // of the second product's operands
     extern __shared__ __align__(1024) uint8_t smem[];
     griddep_launch_dependents();
     if (smem_u32(smem) & 1023) {
@@ -948,6 +979,16 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
         return it.ntok >= 0;
     };
 
+    // CODES: 768 threads begin with 80 registers each; the softmax's take of the others': (2 * 104 + 72 + 72 + 2 * 64) / 6 = 80
+    if constexpr (C::CODE) {
+        static_assert(C::NTHREADS == 768 && C::W_EPI == 8, "shares of registers");
+        if (warp < C::W_EPI)
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+        else if (warp < C::W_CONVERT)
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        else
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    }
     if (C::CODE && warp >= C::W_CONVERT) {
         convert_codes<T, D, KIND>(p, smem, warp - C::W_CONVERT, lane, bar, take);
     } else if (warp >= C::W_ITEMS) {
@@ -1042,9 +1083,9 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
             // QK runs LOOK tiles ahead of PV; each has a cursor over the items
             if (elect_one()) {
                 constexpr int LOOK = C::NS - 1;
-                constexpr uint32_t idesc = (1u << 4) | type_bits<T>() | ((uint32_t)(128 >> 4) << 24);
-                constexpr uint32_t id_pv = idesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // B: N contiguous
-                const uint32_t id_qk = idesc | (p.neg << 13);
+                constexpr uint32_t idesc = (1u << 4) | ((uint32_t)(128 >> 4) << 24);
+                constexpr uint32_t id_pv = idesc | type_bits<X>() | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // B: N contiguous
+                const uint32_t id_qk = idesc | type_bits<T>() | (p.neg << 13);
                 auto wait1 = [&](int b, uint32_t parity) -> bool {
 #pragma unroll 1
                     for (uint32_t i = 0; i < kTries; i++)
@@ -1380,22 +1421,37 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
 #pragma unroll
                     for (int i = 0; i < 16; i++) s[i] = seen & (1u << i) ? s[i] : 0xff800000u;
                 };
-                // CODES: a tile's scales; y(i) is what a logit and the log2 of V's scale come to
-                const float *sc = reinterpret_cast<const float *>(smem + C::SC_OFF) + (g % C::NC) * (3 * TK);
-                if (C::CODE && !wait_warp(bar(B_SCF + g % C::NC), (uint32_t)((g / C::NC) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
-                    ok = false;
-                    break;
+                float shift = 0.f, lower = 1.f;  // CODES: F and 2^-F; sc: the columns' kc
+                const float *sc = reinterpret_cast<const float *>(smem + C::SC_OFF) + (g % C::NC) * C::SC;
+                if (C::CODE) {
+                    if (!wait_warp(bar(B_SCF + g % C::NC), (uint32_t)((g / C::NC) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                        ok = false;
+                        break;
+                    }
+                    shift = sc[2 * TK];
+                    lower = sc[2 * TK + 1];
                 }
                 float mx = -INFINITY;
                 if (busy) {
                     float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (!masked) {
+                    if (C::CODE && !masked) {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < TK; c0 += 32) {
+                            uint32_t s[32];
+                            tmem_ld32(ts + c0, s);
+                            const Columns k0(sc + c0), k1(sc + c0 + 16);  // they arrive while the products do
+                            tmem_wait_ld();
+                            scale_logits(s, k0);
+                            scale_logits(s + 16, k1);
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        }
+                    } else if (!masked) {
 #pragma unroll 1
                         for (int c0 = 0; c0 < TK; c0 += 32) {
                             uint32_t s[32];
                             tmem_ld32(ts + c0, s);
                             tmem_wait_ld();
-                            if constexpr (C::CODE) scale_logits<32>(s, sc + c0);
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
@@ -1405,14 +1461,20 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                         for (int c0 = 0; c0 < nk; c0 += 16) {
                             uint32_t s[16];
                             tmem_ld16(ts + c0, s);
-                            tmem_wait_ld();
-                            if constexpr (C::CODE) scale_logits<16>(s, sc + c0);
+                            if constexpr (C::CODE) {
+                                const Columns k(sc + c0);
+                                tmem_wait_ld();
+                                scale_logits(s, k);
+                            } else {
+                                tmem_wait_ld();
+                            }
                             hide(c0, s, row4c);
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
                     }
-                    mx = max2(max2(mm[0], mm[1]), max2(mm[2], mm[3])) * (C::CODE ? 1.f : p.c);
+                    mx = max2(max2(mm[0], mm[1]), max2(mm[2], mm[3]));
+                    mx = C::CODE ? mx + shift : mx * p.c;
                 }
                 float now = before, alpha = 1.f;
                 if (live && !(mx <= before + kRescaleLog2)) {  // so also from -infinity, and for a NaN
@@ -1448,10 +1510,27 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                     }
                     // a row that has seen nothing yet has only -inf: any finite maximum gives it zeros
                     const float2 cc = make_float2(p.c, p.c);
-                    const float mneg = m == -INFINITY ? 0.f : -m;
+                    const float mneg = C::CODE ? (m == -INFINITY ? 0.f : shift - m) : m == -INFINITY ? 0.f : -m;
                     const float2 mm = make_float2(mneg, mneg);
                     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-                    if (!masked) {
+                    if (C::CODE && !masked) {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < TK; c0 += 16) {
+                            uint32_t s[16], pk[8];
+                            tmem_ld16(ts + c0, s);
+                            const Columns k(sc + c0), v(sc + TK + c0);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k[i], mm);
+                                x = i % kPoly == kPoly - 1 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                                sum[i & 1] = add2(sum[i & 1], x);
+                                x = mul2(x, v[i]);
+                                pk[i] = pack2<X>(x.x, x.y);
+                            }
+                            tmem_st8(ts + c0 / 2, pk);
+                        }
+                    } else if (!masked) {
 #pragma unroll 1
                         for (int c0 = 0; c0 < TK; c0 += 32) {
                             uint32_t s[32], pk[16];
@@ -1459,12 +1538,10 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
-                                const float2 k2 = C::CODE ? *reinterpret_cast<const float2 *>(sc + c0 + 2 * i) : cc;
-                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k2, mm);
+                                float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), cc, mm);
                                 x = i % kPoly == kPoly - 1 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
-                                if constexpr (C::CODE) x = mul2(x, *reinterpret_cast<const float2 *>(sc + 2 * TK + c0 + 2 * i));
-                                pk[i] = pack2<T>(x.x, x.y);
+                                pk[i] = pack2<X>(x.x, x.y);
                             }
                             tmem_st16(ts + c0 / 2, pk);
                         }
@@ -1473,30 +1550,28 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                         for (int c0 = 0; c0 < nk; c0 += 16) {
                             uint32_t s[16], pk[8];
                             tmem_ld16(ts + c0, s);
-                            tmem_wait_ld();
                             if constexpr (C::CODE) {  // before what is hidden becomes -infinity: a scale may be zero
-#pragma unroll
-                                for (int i = 0; i < 8; i++) {
-                                    const float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])),
-                                                          *reinterpret_cast<const float2 *>(sc + c0 + 2 * i), mm);
-                                    s[2 * i] = __float_as_uint(x.x), s[2 * i + 1] = __float_as_uint(x.y);
-                                }
+                                const Columns k(sc + c0);
+                                tmem_wait_ld();
+                                scale_logits(s, k);
+                            } else {
+                                tmem_wait_ld();
                             }
                             hide(c0, s, row4);
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
-                                float2 x = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-                                if constexpr (!C::CODE) x = fma2(x, cc, mm);
+                                const float2 y = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+                                float2 x = C::CODE ? add2(y, mm) : fma2(y, cc, mm);
                                 x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
-                                if constexpr (C::CODE) x = mul2(x, *reinterpret_cast<const float2 *>(sc + 2 * TK + c0 + 2 * i));
-                                pk[i] = pack2<T>(x.x, x.y);
+                                if constexpr (C::CODE) x = mul2(x, *reinterpret_cast<const float2 *>(sc + TK + c0 + 2 * i));
+                                pk[i] = pack2<X>(x.x, x.y);
                             }
                             tmem_st8(ts + c0 / 2, pk);
                         }
                     }
                     const float2 all = add2(sum[0], sum[1]);
-                    l += all.x + all.y;
+                    l += C::CODE ? (all.x + all.y) * lower : all.x + all.y;
                     tmem_wait_st();
                 }
                 if (C::CODE) {  // the tile's scales have been read
@@ -1760,9 +1835,9 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
     CUtensorMap tq, tqp, tk, tv;
     if (e2c_tmap_3d(&tq, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, q_box) ||
         (prefix && e2c_tmap_3d(&tqp, q, dt, 2, D, a.H, a.T, D * 2, (uint64_t)ldq * 2, 64, a.G, qp_box)) ||
-        (C::CODE ? e2c_tmap_bytes(&tk, a.pc.k, width, rows, C::ROW, box, 0)
+        (C::CODE ? e2c_tmap_bytes(&tk, a.pc.k, width, rows, C::ROW, box, 1)
                  : e2c_tmap_2d(&tk, a.pc.k, dt, 2, width, rows, width * 2, 64, box)) ||
-        (C::CODE ? e2c_tmap_bytes(&tv, a.pc.v, width, rows, C::ROW, box, 0)
+        (C::CODE ? e2c_tmap_bytes(&tv, a.pc.v, width, rows, C::ROW, box, 1)
                  : e2c_tmap_2d(&tv, a.pc.v, dt, 2, width, rows, width * 2, 64, box)))
         return -3;
     if (!prefix) tqp = tq;

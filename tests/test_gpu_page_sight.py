@@ -1,10 +1,12 @@
 """Attention over pages with sinks, over trees of drafted tokens and over pages of 8 bits; the store into such pages and
 their reading back; trees and what is kept of them: on the GPU, against plain 64-bit forms.
 
-Tolerances are those of test_gpu_prompt_cache.py, with u the unit roundoff of q's type: over pages of 8 bits the exponential
-times its token's scale of v takes the probability's place, so that it, too, is rounded once, against p |v| with v = code * scale;
-a product below 2^-14 of a row's largest loses 2^-25 of that absolutely in fp16, times a code of at most 127: 2^-25 of the
-largest |v|. Logits are the same 32-bit sums of products, and one product more for the key's scale.
+Tolerances are those of test_gpu_prompt_cache.py, with u the unit roundoff of q's type, and for pages of 8 bits, whose second
+product has fp16 operands whatever q's type:
+  attention  besides u |out| for the result, 2^-11 sum p|v| each for the exponential (times its token's scale, where that is
+             applied there) and for v = code * scale where that becomes an operand; an exponential below 2^-14 of the row's
+             largest (times its scale) loses 2^-25 of that absolutely, so that a row is off by 2^-25 of the largest |v| a key.
+             Logits are the same 32-bit sums of products, and one product more for the key's scale
   codes      a head's values are within half a step (scale / 2) of the 64-bit rotation, and 2^-22 of the largest magnitude for
              the rotation, the scale and the quotient in 32 bits; equal to the 32-bit arithmetic written out
   read back  code * scale in fp32 (2^-24), rounded once to the output type
@@ -99,6 +101,18 @@ def sight64(torch, cache, layer, q, seqs, q_start, causal, window, scale, sinks=
         lse[a:b] = r.T
         big[a:b] = x.abs().masked_fill(~sees, 0).amax(-1).T
     return out, mag, lse, big
+
+
+def assert_codes(torch, got, lse, want, name, keys, largest):
+    """assert_attention for pages of 8 bits whose values are at most `largest`."""
+    out, mag, ref, big = want
+    logit = 2.0 ** -18 * (1 + big)
+    tol = UNIT[name] * out.abs() + (2.02 * 2.0 ** -11 + 2 * logit[..., None]) * mag + 2.0 ** -25 * (1 + keys * largest) + 1e-7
+    assert not torch.isnan(got).any()
+    assert ((got.double() - out).abs() - tol).max().item() <= 0
+    empty = torch.isinf(ref)
+    assert torch.equal(torch.isinf(lse), empty) and (lse[empty] < 0).all()
+    assert ((lse.double() - ref).abs() - logit)[~empty].max().item() <= 0
 
 
 # ------------------------------------------------------------------------------------------ sinks
@@ -366,6 +380,10 @@ def make_codes(e2c, torch, seed, lens, queries, shared, H, KV, D, page, dtype, s
     return e2c.PageCache(k, v, cache.table, cache.length, cache.refs, ks, vs), q, seqs, q_start, max_q
 
 
+def largest(cache):
+    return 127.0 * cache.v_scale.nan_to_num().abs().max().item()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("causal,window,sinks", [(True, -1, 0), (False, 37, 0), (True, 130, 4), (False, 0, 129)])
 @pytest.mark.parametrize("case", list(CASES))
@@ -375,7 +393,8 @@ def test_codes_attention(e2c, torch_cuda, case, causal, window, sinks, dtype):
     cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 14, lens, queries, shared, H, KV, D, page, dtype, spread=0.3)
     out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, causal=causal, window=window, sinks=sinks, lse=True)
     e2c.check()
-    assert_attention(torch, out, lse, sight64(torch, cache, 0, q, seqs, q_start, causal, window, D ** -0.5, sinks), dtype, max(lens))
+    want = sight64(torch, cache, 0, q, seqs, q_start, causal, window, D ** -0.5, sinks)
+    assert_codes(torch, out, lse, want, dtype, max(lens), largest(cache))
     again = cache.attention(0, q, seqs, q_start, max_q, shared=shared, causal=causal, window=window, sinks=sinks)
     assert torch.equal(again, out), "two calls differ"
 
@@ -393,4 +412,4 @@ def test_codes_tree_attention(e2c, torch_cuda, case, dtype):
         out, lse = cache.attention(0, q, seqs, q_start, max_q, shared=shared, window=window, sinks=sinks, tree=tree, lse=True)
         e2c.check()
         want = sight64(torch, cache, 0, q, seqs, q_start, True, window, D ** -0.5, sinks, [tree_mask(p) for p in parents])
-        assert_attention(torch, out, lse, want, dtype, max(lens))
+        assert_codes(torch, out, lse, want, dtype, max(lens), largest(cache))
