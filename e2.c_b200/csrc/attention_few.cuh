@@ -17,7 +17,8 @@
 // through one head after the other). Calls of few and short items (a window, or a short table) take a block an item: no
 // plan, and no join.
 //
-// Codes (8 bits) become fp16, exactly, in registers; scales are factors of a lane's own keys, applied as in attention_pages.cuh.
+// Codes (8 bits) become fp16, exactly, in registers; scales are factors of a lane's own keys, and m is the largest
+// logit_j + log2 vs_j (less 2^8 at most), vs V's scale, so that P_j = 2^(logit_j - m) vs_j has the size that it has without scales.
 // Q in bf16 is scaled by a power of two, one for an item, so that fp16 holds it: exact but for values below 2^-28 of the item's
 // largest, which lose 2^-39 of that at most.
 #pragma once
@@ -678,7 +679,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
 
 // Items of which a block can take one each, and the keys of which are few enough that reading them takes no longer than a join of
 // their parts would
-constexpr int WHOLE_BYTES = 512 << 10;
+constexpr int WHOLE_BYTES = 256 << 10;
 template <typename T, bool CODE, int D, int NT>
 int run_few(Args a, const void *q, int64_t ldq, int sms, cudaStream_t st) {
     using C = Few<CODE, D, NT>;

@@ -785,7 +785,7 @@ struct Columns {
     E2C_DEV float2 operator[](int i) const { return i & 1 ? make_float2(x[i / 2].z, x[i / 2].w) : make_float2(x[i / 2].x, x[i / 2].y); }
 };
 // the products of sixteen columns times their kc
-E2C_DEV void scale_logits(uint32_t *s, const Columns &k) {
+E2C_DEV void scale_logits(uint32_t (&s)[16], const Columns &k) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const float2 y = mul2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k[i]);
@@ -797,33 +797,34 @@ E2C_DEV void scale_logits(uint32_t *s, const Columns &k) {
 // take four pieces of 16 codes of row r and of row r ^ 5: with the loads' and the products' 128-byte swizzles these reads and both
 // writes of each are in all banks. A thread's rows are 32 apart, which no swizzle tells apart, so that their addresses are constants
 // away from one another: worked out for each piece they took half of this code.
-template <typename T, int D, int KIND, bool IS_V>
+// One piece a step: with two dozen warps in seven roles, code that does not stay in the instruction caches slows all of them (four at
+// once: 189 us where this takes 173, 6 prompts of 2500 tokens, 12 heads of 64).
+template <typename X, int D, int KIND, int ROWS>
 E2C_DEV void convert_stage(const uint8_t *x, uint8_t *y, int here, int upto, int tid) {
     using C = Cfg<D, KIND>;
-    using X = std::conditional_t<IS_V, __half, T>;
     // a panel of codes has ROWS rows of ROW bytes; the four warps take 32 rows by 64 bytes at a time
-    constexpr int ROWS = IS_V ? C::VROWS : TK, HALVES = C::ROW / 64, EACH = ROWS / 32, PARTS = C::CSTAGE / (ROWS * 64);
+    constexpr int HALVES = C::ROW / 64, EACH = ROWS / 32, PARTS = C::CSTAGE / (ROWS * 64);
     const int pair = tid >> 3 & 3, r0 = (tid >> 5) * 8 + (tid & 4 ? pair ^ 5 : pair), piece = tid & 3;
     const uint32_t from = r0 * C::ROW + ((HALVES == 2 ? piece ^ (r0 & 7) : piece ^ (r0 >> 1 & 3)) << 4);
     y += r0 * 128;
     const int first = ((2 * piece) ^ (r0 & 7)) << 4;
 #pragma unroll 1
-    for (int part = 0; part < PARTS; part++, y += ROWS * 128) {  // of a panel's halves
+    for (int part = 0; part < PARTS; part++) {  // of a panel's halves
         const uint8_t *p = x + (HALVES == 2 ? (part >> 1) * (ROWS * C::ROW) + (from ^ (part & 1) << 6) : from);
-        uint4 c[EACH];
-#pragma unroll
-        for (int i = 0; i < EACH; i++) c[i] = *reinterpret_cast<const uint4 *>(p + i * (32 * C::ROW));
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
+        uint4 next = *reinterpret_cast<const uint4 *>(p);
+#pragma unroll 1
+        for (int i = 0; i < EACH; i++, y += 32 * 128) {
+            const uint4 c = next;
+            if (i + 1 < EACH) next = *reinterpret_cast<const uint4 *>(p += 32 * C::ROW);
             uint2 s[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) s[k] = from_codes<X>((&c[i].x)[k]);
+            for (int k = 0; k < 4; k++) s[k] = from_codes<X>((&c.x)[k]);
             if (here < ROWS) {  // the last keys' tile
                 if (r0 + 32 * i >= here) s[0] = s[1] = s[2] = s[3] = make_uint2(0, 0);
                 if (r0 + 32 * i >= upto) continue;
             }
-            *reinterpret_cast<uint4 *>(y + i * (32 * 128) + first) = make_uint4(s[0].x, s[0].y, s[1].x, s[1].y);
-            *reinterpret_cast<uint4 *>(y + i * (32 * 128) + (first ^ 16)) = make_uint4(s[2].x, s[2].y, s[3].x, s[3].y);
+            *reinterpret_cast<uint4 *>(y + first) = make_uint4(s[0].x, s[0].y, s[1].x, s[1].y);
+            *reinterpret_cast<uint4 *>(y + (first ^ 16)) = make_uint4(s[2].x, s[2].y, s[3].x, s[3].y);
         }
     }
 }
@@ -870,10 +871,10 @@ E2C_DEV void convert_codes(const Args &p, uint8_t *smem, int w, int lane, Bar ba
                 if (!wait_warp(bar(TAKEN + out), op, p.status, E2C_ERR_WAIT_PRODUCER)) return;
                 const int here = is_v ? min(nk - h * C::VROWS, C::VROWS) : nk, upto = (here + 15) & ~15;
                 uint8_t *y = to + out * C::STAGE;
-                if (is_v)
-                    convert_stage<T, D, KIND, true>(x, y, here, upto, tid);
+                if (is_v || (__is_same(T, __half) && C::VROWS == TK))
+                    convert_stage<__half, D, KIND, C::VROWS>(x, y, here, upto, tid);
                 else
-                    convert_stage<T, D, KIND, false>(x, y, here, upto, tid);
+                    convert_stage<T, D, KIND, TK>(x, y, here, upto, tid);
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
@@ -1436,15 +1437,14 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                     float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (C::CODE && !masked) {
 #pragma unroll 1
-                        for (int c0 = 0; c0 < TK; c0 += 32) {
-                            uint32_t s[32];
-                            tmem_ld32(ts + c0, s);
-                            const Columns k0(sc + c0), k1(sc + c0 + 16);  // they arrive while the products do
+                        for (int c0 = 0; c0 < TK; c0 += 16) {  // (and below: 32 columns a step are too much code)
+                            uint32_t s[16];
+                            tmem_ld16(ts + c0, s);
+                            const Columns k(sc + c0);  // they arrive while the products do
                             tmem_wait_ld();
-                            scale_logits(s, k0);
-                            scale_logits(s + 16, k1);
+                            scale_logits(s, k);
 #pragma unroll
-                            for (int i = 0; i < 32; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                            for (int i = 0; i < 16; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
                     } else if (!masked) {
 #pragma unroll 1
@@ -1523,7 +1523,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
                                 float2 x = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k[i], mm);
-                                x = i % kPoly == kPoly - 1 ? ex2_poly(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                                x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
                                 x = mul2(x, v[i]);
                                 pk[i] = pack2<X>(x.x, x.y);

@@ -413,3 +413,221 @@ def test_codes_tree_attention(e2c, torch_cuda, case, dtype):
         e2c.check()
         want = sight64(torch, cache, 0, q, seqs, q_start, True, window, D ** -0.5, sinks, [tree_mask(p) for p in parents])
         assert_codes(torch, out, lse, want, dtype, max(lens), largest(cache))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("src,dtype", [("bf16", "bf16"), ("f32", "f16"), ("f16", "bf16")])
+@pytest.mark.parametrize("lens,queries,H,KV,D,page,rot,pad", [([5], [5], 1, 1, 64, 8, 64, 0), ([1, 40, 17], [1, 1, 1], 8, 2, 128, 16, 128, 8),
+                                                              ([70, 33], [70, 20], 6, 5, 256, 32, 96, 8), ([19, 64], [3, 64], 4, 2, 64, 16, 20, 3)])
+def test_codes_store_and_load(e2c, torch_cuda, lens, queries, H, KV, D, page, rot, pad, src, dtype, interleaved):
+    """Codes and scales against the 32-bit arithmetic and against 64 bits, what is read back, and all else left as it was."""
+    torch = torch_cuda
+    cache, _, seqs, q_start, _ = make_codes(e2c, torch, 21, lens, queries, 0, H, KV, D, page, "f16", layers=2)
+    T = int(q_start[-1])
+    rows = torch.randn(T, (H + 2 * KV) * D + pad, device="cuda").to(getattr(torch, DT[src]))[:, pad:]  # an odd pad: no 16-byte accesses
+    q, k, v = rows.unflatten(1, (H + 2 * KV, D)).split([H, KV, KV], 1)
+    v[0] = 0  # an all-zero head
+    cos, sin = e2c.rope_table(max(lens), rot)
+    before = [x.clone() for x in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    out = cache.store(1, q, k, v, cos, sin, seqs, q_start, interleaved=interleaved, dtype=getattr(torch, DT[dtype]))
+    e2c.check()
+    pos = torch.cat([torch.arange(lens[s] - queries[s], lens[s]) for s in seqs.tolist()]).cuda()
+    owner = torch.cat([torch.full((queries[s],), s) for s in seqs.tolist()]).cuda()
+    want, mag = turn64(torch, q, cos, sin, pos, interleaved, False)
+    assert ((out.double() - want).abs() <= UNIT[dtype] * want.abs() + 2.0 ** -25 + 4 * 2.0 ** -24 * mag).all()
+    p, slot = cache.table[owner, pos // page].long(), pos % page
+    turned, mag = turn64(torch, k, cos, sin, pos, interleaved, False)
+    for x, s, exact, err in ((cache.k, cache.k_scale, turned, 4 * 2.0 ** -24 * mag), (cache.v, cache.v_scale, v.double(), torch.zeros_like(mag))):
+        codes, scale = x[1][p, slot], s[1][p, :, slot]
+        amax = exact.abs().amax(-1, keepdim=True)
+        step = torch.where(amax > 0, amax / 127, 1.0)
+        assert ((scale.double() - step[..., 0]).abs() <= 2.0 ** -22 * step[..., 0]).all()
+        assert ((codes.double() * step - exact).abs() <= step * (0.5 + 127 * 2.0 ** -21) + err).all()
+        assert codes.abs().max() <= 127 and (codes[0].abs().amax(-1) == 127).sum() == (amax[0] > 0).sum()
+    assert torch.equal(cache.v[1][p, slot], quantised(torch, v)[0]) and torch.equal(cache.v_scale[1][p, :, slot], quantised(torch, v)[1])
+    for name in ("bfloat16", "float32", "float16"):
+        t = getattr(torch, name)
+        got = cache.load(1, seqs, q_start, T, dtype=t)
+        e2c.check()
+        for y, x, s in zip(got, (cache.k, cache.v), (cache.k_scale, cache.v_scale)):
+            assert torch.equal(y, (x[1][p, slot].float() * s[1][p, :, slot][..., None]).to(t))
+    for x, y in zip((cache.k, cache.v), before[:2]):  # the other layer, and tokens that are not the batch's
+        keep = torch.ones_like(x[..., 0, 0], dtype=torch.bool)
+        keep[1, p, slot] = False
+        assert torch.equal(x[keep], y[keep])
+
+
+def test_load_first_and_rows_that_are_not_there(e2c, torch_cuda):
+    torch = torch_cuda
+    for dtype in ("f16", "bf16"):
+        cache, _, seqs, _, _ = make_batch(e2c, torch, 4, [50, 20, 9], [1, 1, 1], 0, 2, 2, 64, 8, dtype)
+        order = dev(torch, [2, 0, 1])
+        k, v = cache.load(0, order, dev(torch, [0, 4, 10, 12]), 12, first=dev(torch, [5, 13, 18]))
+        e2c.check()
+        for i, (s, t) in enumerate([(2, j) for j in range(5, 9)] + [(0, j) for j in range(13, 19)] + [(1, 18), (1, 19)]):
+            assert torch.equal(k[i], cache.k[0, cache.table[s, t // 8].long(), t % 8]) and torch.equal(v[i], cache.v[0, cache.table[s, t // 8].long(), t % 8])
+        # before the first token, past the last, a sequence that is not there
+        k, _ = cache.load(0, dev(torch, [2, 0, 77]), dev(torch, [0, 2, 4, 5]), 5, first=dev(torch, [-1, 49, 0]))
+        with pytest.raises(e2c.E2CudaError, match="outside the cache"):
+            e2c.check()
+        assert torch.equal(k[1], cache.k[0, cache.table[2, 0].long(), 0]) and torch.equal(k[2], cache.k[0, cache.table[0, 6].long(), 1])
+
+
+def test_heads_that_are_not_finite_or_tiny(e2c, torch_cuda):
+    """Such a head stands for NaN, one below 2^-100 for zeros; a row that sees the key is NaN, and others are as before."""
+    torch = torch_cuda
+    cache = e2c.PageCache.new(1, 40, 16, 2, 64, 2, 16, torch.int8)
+    seqs, qs = dev(torch, [0]), dev(torch, [0, 200])
+    cache.append(seqs, dev(torch, [200]))
+    cos, sin = e2c.rope_table(256, 64)
+    q, k, v = (torch.randn(200, h, 64, device="cuda") for h in (4, 2, 2))
+    k[150, 0, 3], k[160, 0, 5], k[10, 1], v[170, 1, 7] = float("nan"), float("inf"), 1e-35, float("-inf")
+    x = cache.store(0, q, k, v, cos, sin, seqs, qs)
+    k2, v2 = cache.load(0, seqs, qs, 200)
+    e2c.check()
+    assert x.dtype == torch.bfloat16
+    assert torch.isnan(k2[[150, 160], 0]).all() and not torch.isnan(k2[[150, 160], 1]).any() and (k2[10, 1] == 0).all()
+    assert torch.isnan(v2[170, 1]).all() and torch.isnan(v2).sum() == 64
+    for rows in (200, 3):  # the form of many rows and of few: the last tokens
+        out, lse = cache.attention(0, x[200 - rows:].contiguous(), seqs, dev(torch, [0, rows]), rows, lse=True)
+        e2c.check()
+        at = torch.arange(200 - rows, 200, device="cuda")
+        assert torch.equal(torch.isnan(out[:, :2]).all(-1).all(-1), at >= 150) and torch.equal(torch.isnan(lse[:, 0]), at >= 150)
+        assert torch.isnan(out[at >= 170][:, 2:]).all() and not torch.isnan(lse[:, 2:]).any()
+
+
+def test_page_operations_move_scales(e2c, torch_cuda):
+    torch = torch_cuda
+    cache = tagged(e2c, torch, "int8", 3, 40, 16, 2, 64, 6, 8, 3)
+    cache.append(dev(torch, [0, 1, 2]), dev(torch, [30, 50, 10]))
+    e2c.check()
+    parent = [x.clone() for x in tokens_of(cache, 0, 30)]
+    other = [x.clone() for x in tokens_of(cache, 2, 10)]
+    cache.fork(dev(torch, [0]), dev(torch, [4]))
+    cache.append(dev(torch, [4]), dev(torch, [1]))  # copies the partly filled page
+    cache.free(dev(torch, [1]))
+    cache.compact()
+    e2c.check()
+    assert cache.table[0, 1] != cache.table[4, 1]
+    for s, want in ((0, parent), (4, parent), (2, other)):
+        for x, y in zip(tokens_of(cache, s, want[0].shape[1] if s != 2 else 10), want):
+            assert torch.equal(x, y)
+
+
+def test_refusals_of_tensors(e2c, torch_cuda):
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 2, [40, 20], [3, 2], 0, 4, 2, 64, 16, "f16")
+    good = (cache.k, cache.v, cache.table, cache.length, cache.refs)
+    for scales in ((), (cache.k_scale, None), (cache.k_scale, cache.v_scale.half()), (cache.k_scale, cache.v_scale[..., :-1]), (cache.k_scale.cpu(), cache.v_scale)):
+        with pytest.raises(e2c.E2CudaError, match="PageCache"):
+            e2c.PageCache(*good, *scales)
+    plain = make_batch(e2c, torch, 2, [40], [3], 0, 4, 2, 64, 16, "f16")[0]
+    with pytest.raises(e2c.E2CudaError, match="only there"):
+        e2c.PageCache(plain.k, plain.v, plain.table, plain.length, plain.refs, cache.k_scale, cache.v_scale)
+    with pytest.raises(e2c.E2CudaError, match="attention: q"):
+        cache.attention(0, q.float(), seqs, q_start, max_q)
+    for tree in (torch.zeros(5, 1, dtype=torch.int32), torch.zeros(4, 1, dtype=torch.int32, device="cuda"),
+                 torch.zeros(5, 1, dtype=torch.int64, device="cuda"), torch.zeros(5, 2, dtype=torch.int32, device="cuda")[:, :1]):
+        with pytest.raises(e2c.E2CudaError, match="tree"):
+            cache.attention(0, q, seqs, q_start, max_q, tree=tree)
+    with pytest.raises(e2c.E2CudaError, match="sinks"):
+        cache.attention(0, q, seqs, q_start, max_q, window=3, sinks=-1)
+    with pytest.raises(e2c.E2CudaError):
+        cache.tree(torch.zeros(5, dtype=torch.int32), seqs, q_start, max_q)
+    with pytest.raises(e2c.E2CudaError):
+        cache.keep(seqs, q_start, torch.zeros(5, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"))
+    with pytest.raises(e2c.E2CudaError):
+        cache.store(0, q, q[:, :2], q[:, :2], *e2c.rope_table(64, 64), seqs, q_start, pos=torch.zeros(5, dtype=torch.int64, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", ["int8", "bfloat16"])
+def test_drafting_steps_in_a_graph(e2c, torch_cuda, dtype):
+    """Steps of append, tree, store, attention and keep as a program runs them, captured on another stream and replayed,
+    against the same steps of a cache whose accepted tokens were all that was ever stored."""
+    torch = torch_cuda
+    rng = np.random.default_rng(7)
+    n, m, steps, H, KV, D, page = 3, 6, 5, 4, 2, 128, 16
+    cos, sin = e2c.rope_table(256, D)
+    g = torch.Generator(device="cuda").manual_seed(9)
+
+    def new():
+        cache = e2c.PageCache.new(1, 64, page, KV, D, n, 12, getattr(torch, dtype))
+        cache.append(dev(torch, range(n)), dev(torch, [21] * n))
+        return cache
+
+    text = [torch.randn(21 * n, h, D, generator=g, device="cuda").bfloat16() for h in (H, KV, KV)]
+    seqs, grow, qs = dev(torch, range(n)), dev(torch, [m] * n), dev(torch, range(0, n * m + 1, m))
+    cache, plain = new(), new()
+    for c in (cache, plain):
+        c.store(0, *text, cos, sin, seqs, dev(torch, range(0, 21 * n + 1, 21)))
+    q, k, v = (torch.zeros(n * m, h, D, device="cuda", dtype=torch.bfloat16) for h in (H, KV, KV))
+    parents, kept, counts = (torch.zeros(s, dtype=torch.int32, device="cuda") for s in (n * m, n * m, n))
+    out = torch.zeros_like(q)
+
+    def step(stream=None):
+        cache.append(seqs, grow, stream=stream)
+        tree, pos = cache.tree(parents, seqs, qs, m, stream=stream)
+        x = cache.store(0, q, k, v, cos, sin, seqs, qs, pos=pos, stream=stream)
+        cache.attention(0, x, seqs, qs, m, tree=tree, out=out, stream=stream)
+        cache.keep(seqs, qs, kept, counts, stream=stream)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph, drafts = None, []
+    for i in range(steps):
+        trees = [random_parents(rng, m) for _ in range(n)]
+        paths = []
+        for t in trees:
+            path, r = [], int(rng.integers(0, m))
+            while r >= 0:
+                path.append(r)
+                r = t[r]
+            paths.append(path[::-1])
+        with torch.cuda.stream(stream):
+            for x in (q, k, v):
+                x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+            parents.copy_(dev(torch, sum(trees, [])))
+            kept.copy_(dev(torch, sum([p + [0] * (m - len(p)) for p in paths], [])))
+            counts.copy_(dev(torch, [len(p) for p in paths]))
+            if i < 2:
+                step()
+            else:
+                if graph is None:
+                    torch.cuda.synchronize()
+                    graph = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(graph, stream=stream):
+                        step()
+                graph.replay()
+        torch.cuda.synchronize()
+        e2c.check()
+        # the accepted path as it would have been decoded: causal rows behind the same text
+        sizes = [len(p) for p in paths]
+        rows = torch.tensor([s * m + r for s in range(n) for r in paths[s]], device="cuda")
+        plain.append(seqs, dev(torch, sizes))
+        starts = dev(torch, np.concatenate([[0], np.cumsum(sizes)]))
+        x = plain.store(0, q[rows], k[rows], v[rows], cos, sin, seqs, starts)
+        want = plain.attention(0, x, seqs, starts, max(sizes))
+        e2c.check()
+        assert torch.equal(cache.length, plain.length)
+        for a, b in zip(cache.load(0, seqs, starts, len(rows)), plain.load(0, seqs, starts, len(rows))):
+            assert torch.equal(a, b)
+        # keys in another order in the sums, and other tiles: both are rounded from the same 32-bit sums within bf16's half steps
+        assert (out[rows].float() - want.float()).abs().max() <= 2.0 ** -6 * want.float().abs().max()
+    assert int((cache.refs > 0).sum()) == sum(-(-int(x) // page) for x in cache.length)
+
+
+def test_two_streams_with_workspaces_of_their_own(e2c, torch_cuda):
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 8, [900, 1000, 1100] * 20, [2] * 60, 0, 8, 4, 128, 16, "bf16")
+    big, qb, seqb, startb, maxb = make_batch(e2c, torch, 8, [3000, 2500], [300, 200], 0, 8, 2, 64, 32, "f16")
+    want = cache.attention(0, q, seqs, q_start, max_q), big.attention(0, qb, seqb, startb, maxb, window=300, sinks=5)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(10):
+        got.append((cache.attention(0, q, seqs, q_start, max_q, stream=streams[0]), big.attention(0, qb, seqb, startb, maxb, window=300, sinks=5, stream=streams[1])))
+        got.append((cache.attention(0, q, seqs, q_start, max_q, stream=streams[1]), big.attention(0, qb, seqb, startb, maxb, window=300, sinks=5, stream=streams[0])))
+    torch.cuda.synchronize()
+    e2c.check()
+    for a, b in got:
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1])
