@@ -361,7 +361,8 @@ def quantised(torch, x):
     """Codes and scales of heads, in the 32-bit arithmetic of the engine's activation quantiser."""
     amax = x.float().abs().amax(-1, keepdim=True)
     some = amax > 0
-    codes = (x.float() * torch.where(some, 127.0 / amax, 1.0)).round().to(torch.int8)
+    # one division, rounded once: torch takes 127.0 / amax as a reciprocal times 127
+    codes = (x.float() * torch.where(some, torch.full_like(amax, 127.0) / amax, 1.0)).round().to(torch.int8)
     return codes, torch.where(some, amax * float(np.float32(1 / 127)), 1.0)[..., 0]
 
 
@@ -418,7 +419,7 @@ def test_codes_tree_attention(e2c, torch_cuda, case, dtype):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("src,dtype", [("bf16", "bf16"), ("f32", "f16"), ("f16", "bf16")])
 @pytest.mark.parametrize("lens,queries,H,KV,D,page,rot,pad", [([5], [5], 1, 1, 64, 8, 64, 0), ([1, 40, 17], [1, 1, 1], 8, 2, 128, 16, 128, 8),
-                                                              ([70, 33], [70, 20], 6, 5, 256, 32, 96, 8), ([19, 64], [3, 64], 4, 2, 64, 16, 20, 3)])
+                                                              ([70, 33], [70, 20], 10, 5, 256, 32, 96, 8), ([19, 64], [3, 64], 4, 2, 64, 16, 20, 3)])
 def test_codes_store_and_load(e2c, torch_cuda, lens, queries, H, KV, D, page, rot, pad, src, dtype, interleaved):
     """Codes and scales against the 32-bit arithmetic and against 64 bits, what is read back, and all else left as it was."""
     torch = torch_cuda
