@@ -94,11 +94,6 @@ E2C_DEV void mma_16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, u
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-E2C_DEV float lg2_approx(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // the transpose of an 8 x 8 matrix of 16-bit values, a row's pair in each lane
 E2C_DEV uint32_t transpose8(uint32_t x) {
     uint32_t y;

@@ -153,8 +153,8 @@ struct Cfg {
     static constexpr int K_OFF = NQ * Q_BYTES;
     static constexpr int V_OFF = K_OFF + NKS * STAGE;
     static constexpr int KC_OFF = V_OFF + NVS * STAGE, VC_OFF = KC_OFF + NKC * KCSTAGE;
-    static constexpr int SC_OFF = VC_OFF + NVC * CSTAGE;        // [NC]: K's times c, V's, and the tile's powers
-    static constexpr int SC = 2 * TK + 4;
+    static constexpr int SC_OFF = VC_OFF + NVC * CSTAGE;        // [NC]: K's times c; V's, their log2 and they themselves
+    static constexpr int SC = 3 * TK;
     static constexpr int XM = SC_OFF + (CODE ? NC * SC * 4 : 0);  // running maxima handed on [NG][128]
     static constexpr int ML = XM + NG * TR * 4;                 // item's (m, l) [2 items][NG][128] x 2
     static constexpr int ITEMS = ML + 2 * NG * TR * 8;
@@ -664,6 +664,11 @@ E2C_DEV float ex2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+E2C_DEV float lg2_approx(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // Maxima that a NaN stays in. A row whose largest logit is NaN or +infinity has no softmax: its running maximum
 // keeps that value to the end, and the result is NaN whatever the sums became meanwhile.
@@ -740,12 +745,19 @@ __host__ __device__ constexpr uint32_t type_bits() {  // A and B formats of the 
 
 // ---- pages of 8 bits (CODES). Codes become 16-bit numbers on their way from the stages that the loads fill to those that the
 // products read, exactly (they are whole and at most 127): K's in q's type, V's in fp16. Scales stay out of the products; the
-// softmax applies them, column by column. With kc = K's scale * c and a power of two for each tile, 2^F, near its largest
-// scale of V:
-//   logit_j = (q . code_j) kc_j,   w_j = 2^(logit_j + F - m),   m the largest logit_j + F (less 2^8 at most)
-//   out = sum_j P_j code_j / l,    P_j = w_j (vs_j 2^-F) in fp16,   l = sum_j 2^(logit_j - m) = sum over tiles of 2^-F sum_j w_j
-// so that P has the size that it has without scales, whatever theirs is. A scale that is not finite makes its key, or the rows that
-// meet its value, NaN.
+// softmax applies them, column by column. With kc = K's scale * c and vs V's:
+//   logit_j = (q . code_j) kc_j,   m the largest logit_j + log2 vs_j of the keys that a row sees (less 2^8 at most)
+//   out = sum_j P_j code_j / l,    P_j = 2^(logit_j - m) vs_j in fp16,   l = sum_j 2^(logit_j - m)
+// so that P has the size that it has without scales, whatever theirs is, and a key adds what it adds whatever its neighbours
+// and the keys out of sight are. (One power of two for a tile instead, near its largest scale, saves the logarithms' reads and
+// loses every key whose scale is 2^14 below that one: a large token's neighbours, in sight of it or not.) Exponentials are held
+// times 2^kSpare, and log2 vs is at least kLeastLog2: they reach 2^(8 + 96 + 16), a tile's sum 2^127, and at vs = 2^121,
+// fp32's largest divided by 127, l still has the keys of weights down to 2^-21. A scale that is not finite makes its key, or the rows
+// that meet its value, NaN.
+constexpr float kSpare = 16.0f, kLeastLog2 = -96.0f;
+// log2 of a scale of V, and the scale as P's factor
+E2C_DEV float scale_log2(float x) { return fabsf(x) < INFINITY ? fmaxf(lg2_approx(fabsf(x)), kLeastLog2) : 0.f; }
+E2C_DEV float scale_factor(float x) { return fabsf(x) < INFINITY ? x * 0x1p-16f : NAN; }
 
 // four codes as 16-bit floats
 template <typename T>
@@ -769,12 +781,6 @@ E2C_DEV uint2 from_codes<__half>(uint32_t w) {
     const __half2 y = __hsub2(reinterpret_cast<const __half2 &>(b), reinterpret_cast<const __half2 &>(less));
     return make_uint2(reinterpret_cast<const uint32_t &>(x), reinterpret_cast<const uint32_t &>(y));
 }
-// 2^(e - 127) for 1 <= e <= 254
-E2C_DEV float power(int e) { return __uint_as_float((uint32_t)e << 23); }
-E2C_DEV uint32_t finite_bits(float x) {
-    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
-}
 // sixteen columns' numbers, in registers
 struct Columns {
     float4 x[4];
@@ -789,6 +795,14 @@ E2C_DEV void scale_logits(uint32_t (&s)[16], const Columns &k) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const float2 y = mul2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k[i]);
+        s[2 * i] = __float_as_uint(y.x), s[2 * i + 1] = __float_as_uint(y.y);
+    }
+}
+// the same with the log2 of V's scales added, f
+E2C_DEV void scale_logits(uint32_t (&s)[16], const Columns &k, const Columns &f) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float2 y = fma2(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), k[i], f[i]);
         s[2 * i] = __float_as_uint(y.x), s[2 * i + 1] = __float_as_uint(y.y);
     }
 }
@@ -855,16 +869,11 @@ E2C_DEV void convert_codes(const Args &p, uint8_t *smem, int w, int lane, Bar ba
                 const uint8_t *x = ring + st * pitch;
                 if (h == 0 && !is_v) {
                     const float *from = reinterpret_cast<const float *>(x + C::CSTAGE);
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int i = 0; i < TK; i += 32)
-                        if (i + lane < nk) top = max(top, finite_bits(from[TK + i + lane]));
-                    // the largest's exponent, from 2^-100 to 2^126: l does not leave fp32's range
-                    const int e = min(max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), 27), 253);
                     if (!wait_warp(bar(B_SCE + sb), (uint32_t)(((g / C::NC) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) return;
                     sc[tid] = tid < nk ? from[tid] * p.c : 0.f;
-                    sc[TK + tid] = tid < nk ? from[TK + tid] * power(254 - e) : 0.f;
-                    if (tid == 0) *reinterpret_cast<float2 *>(sc + 2 * TK) = make_float2((float)(e - 127), power(254 - e));
+                    const float vs = tid < nk ? from[TK + tid] : 0.f;
+                    sc[TK + tid] = scale_log2(vs);
+                    sc[2 * TK + tid] = scale_factor(vs);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(B_SCF + sb));
                 }
@@ -1422,15 +1431,10 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
 #pragma unroll
                     for (int i = 0; i < 16; i++) s[i] = seen & (1u << i) ? s[i] : 0xff800000u;
                 };
-                float shift = 0.f, lower = 1.f;  // CODES: F and 2^-F; sc: the columns' kc
                 const float *sc = reinterpret_cast<const float *>(smem + C::SC_OFF) + (g % C::NC) * C::SC;
-                if (C::CODE) {
-                    if (!wait_warp(bar(B_SCF + g % C::NC), (uint32_t)((g / C::NC) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
-                        ok = false;
-                        break;
-                    }
-                    shift = sc[2 * TK];
-                    lower = sc[2 * TK + 1];
+                if (C::CODE && !wait_warp(bar(B_SCF + g % C::NC), (uint32_t)((g / C::NC) & 1), p.status, E2C_ERR_WAIT_ATTN)) {
+                    ok = false;
+                    break;
                 }
                 float mx = -INFINITY;
                 if (busy) {
@@ -1440,9 +1444,9 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                         for (int c0 = 0; c0 < TK; c0 += 16) {  // (and below: 32 columns a step are too much code)
                             uint32_t s[16];
                             tmem_ld16(ts + c0, s);
-                            const Columns k(sc + c0);  // they arrive while the products do
+                            const Columns k(sc + c0), f(sc + TK + c0);  // they arrive while the products do
                             tmem_wait_ld();
-                            scale_logits(s, k);
+                            scale_logits(s, k, f);
 #pragma unroll
                             for (int i = 0; i < 16; i += 2) mm[i / 2 & 3] = max3(mm[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
                         }
@@ -1462,9 +1466,9 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                             uint32_t s[16];
                             tmem_ld16(ts + c0, s);
                             if constexpr (C::CODE) {
-                                const Columns k(sc + c0);
+                                const Columns k(sc + c0), f(sc + TK + c0);
                                 tmem_wait_ld();
-                                scale_logits(s, k);
+                                scale_logits(s, k, f);
                             } else {
                                 tmem_wait_ld();
                             }
@@ -1474,7 +1478,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                         }
                     }
                     mx = max2(max2(mm[0], mm[1]), max2(mm[2], mm[3]));
-                    mx = C::CODE ? mx + shift : mx * p.c;
+                    if (!C::CODE) mx *= p.c;
                 }
                 float now = before, alpha = 1.f;
                 if (live && !(mx <= before + kRescaleLog2)) {  // so also from -infinity, and for a NaN
@@ -1510,7 +1514,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                     }
                     // a row that has seen nothing yet has only -inf: any finite maximum gives it zeros
                     const float2 cc = make_float2(p.c, p.c);
-                    const float mneg = C::CODE ? (m == -INFINITY ? 0.f : shift - m) : m == -INFINITY ? 0.f : -m;
+                    const float mneg = m == -INFINITY ? 0.f : C::CODE ? kSpare - m : -m;
                     const float2 mm = make_float2(mneg, mneg);
                     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                     if (C::CODE && !masked) {
@@ -1518,7 +1522,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                         for (int c0 = 0; c0 < TK; c0 += 16) {
                             uint32_t s[16], pk[8];
                             tmem_ld16(ts + c0, s);
-                            const Columns k(sc + c0), v(sc + TK + c0);
+                            const Columns k(sc + c0), v(sc + 2 * TK + c0);
                             tmem_wait_ld();
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
@@ -1564,14 +1568,14 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                                 float2 x = C::CODE ? add2(y, mm) : fma2(y, cc, mm);
                                 x = make_float2(ex2_approx(x.x), ex2_approx(x.y));
                                 sum[i & 1] = add2(sum[i & 1], x);
-                                if constexpr (C::CODE) x = mul2(x, *reinterpret_cast<const float2 *>(sc + TK + c0 + 2 * i));
+                                if constexpr (C::CODE) x = mul2(x, *reinterpret_cast<const float2 *>(sc + 2 * TK + c0 + 2 * i));
                                 pk[i] = pack2<X>(x.x, x.y);
                             }
                             tmem_st8(ts + c0 / 2, pk);
                         }
                     }
                     const float2 all = add2(sum[0], sum[1]);
-                    l += C::CODE ? (all.x + all.y) * lower : all.x + all.y;
+                    l += C::CODE ? (all.x + all.y) * 0x1p-16f : all.x + all.y;
                     tmem_wait_st();
                 }
                 if (C::CODE) {  // the tile's scales have been read
