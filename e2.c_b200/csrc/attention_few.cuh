@@ -18,7 +18,8 @@
 // plan, and no join.
 //
 // Codes (8 bits) become fp16, exactly, in registers; scales are factors of a lane's own keys, and m is the largest
-// logit_j + log2 vs_j (less 2^8 at most), vs V's scale, so that P_j = 2^(logit_j - m) vs_j has the size that it has without scales.
+// logit_j + log2 vs_j (less 2^8 at most), vs V's scale, so that P_j = 2^(logit_j - m) vs_j has the size that it has without scales;
+// a head of zeros, held with the scale 1, counts as one of scale 0.
 // Q in bf16 is scaled by a power of two, one for an item, so that fp16 holds it: exact but for values below 2^-28 of the item's
 // largest, which lose 2^-39 of that at most.
 #pragma once
@@ -397,6 +398,23 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                 const bool fine = fabsf(x) < INFINITY;
                 lv[h] = fine ? fminf(fmaxf(lg2_approx(fabsf(x)), -100.f), 100.f) : 0.f;
                 vs[h] = fine ? x : NAN;
+            }
+            if (__any_sync(0xffffffffu, vs[0] == 1.f || vs[1] == 1.f)) {  // heads of zeros, if their codes are that
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < D / 64; i++) {  // the quad has a key's 16-byte pieces in turn
+                        const uint4 w = *reinterpret_cast<const uint4 *>(v + C::piece(oct + 8 * h, 4 * i + quad));
+                        any |= w.x | w.y | w.z | w.w;
+                    }
+                    any |= __shfl_xor_sync(0xffffffffu, any, 1);
+                    any |= __shfl_xor_sync(0xffffffffu, any, 2);
+                    if (vs[h] == 1.f && any == 0) {
+                        lv[h] = kLeastLog2;
+                        vs[h] = 0.f;
+                    }
+                }
             }
         }
         // the logits, and, as y, with the log2 of their weights' scale

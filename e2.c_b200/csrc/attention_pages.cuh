@@ -753,7 +753,7 @@ __host__ __device__ constexpr uint32_t type_bits() {  // A and B formats of the 
 // loses every key whose scale is 2^14 below that one: a large token's neighbours, in sight of it or not.) Exponentials are held
 // times 2^kSpare, and log2 vs is at least kLeastLog2: they reach 2^(8 + 96 + 16), a tile's sum 2^127, and at vs = 2^121,
 // fp32's largest divided by 127, l still has the keys of weights down to 2^-21. A scale that is not finite makes its key, or the rows
-// that meet its value, NaN.
+// that meet its value, NaN. A head of zeros is held with the scale 1, but adds nothing: as a scale of 0 it leaves m to the others.
 constexpr float kSpare = 16.0f, kLeastLog2 = -96.0f;
 // log2 of a scale of V, and the scale as P's factor
 E2C_DEV float scale_log2(float x) { return fabsf(x) < INFINITY ? fmaxf(lg2_approx(fabsf(x)), kLeastLog2) : 0.f; }
@@ -843,6 +843,23 @@ E2C_DEV void convert_stage(const uint8_t *x, uint8_t *y, int here, int upto, int
     }
 }
 
+// Whether the codes of a key's head of v, whose scale is 1, are zeros. From the pages, since scales are prepared before V's codes
+// have arrived; other heads' scales are hardly ever 1.
+template <int D>
+E2C_DEV bool zero_codes(const Args &p, const Item &it, int key) {
+    if (it.seq < 0) return false;
+    const int shift = 31 - __clz(p.pc.page), page = p.pc.table[(int64_t)it.seq * p.pc.max_blocks + (key >> shift)];
+    if ((unsigned)page >= (unsigned)p.pc.n_pages) return false;  // reported where its codes are loaded
+    const int64_t row = ((int64_t)page << shift) + (key & (p.pc.page - 1));
+    const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const int8_t *>(p.pc.v) + (row * p.pc.KV + it.kvh) * D);
+    uint32_t any = 0;
+#pragma unroll 1
+    for (int i = 0; i < D / 16 && any == 0; i += 4)
+#pragma unroll
+        for (int k = 0; k < 4; k++) any |= x[i + k].x | x[i + k].y | x[i + k].z | x[i + k].w;
+    return any == 0;
+}
+
 // Four warps for K (w < 4) and four for V: every stage's codes, of as many keys as the product takes, into the 128-byte swizzle that
 // it reads; rows past the last key become zeros. K's warps also prepare the tile's scales.
 template <typename T, int D, int KIND, typename Bar, typename Take>
@@ -871,7 +888,8 @@ E2C_DEV void convert_codes(const Args &p, uint8_t *smem, int w, int lane, Bar ba
                     const float *from = reinterpret_cast<const float *>(x + C::CSTAGE);
                     if (!wait_warp(bar(B_SCE + sb), (uint32_t)(((g / C::NC) & 1) ^ 1), p.status, E2C_ERR_WAIT_PRODUCER)) return;
                     sc[tid] = tid < nk ? from[tid] * p.c : 0.f;
-                    const float vs = tid < nk ? from[TK + tid] : 0.f;
+                    float vs = tid < nk ? from[TK + tid] : 0.f;
+                    if (vs == 1.f && zero_codes<D>(p, it, tile_key<KIND>(it, j) + tid)) vs = 0.f;
                     sc[TK + tid] = scale_log2(vs);
                     sc[2 * TK + tid] = scale_factor(vs);
                     __syncwarp();

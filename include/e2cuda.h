@@ -350,7 +350,8 @@ typedef struct e2cuda_sight {
 } e2cuda_sight;
 /* The same for q and out of q_type: the cache's type, or with pages of E2CUDA_I8 either of 16 bits. Over such pages the logits
  * are the codes' products times the key's scale, exact up to 32-bit sums; an exponential times its token's scale of v is rounded
- * to fp16, relative to the largest such product of its row, before the product with the codes. Scales are not negative. */
+ * to fp16, relative to the largest such product of its row, before the product with the codes. Scales are not negative; a head
+ * of zeros whose scale is 1, as a store leaves it, does not count among these products. */
 int e2cuda_pages_attention_sight(const e2cuda_pages *pc, int layer, int q_type, const void *q, int ldq, const int32_t *seqs,
                                  const int32_t *q_start, int n, int T, int max_q, int heads, int shared, const e2cuda_sight *sight,
                                  float scale, void *out, int ldo, float *lse, void *ws, size_t ws_bytes, void *stream);

@@ -1,6 +1,6 @@
-"""Attention over pages of 8 bits whose heads of v differ in size by many powers of two: tokens that outweigh their neighbours in and
-out of sight. On the GPU, against the 64-bit form of test_gpu_page_sight.py, in the forms for few rows, for many, and behind a
-packed prefix.
+"""Attention over pages of 8 bits whose heads of v differ in size by many powers of two: heads of zeros, tokens that outweigh
+their neighbours in and out of sight. On the GPU, against the 64-bit form of test_gpu_page_sight.py, in the forms for few rows,
+for many, and behind a packed prefix.
 
 A row's tolerance comes from what it sees alone (u: unit roundoff of q's type; p: its 64-bit weights; s: scales of v):
   result      u |out|, and in fp16 2^-25 for a subnormal
@@ -90,6 +90,12 @@ def some_heads(torch, cache, g, part):
     return torch.rand(cache.v_scale.shape, generator=g, device="cuda") < part
 
 
+def zero_heads(torch, cache, heads):
+    """As a store leaves heads of zeros."""
+    cache.v.masked_fill_(heads.transpose(-1, -2)[..., None], 0)
+    cache.v_scale.masked_fill_(heads, 1.0)
+
+
 def outliers(torch, cache, g, low, high, part=0.01):
     heads = some_heads(torch, cache, g, part)
     up = torch.exp2(low + (high - low) * torch.rand(cache.v_scale.shape, generator=g, device="cuda"))
@@ -109,6 +115,9 @@ def light_outliers(torch, cache, g, q):
 
 SPREADS = {
     "wide": lambda t, c, g, q: random_scales(t, c, g, -10, 10),
+    "zeros": lambda t, c, g, q: (random_scales(t, c, g, -9, -8), zero_heads(t, c, some_heads(t, c, g, 0.1))),
+    "zeros among tiny ones": lambda t, c, g, q: (random_scales(t, c, g, -26, -25), zero_heads(t, c, some_heads(t, c, g, 0.02))),
+    "ones": lambda t, c, g, q: c.v_scale.masked_fill_(~t.isnan(c.v_scale), 1.0),  # of heads that are not zeros
     "outliers": lambda t, c, g, q: outliers(t, c, g, 20, 60),
     "light outliers": lambda t, c, g, q: light_outliers(t, c, g, q),
 }
@@ -130,14 +139,19 @@ def test_scales_of_many_sizes(e2c, torch_cuda, spread, case, causal, window, sin
 
 
 @pytest.mark.parametrize("rows,H,KV,D", [(4, 8, 2, 128), (9, 8, 2, 128), (40, 4, 2, 64), (30, 2, 1, 256), (3, 2, 2, 64)])
-def test_scales_of_many_sizes_in_trees(e2c, torch_cuda, rows, H, KV, D):
-    """Large tokens on other branches."""
+@pytest.mark.parametrize("spread", ["zeros", "outliers"])
+def test_scales_of_many_sizes_in_trees(e2c, torch_cuda, spread, rows, H, KV, D):
+    """Large tokens on other branches, and zeros."""
     torch = torch_cuda
     rng = np.random.default_rng(rows)
     lens = [rows + x for x in (0, 70, 1000)]
     cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 32, lens, [rows] * 3, 0, H, KV, D, 16, "f16", spread=0.3)
     g = torch.Generator(device="cuda").manual_seed(rows)
-    outliers(torch, cache, g, 5, 8, 0.1)
+    if spread == "zeros":
+        random_scales(torch, cache, g, -6, -5)  # fp16's result keeps its bits
+        zero_heads(torch, cache, some_heads(torch, cache, g, 0.2))
+    else:
+        outliers(torch, cache, g, 5, 8, 0.1)
     parents = [random_parents(rng, rows) for _ in lens]
     tree, _ = cache.tree(dev(torch, sum(parents, [])), seqs, q_start, max_q)
     got = cache.attention(0, q, seqs, q_start, max_q, tree=tree, lse=True)
@@ -156,3 +170,25 @@ def test_a_large_token_out_of_sight_changes_nothing(e2c, torch_cuda, rows):
     e2c.check()
     assert torch.equal(now[:-1], was[:-1]) and torch.equal(lse[:-1], lse0[:-1])
     assert not torch.equal(now[-1], was[-1])
+
+
+@pytest.mark.parametrize("rows", [1, 64])
+def test_stored_zeros_beside_small_values(e2c, torch_cuda, rows):
+    """From the store on: a first token whose value is zero and which draws half of the weight."""
+    torch = torch_cuda
+    H, KV, D, L = 4, 2, 128, 700
+    cache = e2c.PageCache.new(1, 50, 16, KV, D, 1, 50, torch.int8)
+    seqs = dev(torch, [0])
+    cache.append(seqs, dev(torch, [L]))
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    q, k, v = (torch.randn(L, h, D, generator=g, device="cuda") for h in (H, KV, KV))
+    v *= 1e-3
+    q[..., 0], k[..., 0], k[0], v[0] = 8.0, 0.0, 0.0, 0.0
+    k[0, :, 0] = 11.0
+    ones, none = torch.ones(L, 1, device="cuda"), torch.zeros(L, 1, device="cuda")  # no rotation
+    x = cache.store(0, q.bfloat16(), k.bfloat16(), v.bfloat16(), ones, none, seqs, dev(torch, [0, L]))
+    assert (cache.v_scale[0, cache.table[0, 0].long(), :, 0] == 1).all()
+    x, starts = x[L - rows:].contiguous(), dev(torch, [0, rows])
+    got = cache.attention(0, x, seqs, starts, rows, lse=True)
+    e2c.check()
+    assert_scaled(torch, cache, got, x, seqs, starts, True, -1, D ** -0.5, "bf16")
