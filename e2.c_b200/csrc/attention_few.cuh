@@ -19,7 +19,7 @@
 //
 // Codes (8 bits) become fp16, exactly, in registers; scales are factors of a lane's own keys, and m is the largest
 // logit_j + log2 vs_j (less 2^8 at most), vs V's scale, so that P_j = 2^(logit_j - m) vs_j has the size that it has without scales;
-// a head of zeros, held with the scale 1, counts as one of scale 0.
+// a head of zeros, held with the scale 1, counts as one of scale 0. Exponentials are held as those of the tiles are (kSpare).
 // Q in bf16 is scaled by a power of two, one for an item, so that fp16 holds it: exact but for values below 2^-28 of the item's
 // largest, which lose 2^-39 of that at most.
 #pragma once
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
     float2 *ml = reinterpret_cast<float2 *>(smem + C::ML);
     uint32_t qf[D / 16][NT][2];
     float o[D / 16][NT][4];
-    float m[NT][2], l[NT][2], less[NT][2];  // less: -m, or 0 for a row that has only seen -infinity
+    float m[NT][2], l[NT][2], less[NT][2];  // less: -m (CODE: + kSpare), or 0 for a row that has only seen -infinity
     int4 *seen = reinterpret_cast<int4 *>(smem + C::SEEN) + warp * C::ROWS;
     int all_lo = 0, all_hi = 0;             // keys that every row sees
     float cu;                               // what a product times its key's scale is multiplied by
@@ -394,12 +394,11 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 kc[h] = sc[8 * h] * cu;
-                const float x = sc[C::KEYS + 8 * h];
-                const bool fine = fabsf(x) < INFINITY;
-                lv[h] = fine ? fminf(fmaxf(lg2_approx(fabsf(x)), -100.f), 100.f) : 0.f;
-                vs[h] = fine ? x : NAN;
+                lv[h] = scale_log2(sc[C::KEYS + 8 * h]);
+                vs[h] = scale_factor(sc[C::KEYS + 8 * h]);
             }
-            if (__any_sync(0xffffffffu, vs[0] == 1.f || vs[1] == 1.f)) {  // heads of zeros, if their codes are that
+            constexpr float ONE = 0x1p-16f;  // scale_factor(1)
+            if (__any_sync(0xffffffffu, vs[0] == ONE || vs[1] == ONE)) {  // heads of zeros, if their codes are that
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t any = 0;
@@ -410,7 +409,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                     }
                     any |= __shfl_xor_sync(0xffffffffu, any, 1);
                     any |= __shfl_xor_sync(0xffffffffu, any, 2);
-                    if (vs[h] == 1.f && any == 0) {
+                    if (vs[h] == ONE && any == 0) {
                         lv[h] = kLeastLog2;
                         vs[h] = 0.f;
                     }
@@ -476,9 +475,9 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                     x = max2(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     if (x <= m[nt][i] + kRescaleLog2) continue;
                     const float now = max2(m[nt][i], x), alpha = ex2_approx(m[nt][i] - now);
+                    l[nt][i] = CODE ? times_exp2(l[nt][i], m[nt][i] - now) : l[nt][i] * alpha;
                     m[nt][i] = now;
-                    less[nt][i] = now == -INFINITY ? 0.f : -now;
-                    l[nt][i] *= alpha;
+                    less[nt][i] = now == -INFINITY ? 0.f : CODE ? kSpare - now : -now;
 #pragma unroll
                     for (int d = 0; d < D / 16; d++) o[d][nt][i] *= alpha, o[d][nt][2 + i] *= alpha;
                 }
@@ -491,7 +490,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const float x = ex2_approx(s[nt][2 * h + i] + less[nt][i]);
-                    l[nt][i] += x;
+                    l[nt][i] = CODE ? fmaf(x, 0x1p-16f, l[nt][i]) : l[nt][i] + x;
                     s[nt][2 * h + i] = CODE ? x * vs[h] : x;
                 }
             }
@@ -571,8 +570,8 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                     const float top = max2(m[nt][i], x.x), ref = top == -INFINITY ? 0.f : top;
                     f[nt][i] = ex2_approx(m[nt][i] - ref);
                     g[nt][i] = ex2_approx(x.x - ref);
+                    l[nt][i] = CODE ? times_exp2(l[nt][i], m[nt][i] - ref) + times_exp2(x.y, x.x - ref) : l[nt][i] * f[nt][i] + x.y * g[nt][i];
                     m[nt][i] = top;
-                    l[nt][i] = l[nt][i] * f[nt][i] + x.y * g[nt][i];
                 }
 #pragma unroll
             for (int i = 0; i < D / 16; i++)

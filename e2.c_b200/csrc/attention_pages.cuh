@@ -758,6 +758,11 @@ constexpr float kSpare = 16.0f, kLeastLog2 = -96.0f;
 // log2 of a scale of V, and the scale as P's factor
 E2C_DEV float scale_log2(float x) { return fabsf(x) < INFINITY ? fmaxf(lg2_approx(fabsf(x)), kLeastLog2) : 0.f; }
 E2C_DEV float scale_factor(float x) { return fabsf(x) < INFINITY ? x * 0x1p-16f : NAN; }
+// l 2^x by halves: m moves with the scales, by more than one factor can have, and l holds as much more or less
+E2C_DEV float times_exp2(float l, float x) {
+    const float half = ex2_approx(0.5f * x);
+    return l * half * half;
+}
 
 // four codes as 16-bit floats
 template <typename T>
@@ -1508,7 +1513,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                 if (lane == 0) mbar_arrive(bar(B_MX + group * 4 + quad));
                 if (busy) {
                     if (now != m) {
-                        l *= ex2_approx(m - now);
+                        l = C::CODE ? times_exp2(l, m - now) : l * ex2_approx(m - now);
                         m = now;
                     }
                     if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
@@ -1658,7 +1663,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
             for (int i = 1; i < C::NG; i++) m = max2(m, a[i].x);
             const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-            for (int i = 0; i < C::NG; i++) l += a[i].y * ex2_approx(a[i].x - ref);
+            for (int i = 0; i < C::NG; i++) l += C::CODE ? times_exp2(a[i].y, a[i].x - ref) : a[i].y * ex2_approx(a[i].x - ref);
             const bool live = tok < it.ntok, bad = no_softmax(m), some = bad || l > 0.f;
             const float inv = bad ? NAN : some ? __fdividef(1.0f, l) : 0.f;
             float none = 0.f;  // the result of a row with l = 0; a part leaves that to the join

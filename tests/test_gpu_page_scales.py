@@ -1,6 +1,6 @@
 """Attention over pages of 8 bits whose heads of v differ in size by many powers of two: heads of zeros, tokens that outweigh
-their neighbours in and out of sight. On the GPU, against the 64-bit form of test_gpu_page_sight.py, in the forms for few rows,
-for many, and behind a packed prefix.
+their neighbours in and out of sight, the largest and the smallest scales that a store leaves. On the GPU, against the 64-bit form
+of test_gpu_page_sight.py, in the forms for few rows, for many, and behind a packed prefix.
 
 A row's tolerance comes from what it sees alone (u: unit roundoff of q's type; p: its 64-bit weights; s: scales of v):
   result      u |out|, and in fp16 2^-25 for a subnormal
@@ -192,3 +192,35 @@ def test_stored_zeros_beside_small_values(e2c, torch_cuda, rows):
     got = cache.attention(0, x, seqs, starts, rows, lse=True)
     e2c.check()
     assert_scaled(torch, cache, got, x, seqs, starts, True, -1, D ** -0.5, "bf16")
+
+
+@pytest.mark.parametrize("low,high,part", [(100, 118, 1.0), (116, 118, 0.02), (-104, -100, 1.0), (-104, -90, 1.0), (-100, 100, 1.0)])
+@pytest.mark.parametrize("rows,H,KV,D", [(1, 8, 2, 128), (16, 1, 1, 64), (3, 8, 4, 256), (60, 4, 2, 64), (100, 2, 1, 256), (33, 4, 1, 128)])
+def test_largest_and_smallest_scales(e2c, torch_cuda, low, high, part, rows, H, KV, D):
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 34, [300, 45], [rows, min(rows, 45)], 0, H, KV, D, 16, "bf16", spread=0.0)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    cache.v_scale.mul_(32)  # about 1: a head's largest of D normal values is 2.5 to 3
+    if part == 1.0:
+        random_scales(torch, cache, g, low, high)
+    else:
+        outliers(torch, cache, g, low, high, part)
+    got = cache.attention(0, q, seqs, q_start, max_q, lse=True)
+    e2c.check()
+    assert_scaled(torch, cache, got, q, seqs, q_start, True, -1, D ** -0.5, "bf16")
+
+
+@pytest.mark.parametrize("rows,H,KV,D", [(1, 8, 2, 128), (2, 8, 1, 64), (3, 8, 4, 256), (60, 4, 2, 64), (100, 2, 1, 256), (33, 4, 1, 128)])
+@pytest.mark.parametrize("up", [False, True])
+def test_scales_in_steps(e2c, torch_cuda, up, rows, H, KV, D):
+    """Runs of tokens whose values are 2^180 times the others': the weights of the small ones count all the same."""
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 35, [900], [rows], 0, H, KV, D, 16, "bf16", spread=0.0)
+    t = torch.arange(900, device="cuda")
+    at = torch.where((t // 150 % 2 == 1) == up, 90.0, -90.0)
+    pages = cache.table[0, :57].long()
+    size = torch.exp2(torch.nn.functional.pad(at, (0, 912 - 900))).view(57, 1, 16)
+    cache.v_scale[0, pages] *= size
+    got = cache.attention(0, q, seqs, q_start, max_q, lse=True)
+    e2c.check()
+    assert_scaled(torch, cache, got, q, seqs, q_start, True, -1, D ** -0.5, "bf16")
