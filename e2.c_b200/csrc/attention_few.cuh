@@ -20,7 +20,7 @@
 // Codes (8 bits) become fp16, exactly, in registers; scales are factors of a lane's own keys, and m is the largest
 // logit_j + log2 vs_j (less 2^8 at most), vs V's scale, so that P_j = 2^(logit_j - m) vs_j has the size that it has without scales;
 // a head of zeros, held with the scale 1, counts as one of scale 0. Exponentials are held as those of the tiles are (kSpare).
-// Q in bf16 is scaled by a power of two, one for an item, so that fp16 holds it: exact but for values below 2^-28 of the item's
+// Q in bf16 is scaled by a power of two, one for a row, so that fp16 holds it: exact but for values below 2^-28 of the row's
 // largest, which lose 2^-39 of that at most.
 #pragma once
 #include "attention_pages.cuh"
@@ -285,7 +285,9 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
     float m[NT][2], l[NT][2], less[NT][2];  // less: -m (CODE: + kSpare), or 0 for a row that has only seen -infinity
     int4 *seen = reinterpret_cast<int4 *>(smem + C::SEEN) + warp * C::ROWS;
     int all_lo = 0, all_hi = 0;             // keys that every row sees
-    float cu;                               // what a product times its key's scale is multiplied by
+    constexpr bool TURNED = CODE && !std::is_same<T, __half>::value;  // Q becomes fp16 too, times a power of two for each row
+    const float c = p.neg ? -p.c : p.c;
+    float up[NT][2];                        // TURNED: back from that
     auto begin = [&](const Item &it) {
         const int rows = it.ntok * p.G;
         // Q: a lane's 16 (8 bits) or 8 neighbouring dimensions of each 64 or 32, of row `oct`
@@ -301,27 +303,27 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                 for (int k = 0; k < PER / 8; k++)
                     w[nt][j * (PER / 8) + k] = row < rows ? *reinterpret_cast<const uint4 *>(q + j * 4 * PER + quad * PER + k * 8) : make_uint4(0, 0, 0, 0);
         }
-        float up = 1.f;
-        if constexpr (CODE && !std::is_same<T, __half>::value) {
-            uint32_t top = 0;  // the largest finite magnitude
+        if constexpr (TURNED) {
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++) {
+                uint32_t top = 0;  // the row's largest finite magnitude
 #pragma unroll
                 for (int k = 0; k < D / 8; k++) {
                     const uint32_t b = reinterpret_cast<const uint32_t *>(w[nt])[k], b0 = b << 16 & 0x7fffffffu, b1 = b & 0x7fff0000u;
                     top = max(top, max(b0 < 0x7f800000u ? b0 : 0u, b1 < 0x7f800000u ? b1 : 0u));
                 }
-            top = __reduce_max_sync(0xffffffffu, top);
-            const uint32_t ex = max(top >> 23, 15u);  // its exponent becomes 14
-            const float scale = __uint_as_float((268u - ex) << 23);
-            up = __uint_as_float((ex - 14u) << 23);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const uint32_t ex = max(top >> 23, 15u);  // its exponent becomes 14
+                const float scale = __uint_as_float((268u - ex) << 23);
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
+                for (int i = 0; i < 2; i++) up[nt][i] = __uint_as_float((__shfl_sync(0xffffffffu, ex, 4 * (2 * quad + i)) - 14u) << 23);
 #pragma unroll
                 for (int k = 0; k < D / 8; k++) {
                     const float2 f = __bfloat1622float2(reinterpret_cast<const __nv_bfloat162 *>(w[nt])[k]);
                     reinterpret_cast<uint32_t *>(w[nt])[k] = pack2<__half>(f.x * scale, f.y * scale);
                 }
+            }
         }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -330,7 +332,6 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                 qf[k][nt][0] = reinterpret_cast<const uint32_t *>(w[nt])[2 * k];
                 qf[k][nt][1] = reinterpret_cast<const uint32_t *>(w[nt])[2 * k + 1];
             }
-        cu = (p.neg ? -p.c : p.c) * up;
         int lo = 0, hi = it.klim;
         if (lane < rows) {
             const int tok = lane / p.G;
@@ -388,12 +389,12 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
             }
         }
         // s[nt][2 h + i]: key oct + 8 h, row 8 nt + 2 quad + i
-        float lv[2] = {0.f, 0.f}, vs[2] = {1.f, 1.f}, kc[2] = {cu, cu};
+        float lv[2] = {0.f, 0.f}, vs[2] = {1.f, 1.f}, kc[2] = {c, c};
         if constexpr (CODE) {
             const float *sc = reinterpret_cast<const float *>(smem + C::SCALES) + st * (2 * C::KEYS) + r0 + oct;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                kc[h] = sc[8 * h] * cu;
+                kc[h] = sc[8 * h] * c;
                 lv[h] = scale_log2(sc[C::KEYS + 8 * h]);
                 vs[h] = scale_factor(sc[C::KEYS + 8 * h]);
             }
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                s[nt][e] = (s[nt][e] + s2[nt][e]) * kc[e >> 1];
+                s[nt][e] = (s[nt][e] + s2[nt][e]) * (TURNED ? kc[e >> 1] * up[nt][e & 1] : kc[e >> 1]);
                 y[nt][e] = CODE ? s[nt][e] + lv[e >> 1] : s[nt][e];
             }
         if (kk < all_lo || kk + 16 > min(end, all_hi)) {  // some row does not see some of them

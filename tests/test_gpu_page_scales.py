@@ -224,3 +224,20 @@ def test_scales_in_steps(e2c, torch_cuda, up, rows, H, KV, D):
     got = cache.attention(0, q, seqs, q_start, max_q, lse=True)
     e2c.check()
     assert_scaled(torch, cache, got, q, seqs, q_start, True, -1, D ** -0.5, "bf16")
+
+
+@pytest.mark.parametrize("rows,H,KV,D", [(1, 8, 1, 128), (2, 16, 2, 64), (3, 10, 2, 256), (40, 4, 2, 128)])
+@pytest.mark.parametrize("by", [2.0 ** 60, 1e38, 2.0 ** -60])
+def test_a_query_of_another_size_changes_no_other(e2c, torch_cuda, by, rows, H, KV, D):
+    """Rows of one product, whose queries are heads of very different sizes."""
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_codes(e2c, torch, 36, [500, 70], [rows] * 2, 0, H, KV, D, 16, "bf16", spread=0.3)
+    was, lse0 = cache.attention(0, q, seqs, q_start, max_q, lse=True)
+    odd = q.clone()
+    odd[rows - 1, 1] *= by
+    now, lse = cache.attention(0, odd, seqs, q_start, max_q, lse=True)
+    e2c.check()
+    same = torch.ones(2 * rows, H, dtype=torch.bool, device="cuda")
+    same[rows - 1, 1] = False
+    assert torch.equal(now[same], was[same]) and torch.equal(lse[same], lse0[same])
+    assert not torch.equal(now[~same], was[~same])
