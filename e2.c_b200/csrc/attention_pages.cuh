@@ -130,6 +130,9 @@ struct Cfg {
     static constexpr int W_EPI = 4 * NG, W_ITEMS = W_EPI + 4, W_MMA = W_ITEMS + 1, W_K = W_MMA + 1, W_V = W_K + 1;
     static constexpr int W_CONVERT = W_V + 1;  // CODES: four warps for K, then four for V
     static constexpr int WARPS = W_CONVERT + (CODE ? 8 : 0), NTHREADS = 32 * WARPS;
+    // CODES: registers of a thread by role, and of the block
+    static constexpr int R_SOFTMAX = 104, R_OTHERS = 72, R_CONVERT = 64;
+    static constexpr int REGISTERS = 32 * (W_EPI * R_SOFTMAX + (W_CONVERT - W_EPI) * R_OTHERS + (WARPS - W_CONVERT) * R_CONVERT);
     static constexpr int PANELS = D / 64;  // 64 of the head's dimensions each, 128 bytes a row
     static constexpr int NQ = D == 64 ? 2 : 1;  // Q buffers
     // K and V have a ring of stages each: of a tile, or for D = 256 of half a one (K: half of the
@@ -1014,13 +1017,13 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
 
     // CODES: 768 threads begin with 80 registers each; the softmax's take of the others': (2 * 104 + 72 + 72 + 2 * 64) / 6 = 80
     if constexpr (C::CODE) {
-        static_assert(C::NTHREADS == 768 && C::W_EPI == 8, "shares of registers");
+        static_assert(C::REGISTERS == 768 * 80 && C::NTHREADS == 768, "shares of registers");
         if (warp < C::W_EPI)
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::R_SOFTMAX));
         else if (warp < C::W_CONVERT)
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_OTHERS));
         else
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::R_CONVERT));
     }
     if (C::CODE && warp >= C::W_CONVERT) {
         convert_codes<T, D, KIND>(p, smem, warp - C::W_CONVERT, lane, bar, take);
@@ -1852,6 +1855,15 @@ int run(const Args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStr
             cudaGetLastError();
             e2c_set_msg("pages_attention: cannot reserve %d bytes of shared memory", smem_bytes<D, KIND>());
             return -2;
+        }
+        if constexpr (C::CODE) {  // fewer than the roles' shares add up to: the softmax would wait for registers for good
+            cudaFuncAttributes has = {};
+            if (cudaFuncGetAttributes(&has, k_attention_pages<T, D, KIND>) != cudaSuccess || has.numRegs * C::NTHREADS < C::REGISTERS) {
+                cudaGetLastError();
+                e2c_set_msg("pages_attention: the kernel for pages of 8 bits was built with %d registers a thread, and needs %d", has.numRegs,
+                            C::REGISTERS / C::NTHREADS);
+                return -2;
+            }
         }
         attr.set(dev, 1);
     }
