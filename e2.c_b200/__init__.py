@@ -597,10 +597,10 @@ class PageCache:
 
     def tree(self, parents, seqs, q_start, max_q: int, stream=None):
         """The rows' trees, for attention and store: parents [T] int32 (each row's parent among its entry's rows, before it; -1: the text)
-        -> (tree [T][(max_q + 31) / 32] int32, pos [T] int32): the bits of each row's ancestors and its own, and its rotary position."""
+        -> (tree [T][(min(max_q, T) + 31) / 32] int32, pos [T] int32): the bits of each row's ancestors and its own, and its rotary position."""
         here = self._here()
         torch, T, n = _torch_mod, parents.shape[0], seqs.shape[0]
-        words = max(1, (max_q + 31) // 32)
+        words = max(1, (min(max_q, T) + 31) // 32)
         tree, pos = _result(stream, lambda: (torch.empty((T, words), dtype=torch.int32, device=self.k.device),
                                              torch.empty(T, dtype=torch.int32, device=self.k.device)))
         _ok(lib().e2cuda_pages_tree(self._p, _ints(parents, T, "tree parents", here), _ints(seqs, n, "tree seqs", here),
@@ -638,7 +638,7 @@ class PageCache:
         st = _stream(stream, here)
         max_q = min(max_q, T)  # a bound kept for batches of any size
         window = max(-1, min(window, INT_MAX))  # none, or wider than any sequence
-        sight = Sight(causal, window, min(sinks, INT_MAX), 0, None)
+        sight = Sight(causal, window, max(-1, min(sinks, INT_MAX)), 0, None)
         if tree is not None:
             if tree.get_device() != here:
                 raise _elsewhere(tree, "attention tree", here)

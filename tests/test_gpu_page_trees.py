@@ -75,3 +75,19 @@ def test_rows_without_bits(e2c, torch_cuda, n, held):
         out, lse = cache.attention(0, q, seqs, q_start, max_q, tree=tree, lse=True)
         e2c.check()
         assert torch.isnan(out[~none]).all() and (out[none] == 0).all() and (lse == -float("inf")).all()
+
+
+def test_bounds_of_any_size(e2c, torch_cuda):
+    """A bound on an entry's rows may be one kept for all batches; a number of sinks below zero is refused, however far."""
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 18, [50, 40], [3, 2], 0, 4, 2, 64, 16, "f16")
+    parents = dev(torch, [-1, 0, 0, -1, -1])
+    want, pos = cache.tree(parents, seqs, q_start, max_q)
+    tree, at = cache.tree(parents, seqs, q_start, 2 ** 31 - 1)
+    assert torch.equal(tree, want) and torch.equal(at, pos)
+    out = cache.attention(0, q, seqs, q_start, 2 ** 31 - 1, tree=tree)
+    assert torch.equal(out, cache.attention(0, q, seqs, q_start, max_q, tree=want))
+    e2c.check()
+    for sinks in (-1, -2 ** 31 - 5, -2 ** 32):
+        with pytest.raises(e2c.E2CudaError, match="sinks"):
+            cache.attention(0, q, seqs, q_start, max_q, window=3, sinks=sinks)
