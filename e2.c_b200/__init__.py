@@ -642,8 +642,8 @@ class PageCache:
         if tree is not None:
             if tree.get_device() != here:
                 raise _elsewhere(tree, "attention tree", here)
-            if tree.dtype is not _torch_mod.int32 or tree.dim() != 2 or tree.shape[0] != T or not tree.is_contiguous():
-                raise E2CudaError(f"attention: a contiguous int32 tree of {T} rows, got {tree.dtype} {tuple(tree.shape)}")
+            if tree.dtype is not _torch_mod.int32 or tree.dim() != 2 or tree.shape[0] != T or tree.shape[1] < 1 or not tree.is_contiguous():
+                raise E2CudaError(f"attention: a contiguous int32 tree of {T} rows of words, got {tree.dtype} {tuple(tree.shape)}")
             sight.words, sight.tree = tree.shape[1], tree.data_ptr()
         batch = (n, T, max_q, H, shared)
         need = self._needs.get(batch)

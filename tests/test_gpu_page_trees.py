@@ -91,3 +91,11 @@ def test_bounds_of_any_size(e2c, torch_cuda):
     for sinks in (-1, -2 ** 31 - 5, -2 ** 32):
         with pytest.raises(e2c.E2CudaError, match="sinks"):
             cache.attention(0, q, seqs, q_start, max_q, window=3, sinks=sinks)
+
+
+def test_a_tree_without_words_is_refused(e2c, torch_cuda):
+    """An empty tensor has no address, and is not taken for no tree."""
+    torch = torch_cuda
+    cache, q, seqs, q_start, max_q = make_batch(e2c, torch, 19, [50, 40], [3, 2], 0, 4, 2, 64, 16, "f16")
+    with pytest.raises(e2c.E2CudaError, match="tree of 5 rows of words"):
+        cache.attention(0, q, seqs, q_start, max_q, tree=torch.zeros(5, 0, dtype=torch.int32, device="cuda"))
