@@ -8,7 +8,8 @@
 //   S' = K Q'      16 keys x 8 rows, fp32
 //   P' = 2^(S' - m) in 16 bits, transposed in registers (movmatrix) into the second product's operand
 //   O' += V' P'    head dim x 8 rows, fp32
-// One more warp walks the block's share of items (those of attention_pages.cuh, as are the joins) and loads their keys by TMA, 16 for
+// P is rounded to the operands' type, as in the tiles' kernel (the error that it adds is given there), so that a row comes out as
+// exact in either. One more warp walks the block's share of items (those of attention_pages.cuh, as are the joins) and loads their keys by TMA, 16 for
 // each warp at once, a lane for each page; at an item's end the warps' sums are added up pair by pair, in a fixed order. Head
 // dimensions are contracted in the order in which 16-byte loads from shared memory hold them.
 //
@@ -549,8 +550,8 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 l[nt][i] = x;
             }
-        // (a loop, not its steps one after the other: this code runs once an item, and for short ones fetching it is
-        // what it takes)
+        // (a loop, not its steps one after the other: this code runs once an item, and the small calls wait for
+        // instructions a seventh of their time as it is)
         auto slot = [&](int w) { return reinterpret_cast<float4 *>(smem + C::MERGE + (C::GIVES >> 4 * w & 15) * C::SLOT_BYTES) + lane; };
         auto slot_rows = [&](int w) { return ml + (C::GIVES >> 4 * w & 15) * C::ROWS + 2 * quad; };
 #pragma unroll 1
@@ -690,9 +691,13 @@ __global__ void __launch_bounds__(32 * (Few<CODE, D, NT>::WARPS + 1), Few<CODE, 
     }
 }
 
-// Items of which a block can take one each, and the keys of which are few enough that reading them takes no longer than a join of
-// their parts would
-constexpr int WHOLE_BYTES = 256 << 10;
+// Calls with an item a block at most, and so few keys an item that reading them takes one block no longer than the plan and the join of
+// divided items take. One token an entry, us whole and divided: 4 sequences of 300, 500, 700 and 1000 tokens (256 bytes of a key
+// and value; 77, 128, 179 and 256 KB), 8-bit heads of 128 over 4, in a graph 9.8, 12.0, 14.5 and 18.2, divided 12.0, 12.9, 12.9 and 13.9, and
+// through Python, which saves a launch, 14.7, -, 14.9 and 18.7, divided 16.7; 30 sequences of 500 and 1000 in a graph 13.5 and 20.7, divided 15.1 and
+// 19.3; 3 sequences, 16-bit heads of 256 over 2, windows of 100, 200 and 400 (1 KB a key) 7.9, 10.2 and 14.2, divided 10.9, 11.4 and 11.7. So it turns at 140 KB
+// (few items, in a graph) to 250 KB (many, or without one).
+constexpr int WHOLE_BYTES = 192 << 10;
 template <typename T, bool CODE, int D, int NT>
 int run_few(Args a, const void *q, int64_t ldq, int sms, cudaStream_t st) {
     using C = Few<CODE, D, NT>;
@@ -707,10 +712,11 @@ int run_few(Args a, const void *q, int64_t ldq, int sms, cudaStream_t st) {
         }
         attr.set(dev, 1);
     }
-    // the most keys that an item can have: the table's, or those of a window on both sides of its rows and the sinks
+    // a bound on an item's keys, whose lengths are on the device: the table's (a short text in a wide table counts as a long one), or
+    // those of a window before its rows, and behind them where they see that side, and the sinks
     int64_t keys = (int64_t)a.pc.max_blocks * a.pc.page;
     if (a.window >= 0) {
-        const int64_t seen = 2 * (int64_t)a.window + 1 + a.max_q + a.sinks + 2 * a.align;
+        const int64_t seen = (a.causal || a.tree ? 1 : 2) * (int64_t)a.window + 1 + a.max_q + a.sinks + 2 * a.align;
         keys = keys < seen ? keys : seen;
     }
     int grid = sms * C::CTAS;
