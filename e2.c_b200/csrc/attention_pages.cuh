@@ -85,7 +85,11 @@ int e2c_attn_plain(const e2c_attn_args &a, const void *q, int64_t ldq, bool pref
 int e2c_attn_sight(const e2c_attn_args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st);
 // The same over pages of 8 bits, with SIGHT.
 int e2c_attn_codes(const e2c_attn_args &a, const void *q, int64_t ldq, bool prefix, int sms, cudaStream_t st);
-// The same over pages of 16 and of 8 bits, for entries of at most FEW_ROWS rows (tokens by the heads of a key head), without a prefix.
+// The same over pages of 16 and of 8 bits, for entries of at most FEW_ROWS rows (tokens by the heads of a key head), without a prefix:
+// two N tiles, beyond which O alone is 32 registers more a tile (heads of 128). us a call with 9 to 16 rows, here and by tiles of 128 rows: 8 bits,
+// 64 sequences of 5461 to 8192 tokens, heads of 64 291 and 345, of 128 236 and 363, of 256 243 and 367, 4 of 700 15.9 and 17.6; 16 bits,
+// 128 windows of 2047 and sinks, heads of 64 131 and 141, of 128 194 and 190, of 256 192 and 188, 40 windows of 300 30.6 and 29.0, 3 of 511 15.0 and
+// 16.4, 4 trees behind 300 tokens 12.9 and 15.5.
 constexpr int FEW_ROWS = 16;
 int e2c_attn_few(const e2c_attn_args &a, const void *q, int64_t ldq, int sms, cudaStream_t st);
 int e2c_attn_few_codes(const e2c_attn_args &a, const void *q, int64_t ldq, int sms, cudaStream_t st);
@@ -287,19 +291,19 @@ E2C_DEV Entry entry_of(const Args &p, int i, bool report) {
     return e;
 }
 
-// A run of key tiles: nt of them from k0 on, keys before klim; gap keys are skipped after the first ns.
-// a window's first tile begins at a multiple of it (past the prefix): of what one load brings, at least
+// A window's first tile begins at a multiple of it (past the prefix): of what one load brings, at least
 template <int KIND>
 E2C_DEV int aligned(const Args &p, int x) {
     return KIND & FEW ? x & -p.align : x / TK * TK;
 }
-// The block's share and key head among `hs` blocks that have the same share of the entries' tiles, and those blocks' number
+// the blocks side by side that have the same share of the entries' tiles, for a key head each
 template <int KIND>
 E2C_DEV int hs_of(const Args &p) {
     return KIND & FEW ? p.hs : 1;
 }
 template <int KIND>
 constexpr int SLOT = KIND & FEW ? FEW_ROWS : TR;  // rows of a part in the workspace
+// A run of key tiles: nt of them from k0 on, keys before klim; gap keys are skipped after the first ns.
 struct Span {
     int nt, k0, klim, ns, gap;
     // the part of nt tiles from tile off on, in an item's fields
@@ -819,8 +823,8 @@ E2C_DEV void scale_logits(uint32_t (&s)[16], const Columns &k, const Columns &f)
 // take four pieces of 16 codes of row r and of row r ^ 5: with the loads' and the products' 128-byte swizzles these reads and both
 // writes of each are in all banks. A thread's rows are 32 apart, which no swizzle tells apart, so that their addresses are constants
 // away from one another: worked out for each piece they took half of this code.
-// One piece a step: with two dozen warps in seven roles, code that does not stay in the instruction caches slows all of them (four at
-// once: 189 us where this takes 173, 6 prompts of 2500 tokens, 12 heads of 64).
+// One piece a step: four at once took 189 us where this took 173 (6 prompts of 2000 tokens of texts of 2500, 12 heads of 64; 176 with
+// the scales by column).
 template <typename X, int D, int KIND, int ROWS>
 E2C_DEV void convert_stage(const uint8_t *x, uint8_t *y, int here, int upto, int tid) {
     using C = Cfg<D, KIND>;
@@ -1467,7 +1471,7 @@ __global__ void __launch_bounds__(Cfg<D, KIND>::NTHREADS, 1)
                     float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (C::CODE && !masked) {
 #pragma unroll 1
-                        for (int c0 = 0; c0 < TK; c0 += 16) {  // (and below: 32 columns a step are too much code)
+                        for (int c0 = 0; c0 < TK; c0 += 16) {  // (and below: with 32 columns a step a call of 173 us took 200)
                             uint32_t s[16];
                             tmem_ld16(ts + c0, s);
                             const Columns k(sc + c0), f(sc + TK + c0);  // they arrive while the products do
